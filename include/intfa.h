@@ -235,6 +235,98 @@ int intfa_scales_f16_to_f32(const void* src_f16, float* dst_f32, int64_t n, void
 /* Number of SMs of the current device (persistent-grid sizing); <0 on error. */
 int intfa_sm_count(void);
 
+/* ---------------------------------------------------------------------------------------------------------------------------
+ * Serving: rotary positions, a paged int8 K/V cache, attention over it.  No counterpart in the reference, whose operators take whole
+ * [B,H,N,D] tensors.  Indices that these entry points read on the DEVICE (positions, lengths, pages) are checked there: where one lies
+ * outside its table or cache nothing is read or written through it and `status` receives INTFA_STATUS_BAD_INDEX in its low byte.
+ */
+#define INTFA_STATUS_BAD_INDEX 96
+
+#define INTFA_TYPE_FP16 0
+#define INTFA_TYPE_BF16 1
+#define INTFA_TYPE_FP32 2
+
+/*
+ * Rotary positions: pair j of a head's first rot_dim channels, (a, b) = channels (j, j + rot_dim/2), or (2j, 2j+1) if interleaved,
+ * becomes (a c - b s, b c + a s) with (c, s) = table[position][j]; inverse: s with the other sign, which is the gradient.  Computed in
+ * fp32, rounded once; further channels are copied.  Rows whose position is outside the table become zeros.
+ * q [B,H,N,D] and, if k is not NULL, k [B,H_kv,N,D]: element strides for (B,H,N), last dim contiguous, 16-byte aligned rows; the same
+ * for the outputs, which may not overlap the inputs.  positions: [N], or [B,N] with positions_stride elements between batches.
+ */
+typedef struct IntfaRotaryParams {
+  const void* q; const void* k; void* q_out; void* k_out;
+  int64_t q_stride[3]; int64_t k_stride[3]; int64_t q_out_stride[3]; int64_t k_out_stride[3];
+  int32_t B, H, H_kv, N, D;             /* D in {16,32,64,128,256} */
+  int32_t dtype;                        /* INTFA_TYPE_* */
+  const float* table;                   /* [table_rows][rot_dim/2][2]: cos, sin; contiguous, 16-byte aligned */
+  int64_t table_rows; int32_t rot_dim;  /* even, 2 .. D */
+  int32_t interleaved, inverse;
+  const void* positions; int32_t positions_i64; int64_t positions_stride;
+  int32_t* status;                      /* device int32 or NULL */
+} IntfaRotaryParams;
+int intfa_rotary(const IntfaRotaryParams* p, void* stream);
+
+/*
+ * A paged int8 K/V cache and which of its pages hold which tokens.  k, v: [pages, H_kv, page_size, D] int8, element strides for
+ * (page, head, token) that are multiples of 16, last dim contiguous, 16-byte aligned.  k_scale, v_scale: fp32
+ * [pages, H_kv, page_size/block], any positive strides: a value is its code times the scale of its block of `block` tokens and head.
+ * Token i of sequence s is in slot i % page_size of page block_table[s][i / page_size]; entries past the last token are not read.
+ * seq_lens [S]: tokens in the cache, those of the call included (the new tokens of intfa_paged_append, the query rows of a causal
+ * intfa_paged_attention are the last of them).
+ */
+typedef struct IntfaPagedCache {
+  void* k; void* v; float* k_scale; float* v_scale;
+  int64_t k_stride[3]; int64_t v_stride[3]; int64_t ks_stride[3]; int64_t vs_stride[3];
+  const int32_t* block_table; int64_t table_stride; int32_t table_width;
+  const int32_t* seq_lens;
+  int32_t S, pages, H_kv, D;            /* D in {64,128,256} */
+  int32_t page_size, block;             /* powers of two, page_size 8 .. 256, block 1 .. page_size */
+} IntfaPagedCache;
+
+/*
+ * Appends k, v [tokens, H_kv, D] (fp16 or bf16) to the cache: the tokens of sequence s are cu_seqlens[s] .. cu_seqlens[s+1]-1 (NULL: one
+ * token a sequence) and become its last ones.  With a table, k is rotated by the tokens' positions first (as intfa_rotary, without
+ * rounding in between).  scale = max|x|/127 over the block, code = rint(x/scale); 0 where the scale is 0 or not finite.  A block that
+ * began before this call keeps the larger of its old scale and the new tokens', and where that grew its older codes become
+ * rint(code * (old/new)).  Rows behind the last sequence, and those of a sequence with seq_lens 0
+ * (padding), are left out.  Two sequences may not append to the same page in one call.
+ * q [tokens, H, D] if not NULL: rotated alike and quantised per row into q8 [tokens, H, D], q_scale [tokens, H] (both contiguous).
+ */
+typedef struct IntfaAppendParams {
+  IntfaPagedCache cache;
+  const void* q; const void* k; const void* v;
+  int64_t q_stride[2]; int64_t k_stride[2]; int64_t v_stride[2];      /* elements, (token, head); 16-byte aligned rows */
+  void* q8; float* q_scale;
+  int64_t tokens; int32_t H;
+  int32_t dtype;                        /* INTFA_TYPE_FP16 or _BF16 */
+  const int32_t* cu_seqlens;            /* [S+1] or NULL (tokens == S) */
+  const float* table; int64_t table_rows; int32_t rot_dim; int32_t interleaved;      /* as IntfaRotaryParams; table NULL: no rotation */
+  int32_t* status;
+} IntfaAppendParams;
+int intfa_paged_append(const IntfaAppendParams* p, void* stream);
+
+/*
+ * Attention of int8 query rows q [tokens, H, D] (their scales fp32 [tokens, H]) over the cache: the rows of sequence s are
+ * cu_seqlens[s] .. cu_seqlens[s+1]-1 (NULL: one row a sequence); causal: row i of n sees the keys up to seq_lens[s] - n + i, else all.
+ * Softmax, sums and the running output in fp32, p * v_scale rounded to fp16 for the product with v.  A row that sees nothing is zero
+ * (lse -inf); rows behind the last sequence are not written.  o [tokens, H, D]: strides for (token, head), multiples of 8.
+ * lse_out (or NULL): [tokens, H] fp32 contiguous, log2 domain, as intfa_fwd's.
+ * workspace: device scratch of intfa_paged_workspace_bytes() bytes, 256-byte aligned, contents irrelevant.
+ */
+typedef struct IntfaPagedParams {
+  IntfaPagedCache cache;
+  const void* q; const float* q_scale; void* o; float* lse_out;
+  int64_t q_stride[2]; int64_t qs_stride[2]; int64_t o_stride[2];
+  int64_t tokens; int32_t H;
+  int32_t o_dtype;                      /* INTFA_OUT_* */
+  const int32_t* cu_seqlens;
+  int32_t causal; float sm_scale;
+  void* workspace; uint64_t workspace_bytes;
+  int32_t* status;
+} IntfaPagedParams;
+int intfa_paged_attention(const IntfaPagedParams* p, void* stream);
+size_t intfa_paged_workspace_bytes(const IntfaPagedParams* p);
+
 #ifdef __cplusplus
 }
 #endif

@@ -14,12 +14,15 @@ ERR_INVALID_ARG, ERR_UNSUPPORTED, ERR_CUDA, ERR_DEVICE_WAIT, ERR_TOO_LARGE = -1,
 VARIANT_FULL, VARIANT_HALF, VARIANT_HALF_FP8 = 0, 1, 2
 VSCALE_PER_TENSOR, VSCALE_PER_CHANNEL = 0, 1
 SCALE_F16_Q, SCALE_F16_K, SCALE_F16_V = 1, 2, 4
+TYPE_FP16, TYPE_BF16, TYPE_FP32 = 0, 1, 2
+STATUS_BAD_INDEX = 96
 
 EXPORTS = ("intfa_version", "intfa_last_error", "intfa_fwd", "intfa_fwd_workspace_bytes", "intfa_quant_pertoken",
            "intfa_quant_v_workspace_bytes", "intfa_quant_v", "intfa_quant_v_partial_workspace_bytes", "intfa_quant_v_partial",
            "intfa_quant_qkv_workspace_bytes", "intfa_quant_qkv",
            "intfa_v_colmax", "intfa_v_quant_from_colmax", "intfa_quant_v_static",
-           "intfa_quant_v_static_max_words", "intfa_scales_f16_to_f32", "intfa_sm_count")
+           "intfa_quant_v_static_max_words", "intfa_scales_f16_to_f32", "intfa_sm_count",
+           "intfa_rotary", "intfa_paged_append", "intfa_paged_attention", "intfa_paged_workspace_bytes")
 
 _i64x3 = ctypes.c_int64 * 3
 _i64x2 = ctypes.c_int64 * 2
@@ -48,6 +51,49 @@ class IntfaFwdParams(ctypes.Structure):
         ("debug_wait_limit_kcycles", ctypes.c_int32), ("debug_skip_k_load", ctypes.c_int32),
         ("scale_f16", ctypes.c_int32),
         ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64),
+    ]
+
+
+class IntfaRotaryParams(ctypes.Structure):
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("q_out", ctypes.c_void_p), ("k_out", ctypes.c_void_p),
+        ("q_stride", _i64x3), ("k_stride", _i64x3), ("q_out_stride", _i64x3), ("k_out_stride", _i64x3),
+        ("B", ctypes.c_int32), ("H", ctypes.c_int32), ("H_kv", ctypes.c_int32), ("N", ctypes.c_int32), ("D", ctypes.c_int32),
+        ("dtype", ctypes.c_int32), ("table", ctypes.c_void_p), ("table_rows", ctypes.c_int64), ("rot_dim", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32), ("inverse", ctypes.c_int32),
+        ("positions", ctypes.c_void_p), ("positions_i64", ctypes.c_int32), ("positions_stride", ctypes.c_int64),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class IntfaPagedCache(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+        ("k_stride", _i64x3), ("v_stride", _i64x3), ("ks_stride", _i64x3), ("vs_stride", _i64x3),
+        ("block_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("table_width", ctypes.c_int32),
+        ("seq_lens", ctypes.c_void_p),
+        ("S", ctypes.c_int32), ("pages", ctypes.c_int32), ("H_kv", ctypes.c_int32), ("D", ctypes.c_int32),
+        ("page_size", ctypes.c_int32), ("block", ctypes.c_int32),
+    ]
+
+
+class IntfaAppendParams(ctypes.Structure):
+    _fields_ = [
+        ("cache", IntfaPagedCache), ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("q_stride", _i64x2), ("k_stride", _i64x2), ("v_stride", _i64x2), ("q8", ctypes.c_void_p), ("q_scale", ctypes.c_void_p),
+        ("tokens", ctypes.c_int64), ("H", ctypes.c_int32), ("dtype", ctypes.c_int32), ("cu_seqlens", ctypes.c_void_p),
+        ("table", ctypes.c_void_p), ("table_rows", ctypes.c_int64), ("rot_dim", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class IntfaPagedParams(ctypes.Structure):
+    _fields_ = [
+        ("cache", IntfaPagedCache), ("q", ctypes.c_void_p), ("q_scale", ctypes.c_void_p), ("o", ctypes.c_void_p),
+        ("lse_out", ctypes.c_void_p), ("q_stride", _i64x2), ("qs_stride", _i64x2), ("o_stride", _i64x2),
+        ("tokens", ctypes.c_int64), ("H", ctypes.c_int32), ("o_dtype", ctypes.c_int32), ("cu_seqlens", ctypes.c_void_p),
+        ("causal", ctypes.c_int32), ("sm_scale", ctypes.c_float), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64),
+        ("status", ctypes.c_void_p),
     ]
 
 
@@ -109,6 +155,14 @@ def load():
     lib.intfa_scales_f16_to_f32.argtypes = [vp, vp, i64, vp]
     lib.intfa_sm_count.restype = ctypes.c_int
     lib.intfa_sm_count.argtypes = []
+    lib.intfa_rotary.restype = ctypes.c_int
+    lib.intfa_rotary.argtypes = [ctypes.POINTER(IntfaRotaryParams), vp]
+    lib.intfa_paged_append.restype = ctypes.c_int
+    lib.intfa_paged_append.argtypes = [ctypes.POINTER(IntfaAppendParams), vp]
+    lib.intfa_paged_attention.restype = ctypes.c_int
+    lib.intfa_paged_attention.argtypes = [ctypes.POINTER(IntfaPagedParams), vp]
+    lib.intfa_paged_workspace_bytes.restype = ctypes.c_size_t
+    lib.intfa_paged_workspace_bytes.argtypes = [ctypes.POINTER(IntfaPagedParams)]
     _lib = lib
     return lib
 

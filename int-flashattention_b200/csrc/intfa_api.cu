@@ -236,4 +236,90 @@ int intfa_scales_f16_to_f32(const void* src_f16, float* dst_f32, int64_t n, void
   return scales_f16_to_f32(src_f16, dst_f32, n, reinterpret_cast<cudaStream_t>(stream));
 }
 
+// ---------------------------------------------------------------------------------------------------------------
+// rotary positions, paged cache
+// ---------------------------------------------------------------------------------------------------------------
+// rows of `esize`-byte elements: pointer and every stride on a 16-byte boundary
+static int check_rows(const char* name, const void* ptr, const int64_t* st, int n, int esize) {
+  if (!ptr) return set_error(INTFA_ERR_INVALID_ARG, "%s is NULL", name);
+  if (!aligned16(ptr)) return set_error(INTFA_ERR_INVALID_ARG, "%s must be 16-byte aligned", name);
+  for (int i = 0; i < n; ++i)
+    if (st[i] < 0 || (st[i] * esize) % 16 != 0)
+      return set_error(INTFA_ERR_INVALID_ARG, "%s stride[%d]=%lld: byte strides must be multiples of 16 and not negative", name, i, (long long)st[i]);
+  return INTFA_OK;
+}
+static int check_table(const float* table, int64_t rows, int rot, int D) {
+  if (!aligned16(table)) return set_error(INTFA_ERR_INVALID_ARG, "the table must be 16-byte aligned");
+  if (rows <= 0) return set_error(INTFA_ERR_INVALID_ARG, "the table has no rows");
+  if (rot < 2 || rot > D || rot % 2) return set_error(INTFA_ERR_INVALID_ARG, "rot_dim must be even and 2 .. head_dim, got %d", rot);
+  return INTFA_OK;
+}
+static bool power_of_two(int n) { return n > 0 && (n & (n - 1)) == 0; }
+static int check_cache(const IntfaPagedCache* c) {
+  int rc;
+  if (c->D != 64 && c->D != 128 && c->D != 256) return set_error(INTFA_ERR_UNSUPPORTED, "head_dim %d unsupported in a paged cache: 64, 128 or 256", c->D);
+  if (!power_of_two(c->page_size) || c->page_size < 8 || c->page_size > 256)
+    return set_error(INTFA_ERR_UNSUPPORTED, "page_size %d unsupported: a power of two, 8 to 256", c->page_size);
+  if (!power_of_two(c->block) || c->block > c->page_size)
+    return set_error(INTFA_ERR_UNSUPPORTED, "block %d unsupported: a power of two up to page_size = %d", c->block, c->page_size);
+  if (c->S <= 0 || c->pages <= 0 || c->H_kv <= 0 || c->table_width <= 0) return set_error(INTFA_ERR_INVALID_ARG, "S, pages, H_kv and table_width must be positive");
+  if ((rc = check_tma_tensor("k_cache", c->k, c->k_stride, 1)) || (rc = check_tma_tensor("v_cache", c->v, c->v_stride, 1))) return rc;
+  if (!c->k_scale || !c->v_scale) return set_error(INTFA_ERR_INVALID_ARG, "k_scale / v_scale is NULL");
+  if (!c->block_table || !c->seq_lens) return set_error(INTFA_ERR_INVALID_ARG, "block_table / seq_lens is NULL");
+  return INTFA_OK;
+}
+
+int intfa_rotary(const IntfaRotaryParams* p, void* stream) {
+  if (!p) return set_error(INTFA_ERR_INVALID_ARG, "params is NULL");
+  if (p->B <= 0 || p->H <= 0 || p->N <= 0 || (p->k && p->H_kv <= 0)) return set_error(INTFA_ERR_INVALID_ARG, "B, H, H_kv, N must be positive");
+  if (!head_dim_ok(p->D)) return set_error(INTFA_ERR_UNSUPPORTED, "head_dim %d unsupported: 16, 32, 64, 128 or 256", p->D);
+  if (p->dtype != INTFA_TYPE_FP16 && p->dtype != INTFA_TYPE_BF16 && p->dtype != INTFA_TYPE_FP32) return set_error(INTFA_ERR_INVALID_ARG, "unknown dtype %d", p->dtype);
+  const int es = p->dtype == INTFA_TYPE_FP32 ? 4 : 2;
+  int rc;
+  if ((rc = check_rows("q", p->q, p->q_stride, 3, es)) || (rc = check_rows("q_out", p->q_out, p->q_out_stride, 3, es))) return rc;
+  if (p->k && ((rc = check_rows("k", p->k, p->k_stride, 3, es)) || (rc = check_rows("k_out", p->k_out, p->k_out_stride, 3, es)))) return rc;
+  if (!p->table || !p->positions) return set_error(INTFA_ERR_INVALID_ARG, "table / positions is NULL");
+  if ((rc = check_table(p->table, p->table_rows, p->rot_dim, p->D))) return rc;
+  return rotary(p, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int intfa_paged_append(const IntfaAppendParams* p, void* stream) {
+  if (!p) return set_error(INTFA_ERR_INVALID_ARG, "params is NULL");
+  int rc;
+  if ((rc = check_cache(&p->cache))) return rc;
+  if (p->tokens <= 0 || (p->q && p->H <= 0)) return set_error(INTFA_ERR_INVALID_ARG, "tokens and H must be positive");
+  if (!p->cu_seqlens && p->tokens != p->cache.S) return set_error(INTFA_ERR_INVALID_ARG, "without cu_seqlens there is one token a sequence: %lld tokens, %d sequences", (long long)p->tokens, p->cache.S);
+  if (p->dtype != INTFA_TYPE_FP16 && p->dtype != INTFA_TYPE_BF16) return set_error(INTFA_ERR_INVALID_ARG, "dtype must be INTFA_TYPE_FP16 or INTFA_TYPE_BF16");
+  if (p->tokens > 0x7fffffffLL) return set_error(INTFA_ERR_TOO_LARGE, "too many tokens");
+  if ((rc = check_rows("k", p->k, p->k_stride, 2, 2)) || (rc = check_rows("v", p->v, p->v_stride, 2, 2))) return rc;
+  if (p->q) {
+    if ((rc = check_rows("q", p->q, p->q_stride, 2, 2))) return rc;
+    if (!p->q8 || !aligned16(p->q8) || !p->q_scale) return set_error(INTFA_ERR_INVALID_ARG, "q8 (16-byte aligned) and q_scale are needed with q");
+  }
+  if (p->table && (rc = check_table(p->table, p->table_rows, p->rot_dim, p->cache.D))) return rc;
+  return paged_append(p, reinterpret_cast<cudaStream_t>(stream));
+}
+
+static int check_paged(const IntfaPagedParams* p) {
+  int rc;
+  if ((rc = check_cache(&p->cache))) return rc;
+  if (p->tokens <= 0 || p->H <= 0) return set_error(INTFA_ERR_INVALID_ARG, "tokens and H must be positive");
+  if (p->H % p->cache.H_kv) return set_error(INTFA_ERR_INVALID_ARG, "H=%d must be a multiple of H_kv=%d", p->H, p->cache.H_kv);
+  if (!p->cu_seqlens && p->tokens != p->cache.S) return set_error(INTFA_ERR_INVALID_ARG, "without cu_seqlens there is one row a sequence: %lld rows, %d sequences", (long long)p->tokens, p->cache.S);
+  if (p->tokens * p->H > 0x7fffffffLL) return set_error(INTFA_ERR_TOO_LARGE, "too many query rows");
+  if (p->o_dtype != INTFA_OUT_FP16 && p->o_dtype != INTFA_OUT_BF16) return set_error(INTFA_ERR_INVALID_ARG, "o_dtype must be INTFA_OUT_FP16 or INTFA_OUT_BF16");
+  return INTFA_OK;
+}
+size_t intfa_paged_workspace_bytes(const IntfaPagedParams* p) { return p && check_paged(p) == INTFA_OK ? paged_workspace_bytes(p) : 0; }
+
+int intfa_paged_attention(const IntfaPagedParams* p, void* stream) {
+  if (!p) return set_error(INTFA_ERR_INVALID_ARG, "params is NULL");
+  int rc;
+  if ((rc = check_paged(p))) return rc;
+  if ((rc = check_rows("q", p->q, p->q_stride, 2, 1)) || (rc = check_rows("o", p->o, p->o_stride, 2, 2))) return rc;
+  if (!p->q_scale || p->qs_stride[0] < 0 || p->qs_stride[1] < 0) return set_error(INTFA_ERR_INVALID_ARG, "q_scale is NULL or has a negative stride");
+  if (!p->workspace || (reinterpret_cast<uintptr_t>(p->workspace) & 255u)) return set_error(INTFA_ERR_INVALID_ARG, "workspace is NULL or not 256-byte aligned");
+  return paged_attention(p, reinterpret_cast<cudaStream_t>(stream));
+}
+
 }  // extern "C"

@@ -162,9 +162,8 @@ static int next_tile_counter(unsigned int** out) {
   return INTFA_OK;
 }
 
-// [B,H,N,D] tensor, element strides for (B,H,N); box = (box_d, box_rows, 1, 1)
-static int make_tmap(CUtensorMap* tm, const void* base, int esize, const int64_t* stride, int B, int H, int N, int D,
-                     int box_d, int box_rows, CUtensorMapSwizzle swz) {
+int make_tmap(CUtensorMap* tm, const void* base, int esize, const int64_t* stride, int B, int H, int N, int D, int box_d, int box_rows,
+              CUtensorMapSwizzle swz) {
   EncodeTiledFn fn = get_encode_fn();
   if (!fn) return set_error(INTFA_ERR_CUDA, "cuTensorMapEncodeTiled entry point not available");
   cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)N, (cuuint64_t)H, (cuuint64_t)B};

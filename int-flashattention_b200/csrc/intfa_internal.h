@@ -1,5 +1,6 @@
 // Internal declarations shared by the translation units of libintfa.so.
 #pragma once
+#include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -40,6 +41,14 @@ struct KParams {
 int set_error(int code, const char* fmt, ...);
 // SM count of the current device, cached per device; <=0 on failure.
 int sm_count_cached();
+
+// What a kernel stores in the status word where an index that it reads on the device (a position, page or length) lies outside its table or
+// cache; the codes of the waits are others.
+constexpr int kStatusBadIndex = INTFA_STATUS_BAD_INDEX;
+
+// [B,H,N,D] tensor, element strides for (B,H,N); box = (box_d, box_rows, 1, 1)
+int make_tmap(CUtensorMap* tm, const void* base, int esize, const int64_t* stride, int B, int H, int N, int D, int box_d, int box_rows,
+              CUtensorMapSwizzle swz);
 
 // Few query rows against many keys (intfa_decode.cu).  Returns false where the call is not one for that path.
 bool decode_dispatch(const IntfaFwdParams* a, cudaStream_t stream, int* rc);
@@ -89,6 +98,10 @@ size_t quant_qkv_workspace_bytes(int B, int Hkv, int Nk, int D);
 int quant_qkv(const void* q, const void* k, const void* v, const int64_t* v_st, void* q8, void* k8, void* v8, float* qs,
               float* ks, float* vs, int mode, int B, int H, int Hkv, int Nq, int Nk, int D, void* workspace,
               cudaStream_t stream);
+int rotary(const IntfaRotaryParams* a, cudaStream_t stream);
+int paged_append(const IntfaAppendParams* a, cudaStream_t stream);
+int paged_attention(const IntfaPagedParams* a, cudaStream_t stream);
+size_t paged_workspace_bytes(const IntfaPagedParams* a);
 int scales_f16_to_f32(const void* src, float* dst, long long n, cudaStream_t stream);
 
 }  // namespace intfa

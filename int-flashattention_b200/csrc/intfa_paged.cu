@@ -1,0 +1,348 @@
+// New tokens into a paged int8 cache: keys rotated by their positions, keys and values quantised with one scale for each block of
+// `block` tokens and head, queries of the same tokens rotated and quantised per token, all in one launch.
+//
+// Reads 2 bytes a value, writes 1 (10 000 tokens of 32 + 8 + 8 heads x 128: 345 MB, 53 us at the measured copy rate): bound by HBM, and
+// by launch and latency for the few tokens of a decode step.
+//   block = 1   a row (one head of one token) is quantised by the lanes that loaded it; a CTA takes one token, or a few of few heads
+//   block > 1   a CTA takes what a sequence adds to one block, for some heads: the largest magnitudes first, then the codes.  A block that
+//               began in an earlier call keeps the larger of its old scale and the new tokens'; where that grew its older codes become
+//               rint(code * (old / new)).  So a block's codes depend on how its tokens were handed over, as its scale must.
+#include "intfa_rows.cuh"
+
+namespace intfa {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxTokens = 16;           // tokens of a CTA: 32 rows at 64 channels, two tensors
+
+struct AppendJob {
+  const void* x[3];                      // q, k, v: packed [tokens, heads, D]
+  long long xn[3], xh[3];
+  int heads[3];
+  int8_t* q8; float* qs;                 // contiguous
+  int8_t* cache[2]; float* scale[2];     // k, v
+  long long cp[2], ch[2], cn[2], sp[2], sh[2], sb[2];
+  const int* table; long long table_stride; int width;
+  const int* lens; const int* cu;
+  int S, pages, page_log, block_log;
+  long long tokens;
+  const float* rot_table; long long rot_rows; int rot, interleaved;
+  int* status;
+};
+
+__device__ __forceinline__ int cu_at(const AppendJob& p, int s) { return p.cu ? p.cu[s] : s; }
+__device__ __forceinline__ void report(const AppendJob& p) {
+  if (p.status) atomicCAS(p.status, 0, kStatusBadIndex);
+}
+
+// Where a token goes.  page < 0: nowhere (it is behind the last sequence, or of one without tokens, or an index lies outside the cache).
+// Called by a warp.
+struct Place {
+  long long pos;
+  int page, slot;
+  int own;                               // belongs to a sequence
+};
+__device__ __forceinline__ Place place_of(const AppendJob& p, long long t) {
+  Place r;
+  r.pos = 0;
+  r.page = -1;
+  r.slot = r.own = 0;
+  if (t >= p.tokens) return r;
+  int s = 0;
+  if (p.cu) {
+    const int first = p.cu[0], last = p.cu[p.S];
+    if (last > p.tokens) report(p);
+    if (t < first || t >= last) return r;
+    s = find_last(p.S, t, [&](int i) { return (long long)p.cu[i]; });
+  } else {
+    s = (int)t;
+  }
+  const int end = cu_at(p, s + 1), len = p.lens[s];
+  if (len == 0) return r;                // (padding)
+  const long long pos = (long long)len - (end - t);
+  r.own = 1;
+  r.pos = pos;
+  const long long col = pos >> p.page_log;
+  if (t < end && pos >= 0 && col < p.width) {
+    const int page = p.table[s * p.table_stride + col];
+    if (page >= 0 && page < p.pages) {
+      r.page = page;
+      r.slot = (int)(pos & ((1 << p.page_log) - 1));
+    }
+  }
+  if (r.page < 0) report(p);
+  return r;
+}
+
+// Rows of the tensors from `first` on, one CTA of `tokens_cta` tokens; each row has its own scale.
+template <typename T, int D, int FIRST, int COUNT>
+__device__ __forceinline__ void token_rows(const AppendJob& p, long long cta, int tokens_cta, Place* place) {
+  constexpr int LPR = D / 8, SLOTS = kThreads / LPR, U = 4;
+  const int e0 = threadIdx.x % LPR * 8, slot = threadIdx.x / LPR, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per_token = SLOTS / tokens_cta, mine = slot / per_token, row0 = slot % per_token;
+  const long long token = cta * tokens_cta + mine;
+  const bool in = token < p.tokens;
+  const int h0 = p.heads[FIRST], h1 = COUNT > 1 ? p.heads[FIRST + 1] : 0, rows = h0 + h1 + (COUNT > 2 ? p.heads[FIRST + 2] : 0);
+  Raw<T> raw[U];
+  auto split = [&](int r, int& w, int& h) {
+    w = FIRST;
+    h = r;
+    if (COUNT > 1 && r >= h0) {
+      w = FIRST + 1;
+      h = r - h0;
+      if (COUNT > 2 && h >= h1) {
+        w = FIRST + 2;
+        h -= h1;
+      }
+    }
+  };
+  auto src = [&](int r) {
+    int w, h;
+    split(r, w, h);
+    return static_cast<const T*>(p.x[w]) + token * p.xn[w] + h * p.xh[w];
+  };
+  auto load = [&](int r) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      raw[u].zero();
+      if (in && r + u * per_token < rows) raw[u].load(src(r + u * per_token) + e0);
+    }
+  };
+  load(row0);
+  for (int i = warp; i < tokens_cta; i += kThreads / 32) {
+    const Place x = place_of(p, cta * tokens_cta + i);
+    if (lane == 0) place[i] = x;
+  }
+  __syncthreads();
+  const Place at = place[mine];
+  Turn turn;
+  const bool turns = p.rot_table != nullptr, pos_ok = !turns || (at.pos >= 0 && at.pos < p.rot_rows);
+  if (turns) {
+    turn.load(p.rot_table, pos_ok ? at.pos : 0, p.rot, p.interleaved, false, e0);
+    if (!pos_ok && at.own && threadIdx.x % (per_token * LPR) == 0) report(p);
+  }
+  const bool goes = in && at.page >= 0 && pos_ok;
+  const int rounds = (rows + per_token * U - 1) / (per_token * U);
+#pragma unroll 1
+  for (int k = 0; k < rounds; ++k) {
+    const int r = row0 + k * per_token * U;
+    if (k > 0) load(r);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int row = r + u * per_token;
+      const bool row_ok = goes && row < rows;
+      int w, h;
+      split(row, w, h);
+      float x[8];
+      widen(raw[u], x);
+      if (turns) turn.apply(x, raw[u], src(row_ok ? row : 0), row_ok, p.rot, p.interleaved, e0, w < 2);
+      const float s = scale_of(row_max<LPR>(absmax8(x)));
+      const uint2 c = codes8(x, s, __fdiv_rn(1.0f, s));
+      if (row_ok) {
+        if (w == 0) {
+          *reinterpret_cast<uint2*>(p.q8 + (token * p.heads[0] + h) * D + e0) = c;
+          if (e0 == 0) p.qs[token * p.heads[0] + h] = s;
+        } else {
+          *reinterpret_cast<uint2*>(p.cache[w - 1] + at.page * p.cp[w - 1] + h * p.ch[w - 1] + at.slot * p.cn[w - 1] + e0) = c;
+          if (e0 == 0) p.scale[w - 1][at.page * p.sp[w - 1] + h * p.sh[w - 1] + at.slot * p.sb[w - 1]] = s;
+        }
+      }
+    }
+  }
+}
+
+// block = 1
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) append_tokens_kernel(const AppendJob p, int tokens_cta) {
+  __shared__ Place place[kMaxTokens];
+  pdl_wait();
+  pdl_launch();
+  if (p.q8) token_rows<T, D, 0, 3>(p, blockIdx.x, tokens_cta, place);
+  else token_rows<T, D, 1, 2>(p, blockIdx.x, tokens_cta, place);
+}
+
+// block > 1.  CTAs 0 .. units * groups - 1: what one sequence adds to one block, `heads_cta` heads of K and V; the rest: q.
+// Unit u of sequence s: u = cu[s] / block + 2 s + i for the i-th block that the sequence touches (it touches at most n / block + 2).
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) append_blocks_kernel(const AppendJob p, int units, int groups, int heads_cta, int tokens_cta) {
+  constexpr int LPR = D / 8, SLOTS = kThreads / LPR;
+  __shared__ Place place[kMaxTokens];
+  __shared__ unsigned int most[2 * kThreads];        // [K, V][heads_cta]
+  __shared__ float s_old[2 * kThreads], s_new[2 * kThreads];
+  pdl_wait();
+  pdl_launch();
+  if ((long long)blockIdx.x >= (long long)units * groups) {
+    token_rows<T, D, 0, 1>(p, (long long)blockIdx.x - (long long)units * groups, tokens_cta, place);
+    return;
+  }
+  const int u = blockIdx.x / groups, head0 = (blockIdx.x - u * groups) * heads_cta;
+  const int nh = min(heads_cta, p.heads[1] - head0), block = 1 << p.block_log;
+  const int s = p.cu ? find_last(p.S, u, [&](int i) { return (long long)(p.cu[i] >> p.block_log) + 2 * i; })
+                     : find_last(p.S, u, [&](int i) { return (long long)(i >> p.block_log) + 2 * i; });
+  const int t0 = cu_at(p, s), t1 = cu_at(p, s + 1);
+  const long long len = p.lens[s], first = len - (t1 - t0);
+  if (t0 < 0 || t1 <= t0 || len == 0) return;
+  if (first < 0 || t1 > p.tokens) {
+    if (threadIdx.x == 0) report(p);
+    return;
+  }
+  // the block, its new tokens [n0, n1) (positions) and where its older ones begin
+  const long long bi = (first >> p.block_log) + (u - ((t0 >> p.block_log) + 2 * s)), b0 = bi << p.block_log;
+  const long long n0 = b0 > first ? b0 : first, n1 = b0 + block < len ? b0 + block : len;
+  if (n0 >= n1) return;
+  const bool began = b0 < n0;
+  const long long col = b0 >> p.page_log;
+  const int page = col < p.width ? p.table[s * p.table_stride + col] : -1;
+  if (page < 0 || page >= p.pages || (p.rot_table && n1 > p.rot_rows)) {
+    if (threadIdx.x == 0) report(p);
+    return;
+  }
+  const int slot0 = (int)(b0 & ((1 << p.page_log) - 1)), blk = slot0 >> p.block_log;
+  const int e0 = threadIdx.x % LPR * 8, slot = threadIdx.x / LPR;
+  for (int i = threadIdx.x; i < 2 * nh; i += kThreads) most[i] = 0u;
+  __syncthreads();
+  const int nt = (int)(n1 - n0), rows = nt * nh * 2, rounds = (rows + SLOTS - 1) / SLOTS;
+  // row r: token r / (2 nh), then K's heads and V's
+  Turn turn;
+  float x[8];
+  auto fetch = [&](int k, int& token, int& wh) {
+    const int r = k * SLOTS + slot;
+    const bool ok = r < rows;
+    token = ok ? r / (2 * nh) : 0;
+    wh = ok ? r - token * 2 * nh : 0;
+    const int w = wh >= nh ? 1 : 0, h = head0 + wh - (w ? nh : 0);
+    const T* row = static_cast<const T*>(p.x[1 + w]) + (t0 + (n0 - first) + token) * p.xn[1 + w] + h * p.xh[1 + w];
+    Raw<T> raw;
+    raw.zero();
+    if (ok) raw.load(row + e0);
+    widen(raw, x);
+    if (p.rot_table) {
+      turn.load(p.rot_table, n0 + token, p.rot, p.interleaved, false, e0);
+      turn.apply(x, raw, row, ok, p.rot, p.interleaved, e0, w == 0);
+    }
+    return ok;
+  };
+  int token = 0, wh = 0;
+  bool ok = false;
+#pragma unroll 1
+  for (int k = 0; k < rounds; ++k) {
+    ok = fetch(k, token, wh);
+    const float m = row_max<LPR>(absmax8(x));
+    if (ok && e0 == 0) atomicMax(&most[wh], __float_as_uint(m));       // (not negative, a NaN above all: they compare as whole numbers)
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * nh; i += kThreads) {
+    const int w = i >= nh ? 1 : 0, h = head0 + i - (w ? nh : 0);
+    float* at = p.scale[w] + page * p.sp[w] + h * p.sh[w] + blk * p.sb[w];
+    const float old = began ? *at : 0.f, now = max_nan(old, scale_of(__uint_as_float(most[i])));
+    s_old[i] = old;
+    s_new[i] = now;
+    *at = now;
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int k = 0; k < rounds; ++k) {
+    if (rounds > 1) ok = fetch(k, token, wh);
+    if (!ok) continue;
+    const int w = wh >= nh ? 1 : 0, h = head0 + wh - (w ? nh : 0);
+    const float sc = s_new[wh];
+    *reinterpret_cast<uint2*>(p.cache[w] + page * p.cp[w] + h * p.ch[w] + (slot0 + (int)(n0 - b0) + token) * p.cn[w] + e0) =
+        codes8(x, sc, __fdiv_rn(1.0f, sc));
+  }
+  if (!began) return;
+  const int older = (int)(n0 - b0) * nh * 2;
+#pragma unroll 1
+  for (int r = slot; r < older; r += SLOTS) {
+    const int tk = r / (2 * nh), i = r - tk * 2 * nh, w = i >= nh ? 1 : 0, h = head0 + i - (w ? nh : 0);
+    const float was = s_old[i], now = s_new[i];
+    if (__float_as_uint(was) == __float_as_uint(now)) continue;
+    uint2* at = reinterpret_cast<uint2*>(p.cache[w] + page * p.cp[w] + h * p.ch[w] + (slot0 + tk) * p.cn[w] + e0);
+    const uint2 c = *at;
+    const float ratio = now > 0.f && now <= 3.402823466e38f ? __fdiv_rn(was, now) : 0.f;
+    float y[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = __fmul_rn((float)(int8_t)((j < 4 ? c.x : c.y) >> (8 * (j & 3))), ratio);
+    *at = codes8(y, 1.0f, 1.0f);
+  }
+}
+
+template <typename T, int D>
+int run(const AppendJob& p, cudaStream_t stream) {
+  constexpr int SLOTS = kThreads / (D / 8);
+  auto tokens_of = [&](int heads) {
+    int n = 1;
+    while (n * 2 * heads <= SLOTS) n *= 2;
+    return n < kMaxTokens ? n : kMaxTokens;
+  };
+  if (p.block_log == 0) {
+    const int n = tokens_of(p.heads[0] + p.heads[1] + p.heads[2]);
+    const long long grid = (p.tokens + n - 1) / n;
+    if (grid > 0x7fffffffLL) return set_error(INTFA_ERR_TOO_LARGE, "too many tokens");
+    return launch_kernel("append", append_tokens_kernel<T, D>, (unsigned)grid, kThreads, 0, stream, p, n);
+  }
+  // Heads a CTA: about 4 rounds of rows where the block is short, so that a step of one token has all its heads in one CTA or two
+  int heads_cta = 4 * SLOTS / (2 << p.block_log);
+  if (heads_cta < 1) heads_cta = 1;
+  if (heads_cta > p.heads[1]) heads_cta = p.heads[1];
+  if (heads_cta > kThreads) heads_cta = kThreads;
+  const int groups = (p.heads[1] + heads_cta - 1) / heads_cta, n = p.q8 ? tokens_of(p.heads[0]) : 1;
+  const long long units = (p.tokens >> p.block_log) + 2LL * p.S, grid = units * groups + (p.q8 ? (p.tokens + n - 1) / n : 0);
+  if (grid > 0x7fffffffLL) return set_error(INTFA_ERR_TOO_LARGE, "too many tokens");
+  return launch_kernel("append", append_blocks_kernel<T, D>, (unsigned)grid, kThreads, 0, stream, p, (int)units, groups, heads_cta, n);
+}
+
+int log2_of(long long n) {
+  int i = 0;
+  while ((1LL << i) < n) ++i;
+  return i;
+}
+
+}  // namespace
+
+int paged_append(const IntfaAppendParams* a, cudaStream_t stream) {
+  AppendJob p;
+  const void* x[3] = {a->q, a->k, a->v};
+  const int64_t* xs[3] = {a->q_stride, a->k_stride, a->v_stride};
+  for (int i = 0; i < 3; ++i) {
+    p.x[i] = x[i];
+    p.xn[i] = xs[i][0];
+    p.xh[i] = xs[i][1];
+  }
+  p.heads[0] = a->q ? a->H : 0;
+  p.heads[1] = p.heads[2] = a->cache.H_kv;
+  p.q8 = a->q ? static_cast<int8_t*>(a->q8) : nullptr;
+  p.qs = a->q_scale;
+  const IntfaPagedCache& c = a->cache;
+  p.cache[0] = static_cast<int8_t*>(c.k);
+  p.cache[1] = static_cast<int8_t*>(c.v);
+  p.scale[0] = c.k_scale;
+  p.scale[1] = c.v_scale;
+  const int64_t *cs[2] = {c.k_stride, c.v_stride}, *ss[2] = {c.ks_stride, c.vs_stride};
+  for (int i = 0; i < 2; ++i) {
+    p.cp[i] = cs[i][0]; p.ch[i] = cs[i][1]; p.cn[i] = cs[i][2];
+    p.sp[i] = ss[i][0]; p.sh[i] = ss[i][1]; p.sb[i] = ss[i][2];
+  }
+  p.table = c.block_table;
+  p.table_stride = c.table_stride;
+  p.width = c.table_width;
+  p.lens = c.seq_lens;
+  p.cu = a->cu_seqlens;
+  p.S = c.S;
+  p.pages = c.pages;
+  p.page_log = log2_of(c.page_size);
+  p.block_log = log2_of(c.block);
+  p.tokens = a->tokens;
+  p.rot_table = a->table;
+  p.rot_rows = a->table_rows;
+  p.rot = a->rot_dim;
+  p.interleaved = a->interleaved;
+  p.status = a->status;
+  const bool f16 = a->dtype == INTFA_TYPE_FP16;
+  switch (c.D) {
+    case 64: return f16 ? run<__half, 64>(p, stream) : run<__nv_bfloat16, 64>(p, stream);
+    case 128: return f16 ? run<__half, 128>(p, stream) : run<__nv_bfloat16, 128>(p, stream);
+    default: return f16 ? run<__half, 256>(p, stream) : run<__nv_bfloat16, 256>(p, stream);
+  }
+}
+
+}  // namespace intfa

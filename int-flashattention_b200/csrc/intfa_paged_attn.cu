@@ -1,0 +1,885 @@
+// Attention of packed int8 query rows over a paged int8 K/V cache: decode, and the few rows of a draft or a chunk.
+//
+//   s = dot(q8, k8) * (q_scale * sm_scale * log2 e) * k_scale[block],   p = exp2(s - max),   o = sum p v_scale[block] v8 / sum p
+//
+// Reads K and V once (64 sequences of up to 8192 keys, 8 heads x 128: 703 MB, 109 us at the measured copy rate): bound by HBM.
+//
+// Work.  A unit is (sequence, K/V head, tile of RT = 8 NT rows); the rows of all query heads that share the K/V head are packed into it, so
+// that K and V are read once for all of them.  Its keys are cut into chunks of 32.  The chunks of all units in a row are dealt out to the
+// warps of the GPU in equal contiguous shares, whatever the sequences' lengths are: the lengths are read on the device, so nothing waits for
+// the host and a captured graph takes other lengths at its next replay.  A warp keeps the softmax state and the output of the unit it is in
+// in registers.  A unit that lies within one warp's share is written at once; the parts of the others go to scratch and combine_kernel adds
+// them up, in the order of the keys.
+//
+// Loads.  Each warp has a ring of NS chunks of its own, filled by TMA (pages of any size and order, 8 to 32 rows a copy) and by cp.async (scales,
+// query rows), so no warp waits for another and NS - 1 chunks a warp (128 KB an SM) are in flight.  A chunk's rows are swizzled by the
+// TMA such that the 16-byte reads below are free of bank conflicts.
+//
+// Arithmetic.  m16n8 warp-level MMAs straight from that ring: 8 or 16 rows are far below the smallest tcgen05 tile.  Q K^T is an int8
+// product, exact in int32; the order of the k index is free, so lane t of a quad takes 16-byte piece 2t of each row and calls it its
+// fragment.  For P V the int8 V becomes fp16 (exact: the byte is put behind fp16's 1024 and 1152 is taken off), two keys of a channel in a word.
+// The V scale of a key multiplies its p ahead of the rounding to fp16.  Since the scales of a cache may differ by any factor, the products
+// w = p * v_scale have a running maximum of their own (of s + log2 v_scale), so the largest w is 1 whatever the scales are and the rounding
+// (2^-11 of each w, or 2^-25 of the largest) costs no more than with equal scales; sums and both maxima are fp32.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <atomic>
+
+#include "intfa_internal.h"
+#include "intfa_ptx.cuh"
+#include "intfa_rows.cuh"
+
+namespace intfa {
+namespace {
+
+constexpr int kChunk = 32;                        // keys
+constexpr float kMagicF = 12582912.0f;            // 1.5*2^23: added to an int32 below 2^22 as a bit pattern, it reads as fp32 1.5*2^23 + value
+constexpr int kMagicI = 0x4B400000;
+
+// a unit as combine_kernel sees it
+struct UnitPart {
+  long long chunk0, chunk1;                       // its chunks among all
+  int s, unit;                                    // sequence, unit in it
+  int open;                                       // 1: its parts are in scratch
+  int pad;
+};
+
+struct PParams {
+  const int8_t* q; const float* qs; void* o; float* lse;
+  long long qn, qh, qsn, qsh, on, oh;
+  const float* ks; const float* vs;
+  long long ksP, ksH, ksB, vsP, vsH, vsB;
+  const int* table; long long table_stride; int width;
+  const int* lens; const int* cu;
+  int S, H, Hkv, ratio, pages, page_log, block_log, box_log;
+  long long T;
+  int causal, o_bf16;
+  float c;                                        // sm_scale * log2(e)
+  int workers, least;                             // warps of the grid; fewest chunks a warp takes
+  int rows_tile;                                  // RT
+  float* part; float* part_ml;                    // [2*workers][RT][D]; [2*workers][RT]{m, mw, l, -}
+  UnitPart* units; long long max_units;           // [max_units]
+  long long* head;                                // {units, share, chunks}
+  int* status;
+};
+
+__device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 lds8(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 lds_f2(uint32_t a) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ float lds_f(uint32_t a) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(ok ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ float log2_approx(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// what a sequence asks for
+struct Seq {
+  int t0, n;                 // its query rows: tokens t0 .. t0 + n - 1
+  int keys;                  // that are looked at
+  long long len;
+  int tiles, chunks;         // row tiles and chunks of each K/V head
+};
+__device__ __forceinline__ Seq seq_of(const PParams& p, int s) {
+  Seq q;
+  const long long t0 = p.cu ? p.cu[s] : s, t1 = p.cu ? p.cu[s + 1] : s + 1;
+  q.t0 = (int)t0;
+  q.n = t0 >= 0 && t1 > t0 && t1 <= p.T ? (int)(t1 - t0) : 0;
+  q.len = p.lens[s];
+  const long long most = (long long)p.width << p.page_log;
+  q.keys = (int)(q.len < 0 ? 0 : q.len < most ? q.len : most);
+  q.tiles = (int)(((long long)q.n * p.ratio + p.rows_tile - 1) / p.rows_tile);
+  q.chunks = q.keys > kChunk ? (q.keys + kChunk - 1) / kChunk : 1;      // (a row without keys is written, too)
+  return q;
+}
+
+// a place in the row of all chunks
+struct Cursor {
+  Seq q;
+  int s, unit, chunk;        // sequence; unit in it (K/V head * tiles + tile); chunk in that
+  __device__ __forceinline__ void next(const PParams& p) {
+    if (++chunk < q.chunks) return;
+    chunk = 0;
+    if (++unit < q.tiles * p.Hkv) return;
+    unit = 0;
+    next_seq(p);
+  }
+  // to the next sequence with query rows, if there is one
+  __device__ __forceinline__ void next_seq(const PParams& p) {
+    q.n = 0;
+    while (++s < p.S) {
+      q = seq_of(p, s);
+      if (q.n > 0) break;
+    }
+  }
+};
+
+template <int D, int NT, int WARPS, int NS>
+struct DecodeCfg {
+  static constexpr int RT = 8 * NT, KV = kChunk * D;                    // rows of a tile; bytes of K or V of a chunk
+  static constexpr int PANEL = D < 128 ? D : 128, PANELS = D / PANEL;   // a row lies in panels of at most 128 bytes
+  static constexpr int EXTRA = 2 * kChunk * 4 + RT * D + RT * 4;        // scales, query rows and their scales
+  static constexpr int OFF_EXTRA = WARPS * NS * 2 * KV;
+  static constexpr int OFF_BAR = OFF_EXTRA + WARPS * NS * EXTRA;
+  static constexpr int OFF_PRE = OFF_BAR + WARPS * NS * 8;              // [threads + 1] chunks (long long) and units (int) before a thread's sequences
+  static constexpr int OFF_MISC = OFF_PRE + ((32 * WARPS + 1) * 12 + 15) / 16 * 16;
+  static constexpr int SMEM = OFF_MISC + 32 + 1024;
+  static constexpr int MERGE = WARPS * RT * ((D + 4) + 4) * 4;          // (over the ring, when it is done with)
+  static_assert(MERGE <= OFF_EXTRA, "merge");
+  static_assert(EXTRA % 16 == 0, "alignment");
+  static_assert(SMEM <= 227 * 1024, "shared memory");
+};
+
+// state of the rows of a unit in one warp: rows n*8 + lane/4 (maxima, l: of this lane's keys only until reduced), channels as `acc`
+template <int D, int NT>
+struct RowState {
+  static constexpr int PANELS = D < 128 ? 1 : D / 128, W = D < 128 ? D / 32 : 4, MT = PANELS * W * 2;
+  float m[NT], mw[NT], l[NT];
+  float acc[NT][MT][4];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      m[n] = mw[n] = -INFINITY;
+      l[n] = 0.f;
+#pragma unroll
+      for (int i = 0; i < MT; ++i) acc[n][i][0] = acc[n][i][1] = acc[n][i][2] = acc[n][i][3] = 0.f;
+    }
+  }
+  __device__ __forceinline__ void reduce_l() {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      l[n] += __shfl_xor_sync(0xffffffffu, l[n], 1);
+      l[n] += __shfl_xor_sync(0xffffffffu, l[n], 2);
+    }
+  }
+};
+// channel of entry (i, 0/1) of a lane; entries 2, 3: the next channel
+template <int D>
+__device__ __forceinline__ int channel_of(int i, int g) {
+  constexpr int W = D < 128 ? D / 32 : 4;
+  return i / (2 * W) * 128 + g * (4 * W) + i % (2 * W) * 2;
+}
+
+__device__ __forceinline__ float safe(float m) { return m == -INFINITY ? 0.f : m; }
+
+// what the sum of a row is multiplied by: 2^(mw - m) / l.  A row that sees nothing has l = 0, one whose values are all zero mw = -inf.
+__device__ __forceinline__ float row_factor(float m, float mw, float l) {
+  return l == 0.f ? 0.f : mw == -INFINITY ? l * 0.f : ex2_approx(mw - safe(m)) / l;
+}
+
+template <int D, int NT>
+__device__ __forceinline__ void write_rows(const PParams& p, const Seq& q, int head, int tile, const RowState<D, NT>& st) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  constexpr int MT = RowState<D, NT>::MT, W = RowState<D, NT>::W, PANELS = RowState<D, NT>::PANELS;
+  const int R = q.n * p.ratio;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const float f = row_factor(st.m[n], st.mw[n], st.l[n]);
+    const int rg = tile * (8 * NT) + n * 8 + g;
+    if (p.lse && t == 0 && rg < R) p.lse[(q.t0 + rg / p.ratio) * (long long)p.H + head * p.ratio + rg % p.ratio] = st.m[n] + log2f(st.l[n]);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float fe = __shfl_sync(0xffffffffu, f, (2 * t + e) * 4);
+      const int r = tile * (8 * NT) + n * 8 + 2 * t + e;
+      if (r >= R) continue;
+      uint16_t* o = static_cast<uint16_t*>(p.o) + (q.t0 + r / p.ratio) * p.on + (head * p.ratio + r % p.ratio) * p.oh;
+#pragma unroll
+      for (int pn = 0; pn < PANELS; ++pn) {
+        uint32_t w[2 * W];
+#pragma unroll
+        for (int i = 0; i < 2 * W; ++i) {
+          const float a = st.acc[n][pn * 2 * W + i][e] * fe, b = st.acc[n][pn * 2 * W + i][2 + e] * fe;
+          if (p.o_bf16) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+            w[i] = *reinterpret_cast<const uint32_t*>(&h);
+          } else {
+            const __half2 h = __floats2half2_rn(a, b);
+            w[i] = *reinterpret_cast<const uint32_t*>(&h);
+          }
+        }
+        uint4* d = reinterpret_cast<uint4*>(o + channel_of<D>(pn * 2 * W, g));
+#pragma unroll
+        for (int i = 0; i < 2 * W; i += 4) d[i / 4] = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+      }
+    }
+  }
+  static_assert(MT == PANELS * 2 * W, "tiles");
+}
+
+// 4 channels of a row, added up part by part
+struct Sum {
+  float m, mw, l;
+  float4 a;
+  __device__ __forceinline__ void clear() {
+    m = mw = -INFINITY;
+    l = 0.f;
+    a = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  __device__ __forceinline__ void add(const float4& ml, const float4& x) {
+    const float m1 = fmaxf(m, ml.x), w1 = fmaxf(mw, ml.y);
+    l = l * ex2_approx(m - safe(m1)) + ml.z * ex2_approx(ml.x - safe(m1));
+    const float f = ex2_approx(mw - safe(w1)), h = ex2_approx(ml.y - safe(w1));
+    a.x = a.x * f + x.x * h; a.y = a.y * f + x.y * h; a.z = a.z * f + x.z * h; a.w = a.w * f + x.w * h;
+    m = m1;
+    mw = w1;
+  }
+};
+// ... and written: row r of a unit's sequence, whose first query row is token t0
+__device__ __forceinline__ void write_sum(const PParams& p, int t0, int r, int head, int ch, const Sum& x) {
+  const float f = row_factor(x.m, x.mw, x.l);
+  const long long n = t0 + r / p.ratio;
+  const int h = head * p.ratio + r % p.ratio;
+  uint2 w;
+  if (p.o_bf16) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(x.a.x * f, x.a.y * f), b = __floats2bfloat162_rn(x.a.z * f, x.a.w * f);
+    w.x = *reinterpret_cast<const uint32_t*>(&a);
+    w.y = *reinterpret_cast<const uint32_t*>(&b);
+  } else {
+    const __half2 a = __floats2half2_rn(x.a.x * f, x.a.y * f), b = __floats2half2_rn(x.a.z * f, x.a.w * f);
+    w.x = *reinterpret_cast<const uint32_t*>(&a);
+    w.y = *reinterpret_cast<const uint32_t*>(&b);
+  }
+  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.o) + n * p.on + h * p.oh + ch) = w;
+  if (p.lse && ch == 0) p.lse[n * p.H + h] = x.m + log2f(x.l);
+}
+
+template <int D, int NT>
+__device__ __forceinline__ void write_part(float* part, float* ml, int stride, const RowState<D, NT>& st) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  constexpr int MT = RowState<D, NT>::MT;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    if (t == 0) *reinterpret_cast<float4*>(ml + (n * 8 + g) * 4) = make_float4(st.m[n], st.mw[n], st.l[n], 0.f);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float* d = part + (n * 8 + 2 * t + e) * stride;
+#pragma unroll
+      for (int i = 0; i < MT; i += 2)
+        *reinterpret_cast<float4*>(d + channel_of<D>(i, g)) = make_float4(st.acc[n][i][e], st.acc[n][i][2 + e], st.acc[n][i + 1][e], st.acc[n][i + 1][2 + e]);
+    }
+  }
+}
+
+// One chunk.  sK, sV: its rows in shared memory; sS: its K scales, then its V scales; last[n]: the last key of the chunk that row n*8 + g sees.
+template <int D, int NT, bool MASKED>
+__device__ __forceinline__ void chunk_step(RowState<D, NT>& st, const uint32_t (&q)[D / 64][NT][4], const float (&qs)[NT], const int (&last)[NT],
+                                           uint32_t sK, uint32_t sV, uint32_t sS) {
+  constexpr int CH = D / 64, AT = (NT + 1) / 2, W = RowState<D, NT>::W, PANELS = RowState<D, NT>::PANELS, PANEL = D < 128 ? D : 128;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  float x[NT][4][2], lv[4][2];
+#pragma unroll
+  for (int kt = 0; kt < 4; ++kt) {
+    int d[AT][4];
+#pragma unroll
+    for (int a = 0; a < AT; ++a) d[a][0] = d[a][1] = d[a][2] = d[a][3] = kMagicI;
+#pragma unroll
+    for (int ch = 0; ch < CH; ++ch) {
+      // row kt*8 + g; piece 2t + (ch & 1) of a 128-byte panel, or t of a 64-byte one
+      const int row = kt * 8 + g;
+      uint32_t a;
+      if constexpr (PANEL == 128) a = sK + (ch / 2) * (kChunk * 128) + row * 128 + (((2 * t + (ch & 1)) ^ g) << 4);
+      else a = sK + row * 64 + ((t ^ ((g >> 1) & 3)) << 4);
+      const uint4 kw = lds16(a);
+#pragma unroll
+      for (int i = 0; i < AT; ++i) {
+        const bool two = 2 * i + 1 < NT;
+        const uint32_t(&lo)[4] = q[ch][2 * i];
+        const uint32_t(&hi)[4] = q[ch][two ? 2 * i + 1 : 2 * i];
+        mma_s8(d[i], lo[0], two ? hi[0] : 0u, lo[1], two ? hi[1] : 0u, kw.x, kw.y);
+        mma_s8(d[i], lo[2], two ? hi[2] : 0u, lo[3], two ? hi[3] : 0u, kw.z, kw.w);
+      }
+    }
+    const float2 ks = lds_f2(sS + (kt * 8 + 2 * t) * 4), vs = lds_f2(sS + (kChunk + kt * 8 + 2 * t) * 4);
+    lv[kt][0] = log2_approx(vs.x);
+    lv[kt][1] = log2_approx(vs.y);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      x[n][kt][0] = (__int_as_float(d[n / 2][(n & 1) * 2]) - kMagicF) * qs[n] * ks.x;
+      x[n][kt][1] = (__int_as_float(d[n / 2][(n & 1) * 2 + 1]) - kMagicF) * qs[n] * ks.y;
+    }
+  }
+  uint32_t b[NT][4];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    float w[4][2], mx = -INFINITY, mw = -INFINITY;
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        w[kt][e] = x[n][kt][e] + lv[kt][e];
+        // (chosen, not added: what lies in a place that is not looked at may be anything)
+        if (MASKED && kt * 8 + 2 * t + e > last[n]) x[n][kt][e] = w[kt][e] = -INFINITY;
+        mx = fmaxf(mx, x[n][kt][e]);
+        mw = fmaxf(mw, w[kt][e]);
+      }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      mw = fmaxf(mw, __shfl_xor_sync(0xffffffffu, mw, o));
+    }
+    mx = fmaxf(mx, st.m[n]);
+    mw = fmaxf(mw, st.mw[n]);
+    const float ms = safe(mx), mws = safe(mw);
+    st.l[n] *= ex2_approx(st.m[n] - ms);
+    const bool moved = mw != st.mw[n];
+    const float f = ex2_approx(st.mw[n] - mws);
+    st.m[n] = mx;
+    st.mw[n] = mw;
+    float sum = 0.f;
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt) {
+      sum += ex2_approx(x[n][kt][0] - ms) + ex2_approx(x[n][kt][1] - ms);
+      const __half2 h = __floats2half2_rn(ex2_approx(w[kt][0] - mws), ex2_approx(w[kt][1] - mws));
+      b[n][kt] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    st.l[n] += sum;
+    if (__any_sync(0xffffffffu, moved)) {
+      const float f0 = __shfl_sync(0xffffffffu, f, 8 * t), f1 = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+#pragma unroll
+      for (int i = 0; i < RowState<D, NT>::MT; ++i) {
+        st.acc[n][i][0] *= f0;
+        st.acc[n][i][1] *= f1;
+        st.acc[n][i][2] *= f0;
+        st.acc[n][i][3] *= f1;
+      }
+    }
+  }
+  // O^T (channels x rows) += V^T P^T, 16 keys at a time: two 8-key tiles, of which the lane holds keys 2t and 2t + 1
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int pn = 0; pn < PANELS; ++pn) {
+      uint32_t v[4][W];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = h * 16 + (i >> 1) * 8 + 2 * t + (i & 1);
+        if constexpr (W == 4) {
+          const uint4 y = lds16(sV + pn * (kChunk * 128) + row * 128 + ((g ^ (row & 7)) << 4));
+          v[i][0] = y.x; v[i][1] = y.y; v[i][2] = y.z; v[i][3] = y.w;
+        } else {
+          const uint2 y = lds8(sV + row * 64 + (((g >> 1) ^ ((row >> 1) & 3)) << 4) + (g & 1) * 8);
+          v[i][0] = y.x; v[i][1] = y.y;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        uint32_t a[4][2];                        // [channel of four][8-key tile]
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t lo = __byte_perm(v[2 * k][j], v[2 * k + 1][j], 0x5140) ^ 0x80808080u;
+          const uint32_t hi = __byte_perm(v[2 * k][j], v[2 * k + 1][j], 0x7362) ^ 0x80808080u;
+          const uint32_t r[4] = {__byte_perm(lo, 0x64646464u, 0x4140), __byte_perm(lo, 0x64646464u, 0x4342),
+                                 __byte_perm(hi, 0x64646464u, 0x4140), __byte_perm(hi, 0x64646464u, 0x4342)};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&r[i]), __half2half2(__ushort_as_half(0x6480)));
+            a[i][k] = *reinterpret_cast<const uint32_t*>(&y);
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          mma_f16(st.acc[n][(pn * W + j) * 2], a[0][0], a[1][0], a[0][1], a[1][1], b[n][2 * h], b[n][2 * h + 1]);
+          mma_f16(st.acc[n][(pn * W + j) * 2 + 1], a[2][0], a[3][0], a[2][1], a[3][1], b[n][2 * h], b[n][2 * h + 1]);
+        }
+      }
+    }
+  }
+}
+
+enum { kWaitChunk = 64 };
+
+template <int D, int NT, int WARPS, int NS>
+__global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const PParams p) {
+  using C = DecodeCfg<D, NT, WARPS, NS>;
+  constexpr int RT = C::RT, THREADS = 32 * WARPS;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((0u - smem_u32(smem_raw)) & 1023u);
+  const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const uint32_t bar0 = smem_u32(smem + C::OFF_BAR) + warp * NS * 8;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC);
+  long long* pre_c = reinterpret_cast<long long*>(smem + C::OFF_PRE);
+  int* pre_u = reinterpret_cast<int*>(pre_c + THREADS + 1);
+  int* whole = reinterpret_cast<int*>(smem + C::OFF_MISC + 8);           // of the unit that all warps' shares lie in
+  if (lane == 0)
+    for (int i = 0; i < NS; ++i) mbar_init(bar0 + 8 * i, 1);
+  if (threadIdx.x == 0) {
+    abort_flag[0] = 0;
+    abort_flag[1] = (int)(1u << 31);              // (2^31 cycles, about a second)
+    prefetch_tmap(&tmK);
+    prefetch_tmap(&tmV);
+  }
+  mbar_init_fence();
+  pdl_wait();
+  pdl_launch();
+  // ---- the row of all chunks: thread i counts the sequences i*seg .. (i+1)*seg - 1
+  const int seg = (p.S + THREADS - 1) / THREADS;
+  {
+    long long c = 0, u = 0;
+    bool bad = false;
+    for (int s = threadIdx.x * seg; s < (threadIdx.x + 1) * seg && s < p.S; ++s) {
+      const Seq q = seq_of(p, s);
+      const long long units = (long long)q.tiles * p.Hkv;
+      c += units * q.chunks;
+      u += units;
+      bad |= q.n > 0 && q.len > q.keys;
+    }
+    if (p.cu && threadIdx.x == 0) bad |= p.cu[p.S] > p.T;
+    if (bad && p.status && blockIdx.x == 0) atomicCAS(p.status, 0, kStatusBadIndex);
+    pre_c[threadIdx.x + 1] = c;
+    pre_u[threadIdx.x + 1] = (int)(u < p.max_units ? u : p.max_units);       // (more of them only where cu_seqlens overlap)
+    if (threadIdx.x == 0) {
+      pre_c[0] = 0;
+      pre_u[0] = 0;
+    }
+  }
+  __syncthreads();
+  if (warp == 0) {
+    long long c0 = 0, u0 = 0;
+    for (int w = 0; w < WARPS; ++w) {
+      long long c = pre_c[w * 32 + lane + 1], u = pre_u[w * 32 + lane + 1];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, c, o), y = __shfl_up_sync(0xffffffffu, u, o);
+        if (lane >= o) {
+          c += x;
+          u += y;
+        }
+      }
+      pre_c[w * 32 + lane + 1] = c + c0;
+      pre_u[w * 32 + lane + 1] = (int)(u + u0 < p.max_units ? u + u0 : p.max_units);
+      c0 += __shfl_sync(0xffffffffu, c, 31);
+      u0 += __shfl_sync(0xffffffffu, u, 31);
+    }
+  }
+  __syncthreads();
+  const long long total = pre_c[THREADS];
+  long long share = (total + p.workers - 1) / p.workers;
+  if (share < p.least) share = p.least;
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    p.head[0] = pre_u[THREADS];
+    p.head[1] = share;
+    p.head[2] = total;
+  }
+  const int worker = blockIdx.x * WARPS + warp;
+  const long long begin = worker * share;
+  const long long left0 = total - begin < share ? total - begin : share;
+  long long left = left0 < 0 ? 0 : left0;                    // chunks to do
+  Cursor at;
+  long long unit_id = 0;                                     // of all units
+  if (left > 0) {
+    const int i = find_last(THREADS, begin, [&](int j) { return pre_c[j]; });
+    long long off = begin - pre_c[i];
+    unit_id = pre_u[i];
+    at.s = i * seg - 1;
+    do {
+      at.next_seq(p);
+      const long long units = (long long)at.q.tiles * p.Hkv, c = units * at.q.chunks;
+      if (off < c) break;
+      off -= c;
+      unit_id += units;
+    } while (at.s < p.S);
+    at.unit = (int)(off / at.q.chunks);
+    at.chunk = (int)(off - (long long)at.unit * at.q.chunks);
+    unit_id += at.unit;
+  }
+  // ---- loads
+  const uint32_t sKV = smem_u32(smem) + warp * NS * 2 * C::KV;
+  const uint32_t sX = smem_u32(smem + C::OFF_EXTRA) + warp * NS * C::EXTRA;
+  Cursor ahead = at;
+  long long to_load = left;
+  bool fresh = true;                                         // the next chunk to load needs its query rows, too
+  int page = 0;                                              // of key `lane` of the next chunk to load
+  auto look_up = [&]() {
+    const int key = ahead.chunk * kChunk + lane;
+    page = 0;
+    if (to_load > 0 && key < ahead.q.keys) page = p.table[ahead.s * p.table_stride + (key >> p.page_log)];
+  };
+  const int rows_box = 1 << p.box_log, boxes = kChunk >> p.box_log;
+  auto load = [&](int stage) {
+    if (to_load > 0) {
+      const int key0 = ahead.chunk * kChunk, key = key0 + lane, head = ahead.unit / ahead.q.tiles, tile = ahead.unit - head * ahead.q.tiles;
+      const bool in = key < ahead.q.keys;
+      if (page < 0 || page >= p.pages) {
+        if (p.status) atomicCAS(p.status, 0, kStatusBadIndex);
+        page = 0;
+      }
+      const uint32_t bar = bar0 + 8 * stage, dst = sKV + stage * 2 * C::KV, x = sX + stage * C::EXTRA;
+      // the rows of a copy lie in one page; lane j issues copy j
+      const int first_page = __shfl_sync(0xffffffffu, page, (lane << p.box_log) & 31);
+      const int full = min(boxes, (ahead.q.keys - key0 + rows_box - 1) >> p.box_log);
+      if (lane == 0) mbar_expect_tx(bar, full > 0 ? full * rows_box * 2 * D : 0);
+      __syncwarp();
+      if (lane < full) {
+        const int slot = (key0 + (lane << p.box_log)) & ((1 << p.page_log) - 1);
+#pragma unroll
+        for (int pn = 0; pn < C::PANELS; ++pn) {
+          const uint32_t d = dst + pn * (kChunk * C::PANEL) + (lane << p.box_log) * C::PANEL;
+          tma_load_4d(d, &tmK, bar, pn * C::PANEL, slot, head, first_page);
+          tma_load_4d(d + C::KV, &tmV, bar, pn * C::PANEL, slot, head, first_page);
+        }
+      }
+      const long long blk = (key & ((1 << p.page_log) - 1)) >> p.block_log;
+      cp_async4(x + lane * 4, p.ks + (in ? page * p.ksP + head * p.ksH + blk * p.ksB : 0), in);
+      cp_async4(x + (kChunk + lane) * 4, p.vs + (in ? page * p.vsP + head * p.vsH + blk * p.vsB : 0), in);
+      if (fresh) {
+        const uint32_t xq = x + 2 * kChunk * 4;
+        const int R = ahead.q.n * p.ratio;
+#pragma unroll
+        for (int i = lane; i < RT * (D / 16); i += 32) {
+          const int r = tile * RT + i / (D / 16);
+          const bool ok = r < R;
+          const int n = ok ? r / p.ratio : 0, h = head * p.ratio + (ok ? r - n * p.ratio : 0);
+          cp_async16(xq + i * 16, p.q + (ahead.q.t0 + n) * p.qn + h * p.qh + i % (D / 16) * 16, ok);
+        }
+        if (lane < RT) {
+          const int r = tile * RT + lane;
+          const bool ok = r < R;
+          const int n = ok ? r / p.ratio : 0, h = head * p.ratio + (ok ? r - n * p.ratio : 0);
+          cp_async4(xq + RT * D + lane * 4, p.qs + (ahead.q.t0 + n) * p.qsn + h * p.qsh, ok);
+        }
+      }
+      --to_load;
+      const int unit = ahead.unit, s = ahead.s;
+      ahead.next(p);
+      fresh = ahead.unit != unit || ahead.s != s;
+      look_up();
+    }
+    cp_async_commit();
+  };
+  look_up();
+#pragma unroll 1
+  for (int i = 0; i < NS; ++i) load(i);
+
+  // Where the shares of all warps of the CTA lie in one unit, their parts are added up here before they go to scratch.
+  const long long cta0 = (long long)blockIdx.x * WARPS * share, cta1 = cta0 + WARPS * share < total ? cta0 + WARPS * share : total;
+  bool merge = false;
+  RowState<D, NT> st;
+  st.clear();
+  uint32_t q[D / 64][NT][4];
+  float qs[NT];
+  int last[NT], full_keys = 0;
+  int stage = 0, parity = 0;
+  bool open = false, ok = true;
+  long long unit0 = 0, unit1 = 0;                            // the unit's chunks among all
+  long long pos = begin;
+#pragma unroll 1
+  while (left > 0) {
+    cp_async_wait<NS - 1>();
+    __syncwarp();
+    ok = mbar_wait_warp(bar0 + 8 * stage, parity, abort_flag, p.status, (int)(blockIdx.x << 8) | kWaitChunk);
+    if (!ok) break;
+    const uint32_t kv = sKV + stage * 2 * C::KV, x = sX + stage * C::EXTRA;
+    if (!open) {
+      open = true;
+      unit0 = pos - at.chunk;
+      unit1 = unit0 + at.q.chunks;
+      st.clear();
+      const int tile = at.unit % at.q.tiles, R = at.q.n * p.ratio;
+      const uint32_t xq = x + 2 * kChunk * 4;
+      full_keys = at.q.keys;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int ch = 0; ch < D / 64; ++ch) {
+          // (the pieces of K's rows that chunk_step() takes)
+          const int piece = C::PANEL == 128 ? (ch / 2) * 8 + 2 * t + (ch & 1) : t;
+          const uint4 w = lds16(xq + (n * 8 + g) * D + piece * 16);
+          q[ch][n][0] = w.x; q[ch][n][1] = w.y; q[ch][n][2] = w.z; q[ch][n][3] = w.w;
+        }
+        qs[n] = lds_f(xq + RT * D + (n * 8 + g) * 4) * p.c;
+        const int r = tile * RT + n * 8 + g;
+        last[n] = at.q.keys - 1;
+        if (p.causal && r < R) {
+          const long long lim = at.q.len - at.q.n + r / p.ratio;
+          if (lim < last[n]) last[n] = lim < 0 ? -1 : (int)lim;
+        }
+        full_keys = min(full_keys, last[n] + 1);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) full_keys = min(full_keys, __shfl_xor_sync(0xffffffffu, full_keys, o));
+    }
+    const int key0 = at.chunk * kChunk;
+    if (key0 + kChunk <= full_keys) {
+      chunk_step<D, NT, false>(st, q, qs, last, kv, kv + C::KV, x);
+    } else {
+      int rel[NT];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) rel[n] = last[n] - key0;
+      chunk_step<D, NT, true>(st, q, qs, rel, kv, kv + C::KV, x);
+    }
+    __syncwarp();
+    load(stage);
+    if (++stage == NS) {
+      stage = 0;
+      parity ^= 1;
+    }
+    --left;
+    ++pos;
+    if (at.chunk + 1 == at.q.chunks || left == 0) {
+      st.reduce_l();
+      const int head = at.unit / at.q.tiles, tile = at.unit - head * at.q.tiles;
+      const bool starts = unit0 >= begin, ends = unit1 <= pos;
+      if (unit_id >= p.max_units) {
+        if (p.status && lane == 0) atomicCAS(p.status, 0, kStatusBadIndex);            // (cu_seqlens that overlap)
+      } else if (starts && lane == 0) {
+        UnitPart u;
+        u.chunk0 = unit0;
+        u.chunk1 = unit1;
+        u.s = at.s;
+        u.unit = at.unit;
+        u.open = !(ends || (cta0 == unit0 && cta1 == unit1));
+        u.pad = 0;
+        p.units[unit_id] = u;
+      }
+      if (starts && ends) {
+        write_rows(p, at.q, head, tile, st);
+      } else if (cta0 >= unit0 && cta1 <= unit1) {
+        merge = true;
+        if (lane == 0) {
+          whole[0] = cta0 == unit0 && cta1 == unit1;
+          whole[1] = cta0 == unit0;
+          whole[2] = at.q.t0;
+          whole[3] = at.q.n * p.ratio - tile * RT;
+          whole[4] = head;
+          whole[5] = tile;
+        }
+      } else {
+        const long long slot = 2LL * worker + (starts ? 1 : 0);
+        write_part<D, NT>(p.part + slot * RT * D, p.part_ml + slot * RT * 4, D, st);
+      }
+      open = false;
+      ++unit_id;
+    }
+    at.next(p);
+  }
+  if (!__syncthreads_or(merge)) return;
+  // (every warp is done with its ring: what it asked for has come)
+  float* red = reinterpret_cast<float*>(smem);
+  float* red_ml = red + WARPS * RT * (D + 4);
+  write_part<D, NT>(red + warp * RT * (D + 4), red_ml + warp * RT * 4, D + 4, st);
+  __syncthreads();
+  const long long slot = 2LL * blockIdx.x * WARPS + whole[1];
+  for (int i = threadIdx.x; i < RT * (D / 4); i += THREADS) {
+    const int r = i / (D / 4), ch = i % (D / 4) * 4;
+    Sum x;
+    x.clear();
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w)
+      x.add(*reinterpret_cast<const float4*>(red_ml + (w * RT + r) * 4), *reinterpret_cast<const float4*>(red + (w * RT + r) * (D + 4) + ch));
+    if (!whole[0]) {
+      *reinterpret_cast<float4*>(p.part + (slot * RT + r) * D + ch) = x.a;
+      if (ch == 0) *reinterpret_cast<float4*>(p.part_ml + (slot * RT + r) * 4) = make_float4(x.m, x.mw, x.l, 0.f);
+    } else if (r < whole[3]) {
+      write_sum(p, whole[2], whole[5] * RT + r, whole[4], ch, x);
+    }
+  }
+}
+
+// Sum of the parts of the units that lie in several warps' shares.  GROUPS groups of D/4 threads a row take the parts in turn; the groups'
+// sums are added in order, so a call repeats itself bit for bit.  A chain of L2 latencies: with few units, and so many parts each, one
+// row a CTA and all groups on it; else one unit a CTA.
+template <int D, int GROUPS>
+__global__ void __launch_bounds__(GROUPS * (D / 4)) combine_kernel(const PParams p, int cta_warps, int rows_cta) {
+  constexpr int C4 = D / 4;
+  __shared__ float4 red[GROUPS][C4 + 1];
+  __shared__ float4 red_ml[GROUPS];
+  const int per_unit = p.rows_tile / rows_cta;
+  const long long u = blockIdx.x / per_unit;
+  const int grp = threadIdx.x / C4, ch = threadIdx.x % C4 * 4;
+  pdl_wait();
+  pdl_launch();
+  if (u >= p.head[0]) return;
+  const UnitPart up = p.units[u];
+  if (!up.open) return;
+  const long long share = p.head[1], total = p.head[2], cs = share * cta_warps;
+  const Seq q = seq_of(p, up.s);
+  const int head = up.unit / q.tiles, tile = up.unit - head * q.tiles, R = q.n * p.ratio;
+  const long long a = up.chunk0 / share, b = (up.chunk1 - 1) / share;
+  // CTAs ka .. kb lie in the unit as a whole and have left one part each, in their first warp's slot
+  const long long ka = (up.chunk0 + cs - 1) / cs, kb = up.chunk1 == total ? (total - 1) / cs : up.chunk1 / cs - 1;
+  const long long n0 = ka <= kb ? ka * cta_warps - a : b - a + 1, n1 = ka <= kb ? kb - ka + 1 : 0;
+  const long long n2 = ka <= kb && b >= (kb + 1) * cta_warps ? b - (kb + 1) * cta_warps + 1 : 0;
+  const int parts = (int)(n0 + n1 + n2);
+  auto slot_of = [&](int i) {
+    const long long w = i < n0 ? a + i : i < n0 + n1 ? (ka + (i - n0)) * cta_warps : (kb + 1) * cta_warps + (i - n0 - n1);
+    return 2 * w + (w == a ? 1 : 0);
+  };
+  const int first_row = (int)(blockIdx.x % per_unit) * rows_cta;
+  const int row_step = rows_cta == 1 ? 1 : GROUPS, part_step = rows_cta == 1 ? GROUPS : 1;
+  for (int r = first_row + (rows_cta == 1 ? 0 : grp); r < first_row + rows_cta; r += row_step) {
+    if (tile * p.rows_tile + r >= R) continue;
+    Sum x;
+    x.clear();
+#pragma unroll 4
+    for (int i = rows_cta == 1 ? grp : 0; i < parts; i += part_step) {
+      const long long s = slot_of(i) * p.rows_tile + r;
+      x.add(*reinterpret_cast<const float4*>(p.part_ml + s * 4), *reinterpret_cast<const float4*>(p.part + s * D + ch));
+    }
+    if (rows_cta == 1) {
+      red[grp][ch / 4] = x.a;
+      if (ch == 0) red_ml[grp] = make_float4(x.m, x.mw, x.l, 0.f);
+      __syncthreads();
+      if (grp > 0) return;
+      for (int i = 1; i < GROUPS; ++i) x.add(red_ml[i], red[i][ch / 4]);
+    }
+    write_sum(p, q.t0, tile * p.rows_tile + r, head, ch, x);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------------------------------------------
+struct Plan {
+  int NT = 1, ctas = 0, warps = 8;
+  long long max_units = 0;
+  size_t off_ml = 0, off_units = 0, off_head = 0, bytes = 0;
+};
+Plan make_plan(const IntfaPagedParams* a, int sms) {
+  Plan pl;
+  const IntfaPagedCache& c = a->cache;
+  const int ratio = a->H / c.H_kv;
+  // Rows a tile: 16 where an average sequence has more than 8 rows a K/V head
+  pl.NT = (double)a->tokens * ratio > 8.0 * c.S ? 2 : 1;
+  pl.warps = c.D == 256 ? 4 : c.D == 128 && pl.NT == 2 ? 6 : 8;
+  pl.ctas = sms;
+  pl.max_units = (a->tokens * ratio / (8 * pl.NT) + c.S) * c.H_kv;
+  if (pl.max_units > 0x7fffffffLL) return Plan();
+  const int RT = 8 * pl.NT;
+  const long long slots = 2LL * pl.ctas * pl.warps;
+  auto take = [&](size_t bytes) {
+    const size_t r = pl.bytes;
+    pl.bytes += (bytes + 255) / 256 * 256;
+    return r;
+  };
+  take((size_t)slots * RT * c.D * 4);
+  pl.off_ml = take((size_t)slots * RT * 16);
+  pl.off_units = take((size_t)pl.max_units * sizeof(UnitPart));
+  pl.off_head = take(32);
+  return pl;
+}
+
+template <int D, int NT, int WARPS, int NS>
+int run(const IntfaPagedParams* a, const Plan& pl, PParams p, cudaStream_t stream) {
+  using C = DecodeCfg<D, NT, WARPS, NS>;
+  const IntfaPagedCache& c = a->cache;
+  CUtensorMap tmK, tmV;
+  const CUtensorMapSwizzle swz = C::PANEL == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+  int rc;
+  if ((rc = make_tmap(&tmK, c.k, 1, c.k_stride, c.pages, c.H_kv, c.page_size, D, C::PANEL, 1 << p.box_log, swz))) return rc;
+  if ((rc = make_tmap(&tmV, c.v, 1, c.v_stride, c.pages, c.H_kv, c.page_size, D, C::PANEL, 1 << p.box_log, swz))) return rc;
+  auto kern = paged_kernel<D, NT, WARPS, NS>;
+  static std::atomic<bool> attr_done[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return set_error(INTFA_ERR_CUDA, "cannot query the current device");
+  if (!attr_done[dev].load(std::memory_order_acquire)) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (e != cudaSuccess) return set_error(INTFA_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    attr_done[dev].store(true, std::memory_order_release);
+  }
+  if ((rc = launch_kernel("paged attention", kern, pl.ctas, 32 * WARPS, C::SMEM, stream, tmK, tmV, p))) return rc;
+  constexpr int GROUPS = 1024 / D;
+  const int rows_cta = pl.max_units * p.rows_tile <= 16LL * pl.ctas ? 1 : p.rows_tile;
+  const long long grid = pl.max_units * (p.rows_tile / rows_cta);
+  if (grid > 0x7fffffffLL) return set_error(INTFA_ERR_TOO_LARGE, "too many query rows");
+  return launch_kernel("paged combine", combine_kernel<D, GROUPS>, (unsigned)grid, GROUPS * (D / 4), 0, stream, p, WARPS, rows_cta);
+}
+
+int log2_of(long long n) {
+  int i = 0;
+  while ((1LL << i) < n) ++i;
+  return i;
+}
+
+}  // namespace
+
+size_t paged_workspace_bytes(const IntfaPagedParams* a) {
+  const int sms = sm_count_cached();
+  return make_plan(a, sms > 0 ? sms : 148).bytes;
+}
+
+int paged_attention(const IntfaPagedParams* a, cudaStream_t stream) {
+  const int sms = sm_count_cached();
+  if (sms <= 0) return set_error(INTFA_ERR_CUDA, "cannot query SM count");
+  const Plan pl = make_plan(a, sms);
+  if (pl.bytes == 0) return set_error(INTFA_ERR_TOO_LARGE, "too many query rows or sequences");
+  if (!a->workspace || a->workspace_bytes < pl.bytes) return set_error(INTFA_ERR_INVALID_ARG, "workspace missing or smaller than intfa_paged_workspace_bytes()");
+  const IntfaPagedCache& c = a->cache;
+  PParams p;
+  p.q = static_cast<const int8_t*>(a->q);
+  p.qs = a->q_scale;
+  p.o = a->o;
+  p.lse = a->lse_out;
+  p.qn = a->q_stride[0]; p.qh = a->q_stride[1];
+  p.qsn = a->qs_stride[0]; p.qsh = a->qs_stride[1];
+  p.on = a->o_stride[0]; p.oh = a->o_stride[1];
+  p.ks = c.k_scale; p.vs = c.v_scale;
+  p.ksP = c.ks_stride[0]; p.ksH = c.ks_stride[1]; p.ksB = c.ks_stride[2];
+  p.vsP = c.vs_stride[0]; p.vsH = c.vs_stride[1]; p.vsB = c.vs_stride[2];
+  p.table = c.block_table;
+  p.table_stride = c.table_stride;
+  p.width = c.table_width;
+  p.lens = c.seq_lens;
+  p.cu = a->cu_seqlens;
+  p.S = c.S; p.H = a->H; p.Hkv = c.H_kv; p.ratio = a->H / c.H_kv; p.pages = c.pages;
+  p.page_log = log2_of(c.page_size);
+  p.block_log = log2_of(c.block);
+  p.box_log = c.page_size < kChunk ? p.page_log : log2_of(kChunk);
+  p.T = a->tokens;
+  p.causal = a->causal ? 1 : 0;
+  p.o_bf16 = a->o_dtype == INTFA_OUT_BF16;
+  p.c = a->sm_scale * 1.44269504f;
+  p.workers = pl.ctas * pl.warps;
+  p.least = 1;
+  p.rows_tile = 8 * pl.NT;
+  char* ws = static_cast<char*>(a->workspace);
+  p.part = reinterpret_cast<float*>(ws);
+  p.part_ml = reinterpret_cast<float*>(ws + pl.off_ml);
+  p.units = reinterpret_cast<UnitPart*>(ws + pl.off_units);
+  p.max_units = pl.max_units;
+  p.head = reinterpret_cast<long long*>(ws + pl.off_head);
+  p.status = a->status;
+  switch (c.D) {
+    case 64: return pl.NT == 2 ? run<64, 2, 8, 4>(a, pl, p, stream) : run<64, 1, 8, 5>(a, pl, p, stream);
+    case 128: return pl.NT == 2 ? run<128, 2, 6, 3>(a, pl, p, stream) : run<128, 1, 8, 3>(a, pl, p, stream);
+    default: return pl.NT == 2 ? run<256, 2, 4, 2>(a, pl, p, stream) : run<256, 1, 4, 3>(a, pl, p, stream);
+  }
+}
+
+}  // namespace intfa

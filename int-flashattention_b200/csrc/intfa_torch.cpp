@@ -594,6 +594,355 @@ PyObject* flash(PyObject*, PyObject* const* a, Py_ssize_t n, PyObject* kwnames) 
   END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------------------------------------------------------
+// rotary positions, paged cache
+// (shapes and types are looked at before the device, so that a wrong call is told what is wrong with it anywhere)
+// ---------------------------------------------------------------------------------------------------------------
+std::string shape_of(const at::Tensor& t) {
+  std::string s = "[";
+  for (int64_t i = 0; i < t.dim(); ++i) s += (i ? "," : "") + std::to_string(t.size(i));
+  return s + "]";
+}
+[[noreturn]] void bad_shape(const char* what, const char* want, const at::Tensor& t) {
+  raise(PyExc_ValueError, std::string(what) + " must have shape " + want + ", got " + shape_of(t));
+}
+void same_device(std::initializer_list<const at::Tensor*> ts) {
+  const at::Tensor* first = nullptr;
+  for (const at::Tensor* t : ts) {
+    if (!t || !t->defined()) continue;
+    need_cuda(*t);
+    if (first && t->device() != first->device()) raise(PyExc_ValueError, "all tensors must be on one device");
+    if (!first) first = t;
+  }
+}
+void need_int32(const at::Tensor& t, const char* what) {
+  if (!is(t, at::kInt)) raise(PyExc_TypeError, std::string(what) + " must be int32");
+}
+int dtype_of(const at::Tensor& t, const char* what, bool fp32) {
+  if (is(t, at::kHalf)) return INTFA_TYPE_FP16;
+  if (is(t, at::kBFloat16)) return INTFA_TYPE_BF16;
+  if (fp32 && is(t, at::kFloat)) return INTFA_TYPE_FP32;
+  raise(PyExc_TypeError, std::string(what) + (fp32 ? " must be float16, bfloat16 or float32" : " must be float16 or bfloat16"));
+}
+// rows that 16-byte loads can take
+at::Tensor rows_ready(const at::Tensor& t) {
+  bool ok = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int64_t i = 0; ok && i + 1 < t.dim(); ++i) ok = t.stride(i) >= 0 && t.stride(i) * t.element_size() % 16 == 0;
+  return ok ? t : t.is_contiguous() ? t.clone() : t.contiguous();
+}
+at::Tensor rotary_table(const at::Tensor& t, int64_t D) {
+  if (!is(t, at::kFloat)) raise(PyExc_TypeError, "table must be float32");
+  if (t.dim() != 3 || t.size(2) != 2 || t.size(0) < 1) bad_shape("table", "[n, rot_dim/2, 2] with n > 0", t);
+  if (t.size(1) < 1 || 2 * t.size(1) > D) raise(PyExc_ValueError, "the table is for " + std::to_string(2 * t.size(1)) + " channels, the head has " + std::to_string(D));
+  return t;
+}
+at::Tensor aligned16(const at::Tensor& t) {
+  const at::Tensor c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
+}
+
+// rotary(q, k | None, table, positions, interleaved, inverse)
+PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  try {
+    if (n != 6) raise(PyExc_TypeError, "rotary takes 6 arguments");
+    const at::Tensor& q0 = tensor(a[0], "q");
+    const at::Tensor k0 = a[1] == Py_None ? at::Tensor() : tensor(a[1], "k");
+    const at::Tensor &t0 = tensor(a[2], "table"), &p0 = tensor(a[3], "positions");
+    IntfaRotaryParams P{};
+    P.dtype = dtype_of(q0, "q", true);
+    if (q0.dim() != 3 && q0.dim() != 4) bad_shape("q", "[B,H,N,D] or [tokens,heads,D]", q0);
+    const bool packed = q0.dim() == 3;
+    const int64_t B = packed ? 1 : q0.size(0), N = packed ? q0.size(0) : q0.size(2), H = q0.size(1), D = q0.size(-1);
+    if (D != 16 && D != 32 && D != 64 && D != 128 && D != 256) raise(PyExc_ValueError, "head dim must be one of 16, 32, 64, 128, 256, got " + std::to_string(D));
+    if (k0.defined()) {
+      if (k0.scalar_type() != q0.scalar_type()) raise(PyExc_TypeError, "k must have the type of q");
+      if (k0.dim() != q0.dim() || k0.size(0) != q0.size(0) || k0.size(-1) != D || (!packed && k0.size(2) != N))
+        raise(PyExc_ValueError, "k must have the shape of q but for its heads, got " + shape_of(k0) + " with q " + shape_of(q0));
+    }
+    rotary_table(t0, D);
+    if (!is(p0, at::kInt) && !is(p0, at::kLong)) raise(PyExc_TypeError, "positions must be int32 or int64");
+    const bool per_batch = p0.dim() == 2 && !packed;
+    if (!(p0.dim() == 1 && p0.size(0) == N) && !(per_batch && p0.size(0) == B && p0.size(1) == N))
+      bad_shape("positions", packed ? "[tokens]" : "[N] or [B,N]", p0);
+    same_device({&q0, &k0, &t0, &p0});
+    const c10::Device dev = q0.device();
+    c10::cuda::CUDAGuard guard(dev);
+    at::Tensor qo = empty(q0.sizes(), q0.scalar_type(), dev), ko;
+    if (k0.defined()) ko = empty(k0.sizes(), k0.scalar_type(), dev);
+    const bool none = q0.numel() == 0, no_k = !k0.defined() || k0.numel() == 0;
+    if (B * N > 0x7fffffffLL) raise(PyExc_ValueError, "too many tokens");
+    if (!none || !no_k) {
+      if (none) raise(PyExc_ValueError, "q has no rows, k has some");
+      const at::Tensor q = rows_ready(q0), k = no_k ? at::Tensor() : rows_ready(k0), table = aligned16(t0), pos = p0.contiguous();
+      auto strides = [&](int64_t (&d)[3], const at::Tensor& t) {
+        d[0] = packed ? 0 : t.stride(0);
+        d[1] = t.stride(1);
+        d[2] = packed ? t.stride(0) : t.stride(2);
+      };
+      P.q = q.data_ptr();
+      P.q_out = qo.data_ptr();
+      strides(P.q_stride, q);
+      strides(P.q_out_stride, qo);
+      if (!no_k) {
+        P.k = k.data_ptr();
+        P.k_out = ko.data_ptr();
+        strides(P.k_stride, k);
+        strides(P.k_out_stride, ko);
+        P.H_kv = k.size(1);
+      }
+      P.B = B;
+      P.H = H;
+      P.N = N;
+      P.D = D;
+      P.table = table.data_ptr<float>();
+      P.table_rows = table.size(0);
+      P.rot_dim = 2 * table.size(1);
+      P.positions = pos.data_ptr();
+      P.positions_i64 = is(pos, at::kLong);
+      P.positions_stride = per_batch ? N : 0;
+      P.interleaved = truth(a[4]);
+      P.inverse = truth(a[5]);
+      const at::Tensor st = status_word(dev);
+      P.status = st.data_ptr<int>();
+      void* stream = stream_of(dev);
+      int rc;
+      Py_BEGIN_ALLOW_THREADS
+      rc = intfa_rotary(&P, stream);
+      Py_END_ALLOW_THREADS
+      check(rc);
+    }
+    if (!k0.defined()) return THPVariable_Wrap(qo);
+    return tuple_of({qo, ko});
+  } catch (const PySet&) {
+    return nullptr;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
+// The cache's part of a call, checked; holds what has to live until the launch.
+struct CacheArgs {
+  at::Tensor k, v, ks, vs, table, lens, cu;
+};
+CacheArgs cache_in(IntfaPagedCache& C, const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks, const at::Tensor& vs, const at::Tensor& table,
+                   const at::Tensor& lens, PyObject* cu, int64_t tokens) {
+  CacheArgs x;
+  if (!is(k, at::kChar) || !is(v, at::kChar)) raise(PyExc_TypeError, "k_cache and v_cache must be int8");
+  if (k.dim() != 4) bad_shape("k_cache", "[pages, heads, page_size, D]", k);
+  if (v.sizes() != k.sizes()) raise(PyExc_ValueError, "v_cache must have the shape of k_cache " + shape_of(k) + ", got " + shape_of(v));
+  const int64_t P = k.size(0), H = k.size(1), page = k.size(2), D = k.size(3);
+  if (D != 64 && D != 128 && D != 256) raise(PyExc_ValueError, "the head dim of a paged cache must be 64, 128 or 256, got " + std::to_string(D));
+  auto pow2 = [](int64_t n) { return n > 0 && (n & (n - 1)) == 0; };
+  if (!pow2(page) || page < 8 || page > 256) raise(PyExc_ValueError, "page_size must be a power of two from 8 to 256, got " + std::to_string(page));
+  if (P < 1 || H < 1) raise(PyExc_ValueError, "the cache has no pages or no heads");
+  if (P > 0x7fffffffLL || H > 65535) raise(PyExc_ValueError, "the cache has too many pages or heads");
+  for (const at::Tensor* s : {&ks, &vs}) {
+    const char* what = s == &ks ? "k_scale" : "v_scale";
+    if (!is(*s, at::kFloat)) raise(PyExc_TypeError, std::string(what) + " must be float32");
+    if (s->dim() != 3 || s->size(0) != P || s->size(1) != H || !pow2(s->size(2)) || s->size(2) > page) bad_shape(what, "[pages, heads, page_size/block]", *s);
+  }
+  if (vs.size(2) != ks.size(2)) raise(PyExc_ValueError, "k_scale and v_scale must have the same block of tokens");
+  need_int32(table, "block_table");
+  need_int32(lens, "seq_lens");
+  if (table.dim() != 2) bad_shape("block_table", "[sequences, pages of the longest]", table);
+  const int64_t S = table.size(0);
+  if (lens.dim() != 1 || lens.size(0) != S) bad_shape("seq_lens", "[sequences]", lens);
+  if (S > 0x7fffffffLL || table.size(1) > 0x7fffffffLL) raise(PyExc_ValueError, "block_table is too large");
+  if (cu != Py_None) {
+    const at::Tensor& c = tensor(cu, "cu_seqlens");
+    need_int32(c, "cu_seqlens");
+    if (c.dim() != 1 || c.size(0) != S + 1) bad_shape("cu_seqlens", "[sequences + 1]", c);
+    x.cu = c;
+  } else if (tokens != S) {
+    raise(PyExc_ValueError, "without cu_seqlens there is one token a sequence: got " + std::to_string(tokens) + " tokens, " + std::to_string(S) + " sequences");
+  }
+  for (const at::Tensor* c : {&k, &v}) {
+    bool ok = c->stride(3) == 1 && reinterpret_cast<uintptr_t>(c->data_ptr()) % 16 == 0;
+    for (int i = 0; i < 3; ++i) ok = ok && (c->stride(i) > 0 || c->size(i) == 1) && c->stride(i) % 16 == 0;
+    if (!ok) raise(PyExc_ValueError, "k_cache and v_cache must have a contiguous last dim and lie, with every stride, on 16-byte boundaries");
+  }
+  x.k = k;
+  x.v = v;
+  x.ks = ks;
+  x.vs = vs;
+  x.table = table.stride(1) == 1 && table.stride(0) >= 0 ? table : table.contiguous();
+  x.lens = lens.contiguous();
+  if (x.cu.defined()) x.cu = x.cu.contiguous();
+  C.k = k.data_ptr();
+  C.v = v.data_ptr();
+  C.k_scale = ks.data_ptr<float>();
+  C.v_scale = vs.data_ptr<float>();
+  for (int i = 0; i < 3; ++i) {
+    C.k_stride[i] = k.size(i) == 1 && k.stride(i) <= 0 ? D : k.stride(i);
+    C.v_stride[i] = v.size(i) == 1 && v.stride(i) <= 0 ? D : v.stride(i);
+    C.ks_stride[i] = ks.stride(i);
+    C.vs_stride[i] = vs.stride(i);
+  }
+  C.block_table = x.table.data_ptr<int>();
+  C.table_stride = x.table.stride(0);
+  C.table_width = x.table.size(1);
+  C.seq_lens = x.lens.data_ptr<int>();
+  C.S = S;
+  C.pages = P;
+  C.H_kv = H;
+  C.D = D;
+  C.page_size = page;
+  C.block = page / ks.size(2);
+  return x;
+}
+
+// append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_seqlens | None, q | None, table | None, interleaved)
+PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  try {
+    if (n != 12) raise(PyExc_TypeError, "append takes 12 arguments");
+    const at::Tensor &k0 = tensor(a[0], "k"), &v0 = tensor(a[1], "v");
+    const at::Tensor q0 = a[9] == Py_None ? at::Tensor() : tensor(a[9], "q"), t0 = a[10] == Py_None ? at::Tensor() : tensor(a[10], "table");
+    const at::Tensor &kc = tensor(a[2], "k_cache"), &vc = tensor(a[3], "v_cache"), &ks = tensor(a[4], "k_scale"), &vs = tensor(a[5], "v_scale");
+    const at::Tensor &bt = tensor(a[6], "block_table"), &sl = tensor(a[7], "seq_lens");
+    IntfaAppendParams P{};
+    P.dtype = dtype_of(k0, "k", false);
+    if (k0.dim() != 3) bad_shape("k", "[tokens, heads, D]", k0);
+    if (v0.scalar_type() != k0.scalar_type() || (q0.defined() && q0.scalar_type() != k0.scalar_type())) raise(PyExc_TypeError, "q, k and v must have the same type");
+    if (v0.sizes() != k0.sizes()) raise(PyExc_ValueError, "v must have the shape of k " + shape_of(k0) + ", got " + shape_of(v0));
+    const int64_t T = k0.size(0), D = k0.size(2);
+    if (q0.defined() && (q0.dim() != 3 || q0.size(0) != T || q0.size(2) != D || q0.size(1) < 1)) bad_shape("q", "[tokens, heads, D] of k's tokens and head dim", q0);
+    const CacheArgs c = cache_in(P.cache, kc, vc, ks, vs, bt, sl, a[8], T);
+    if (k0.size(1) != P.cache.H_kv || D != P.cache.D) raise(PyExc_ValueError, "k must have the heads and head dim of the cache " + shape_of(kc) + ", got " + shape_of(k0));
+    for (const at::Tensor* s : {&ks, &vs})
+      for (int i = 0; i < 3; ++i)
+        if (s->stride(i) <= 0 && s->size(i) > 1) raise(PyExc_ValueError, "k_scale and v_scale are written: their strides must be positive");
+    if (t0.defined()) rotary_table(t0, D);
+    same_device({&k0, &v0, &kc, &vc, &ks, &vs, &bt, &sl, &c.cu, &q0, &t0});
+    if (T > 0x7fffffffLL) raise(PyExc_ValueError, "too many tokens");
+    const c10::Device dev = k0.device();
+    c10::cuda::CUDAGuard guard(dev);
+    at::Tensor q8, qs;
+    if (q0.defined()) {
+      q8 = empty(q0.sizes(), at::kChar, dev);
+      qs = empty({T, q0.size(1)}, at::kFloat, dev);
+    }
+    if (T > 0) {
+      if (P.cache.table_width < 1) raise(PyExc_ValueError, "block_table has no columns");
+      const at::Tensor k = rows_ready(k0), v = rows_ready(v0), q = q0.defined() ? rows_ready(q0) : at::Tensor(), table = t0.defined() ? aligned16(t0) : at::Tensor();
+      P.k = k.data_ptr();
+      P.v = v.data_ptr();
+      for (int i = 0; i < 2; ++i) {
+        P.k_stride[i] = k.stride(i);
+        P.v_stride[i] = v.stride(i);
+      }
+      if (q.defined()) {
+        P.q = q.data_ptr();
+        P.q_stride[0] = q.stride(0);
+        P.q_stride[1] = q.stride(1);
+        P.q8 = q8.data_ptr();
+        P.q_scale = qs.data_ptr<float>();
+        P.H = q.size(1);
+      }
+      P.tokens = T;
+      P.cu_seqlens = c.cu.defined() ? c.cu.data_ptr<int>() : nullptr;
+      if (table.defined()) {
+        P.table = table.data_ptr<float>();
+        P.table_rows = table.size(0);
+        P.rot_dim = 2 * table.size(1);
+      }
+      P.interleaved = truth(a[11]);
+      const at::Tensor st = status_word(dev);
+      P.status = st.data_ptr<int>();
+      void* stream = stream_of(dev);
+      int rc;
+      Py_BEGIN_ALLOW_THREADS
+      rc = intfa_paged_append(&P, stream);
+      Py_END_ALLOW_THREADS
+      check(rc);
+    }
+    if (!q0.defined()) Py_RETURN_NONE;
+    return tuple_of({q8, qs});
+  } catch (const PySet&) {
+    return nullptr;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
+// paged(q, k_cache, v_cache, q_scale, k_scale, v_scale, block_table, seq_lens, cu_seqlens | None, causal, sm_scale, out_dtype | None, out | None,
+//       return_lse)
+PyObject* paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  try {
+    if (n != 14) raise(PyExc_TypeError, "paged takes 14 arguments");
+    const at::Tensor &q0 = tensor(a[0], "q"), &kc = tensor(a[1], "k_cache"), &vc = tensor(a[2], "v_cache"), &qs = tensor(a[3], "q_scale");
+    const at::Tensor &ks = tensor(a[4], "k_scale"), &vs = tensor(a[5], "v_scale"), &bt = tensor(a[6], "block_table"), &sl = tensor(a[7], "seq_lens");
+    if (!is(q0, at::kChar)) raise(PyExc_TypeError, "q must be int8");
+    if (q0.dim() != 3) bad_shape("q", "[tokens, heads, D]", q0);
+    const int64_t T = q0.size(0), H = q0.size(1), D = q0.size(2);
+    if (!is(qs, at::kFloat)) raise(PyExc_TypeError, "q_scale must be float32");
+    if (qs.dim() != 2 || qs.size(0) != T || qs.size(1) != H) bad_shape("q_scale", "[tokens, heads]", qs);
+    Options o;
+    if (a[11] != Py_None) take_option(o, N_OUT, a[11]);
+    IntfaPagedParams P{};
+    const CacheArgs c = cache_in(P.cache, kc, vc, ks, vs, bt, sl, a[8], T);
+    if (D != P.cache.D || H < 1 || H % P.cache.H_kv) raise(PyExc_ValueError, "q must have the head dim of the cache " + shape_of(kc) + " and a multiple of its heads, got " + shape_of(q0));
+    at::Tensor out;
+    if (a[12] != Py_None) {
+      out = tensor(a[12], "out");
+      if (!is(out, at::kHalf) && !is(out, at::kBFloat16)) raise(PyExc_TypeError, "out must be float16 or bfloat16");
+      if (a[11] != Py_None && out.scalar_type() != o.out) raise(PyExc_TypeError, "out has another type than out_dtype");
+      if (out.sizes() != q0.sizes()) bad_shape("out", "that of q", out);
+      o.out = out.scalar_type();
+    }
+    same_device({&q0, &qs, &kc, &vc, &ks, &vs, &bt, &sl, &c.cu, &out});
+    if (T * H > 0x7fffffffLL) raise(PyExc_ValueError, "too many query rows");
+    const c10::Device dev = q0.device();
+    c10::cuda::CUDAGuard guard(dev);
+    if (out.defined()) {
+      bool ok = out.stride(2) == 1 && reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0;
+      for (int i = 0; i < 2; ++i) ok = ok && (out.stride(i) > 0 || out.size(i) <= 1) && out.stride(i) % 8 == 0;
+      if (!ok) raise(PyExc_ValueError, "out must have a contiguous last dim and lie, with every stride, on 16-byte boundaries");
+    } else {
+      out = empty({T, H, D}, o.out, dev);
+    }
+    const bool want_lse = truth(a[13]);
+    at::Tensor lse = want_lse ? empty({T, H}, at::kFloat, dev) : at::Tensor();
+    if (T > 0) {
+      if (P.cache.table_width < 1) raise(PyExc_ValueError, "block_table has no columns");
+      const at::Tensor q = rows_ready(q0);
+      const at::Tensor s = qs.stride(0) >= 0 && qs.stride(1) >= 0 ? qs : qs.contiguous();
+      P.q = q.data_ptr();
+      P.q_scale = s.data_ptr<float>();
+      P.o = out.data_ptr();
+      P.lse_out = want_lse ? lse.data_ptr<float>() : nullptr;
+      for (int i = 0; i < 2; ++i) {
+        P.q_stride[i] = q.stride(i);
+        P.qs_stride[i] = s.stride(i);
+        P.o_stride[i] = out.size(i) <= 1 ? H * D : out.stride(i);
+      }
+      P.tokens = T;
+      P.H = H;
+      P.o_dtype = o.out == at::kBFloat16 ? INTFA_OUT_BF16 : INTFA_OUT_FP16;
+      P.cu_seqlens = c.cu.defined() ? c.cu.data_ptr<int>() : nullptr;
+      P.causal = truth(a[9]);
+      P.sm_scale = static_cast<float>(as_double(a[10]));
+      const size_t bytes = intfa_paged_workspace_bytes(&P);
+      at::Tensor ws = empty({static_cast<int64_t>(bytes)}, at::kByte, dev);
+      P.workspace = ws.data_ptr();
+      P.workspace_bytes = bytes;
+      const at::Tensor st = status_word(dev);
+      P.status = st.data_ptr<int>();
+      void* stream = stream_of(dev);
+      int rc;
+      Py_BEGIN_ALLOW_THREADS
+      rc = intfa_paged_attention(&P, stream);
+      Py_END_ALLOW_THREADS
+      check(rc);
+    }
+    if (!want_lse) return THPVariable_Wrap(out);
+    return tuple_of({out, lse});
+  } catch (const PySet&) {
+    return nullptr;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
 // the status word (int32[1] tensor) of a CUDA device
 PyObject* status(PyObject*, PyObject* arg) {
   HANDLE_TH_ERRORS
@@ -620,6 +969,9 @@ PyMethodDef kMethods[] = {{"fwd", method(fwd), METH_FASTCALL | METH_KEYWORDS, nu
                           {"quant_pertoken", quant_pertoken, METH_O, nullptr},
                           {"quant_v", method(quant_v), METH_FASTCALL, nullptr},
                           {"quant_qkv", method(quant_qkv), METH_FASTCALL, nullptr},
+                          {"rotary", method(rotary), METH_FASTCALL, nullptr},
+                          {"append", method(append), METH_FASTCALL, nullptr},
+                          {"paged", method(paged), METH_FASTCALL, nullptr},
                           {"status", status, METH_O, nullptr},
                           {"set_error_class", set_error_class, METH_O, nullptr},
                           {nullptr, nullptr, 0, nullptr}};

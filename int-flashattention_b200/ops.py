@@ -13,6 +13,8 @@ PyTorch is used for memory and streams only -- every computation runs in libintf
 missing library or a CPU tensor raises.  Argument checks, allocation and launches are native code (csrc/intfa_torch.cpp,
 module _native); the functions here give them their signatures.
 """
+import math
+
 import torch
 
 from . import _lib
@@ -52,12 +54,14 @@ def _status_word(dev):
 
 def check_status(device=None):
     """Synchronise and raise if any kernel launched through this module on `device` gave up a
-    bounded device-side wait.  Returns the raw status word (0 = fine)."""
+    bounded device-side wait, or was given a position, length or page outside its table or cache.  Returns the raw status word (0 = fine)."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     word = _status_word(dev)
     val = int(word.item())
     if val != 0:
         word.zero_()
+        if val & 0xff == _lib.STATUS_BAD_INDEX:
+            raise _lib.IntfaError(_lib.ERR_INVALID_ARG, "a position, length or page lies outside its table or cache (nothing was read or written there)")
         raise _lib.IntfaError(_lib.ERR_DEVICE_WAIT,
                               "device-side wait expired (wait code %d, CTA %d)" % (val & 0xff, val >> 8))
     return val
@@ -153,3 +157,87 @@ def int_flash_attention(q, k, v, causal, sm_scale, variant="full", v_mode="per_c
     per-(batch,head) V for the full-int8 variant) followed by the INT8 attention forward.
     Argument order follows the reference's attention(q, k, v, causal, sm_scale) (flash_atten_fp.py:155)."""
     return (_native_mod or _native()).flash(q, k, v, causal, sm_scale, variant, v_mode, **kw)
+
+
+# ---------------------------------------------------------------------------------------------
+# serving: rotary positions, a paged int8 cache, attention over it
+# ---------------------------------------------------------------------------------------------
+def rotary_table(n, rot_dim, base=10000.0, *, scaling=None, device=None):
+    """(cos, sin) of positions 0 .. n-1 for the first `rot_dim` channels of a head: float32 [n, rot_dim/2, 2], from angles
+    position * base**(-2j/rot_dim) in 64 bits.  `scaling` for contexts longer than those trained on:
+      ("linear", factor)     every position divided by factor
+      ("ntk", factor)        the base raised to base * factor**(rot_dim/(rot_dim-2)): the slowest pair turns factor times slower,
+                             the fastest as before
+      ("by_parts", factor, trained[, fast=32, slow=1[, magnitude]])
+                             pairs that turn more than `fast` times within the `trained` positions stay, those that turn fewer
+                             than `slow` times are divided by factor, in between by a ramp over the logarithm of the turns; cos and sin are
+                             multiplied by `magnitude` (0.1 ln(factor) + 1 unless given)"""
+    if rot_dim < 2 or rot_dim % 2:
+        raise ValueError("rot_dim must be even and at least 2, got %r" % (rot_dim,))
+    if n < 1:
+        raise ValueError("the table needs at least one position")
+    j = torch.arange(0, rot_dim, 2, dtype=torch.float64, device=device) / rot_dim
+    kind, magnitude = (scaling[0] if scaling else None), 1.0
+    if scaling and (len(scaling) < 2 or not scaling[1] > 0):
+        raise ValueError("scaling needs a positive factor")
+    if kind == "ntk":
+        if rot_dim == 2:
+            raise ValueError("ntk scaling needs more than one pair")
+        base = base * scaling[1] ** (rot_dim / (rot_dim - 2))
+    freq = base ** -j
+    if kind == "linear":
+        freq = freq / scaling[1]
+    elif kind == "by_parts":
+        if len(scaling) < 3:
+            raise ValueError("by_parts scaling is (\"by_parts\", factor, trained, ...)")
+        factor, trained = scaling[1:3]
+        fast, slow = scaling[3:5] if len(scaling) > 3 else (32.0, 1.0)
+        if not fast > slow > 0:
+            raise ValueError("by_parts scaling needs fast > slow > 0")
+        magnitude = scaling[5] if len(scaling) > 5 else 0.1 * math.log(factor) + 1.0
+        turns = trained * freq / (2 * math.pi)
+        stay = ((turns / slow).log() / math.log(fast / slow)).clamp(0, 1)
+        freq = freq * stay + freq / factor * (1 - stay)
+    elif kind not in (None, "ntk"):
+        raise ValueError("unknown scaling %r: linear, ntk or by_parts" % (kind,))
+    angle = torch.arange(n, dtype=torch.float64, device=device)[:, None] * freq
+    return (torch.stack([angle.cos(), angle.sin()], -1) * magnitude).float()
+
+
+def rotary(q, k, table, positions, *, interleaved=False, inverse=False):
+    """Rotates q, and k with it unless it is None, by their positions: pair j of a head's first channels, (a, b) = channels
+    (j, j + rot_dim/2), or (2j, 2j+1) where interleaved, becomes (a c - b s, b c + a s) with (c, s) = table[position, j]
+    (rotary_table).  q [B,H,N,D] with positions [N] or [B,N], or packed [tokens, heads, D] with positions [tokens]; k likewise with
+    heads of its own.  float16, bfloat16 or float32; computed in fp32 and rounded once.  inverse=True is the gradient of the call
+    with inverse=False (no autograd here): the rotation back.  Returns q', or (q', k')."""
+    return (_native_mod or _native()).rotary(q, k, table, positions, interleaved, inverse)
+
+
+def append_int8_paged(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_seqlens=None, *, q=None, table=None,
+                      interleaved=False):
+    """Appends the new tokens' k and v [tokens, heads, D] (float16 or bfloat16) to a paged int8 cache, in place: k rotated by its
+    position first where a `table` (rotary_table) is given, then both quantised with one scale for each block of tokens and head.
+      k_cache, v_cache   int8 [pages, heads, page_size, D]: any page and head strides of 16 bytes, D 64, 128 or 256,
+                         page_size a power of two from 8 to 256
+      k_scale, v_scale   float32 [pages, heads, page_size/block]; block 1 is one scale a token
+      block_table        int32 [S, columns]: the page of a sequence's tokens i*page_size ...
+      seq_lens           int32 [S]: tokens in the cache with the new ones, which are the last
+      cu_seqlens         int32 [S+1]: where each sequence's new tokens begin among `tokens`; None: one token a sequence
+    Where a block began in an earlier call its scale becomes the larger of the old one and the new tokens', and the codes of its older
+    tokens follow.  Tokens behind the last sequence, and those of a sequence with seq_lens 0 (padding), are left out.  Two sequences may
+    not append to one page in a call.  With q [tokens, query heads, D]: the same tokens' queries,
+    rotated and quantised per token; returns (q8, q_scale [tokens, heads]) as attention_int8_paged takes them."""
+    return (_native_mod or _native()).append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_seqlens, q, table, interleaved)
+
+
+def attention_int8_paged(q, k_cache, v_cache, q_scale, k_scale, v_scale, block_table, seq_lens, cu_seqlens, causal, sm_scale, *,
+                         out_dtype=None, out=None, return_lse=False):
+    """Attention of packed int8 query rows q [tokens, query heads, D] over a paged int8 cache (append_int8_paged has the tensors):
+    softmax(sm_scale * q k^T) v, with q = q8 * q_scale and the cache's values as codes times scales.  The rows of sequence s are
+    cu_seqlens[s] .. cu_seqlens[s+1]-1 (None: one row each, decode); causal: they are its last tokens, row i of n sees keys up to
+    seq_lens[s] - n + i, else all keys.  Query heads share K/V heads in order, as in attention_int8.  A row that sees no key is
+    zero.  Returns o [tokens, query heads, D] in out_dtype (torch.float16 unless given, or torch.bfloat16); with `out` it is written there,
+    and rows behind the last sequence stay as they were (without it they are not set).  return_lse: and the log2-domain LSE
+    [tokens, query heads]."""
+    return (_native_mod or _native()).paged(q, k_cache, v_cache, q_scale, k_scale, v_scale, block_table, seq_lens, cu_seqlens, causal, sm_scale,
+                                            out_dtype, out, return_lse)
