@@ -15,7 +15,8 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 LIB = os.path.join(PKG_DIR, "libintfa.so")
 SOURCES = ["intfa_api.cu", "intfa_quant.cu", "intfa_fwd.cu", "intfa_decode.cu", "intfa_rotary.cu", "intfa_paged.cu",
            "intfa_paged_attn.cu"]
-HEADERS = ["intfa_internal.h", "intfa_ptx.cuh", "intfa_rows.cuh", "intfa_fwd_pipe.cuh", "intfa_fwd_pipe_softmax.inc",
+HEADERS = ["intfa_internal.h", "intfa_ptx.cuh", "intfa_rows.cuh", "intfa_paged_tile.cuh",
+           "intfa_fwd_pipe.cuh", "intfa_fwd_pipe_softmax.inc",
            "intfa_fwd_pipe_update.inc", os.path.join("..", "..", "include", "intfa.h")]
 NATIVE = os.path.join(PKG_DIR, "_native.so")
 NATIVE_SOURCES = ["intfa_torch.cpp", os.path.join("..", "..", "include", "intfa.h")]

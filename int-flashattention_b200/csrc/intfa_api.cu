@@ -316,7 +316,7 @@ int intfa_paged_attention(const IntfaPagedParams* p, void* stream) {
   if (!p) return set_error(INTFA_ERR_INVALID_ARG, "params is NULL");
   int rc;
   if ((rc = check_paged(p))) return rc;
-  if ((rc = check_rows("q", p->q, p->q_stride, 2, 1)) || (rc = check_rows("o", p->o, p->o_stride, 2, 2))) return rc;
+  if ((rc = check_rows("q", p->q, p->q_stride, 2, 1)) || (rc = (p->q_stride[0] > 0 && p->q_stride[1] > 0 ? INTFA_OK : set_error(INTFA_ERR_INVALID_ARG, "q strides must be positive"))) || (rc = check_rows("o", p->o, p->o_stride, 2, 2))) return rc;
   if (!p->q_scale || p->qs_stride[0] < 0 || p->qs_stride[1] < 0) return set_error(INTFA_ERR_INVALID_ARG, "q_scale is NULL or has a negative stride");
   if (!p->workspace || (reinterpret_cast<uintptr_t>(p->workspace) & 255u)) return set_error(INTFA_ERR_INVALID_ARG, "workspace is NULL or not 256-byte aligned");
   return paged_attention(p, reinterpret_cast<cudaStream_t>(stream));

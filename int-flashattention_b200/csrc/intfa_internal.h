@@ -46,9 +46,9 @@ int sm_count_cached();
 // cache; the codes of the waits are others.
 constexpr int kStatusBadIndex = INTFA_STATUS_BAD_INDEX;
 
-// [B,H,N,D] tensor, element strides for (B,H,N); box = (box_d, box_rows, 1, 1)
+// [B,H,N,D] tensor, element strides for (B,H,N); box = (box_d, box_rows, box_heads, 1)
 int make_tmap(CUtensorMap* tm, const void* base, int esize, const int64_t* stride, int B, int H, int N, int D, int box_d, int box_rows,
-              CUtensorMapSwizzle swz);
+              CUtensorMapSwizzle swz, int box_heads = 1);
 
 // Few query rows against many keys (intfa_decode.cu).  Returns false where the call is not one for that path.
 bool decode_dispatch(const IntfaFwdParams* a, cudaStream_t stream, int* rc);

@@ -60,7 +60,8 @@ struct PParams {
   int causal, o_bf16;
   float c;                                        // sm_scale * log2(e)
   int workers, least;                             // warps of the grid; fewest chunks a warp takes
-  int rows_tile;                                  // RT
+  int rows_tile;                                  // rows of a unit: RT, or 256 on the 128-row tiles
+  int tile_tokens;                                // 128-row tiles: whole tokens in one; 0: packed RT rows
   float* part; float* part_ml;                    // [2*workers][RT][D]; [2*workers][RT]{m, mw, l, -}
   UnitPart* units; long long max_units;           // [max_units]
   long long* head;                                // {units, share, chunks}
@@ -261,11 +262,9 @@ struct Sum {
     mw = w1;
   }
 };
-// ... and written: row r of a unit's sequence, whose first query row is token t0
-__device__ __forceinline__ void write_sum(const PParams& p, int t0, int r, int head, int ch, const Sum& x) {
+// ... and written: query row n, head h
+__device__ __forceinline__ void write_sum(const PParams& p, long long n, int h, int ch, const Sum& x) {
   const float f = row_factor(x.m, x.mw, x.l);
-  const long long n = t0 + r / p.ratio;
-  const int h = head * p.ratio + r % p.ratio;
   uint2 w;
   if (p.o_bf16) {
     const __nv_bfloat162 a = __floats2bfloat162_rn(x.a.x * f, x.a.y * f), b = __floats2bfloat162_rn(x.a.z * f, x.a.w * f);
@@ -707,7 +706,8 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_const
       *reinterpret_cast<float4*>(p.part + (slot * RT + r) * D + ch) = x.a;
       if (ch == 0) *reinterpret_cast<float4*>(p.part_ml + (slot * RT + r) * 4) = make_float4(x.m, x.mw, x.l, 0.f);
     } else if (r < whole[3]) {
-      write_sum(p, whole[2], whole[5] * RT + r, whole[4], ch, x);
+      const int row = whole[5] * RT + r;
+      write_sum(p, whole[2] + row / p.ratio, whole[4] * p.ratio + row % p.ratio, ch, x);
     }
   }
 }
@@ -730,7 +730,20 @@ __global__ void __launch_bounds__(GROUPS * (D / 4)) combine_kernel(const PParams
   if (!up.open) return;
   const long long share = p.head[1], total = p.head[2], cs = share * cta_warps;
   const Seq q = seq_of(p, up.s);
-  const int head = up.unit / q.tiles, tile = up.unit - head * q.tiles, R = q.n * p.ratio;
+  const int tiles = p.tile_tokens ? (q.n + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens) : q.tiles;
+  const int head = up.unit / tiles, tile = up.unit - head * tiles;
+  // row r of the unit: query row (token n of the sequence, head h of the K/V head's)
+  auto row_of = [&](int r, int& n, int& h) {
+    if (p.tile_tokens) {
+      const int rr = r & 127;
+      n = (2 * tile + (r >> 7)) * p.tile_tokens + rr / p.ratio;
+      h = rr % p.ratio;
+      return rr < p.tile_tokens * p.ratio && n < q.n;
+    }
+    n = (tile * p.rows_tile + r) / p.ratio;
+    h = (tile * p.rows_tile + r) % p.ratio;
+    return n < q.n;
+  };
   const long long a = up.chunk0 / share, b = (up.chunk1 - 1) / share;
   // CTAs ka .. kb lie in the unit as a whole and have left one part each, in their first warp's slot
   const long long ka = (up.chunk0 + cs - 1) / cs, kb = up.chunk1 == total ? (total - 1) / cs : up.chunk1 / cs - 1;
@@ -744,7 +757,8 @@ __global__ void __launch_bounds__(GROUPS * (D / 4)) combine_kernel(const PParams
   const int first_row = (int)(blockIdx.x % per_unit) * rows_cta;
   const int row_step = rows_cta == 1 ? 1 : GROUPS, part_step = rows_cta == 1 ? GROUPS : 1;
   for (int r = first_row + (rows_cta == 1 ? 0 : grp); r < first_row + rows_cta; r += row_step) {
-    if (tile * p.rows_tile + r >= R) continue;
+    int n, h;
+    if (!row_of(r, n, h)) continue;
     Sum x;
     x.clear();
 #pragma unroll 4
@@ -759,35 +773,50 @@ __global__ void __launch_bounds__(GROUPS * (D / 4)) combine_kernel(const PParams
       if (grp > 0) return;
       for (int i = 1; i < GROUPS; ++i) x.add(red_ml[i], red[i][ch / 4]);
     }
-    write_sum(p, q.t0, tile * p.rows_tile + r, head, ch, x);
+    write_sum(p, q.t0 + n, head * p.ratio + h, ch, x);
   }
 }
+
+#include "intfa_paged_tile.cuh"
 
 // ---------------------------------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------------------------------
 struct Plan {
+  bool tiles = false;                   // 128-row tiles
   int NT = 1, ctas = 0, warps = 8;
   long long max_units = 0;
   size_t off_ml = 0, off_units = 0, off_head = 0, bytes = 0;
 };
+// An average sequence with more rows a K/V head than this takes 128-row tiles
+constexpr double kFewRows = 32;
 Plan make_plan(const IntfaPagedParams* a, int sms) {
   Plan pl;
   const IntfaPagedCache& c = a->cache;
   const int ratio = a->H / c.H_kv;
-  // Rows a tile: 16 where an average sequence has more than 8 rows a K/V head
-  pl.NT = (double)a->tokens * ratio > 8.0 * c.S ? 2 : 1;
-  pl.warps = c.D == 256 ? 4 : c.D == 128 && pl.NT == 2 ? 6 : 8;
   pl.ctas = sms;
-  pl.max_units = (a->tokens * ratio / (8 * pl.NT) + c.S) * c.H_kv;
-  if (pl.max_units > 0x7fffffffLL) return Plan();
-  const int RT = 8 * pl.NT;
-  const long long slots = 2LL * pl.ctas * pl.warps;
   auto take = [&](size_t bytes) {
     const size_t r = pl.bytes;
     pl.bytes += (bytes + 255) / 256 * 256;
     return r;
   };
+  pl.tiles = c.D <= 128 && ratio <= kTileRows && (double)a->tokens * ratio > kFewRows * c.S;
+  if (pl.tiles) {
+    pl.warps = 1;
+    pl.max_units = pl.ctas;
+    take((size_t)2 * pl.ctas * 2 * kTileRows * c.D * 4);
+    pl.off_ml = take((size_t)2 * pl.ctas * 2 * kTileRows * 16);
+    pl.off_units = take((size_t)pl.max_units * sizeof(UnitPart));
+    pl.off_head = take(32);
+    return pl;
+  }
+  // Rows a tile: 16 where an average sequence has more than 8 rows a K/V head
+  pl.NT = (double)a->tokens * ratio > 8.0 * c.S ? 2 : 1;
+  pl.warps = c.D == 256 ? 4 : c.D == 128 && pl.NT == 2 ? 6 : 8;
+  pl.max_units = (a->tokens * ratio / (8 * pl.NT) + c.S) * c.H_kv;
+  if (pl.max_units > 0x7fffffffLL) return Plan();
+  const int RT = 8 * pl.NT;
+  const long long slots = 2LL * pl.ctas * pl.warps;
   take((size_t)slots * RT * c.D * 4);
   pl.off_ml = take((size_t)slots * RT * 16);
   pl.off_units = take((size_t)pl.max_units * sizeof(UnitPart));
@@ -819,6 +848,31 @@ int run(const IntfaPagedParams* a, const Plan& pl, PParams p, cudaStream_t strea
   const long long grid = pl.max_units * (p.rows_tile / rows_cta);
   if (grid > 0x7fffffffLL) return set_error(INTFA_ERR_TOO_LARGE, "too many query rows");
   return launch_kernel("paged combine", combine_kernel<D, GROUPS>, (unsigned)grid, GROUPS * (D / 4), 0, stream, p, WARPS, rows_cta);
+}
+
+template <int D>
+int run_tiles(const IntfaPagedParams* a, const Plan& pl, PParams p, cudaStream_t stream) {
+  using C = TileCfg<D>;
+  const IntfaPagedCache& c = a->cache;
+  CUtensorMap tmQ, tmK, tmV;
+  const CUtensorMapSwizzle swz = D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+  const int64_t qst[3] = {(int64_t)p.T * p.qn, p.qn, p.qh};
+  int rc;
+  if ((rc = make_tmap(&tmQ, a->q, 1, qst, 1, (int)p.T, a->H, D, D, p.ratio, swz, p.tile_tokens))) return rc;
+  if ((rc = make_tmap(&tmK, c.k, 1, c.k_stride, c.pages, c.H_kv, c.page_size, D, D, 1 << p.box_log, swz))) return rc;
+  if ((rc = make_tmap(&tmV, c.v, 1, c.v_stride, c.pages, c.H_kv, c.page_size, D, D, 1 << p.box_log, swz))) return rc;
+  auto kern = paged_tile_kernel<D>;
+  static std::atomic<bool> attr_done[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return set_error(INTFA_ERR_CUDA, "cannot query the current device");
+  if (!attr_done[dev].load(std::memory_order_acquire)) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (e != cudaSuccess) return set_error(INTFA_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    attr_done[dev].store(true, std::memory_order_release);
+  }
+  if ((rc = launch_kernel("paged attention", kern, pl.ctas, C::THREADS, C::SMEM, stream, tmQ, tmK, tmV, p))) return rc;
+  constexpr int GROUPS = 1024 / D, ROWS = 32;
+  return launch_kernel("paged combine", combine_kernel<D, GROUPS>, (unsigned)(pl.ctas * (2 * kTileRows / ROWS)), GROUPS * (D / 4), 0, stream, p, 1, ROWS);
 }
 
 int log2_of(long long n) {
@@ -875,6 +929,14 @@ int paged_attention(const IntfaPagedParams* a, cudaStream_t stream) {
   p.max_units = pl.max_units;
   p.head = reinterpret_cast<long long*>(ws + pl.off_head);
   p.status = a->status;
+  p.tile_tokens = 0;
+  if (pl.tiles) {
+    p.rows_tile = 2 * kTileRows;
+    p.tile_tokens = kTileRows / p.ratio;
+    p.box_log = c.page_size < kTileKeys ? p.page_log : log2_of(kTileKeys);
+    p.least = 2;
+    return c.D == 64 ? run_tiles<64>(a, pl, p, stream) : run_tiles<128>(a, pl, p, stream);
+  }
   switch (c.D) {
     case 64: return pl.NT == 2 ? run<64, 2, 8, 4>(a, pl, p, stream) : run<64, 1, 8, 5>(a, pl, p, stream);
     case 128: return pl.NT == 2 ? run<128, 2, 6, 3>(a, pl, p, stream) : run<128, 1, 8, 3>(a, pl, p, stream);

@@ -1,0 +1,769 @@
+// Attention over a paged int8 cache where a sequence has many query rows (chunks of a prompt, whole prompts): tiles of 128 rows on tcgen05.
+// (Included by intfa_paged_attn.cu inside namespace intfa, after the shared helpers.)
+//
+// A unit is (sequence, K/V head, 256 rows): two tiles of 128 rows, each the rows of as many whole tokens as fit, all query heads of the
+// K/V head packed.  The units' chunks of 128 keys (those that the last row of a unit sees) are dealt out to the CTAs, one an SM, in equal
+// contiguous shares; parts of units that are cut go to scratch and combine_kernel adds them up, as in the kernel for few rows.
+//
+// 512 threads:
+//   warp 0       TMA: Q once per unit (heads x tokens boxes), K and V pages of 8 to 128 rows each
+//   warp 1       MMA issuer.  For each tile in turn: P V of the last chunk, S = Q K^T of the next
+//   warp 2       TMEM; K scales, log2 and reciprocal of the V scales of a chunk into a ring
+//   warp 3       goes through the units and publishes them
+//   warps 4-7    V from int8 (as TMA left it) to fp16 in the MN-major tiles that P V takes
+//   warps 8-11, 12-15   softmax of tile 0 and of tile 1, one thread a row: while one tile is in the tensor core the other is here
+// TMEM: S of both tiles (128 columns each; P, fp16, over the first half of its own S), two accumulators of D columns.
+//
+// The arithmetic is that of the kernel for few rows: w = p v_scale relative to a running maximum of w, P = fp16(w), l = sum p relative to a
+// reference of its own.  Both references follow their maxima only where these get 2^8 ahead: the accumulator is rescaled in a few
+// chunks of a unit, and w <= 2^8 loses no bits in fp16.  Where a chunk's V scales are within 2^60 of what the references differ by (nearly
+// always: the general way is for zeros and for scales of very different sizes) p = w / v_scale needs no exp2 of its own.
+// S starts from the bit pattern of 1.5*2^23, written by a small fp16 MMA, and reads as fp32 1.5*2^23 + dot.
+#pragma once
+
+constexpr int kTileRows = 128, kTileKeys = 128;
+constexpr int kTileService = 40, kTileConvert = 72, kTileSoftmax = 200;          // registers
+static_assert(128 * (kTileService + kTileConvert) + 256 * kTileSoftmax <= 65536, "setmaxnreg budget");
+
+// a unit, or the part of it that a CTA does
+struct __align__(16) TileUnit {
+  long long lim0;              // causal: the last key that the unit's first token sees
+  int t0, tokens;              // its first token among all, and how many it has
+  int head, s, keys;           // K/V head; sequence; keys that are looked at
+  int c0, c1;                  // chunks to do; c0 < 0: no more units
+  int slot;                    // of its part in scratch; -1: the unit is done here
+  int pad[2];
+};
+static_assert(sizeof(TileUnit) == 48, "unit");
+
+struct TileSeq {
+  int t0, n, keys, tiles, uniform;
+  long long first;
+};
+__device__ __forceinline__ TileSeq tile_seq_of(const PParams& p, int s) {
+  const Seq q = seq_of(p, s);
+  TileSeq w;
+  w.t0 = q.t0;
+  w.n = q.n;
+  w.keys = q.keys;
+  w.first = q.len - q.n;
+  w.tiles = (q.n + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
+  w.uniform = !p.causal || w.first < 0 || q.len > q.keys;        // every unit goes over all keys (for the odd lengths, masked)
+  return w;
+}
+__device__ __forceinline__ int tile_chunks(const PParams& p, const TileSeq& q, int tile) {
+  long long vis = q.keys;
+  if (!q.uniform) vis = min(vis, q.first + (long long)(tile + 1) * 2 * p.tile_tokens);
+  return vis > kTileKeys ? (int)((vis + kTileKeys - 1) / kTileKeys) : 1;
+}
+// sum of floor((a t + b) / m), t = 0 .. n-1 (a, b >= 0)
+__device__ inline long long floor_sum(long long n, long long m, long long a, long long b) {
+  long long sum = 0;
+  while (n > 0) {
+    sum += n * (n - 1) / 2 * (a / m) + n * (b / m);
+    a %= m;
+    b %= m;
+    const long long y = a * n + b;
+    if (y < m) break;
+    n = y / m;
+    b = y % m;
+    const long long t = m;
+    m = a;
+    a = t;
+  }
+  return sum;
+}
+// chunks of the first k units of a K/V head
+__device__ inline long long tile_chunks_before(const PParams& p, const TileSeq& q, int k) {
+  if (k <= 0) return 0;
+  if (q.uniform) return (long long)k * tile_chunks(p, q, 0);
+  const int full = k < q.tiles ? k : q.tiles - 1;
+  const long long step = 2 * p.tile_tokens;
+  return floor_sum(full, kTileKeys, step, q.first + step + kTileKeys - 1) + (k == q.tiles ? tile_chunks(p, q, q.tiles - 1) : 0);
+}
+
+template <int D>
+struct TileCfg {
+  static constexpr int THREADS = 512, NK = 3, NV8 = 2, NV = 2, NSC = 4, NU = 4;
+  static constexpr int Q_BYTES = kTileRows * D, K_BYTES = kTileKeys * D, V_BYTES = kTileKeys * D * 2;
+  static constexpr int SC_FLOATS = 3 * kTileKeys + 4;
+  static constexpr int OFF_Q = 0, OFF_K = OFF_Q + 2 * Q_BYTES, OFF_V8 = OFF_K + NK * K_BYTES, OFF_V = OFF_V8 + NV8 * K_BYTES;
+  static constexpr int OFF_ARM = OFF_V + NV * V_BYTES;
+  static constexpr int OFF_SC = OFF_ARM + 4096;
+  static constexpr int OFF_UNIT = OFF_SC + NSC * SC_FLOATS * 4;
+  static constexpr int OFF_PRE = OFF_UNIT + NU * (int)sizeof(TileUnit);
+  static constexpr int NBARS = 4 + 2 * NK + 2 * NV8 + 2 * NV + 2 * NSC + 2 * NU + 6;
+  static constexpr int OFF_BAR = OFF_PRE + (THREADS + 2) * 8;
+  static constexpr int OFF_MISC = OFF_BAR + NBARS * 8;
+  static constexpr int SMEM = OFF_MISC + 32 + 1024;
+  static_assert(SMEM <= 227 * 1024, "shared memory");
+  static_assert(OFF_UNIT % 16 == 0 && OFF_SC % 16 == 0 && OFF_PRE % 8 == 0, "alignment");
+  static constexpr int COL_S = 0, COL_O = 2 * kTileKeys;
+  static_assert(COL_O + 2 * D <= 512, "TMEM columns");
+  static constexpr uint64_t SWZ_QK = D == 128 ? kSwz128 : kSwz64;
+  static constexpr uint32_t IDESC_QK = make_idesc(2, 1, 1, 0, 0, kTileRows, kTileKeys);
+  static constexpr uint32_t IDESC_PV = make_idesc(1, 0, 0, 0, 1, kTileRows, D);
+  static constexpr uint32_t IDESC_ARM = make_idesc(1, 0, 0, 0, 0, kTileRows, kTileKeys);
+};
+
+enum TileWait { TW_UNIT = 65, TW_UEMPTY, TW_QE, TW_KE, TW_V8E, TW_QF, TW_KF, TW_VF, TW_P, TW_SCE, TW_V8F, TW_VE, TW_SC, TW_S, TW_O };
+
+template <int D>
+__global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                                                            const __grid_constant__ CUtensorMap tmV, const PParams p) {
+  using C = TileCfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((0u - smem_u32(smem_raw)) & 1023u);
+  const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const uint32_t bars = smem_u32(smem + C::OFF_BAR);
+  auto BAR = [&](int i) { return bars + 8u * i; };
+  constexpr int B_QF = 0, B_QE = 2;                              // [2] TMA: Q tile landed; commit: its last S is done
+  constexpr int B_KF = 4, B_KE = B_KF + C::NK;                   // TMA; commit
+  constexpr int B_V8F = B_KE + C::NK, B_V8E = B_V8F + C::NV8;    // TMA; converting warps (4)
+  constexpr int B_VF = B_V8E + C::NV8, B_VE = B_VF + C::NV;      // converting warps (4); commit
+  constexpr int B_SCF = B_VE + C::NV, B_SCE = B_SCF + C::NSC;    // scale loader; softmax warps (8)
+  constexpr int B_UF = B_SCE + C::NSC, B_UE = B_UF + C::NU;      // unit published; taken over by TMA, MMA, scale, converting, softmax warps (15)
+  constexpr int B_S = B_UE + C::NU, B_P = B_S + 2, B_O = B_P + 2;        // [2] commit: S; softmax warps of the tile (4): P; commit: last P V
+  static_assert(B_O + 2 == C::NBARS, "barriers");
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 8);
+  TileUnit* units = reinterpret_cast<TileUnit*>(smem + C::OFF_UNIT);
+  long long* pre = reinterpret_cast<long long*>(smem + C::OFF_PRE);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(BAR(B_QF + i), 1);
+      mbar_init(BAR(B_QE + i), 1);
+      mbar_init(BAR(B_S + i), 1);
+      mbar_init(BAR(B_P + i), 4);
+      mbar_init(BAR(B_O + i), 1);
+    }
+    for (int i = 0; i < C::NK; ++i) {
+      mbar_init(BAR(B_KF + i), 1);
+      mbar_init(BAR(B_KE + i), 1);
+    }
+    for (int i = 0; i < C::NV8; ++i) {
+      mbar_init(BAR(B_V8F + i), 1);
+      mbar_init(BAR(B_V8E + i), 4);
+    }
+    for (int i = 0; i < C::NV; ++i) {
+      mbar_init(BAR(B_VF + i), 4);
+      mbar_init(BAR(B_VE + i), 1);
+    }
+    for (int i = 0; i < C::NSC; ++i) {
+      mbar_init(BAR(B_SCF + i), 1);
+      mbar_init(BAR(B_SCE + i), 8);
+    }
+    for (int i = 0; i < C::NU; ++i) {
+      mbar_init(BAR(B_UF + i), 1);
+      mbar_init(BAR(B_UE + i), 15);
+    }
+    abort_flag[0] = 0;
+    abort_flag[1] = (int)(1u << 31);
+    mbar_init_fence();
+    prefetch_tmap(&tmQ);
+    prefetch_tmap(&tmK);
+    prefetch_tmap(&tmV);
+  }
+  // the constant operand whose product with itself is 1.5*2^23 everywhere: each row's 16 values are (1024, 1024, 2048, 0 ..) twice
+  if (threadIdx.x < 256) reinterpret_cast<uint4*>(smem + C::OFF_ARM)[threadIdx.x] = make_uint4(0x64006400u, 0x00006800u, 0u, 0u);
+  fence_proxy_async_smem();
+  if (warp == 2) {
+    tmem_alloc(smem_u32(tmem_slot), 512);
+    tmem_relinquish();
+    tc_fence_before();
+  }
+  pdl_wait();
+  pdl_launch();
+  // ---- the row of all chunks: thread i counts the sequences i*seg .. (i+1)*seg - 1
+  const int seg = (p.S + C::THREADS - 1) / C::THREADS;
+  {
+    long long c = 0;
+    bool bad = false;
+    for (int s = threadIdx.x * seg; s < (threadIdx.x + 1) * seg && s < p.S; ++s) {
+      const TileSeq q = tile_seq_of(p, s);
+      if (q.n > 0) c += tile_chunks_before(p, q, q.tiles) * p.Hkv;
+      bad |= q.n > 0 && q.first + q.n > q.keys;
+    }
+    if (p.cu && threadIdx.x == 0) bad |= p.cu[p.S] > p.T;
+    if (bad && p.status && blockIdx.x == 0) atomicCAS(p.status, 0, kStatusBadIndex);
+    pre[threadIdx.x + 1] = c;
+    if (threadIdx.x == 0) pre[0] = 0;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    long long c0 = 0;
+    for (int w = 0; w < C::THREADS / 32; ++w) {
+      long long c = pre[w * 32 + lane + 1];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, c, o);
+        if (lane >= o) c += x;
+      }
+      pre[w * 32 + lane + 1] = c + c0;
+      c0 += __shfl_sync(0xffffffffu, c, 31);
+    }
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = warp_uniform(*tmem_slot);
+  const long long total = pre[C::THREADS];
+  long long share = (total + p.workers - 1) / p.workers;
+  if (share < p.least) share = p.least;
+  const int code_hi = (int)(blockIdx.x << 8);
+  auto wait = [&](int bar, uint32_t parity, int code) { return mbar_wait_warp(BAR(bar), parity, abort_flag, p.status, code_hi | code); };
+  uint32_t useq = 0;
+  // the next unit, or false
+  auto next_unit = [&](TileUnit& u) {
+    const uint32_t slot = useq % C::NU;
+    if (!wait(B_UF + slot, (useq / C::NU) & 1u, TW_UNIT)) return false;
+    ++useq;
+    u = units[slot];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(BAR(B_UE + slot));
+    u.t0 = warp_uniform(u.t0);
+    u.tokens = warp_uniform(u.tokens);
+    u.head = warp_uniform(u.head);
+    u.s = warp_uniform(u.s);
+    u.keys = warp_uniform(u.keys);
+    u.c0 = warp_uniform(u.c0);
+    u.c1 = warp_uniform(u.c1);
+    u.slot = warp_uniform(u.slot);
+    return u.c0 >= 0;
+  };
+  const int page_mask = (1 << p.page_log) - 1;
+  auto bad_page = [&](int page) { return page < 0 || page >= p.pages; };
+
+  if (warp < 4) {
+    reg_dealloc<kTileService>();
+    if (warp == 3) {
+      // ------------------------------------------------------------------ units
+      const long long begin = (long long)blockIdx.x * share;
+      const long long end = begin + share < total ? begin + share : total;
+      long long pos = begin;
+      int s = 0, head = 0, tile = 0;
+      TileSeq q;
+      q.n = q.tiles = 0;
+      UnitPart part;
+      part.open = 0;
+      if (pos < end) {
+        const int i = find_last(C::THREADS, begin, [&](int j) { return pre[j]; });
+        long long off = begin - pre[i];
+        for (s = i * seg;; ++s) {
+          q = tile_seq_of(p, s);
+          const long long c = q.n > 0 ? tile_chunks_before(p, q, q.tiles) * p.Hkv : 0;
+          if (off < c || s + 1 >= p.S) break;
+          off -= c;
+        }
+        const long long per_head = tile_chunks_before(p, q, q.tiles);
+        head = (int)(off / per_head);
+        off -= head * per_head;
+        int lo = 0, hi = q.tiles;                              // the last tile whose chunks begin at or before `off`
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) / 2;
+          if (tile_chunks_before(p, q, mid) <= off) lo = mid; else hi = mid;
+        }
+        tile = lo;
+        pos = begin - (off - tile_chunks_before(p, q, tile));  // where the first unit begins
+      }
+      bool ok = true;
+      uint32_t seq = 0;
+      const TileUnit none = {0, 0, 0, 0, 0, 0, -1, -1, -1, {0, 0}};
+      while (ok) {
+        TileUnit u = none;
+        if (pos < end) {
+          const int n = tile_chunks(p, q, tile), token = tile * 2 * p.tile_tokens;
+          u.lim0 = p.causal ? q.first + token : (long long)q.keys;
+          u.t0 = q.t0 + token;
+          u.tokens = min(2 * p.tile_tokens, q.n - token);
+          u.head = head;
+          u.s = s;
+          u.keys = q.keys;
+          u.c0 = pos < begin ? (int)(begin - pos) : 0;
+          u.c1 = pos + n > end ? (int)(end - pos) : n;
+          const bool starts = pos >= begin, ends = pos + n <= end;
+          u.slot = starts && ends ? -1 : 2 * (int)blockIdx.x + (starts ? 1 : 0);
+          if (starts && !ends) {
+            part.chunk0 = pos;
+            part.chunk1 = pos + n;
+            part.s = s;
+            part.unit = head * q.tiles + tile;
+            part.open = 1;
+            part.pad = 0;
+          }
+          pos += n;
+          if (++tile == q.tiles) {
+            tile = 0;
+            if (++head == p.Hkv) {
+              head = 0;
+              if (pos < end) {
+                do q = tile_seq_of(p, ++s); while (q.n == 0 && s + 1 < p.S);
+              }
+            }
+          }
+        }
+        const uint32_t slot = seq % C::NU;
+        if (seq >= C::NU) ok = wait(B_UE + slot, (seq / C::NU - 1) & 1u, TW_UEMPTY);
+        if (!ok) break;
+        if (lane == 0) {
+          units[slot] = u;
+          mbar_arrive(BAR(B_UF + slot));
+        }
+        ++seq;
+        if (u.c0 < 0) break;
+      }
+      if (lane == 0) {
+        p.units[blockIdx.x] = part;
+        if (blockIdx.x == 0) {
+          p.head[0] = gridDim.x;
+          p.head[1] = share;
+          p.head[2] = total;
+        }
+      }
+    } else if (warp == 0) {
+      // ------------------------------------------------------------------ TMA
+      uint32_t kit = 0, uit = 0;                               // chunks, units so far
+      uint32_t qit1 = 0;                                       // units with a second tile
+      const int box_rows = 1 << p.box_log, boxes = kTileKeys >> p.box_log;
+      const uint32_t sQ = smem_u32(smem + C::OFF_Q), sK = smem_u32(smem + C::OFF_K), sV8 = smem_u32(smem + C::OFF_V8);
+      const uint32_t q_box = (uint32_t)(p.tile_tokens * p.ratio * D);
+      TileUnit u;
+      bool ok = true;
+      while (ok && next_unit(u)) {
+        const int* table = p.table + (long long)u.s * p.table_stride;
+        const int two = u.tokens > p.tile_tokens;
+        for (int i = 0; i <= two && ok; ++i) {
+          const uint32_t n = i ? qit1 : uit;
+          ok = wait(B_QE + i, (n & 1u) ^ 1u, TW_QE);
+          if (ok && lane == 0) {
+            mbar_expect_tx(BAR(B_QF + i), q_box);
+            tma_load_4d(sQ + i * C::Q_BYTES, &tmQ, BAR(B_QF + i), 0, u.head * p.ratio, u.t0 + i * p.tile_tokens, 0);
+          }
+          __syncwarp();
+        }
+        ++uit;
+        qit1 += two;
+        // lane j: the page of box j of the next chunk
+        auto look_up = [&](int c) {
+          const int key = c * kTileKeys + lane * box_rows;
+          return lane < boxes && c < u.c1 && key < u.keys ? table[key >> p.page_log] : 0;
+        };
+        int next = look_up(u.c0);
+        for (int c = u.c0; c < u.c1 && ok; ++c, ++kit) {
+          int page = next;
+          next = look_up(c + 1);
+          if (bad_page(page)) {
+            if (p.status) atomicCAS(p.status, 0, kStatusBadIndex);
+            page = 0;
+          }
+          const int key0 = c * kTileKeys, full = max(0, min(boxes, (u.keys - key0 + box_rows - 1) >> p.box_log));
+          const int slot = (key0 + lane * box_rows) & page_mask;
+          const uint32_t bytes = (uint32_t)full * box_rows * D;
+          const uint32_t k = kit % C::NK, v = kit % C::NV8;
+          ok = wait(B_KE + k, ((kit / C::NK) & 1u) ^ 1u, TW_KE);
+          if (!ok) break;
+          if (lane == 0) mbar_expect_tx(BAR(B_KF + k), bytes);
+          __syncwarp();
+          if (lane < full) tma_load_4d(sK + k * C::K_BYTES + lane * box_rows * D, &tmK, BAR(B_KF + k), 0, slot, u.head, page);
+          __syncwarp();
+          ok = wait(B_V8E + v, ((kit / C::NV8) & 1u) ^ 1u, TW_V8E);
+          if (!ok) break;
+          if (lane == 0) mbar_expect_tx(BAR(B_V8F + v), bytes);
+          __syncwarp();
+          if (lane < full) tma_load_4d(sV8 + v * C::K_BYTES + lane * box_rows * D, &tmV, BAR(B_V8F + v), 0, slot, u.head, page);
+          __syncwarp();
+        }
+      }
+    } else if (warp == 1) {
+      // ------------------------------------------------------------------ MMA
+      const uint32_t sQ = smem_u32(smem + C::OFF_Q), sK = smem_u32(smem + C::OFF_K), sV = smem_u32(smem + C::OFF_V);
+      const uint64_t descQ = make_smem_desc(sQ, 16, 8 * D, C::SWZ_QK), descK = make_smem_desc(sK, 16, 8 * D, C::SWZ_QK);
+      const uint64_t descV = make_smem_desc(sV, D > 64 ? kTileKeys * 128 : 16, 8 * 128, kSwz128);
+      const uint64_t descArm = make_smem_desc(smem_u32(smem + C::OFF_ARM), 128, 256, 0);
+      uint32_t kit = 0, vit = 0, uit[2] = {0, 0}, pit[2] = {0, 0};       // chunks of K, of V; units, P tiles
+      TileUnit u;
+      bool ok = true;
+      while (ok && next_unit(u)) {
+        const int n = u.c1 - u.c0, two = u.tokens > p.tile_tokens;
+        for (int j = 0; j <= n && ok; ++j) {
+          const uint32_t k = kit % C::NK, v = vit % C::NV;
+          if (j < n) ok = wait(B_KF + k, (kit / C::NK) & 1u, TW_KF);
+          if (ok && j > 0) ok = wait(B_VF + v, (vit / C::NV) & 1u, TW_VF);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (!ok || i > two) continue;
+            const uint32_t tS = tmem + C::COL_S + i * kTileKeys, tO = tmem + C::COL_O + i * D;
+            if (j == 0) ok = wait(B_QF + i, uit[i] & 1u, TW_QF);
+            else ok = wait(B_P + i, pit[i] & 1u, TW_P);
+            if (!ok) continue;
+            if (j > 0) ++pit[i];
+            tc_fence_after();
+            if (elect_one()) {
+              // (the tensor core takes them in this order: S of the next chunk comes over P when the P V that reads it is done)
+              if (j > 0) {
+                const uint64_t vd = descV + (uint64_t)(v * (C::V_BYTES >> 4));
+#pragma unroll
+                for (int kk = 0; kk < kTileKeys / 16; ++kk)
+                  umma_f16_ts(tO, tS + kk * 8, vd + (uint64_t)(kk * ((16 * 128) >> 4)), C::IDESC_PV, j > 1 || kk > 0 ? 1u : 0u);
+              }
+              if (j < n) {
+                umma_f16(tS, descArm, descArm, C::IDESC_ARM, 0);
+#pragma unroll
+                for (int kk = 0; kk < D / 32; ++kk)
+                  umma_i8(tS, descQ + (uint64_t)(i * (C::Q_BYTES >> 4) + 2 * kk), descK + (uint64_t)(k * (C::K_BYTES >> 4) + 2 * kk), C::IDESC_QK, 1);
+                umma_commit(BAR(B_S + i));
+                if (j + 1 == n) umma_commit(BAR(B_QE + i));
+              } else {
+                umma_commit(BAR(B_O + i));
+              }
+              if (i == two) {
+                if (j < n) umma_commit(BAR(B_KE + k));
+                if (j > 0) umma_commit(BAR(B_VE + v));
+              }
+            }
+            __syncwarp();
+          }
+          if (j < n) ++kit;
+          if (j > 0) ++vit;
+        }
+        ++uit[0];
+        uit[1] += two;
+      }
+    } else {
+      // ------------------------------------------------------------------ scales
+      uint32_t it = 0;
+      TileUnit u;
+      bool ok = true;
+      while (ok && next_unit(u)) {
+        const int* table = p.table + (long long)u.s * p.table_stride;
+        const float* ks = p.ks + u.head * p.ksH;
+        const float* vs = p.vs + u.head * p.vsH;
+        int page[4];
+        auto look_up = [&](int c) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = c * kTileKeys + i * 32 + lane;
+            page[i] = c < u.c1 && key < u.keys ? table[key >> p.page_log] : -1;
+          }
+        };
+        look_up(u.c0);
+        for (int c = u.c0; c < u.c1 && ok; ++c, ++it) {
+          float a[4], b[4];
+          unsigned in = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int blk = ((c * kTileKeys + i * 32 + lane) & page_mask) >> p.block_log;
+            a[i] = 0.f;
+            b[i] = 1.f;
+            if (c * kTileKeys + i * 32 + lane < u.keys) {
+              const long long pg = bad_page(page[i]) ? 0 : page[i];
+              a[i] = ks[pg * p.ksP + blk * p.ksB];
+              b[i] = vs[pg * p.vsP + blk * p.vsB];
+              in |= 1u << i;
+            }
+          }
+          look_up(c + 1);
+          const uint32_t slot = it % C::NSC;
+          float* sc = reinterpret_cast<float*>(smem + C::OFF_SC) + slot * C::SC_FLOATS;
+          ok = wait(B_SCE + slot, ((it / C::NSC) & 1u) ^ 1u, TW_SCE);
+          if (!ok) break;
+          float lo = INFINITY, hi = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float l = log2_approx(b[i]);
+            sc[i * 32 + lane] = a[i];
+            sc[kTileKeys + i * 32 + lane] = l;
+            sc[2 * kTileKeys + i * 32 + lane] = 1.0f / b[i];
+            if (in >> i & 1u) {
+              const bool odd = !(fabsf(l) < INFINITY);         // zero, infinite, NaN: the general way
+              lo = fminf(lo, odd ? -INFINITY : l);
+              hi = fmaxf(hi, odd ? INFINITY : l);
+            }
+          }
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) {
+            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+          }
+          if (lane == 0) {
+            sc[3 * kTileKeys] = lo;
+            sc[3 * kTileKeys + 1] = hi;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(BAR(B_SCF + slot));
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp < 8) {
+    reg_dealloc<kTileConvert>();
+    // -------------------------------------------------------------------- V: int8 -> fp16
+    constexpr int PIECES = D / 16;                             // 16-byte pieces of a key's int8 channels
+    const int tid = threadIdx.x - 128;
+    const uint32_t sV8 = smem_u32(smem + C::OFF_V8), sV = smem_u32(smem + C::OFF_V);
+    uint32_t it = 0;
+    TileUnit u;
+    bool ok = true;
+    while (ok && next_unit(u)) {
+      for (int c = u.c0; c < u.c1 && ok; ++c, ++it) {
+        const uint32_t a = it % C::NV8, b = it % C::NV;
+        ok = wait(B_V8F + a, (it / C::NV8) & 1u, TW_V8F) && wait(B_VE + b, ((it / C::NV) & 1u) ^ 1u, TW_VE);
+        if (!ok) break;
+        const uint32_t src = sV8 + a * C::K_BYTES, dst = sV + b * C::V_BYTES;
+#pragma unroll 2
+        for (int i = tid; i < kTileKeys * PIECES; i += 128) {
+          const int key = i / PIECES, pc = i % PIECES;
+          const int sw = D == 128 ? key & 7 : (key >> 1) & 3;
+          const uint4 x = lds16(src + key * D + ((pc ^ sw) << 4));
+          const uint32_t w[4] = {x.x ^ 0x80808080u, x.y ^ 0x80808080u, x.z ^ 0x80808080u, x.w ^ 0x80808080u};
+          uint32_t h[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const uint32_t r = __byte_perm(w[k / 2], 0x64646464u, k & 1 ? 0x4342 : 0x4140);
+            const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&r), __half2half2(__ushort_as_half(0x6480)));
+            h[k] = *reinterpret_cast<const uint32_t*>(&y);
+          }
+          // channels pc*16 .. +15: chunks 2 (pc % 4) and the next of box pc / 4; the lanes of the second box begin with the other one, so
+          // that a row's eight stores lie in different banks
+          const int swap = (pc >> 2) & 1;
+          const uint32_t row = dst + (pc >> 2) * (kTileKeys * 128) + key * 128;
+          const int ch = (pc & 3) * 2;
+          const uint4 y0 = make_uint4(h[0], h[1], h[2], h[3]), y1 = make_uint4(h[4], h[5], h[6], h[7]);
+          const uint4 f = swap ? y1 : y0, g = swap ? y0 : y1;
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(row + (((ch + swap) ^ (key & 7)) << 4)), "r"(f.x), "r"(f.y), "r"(f.z), "r"(f.w) : "memory");
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(row + (((ch + 1 - swap) ^ (key & 7)) << 4)), "r"(g.x), "r"(g.y), "r"(g.z), "r"(g.w) : "memory");
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(BAR(B_VF + b));
+          mbar_arrive(BAR(B_V8E + a));
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    reg_alloc<kTileSoftmax>();
+    // -------------------------------------------------------------------- softmax, one thread a row
+    const int tile = (warp - 8) >> 2, rr = threadIdx.x & 127;
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;         // (lane 32 * (warp % 4) in bits 16 and up)
+    const uint32_t tS = tmem + C::COL_S + tile * kTileKeys + lanes, tO = tmem + C::COL_O + tile * D + lanes;
+    const int tok = tile * p.tile_tokens + rr / p.ratio, hr = rr % p.ratio;
+    uint32_t sit = 0, it = 0, oit = 0;                         // S tiles, chunks, units of this tile so far
+    TileUnit u;
+    bool ok = true;
+    while (ok && next_unit(u)) {
+      const bool work = tile == 0 || u.tokens > p.tile_tokens;
+      if (!work) {
+        for (int c = u.c0; c < u.c1 && ok; ++c, ++it) {
+          ok = wait(B_SCF + it % C::NSC, (it / C::NSC) & 1u, TW_SC);
+          if (lane == 0) mbar_arrive(BAR(B_SCE + it % C::NSC));
+        }
+        continue;
+      }
+      const bool mine = tok < u.tokens && rr < p.tile_tokens * p.ratio;
+      const int h = u.head * p.ratio + hr;
+      float qs = 0.f;
+      if (mine) qs = p.qs[(long long)(u.t0 + tok) * p.qsn + h * p.qsh] * p.c;
+      long long lim = u.keys - 1;
+      if (p.causal && mine) lim = min(lim, u.lim0 + tok);
+      float mref = -INFINITY, ref = -INFINITY, l = 0.f;        // references of p and of w (of the accumulator)
+      for (int c = u.c0; c < u.c1; ++c, ++it, ++sit) {
+        const uint32_t slot = it % C::NSC;
+        ok = wait(B_SCF + slot, (it / C::NSC) & 1u, TW_SC) && wait(B_S + tile, sit & 1u, TW_S);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t sc = smem_u32(smem + C::OFF_SC) + slot * (C::SC_FLOATS * 4);
+        const uint64_t qs2 = f2_pack(qs, qs), magic2 = f2_pack(-kMagicF, -kMagicF);
+        const long long rel64 = lim - (long long)c * kTileKeys;
+        const int rel = rel64 < -1 ? -1 : rel64 > kTileKeys ? kTileKeys : (int)rel64;        // the last column that the row sees
+        const bool masked = __any_sync(0xffffffffu, rel < kTileKeys - 1);
+        // ---- exponents of w: x + log2 v_scale
+        uint64_t xw[kTileKeys / 2];
+        float mx = -INFINITY;
+        uint32_t buf[2][32];
+        tmem_ld32(tS, buf[0]);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          tmem_ld_wait(buf[b & 1]);
+          if (b < 3) tmem_ld32(tS + (b + 1) * 32, buf[(b + 1) & 1]);
+#pragma unroll
+          for (int k = 0; k < 32; k += 4) {
+            const uint4 a = lds16(sc + (b * 32 + k) * 4), v = lds16(sc + (kTileKeys + b * 32 + k) * 4);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint64_t t = f2_add(f2_packu(buf[b & 1][k + 2 * e], buf[b & 1][k + 2 * e + 1]), magic2);
+              const uint64_t x = f2_fma(t, f2_mul(e ? f2_packu(a.z, a.w) : f2_packu(a.x, a.y), qs2), e ? f2_packu(v.z, v.w) : f2_packu(v.x, v.y));
+              xw[(b * 32 + k) / 2 + e] = x;
+              float x0, x1;
+              f2_unpack(x, x0, x1);
+              mx = max3(mx, x0, x1);
+            }
+          }
+        }
+        if (masked) {
+          mx = -INFINITY;
+#pragma unroll
+          for (int k = 0; k < kTileKeys / 2; ++k) {
+            float x0, x1;
+            f2_unpack(xw[k], x0, x1);
+            x0 = 2 * k <= rel ? x0 : -INFINITY;
+            x1 = 2 * k + 1 <= rel ? x1 : -INFINITY;
+            mx = max3(mx, x0, x1);
+            xw[k] = f2_pack(x0, x1);
+          }
+        }
+        // ---- references
+        const bool up = mx > ref + 8.f || (ref == -INFINITY && mx > -INFINITY);
+        if (__any_sync(0xffffffffu, up)) {
+          const float to = up ? mx : ref, f = ref == -INFINITY ? 0.f : ex2_approx(ref - to);
+          if (up && ref > -INFINITY) {
+            mref += to - ref;
+            l *= f;
+          }
+          ref = to;
+          if (c > u.c0) {                        // (the first P V does not look at what is there)
+            const uint64_t f2 = f2_pack(up ? f : 1.f, up ? f : 1.f);
+#pragma unroll 1
+            for (int b = 0; b < D / 32; ++b) {
+              uint32_t o[32];
+              tmem_ld32(tO + b * 32, o);
+              tmem_ld_wait(o);
+#pragma unroll
+              for (int k = 0; k < 32; k += 2) f2_unpacku(f2_mul(f2_packu(o[k], o[k + 1]), f2), o[k], o[k + 1]);
+              tmem_st32(tO + b * 32, o);
+            }
+          }
+        }
+        float lo, hi;
+        {
+          const float2 r = lds_f2(sc + 3 * kTileKeys * 4);
+          lo = r.x;
+          hi = r.y;
+        }
+        const float d = ref - mref;
+        const bool easy = ref == -INFINITY ? mref == -INFINITY && lo > -INFINITY : lo >= d - 60.f && hi <= d + 60.f;
+        const bool general = !__all_sync(0xffffffffu, easy);
+        if (general) {
+          // p by itself: the scores once more
+          float top = -INFINITY;
+#pragma unroll 1
+          for (int pass = 0; pass < 2; ++pass) {
+            float sum = 0.f;
+            const float base = safe(mref);
+#pragma unroll 1
+            for (int b = 0; b < 4; ++b) {
+              uint32_t o[32];
+              tmem_ld32(tS + b * 32, o);
+              tmem_ld_wait(o);
+#pragma unroll
+              for (int k = 0; k < 32; k += 4) {
+                const uint4 a = lds16(sc + (b * 32 + k) * 4);
+                const uint32_t aa[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  float x = (__uint_as_float(o[k + e]) - kMagicF) * (__uint_as_float(aa[e]) * qs);
+                  if (b * 32 + k + e > rel) x = -INFINITY;
+                  if (pass == 0) top = fmaxf(top, x);
+                  else sum += ex2_approx(x - base);
+                }
+              }
+            }
+            if (pass == 0) {
+              if (top > mref + 8.f || (mref == -INFINITY && top > -INFINITY)) {
+                l = mref == -INFINITY ? 0.f : l * ex2_approx(mref - top);
+                mref = top;
+              }
+            } else {
+              l += sum;
+            }
+          }
+        }
+        // ---- w, its sum over v_scale, P
+        const float base = safe(ref);
+        const uint64_t nb = f2_pack(-base, -base);
+        uint64_t sum = 0;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int k = 0; k < 16; k += 2) {
+            const uint4 iv = lds16(sc + (2 * kTileKeys + b * 32 + 2 * k) * 4);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float x0, x1;
+              f2_unpack(f2_add(xw[b * 16 + k + e], nb), x0, x1);
+              x0 = ex2_approx(x0);
+              x1 = ex2_approx(x1);
+              sum = f2_fma(f2_pack(x0, x1), e ? f2_packu(iv.z, iv.w) : f2_packu(iv.x, iv.y), sum);
+              const __half2 y = __floats2half2_rn(x0, x1);
+              pk[k + e] = *reinterpret_cast<const uint32_t*>(&y);
+            }
+          }
+          tmem_st16(tS + b * 16, pk);
+        }
+        if (!general && ref > -INFINITY) {
+          float s0, s1;
+          f2_unpack(sum, s0, s1);
+          l += (s0 + s1) * ex2_approx(ref - mref);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(BAR(B_P + tile));
+          mbar_arrive(BAR(B_SCE + slot));
+        }
+      }
+      if (!ok) break;
+      // ---- the unit's rows
+      ok = wait(B_O + tile, oit & 1u, TW_O);
+      ++oit;
+      if (!ok) break;
+      tc_fence_after();
+      const float f = u.slot < 0 ? row_factor(mref, ref, l) : 1.f;
+      const long long row = (long long)u.slot * (2 * kTileRows) + tile * kTileRows + rr;
+      uint16_t* o16 = static_cast<uint16_t*>(p.o) + (long long)(u.t0 + tok) * p.on + h * p.oh;
+#pragma unroll 1
+      for (int b = 0; b < D / 32; ++b) {
+        uint32_t o[32];
+        tmem_ld32(tO + b * 32, o);
+        tmem_ld_wait(o);
+        if (mine && u.slot < 0) {
+#pragma unroll
+          for (int k = 0; k < 32; k += 8) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float x0 = __uint_as_float(o[k + 2 * e]) * f, x1 = __uint_as_float(o[k + 2 * e + 1]) * f;
+              if (p.o_bf16) {
+                const __nv_bfloat162 y = __floats2bfloat162_rn(x0, x1);
+                w[e] = *reinterpret_cast<const uint32_t*>(&y);
+              } else {
+                const __half2 y = __floats2half2_rn(x0, x1);
+                w[e] = *reinterpret_cast<const uint32_t*>(&y);
+              }
+            }
+            *reinterpret_cast<uint4*>(o16 + b * 32 + k) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        } else if (mine) {
+#pragma unroll
+          for (int k = 0; k < 32; k += 4) *reinterpret_cast<uint4*>(p.part + row * D + b * 32 + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+        }
+        __syncwarp();
+      }
+      if (mine) {
+        if (u.slot >= 0) *reinterpret_cast<float4*>(p.part_ml + row * 4) = make_float4(mref, ref, l, 0.f);
+        else if (p.lse) p.lse[(long long)(u.t0 + tok) * p.H + h] = mref + log2f(l);
+      }
+      tc_fence_before();
+    }
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}

@@ -905,14 +905,15 @@ PyObject* paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
     at::Tensor lse = want_lse ? empty({T, H}, at::kFloat, dev) : at::Tensor();
     if (T > 0) {
       if (P.cache.table_width < 1) raise(PyExc_ValueError, "block_table has no columns");
-      const at::Tensor q = rows_ready(q0);
+      at::Tensor q = rows_ready(q0);
+      if (q.stride(0) <= 0 || q.stride(1) <= 0) q = q.contiguous();
       const at::Tensor s = qs.stride(0) >= 0 && qs.stride(1) >= 0 ? qs : qs.contiguous();
       P.q = q.data_ptr();
       P.q_scale = s.data_ptr<float>();
       P.o = out.data_ptr();
       P.lse_out = want_lse ? lse.data_ptr<float>() : nullptr;
       for (int i = 0; i < 2; ++i) {
-        P.q_stride[i] = q.stride(i);
+        P.q_stride[i] = q.size(i) == 1 && q.stride(i) <= 0 ? H * D : q.stride(i);
         P.qs_stride[i] = s.stride(i);
         P.o_stride[i] = out.size(i) <= 1 ? H * D : out.stride(i);
       }
