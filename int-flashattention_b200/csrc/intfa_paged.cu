@@ -13,7 +13,7 @@ namespace intfa {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxTokens = 16;           // tokens of a CTA: 32 rows at 64 channels, two tensors
+constexpr int kMaxTokens = 32;           // tokens of a CTA
 
 struct AppendJob {
   const void* x[3];                      // q, k, v: packed [tokens, heads, D]
@@ -26,7 +26,7 @@ struct AppendJob {
   const int* lens; const int* cu;
   int S, pages, page_log, block_log;
   long long tokens;
-  const float* rot_table; long long rot_rows; int rot, interleaved;
+  const float* rot_table; long long rot_rows; int rot;
   int* status;
 };
 
@@ -74,16 +74,19 @@ __device__ __forceinline__ Place place_of(const AppendJob& p, long long t) {
   return r;
 }
 
-// Rows of the tensors from `first` on, one CTA of `tokens_cta` tokens; each row has its own scale.
-template <typename T, int D, int FIRST, int COUNT>
-__device__ __forceinline__ void token_rows(const AppendJob& p, long long cta, int tokens_cta, Place* place) {
-  constexpr int LPR = D / 8, SLOTS = kThreads / LPR, U = 4;
-  const int e0 = threadIdx.x % LPR * 8, slot = threadIdx.x / LPR, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int per_token = SLOTS / tokens_cta, mine = slot / per_token, row0 = slot % per_token;
+// Rows of the tensors from FIRST on, tokens_cta tokens a CTA; each row has its own scale.  A slot (the lanes of a row) goes through several
+// rows of one token, two in flight; what it needs of the rotary table stays in registers for all of them.
+template <typename T, int D, int SPIN, int FIRST, int COUNT>
+__device__ __forceinline__ void token_rows(const AppendJob& p, long long cta, int tokens_cta, int per_token, Place* place) {
+  constexpr int LPR = D / 16, U = 2;
+  const int slot = threadIdx.x / LPR, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int mine = slot / per_token, row0 = slot % per_token;
   const long long token = cta * tokens_cta + mine;
-  const bool in = token < p.tokens;
+  const bool in = token < p.tokens && mine < tokens_cta;
   const int h0 = p.heads[FIRST], h1 = COUNT > 1 ? p.heads[FIRST + 1] : 0, rows = h0 + h1 + (COUNT > 2 ? p.heads[FIRST + 2] : 0);
-  Raw<T> raw[U];
+  Pieces at;
+  at.place<SPIN>(threadIdx.x % LPR, p.rot);
+  Row16<T> raw[U];
   auto split = [&](int r, int& w, int& h) {
     w = FIRST;
     h = r;
@@ -96,16 +99,19 @@ __device__ __forceinline__ void token_rows(const AppendJob& p, long long cta, in
       }
     }
   };
-  auto src = [&](int r) {
-    int w, h;
-    split(r, w, h);
-    return static_cast<const T*>(p.x[w]) + token * p.xn[w] + h * p.xh[w];
-  };
+  const T* base[3];
+#pragma unroll
+  for (int i = 0; i < 3; ++i) base[i] = i >= FIRST && i < FIRST + COUNT ? static_cast<const T*>(p.x[i]) + (in ? token : 0) * p.xn[i] : nullptr;
+  auto src = [&](int w, int h) { return (w == 0 ? base[0] : w == 1 ? base[1] : base[2]) + h * (w == 0 ? p.xh[0] : w == 1 ? p.xh[1] : p.xh[2]); };
   auto load = [&](int r) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       raw[u].zero();
-      if (in && r + u * per_token < rows) raw[u].load(src(r + u * per_token) + e0);
+      if (in && r + u * per_token < rows) {
+        int w, h;
+        split(r + u * per_token, w, h);
+        raw[u].load(src(w, h), at);
+      }
     }
   };
   load(row0);
@@ -114,14 +120,16 @@ __device__ __forceinline__ void token_rows(const AppendJob& p, long long cta, in
     if (lane == 0) place[i] = x;
   }
   __syncthreads();
-  const Place at = place[mine];
-  Turn turn;
-  const bool turns = p.rot_table != nullptr, pos_ok = !turns || (at.pos >= 0 && at.pos < p.rot_rows);
-  if (turns) {
-    turn.load(p.rot_table, pos_ok ? at.pos : 0, p.rot, p.interleaved, false, e0);
-    if (!pos_ok && at.own && threadIdx.x % (per_token * LPR) == 0) report(p);
+  const Place to = place[in ? mine : 0];
+  Turn<SPIN> turn;
+  bool goes = in && to.page >= 0;
+  if constexpr (SPIN != kNone) {
+    const bool pos_ok = to.pos >= 0 && to.pos < p.rot_rows;
+    turn.load(p.rot_table, pos_ok ? to.pos : 0, p.rot, false, at);
+    if (!pos_ok && in && to.own && threadIdx.x % LPR == 0 && row0 == 0) report(p);
+    goes = goes && pos_ok;
   }
-  const bool goes = in && at.page >= 0 && pos_ok;
+  // (every lane of a warp makes every round, for the shuffles)
   const int rounds = (rows + per_token * U - 1) / (per_token * U);
 #pragma unroll 1
   for (int k = 0; k < rounds; ++k) {
@@ -132,47 +140,45 @@ __device__ __forceinline__ void token_rows(const AppendJob& p, long long cta, in
       const int row = r + u * per_token;
       const bool row_ok = goes && row < rows;
       int w, h;
-      split(row, w, h);
-      float x[8];
-      widen(raw[u], x);
-      if (turns) turn.apply(x, raw[u], src(row_ok ? row : 0), row_ok, p.rot, p.interleaved, e0, w < 2);
-      const float s = scale_of(row_max<LPR>(absmax8(x)));
-      const uint2 c = codes8(x, s, __fdiv_rn(1.0f, s));
+      split(row < rows ? row : 0, w, h);
+      float x[16];
+      widen16(raw[u], x);
+      if (w < 2 && row_ok) turn.apply(x, src(w, h), p.rot, at);
+      const float s = scale_of(row_max<LPR>(absmax16(x)));
+      uint32_t c[4];
+      codes(x, s, c);
       if (row_ok) {
-        if (w == 0) {
-          *reinterpret_cast<uint2*>(p.q8 + (token * p.heads[0] + h) * D + e0) = c;
-          if (e0 == 0) p.qs[token * p.heads[0] + h] = s;
-        } else {
-          *reinterpret_cast<uint2*>(p.cache[w - 1] + at.page * p.cp[w - 1] + h * p.ch[w - 1] + at.slot * p.cn[w - 1] + e0) = c;
-          if (e0 == 0) p.scale[w - 1][at.page * p.sp[w - 1] + h * p.sh[w - 1] + at.slot * p.sb[w - 1]] = s;
-        }
+        int8_t* out = w == 0 ? p.q8 + (token * p.heads[0] + h) * D : p.cache[w - 1] + to.page * p.cp[w - 1] + h * p.ch[w - 1] + to.slot * p.cn[w - 1];
+        float* sc = w == 0 ? p.qs + token * p.heads[0] + h : p.scale[w - 1] + to.page * p.sp[w - 1] + h * p.sh[w - 1] + to.slot * p.sb[w - 1];
+        *reinterpret_cast<uint2*>(out + at.a) = make_uint2(c[0], c[1]);
+        *reinterpret_cast<uint2*>(out + at.b) = make_uint2(c[2], c[3]);
+        if (threadIdx.x % LPR == 0) *sc = s;
       }
     }
   }
 }
 
 // block = 1
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) append_tokens_kernel(const AppendJob p, int tokens_cta) {
+template <typename T, int D, int SPIN>
+__global__ void __launch_bounds__(kThreads, SPIN == kAny ? 2 : 3) append_tokens_kernel(const AppendJob p, int tokens_cta, int per_token) {
   __shared__ Place place[kMaxTokens];
   pdl_wait();
   pdl_launch();
-  if (p.q8) token_rows<T, D, 0, 3>(p, blockIdx.x, tokens_cta, place);
-  else token_rows<T, D, 1, 2>(p, blockIdx.x, tokens_cta, place);
+  token_rows<T, D, SPIN, 0, 3>(p, blockIdx.x, tokens_cta, per_token, place);
 }
 
 // block > 1.  CTAs 0 .. units * groups - 1: what one sequence adds to one block, `heads_cta` heads of K and V; the rest: q.
 // Unit u of sequence s: u = cu[s] / block + 2 s + i for the i-th block that the sequence touches (it touches at most n / block + 2).
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) append_blocks_kernel(const AppendJob p, int units, int groups, int heads_cta, int tokens_cta) {
-  constexpr int LPR = D / 8, SLOTS = kThreads / LPR;
+template <typename T, int D, int SPIN>
+__global__ void __launch_bounds__(kThreads, 2) append_blocks_kernel(const AppendJob p, int units, int groups, int heads_cta, int tokens_cta, int per_token) {
+  constexpr int LPR = D / 16, SLOTS = kThreads / LPR;
   __shared__ Place place[kMaxTokens];
   __shared__ unsigned int most[2 * kThreads];        // [K, V][heads_cta]
   __shared__ float s_old[2 * kThreads], s_new[2 * kThreads];
   pdl_wait();
   pdl_launch();
   if ((long long)blockIdx.x >= (long long)units * groups) {
-    token_rows<T, D, 0, 1>(p, (long long)blockIdx.x - (long long)units * groups, tokens_cta, place);
+    token_rows<T, D, SPIN, 0, 1>(p, (long long)blockIdx.x - (long long)units * groups, tokens_cta, per_token, place);
     return;
   }
   const int u = blockIdx.x / groups, head0 = (blockIdx.x - u * groups) * heads_cta;
@@ -198,13 +204,14 @@ __global__ void __launch_bounds__(kThreads) append_blocks_kernel(const AppendJob
     return;
   }
   const int slot0 = (int)(b0 & ((1 << p.page_log) - 1)), blk = slot0 >> p.block_log;
-  const int e0 = threadIdx.x % LPR * 8, slot = threadIdx.x / LPR;
+  const int slot = threadIdx.x / LPR;
+  Pieces at;
+  at.place<SPIN>(threadIdx.x % LPR, p.rot);
   for (int i = threadIdx.x; i < 2 * nh; i += kThreads) most[i] = 0u;
   __syncthreads();
   const int nt = (int)(n1 - n0), rows = nt * nh * 2, rounds = (rows + SLOTS - 1) / SLOTS;
   // row r: token r / (2 nh), then K's heads and V's
-  Turn turn;
-  float x[8];
+  float x[16];
   auto fetch = [&](int k, int& token, int& wh) {
     const int r = k * SLOTS + slot;
     const bool ok = r < rows;
@@ -212,13 +219,14 @@ __global__ void __launch_bounds__(kThreads) append_blocks_kernel(const AppendJob
     wh = ok ? r - token * 2 * nh : 0;
     const int w = wh >= nh ? 1 : 0, h = head0 + wh - (w ? nh : 0);
     const T* row = static_cast<const T*>(p.x[1 + w]) + (t0 + (n0 - first) + token) * p.xn[1 + w] + h * p.xh[1 + w];
-    Raw<T> raw;
+    Row16<T> raw;
     raw.zero();
-    if (ok) raw.load(row + e0);
-    widen(raw, x);
-    if (p.rot_table) {
-      turn.load(p.rot_table, n0 + token, p.rot, p.interleaved, false, e0);
-      turn.apply(x, raw, row, ok, p.rot, p.interleaved, e0, w == 0);
+    if (ok) raw.load(row, at);
+    widen16(raw, x);
+    if (SPIN != kNone && ok && w == 0) {
+      Turn<SPIN> turn;
+      turn.load(p.rot_table, n0 + token, p.rot, false, at);
+      turn.apply(x, row, p.rot, at);
     }
     return ok;
   };
@@ -227,8 +235,8 @@ __global__ void __launch_bounds__(kThreads) append_blocks_kernel(const AppendJob
 #pragma unroll 1
   for (int k = 0; k < rounds; ++k) {
     ok = fetch(k, token, wh);
-    const float m = row_max<LPR>(absmax8(x));
-    if (ok && e0 == 0) atomicMax(&most[wh], __float_as_uint(m));       // (not negative, a NaN above all: they compare as whole numbers)
+    const float m = row_max<LPR>(absmax16(x));
+    if (ok && threadIdx.x % LPR == 0) atomicMax(&most[wh], __float_as_uint(m));       // (not negative, a NaN above all: they compare as whole numbers)
   }
   __syncthreads();
   for (int i = threadIdx.x; i < 2 * nh; i += kThreads) {
@@ -245,9 +253,11 @@ __global__ void __launch_bounds__(kThreads) append_blocks_kernel(const AppendJob
     if (rounds > 1) ok = fetch(k, token, wh);
     if (!ok) continue;
     const int w = wh >= nh ? 1 : 0, h = head0 + wh - (w ? nh : 0);
-    const float sc = s_new[wh];
-    *reinterpret_cast<uint2*>(p.cache[w] + page * p.cp[w] + h * p.ch[w] + (slot0 + (int)(n0 - b0) + token) * p.cn[w] + e0) =
-        codes8(x, sc, __fdiv_rn(1.0f, sc));
+    uint32_t c[4];
+    codes(x, s_new[wh], c);
+    int8_t* out = p.cache[w] + page * p.cp[w] + h * p.ch[w] + (slot0 + (int)(n0 - b0) + token) * p.cn[w];
+    *reinterpret_cast<uint2*>(out + at.a) = make_uint2(c[0], c[1]);
+    *reinterpret_cast<uint2*>(out + at.b) = make_uint2(c[2], c[3]);
   }
   if (!began) return;
   const int older = (int)(n0 - b0) * nh * 2;
@@ -256,39 +266,50 @@ __global__ void __launch_bounds__(kThreads) append_blocks_kernel(const AppendJob
     const int tk = r / (2 * nh), i = r - tk * 2 * nh, w = i >= nh ? 1 : 0, h = head0 + i - (w ? nh : 0);
     const float was = s_old[i], now = s_new[i];
     if (__float_as_uint(was) == __float_as_uint(now)) continue;
-    uint2* at = reinterpret_cast<uint2*>(p.cache[w] + page * p.cp[w] + h * p.ch[w] + (slot0 + tk) * p.cn[w] + e0);
-    const uint2 c = *at;
+    uint4* out = reinterpret_cast<uint4*>(p.cache[w] + page * p.cp[w] + h * p.ch[w] + (slot0 + tk) * p.cn[w] + threadIdx.x % LPR * 16);
+    const uint4 c = *out;
+    const uint32_t cw[4] = {c.x, c.y, c.z, c.w};
     const float ratio = now > 0.f && now <= 3.402823466e38f ? __fdiv_rn(was, now) : 0.f;
-    float y[8];
+    uint32_t b[16], o[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = __fmul_rn((float)(int8_t)((j < 4 ? c.x : c.y) >> (8 * (j & 3))), ratio);
-    *at = codes8(y, 1.0f, 1.0f);
+    for (int j = 0; j < 16; ++j) b[j] = __float_as_uint(__fadd_rn(__fmul_rn((float)(int8_t)(cw[j / 4] >> (8 * (j & 3))), ratio), 12582912.0f));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = __byte_perm(__byte_perm(b[4 * j], b[4 * j + 1], 0x0040), __byte_perm(b[4 * j + 2], b[4 * j + 3], 0x0040), 0x5410);
+    *out = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, int SPIN>
 int run(const AppendJob& p, cudaStream_t stream) {
-  constexpr int SLOTS = kThreads / (D / 8);
-  auto tokens_of = [&](int heads) {
-    int n = 1;
-    while (n * 2 * heads <= SLOTS) n *= 2;
-    return n < kMaxTokens ? n : kMaxTokens;
+  constexpr int SLOTS = kThreads / (D / 16);
+  // Slots a token: one for about 6 rows, but as many as there are rows where that leaves SMs without work (a decode step)
+  auto slots_of = [&](int heads) {
+    int n = (heads + 5) / 6;
+    while (n < heads && n < SLOTS && p.tokens * n < 3LL * SLOTS * sm_count_cached()) ++n;
+    if (n < (SLOTS + kMaxTokens - 1) / kMaxTokens) n = (SLOTS + kMaxTokens - 1) / kMaxTokens;
+    return n < SLOTS ? n : SLOTS;
   };
   if (p.block_log == 0) {
-    const int n = tokens_of(p.heads[0] + p.heads[1] + p.heads[2]);
+    const int per = slots_of(p.heads[0] + p.heads[1] + p.heads[2]), n = SLOTS / per;
     const long long grid = (p.tokens + n - 1) / n;
     if (grid > 0x7fffffffLL) return set_error(INTFA_ERR_TOO_LARGE, "too many tokens");
-    return launch_kernel("append", append_tokens_kernel<T, D>, (unsigned)grid, kThreads, 0, stream, p, n);
+    return launch_kernel("append", append_tokens_kernel<T, D, SPIN>, (unsigned)grid, kThreads, 0, stream, p, n, per);
   }
-  // Heads a CTA: about 4 rounds of rows where the block is short, so that a step of one token has all its heads in one CTA or two
-  int heads_cta = 4 * SLOTS / (2 << p.block_log);
+  // Heads a CTA: one or two rounds of rows, so that a step of one token has all its heads in one CTA
+  int heads_cta = 2 * SLOTS / (2 << p.block_log);
   if (heads_cta < 1) heads_cta = 1;
   if (heads_cta > p.heads[1]) heads_cta = p.heads[1];
   if (heads_cta > kThreads) heads_cta = kThreads;
-  const int groups = (p.heads[1] + heads_cta - 1) / heads_cta, n = p.q8 ? tokens_of(p.heads[0]) : 1;
+  const int groups = (p.heads[1] + heads_cta - 1) / heads_cta, per = p.q8 ? slots_of(p.heads[0]) : SLOTS, n = SLOTS / per;
   const long long units = (p.tokens >> p.block_log) + 2LL * p.S, grid = units * groups + (p.q8 ? (p.tokens + n - 1) / n : 0);
   if (grid > 0x7fffffffLL) return set_error(INTFA_ERR_TOO_LARGE, "too many tokens");
-  return launch_kernel("append", append_blocks_kernel<T, D>, (unsigned)grid, kThreads, 0, stream, p, (int)units, groups, heads_cta, n);
+  return launch_kernel("append", append_blocks_kernel<T, D, SPIN>, (unsigned)grid, kThreads, 0, stream, p, (int)units, groups, heads_cta, n, per);
+}
+template <typename T, int D>
+int run_spin(const AppendJob& p, bool interleaved, cudaStream_t stream) {
+  if (!p.rot_table) return run<T, D, kNone>(p, stream);
+  if (interleaved) return run<T, D, kPairs>(p, stream);
+  return p.rot % 16 == 0 ? run<T, D, kHalf>(p, stream) : run<T, D, kAny>(p, stream);
 }
 
 int log2_of(long long n) {
@@ -335,13 +356,12 @@ int paged_append(const IntfaAppendParams* a, cudaStream_t stream) {
   p.rot_table = a->table;
   p.rot_rows = a->table_rows;
   p.rot = a->rot_dim;
-  p.interleaved = a->interleaved;
   p.status = a->status;
-  const bool f16 = a->dtype == INTFA_TYPE_FP16;
+  const bool f16 = a->dtype == INTFA_TYPE_FP16, pairs = a->interleaved != 0;
   switch (c.D) {
-    case 64: return f16 ? run<__half, 64>(p, stream) : run<__nv_bfloat16, 64>(p, stream);
-    case 128: return f16 ? run<__half, 128>(p, stream) : run<__nv_bfloat16, 128>(p, stream);
-    default: return f16 ? run<__half, 256>(p, stream) : run<__nv_bfloat16, 256>(p, stream);
+    case 64: return f16 ? run_spin<__half, 64>(p, pairs, stream) : run_spin<__nv_bfloat16, 64>(p, pairs, stream);
+    case 128: return f16 ? run_spin<__half, 128>(p, pairs, stream) : run_spin<__nv_bfloat16, 128>(p, pairs, stream);
+    default: return f16 ? run_spin<__half, 256>(p, pairs, stream) : run_spin<__nv_bfloat16, 256>(p, pairs, stream);
   }
 }
 

@@ -1,9 +1,9 @@
 // Rotary positions of one or two tensors (q, and k with it) in one launch; the gradient of a rotation is the rotation back.
 //
-// Moves each value once in and once out (2 * 84 million bf16 values in 52.6 us at the measured copy rate): bound by HBM.  A CTA takes
-// one token, or a few where a token has few heads: all its heads share the (cos, sin) of the position, which each lane reads once for
-// its 8 channels and keeps in registers; the other half of a pair is in another lane of the row and comes by shuffles.  The next rows
-// are loaded ahead of the table, so that the way from the position to its (cos, sin) overlaps them.
+// Moves each value once in and once out (2 * 84 million bf16 values: 340 MB, 52.6 us at the measured copy rate): bound by HBM.  All heads of
+// a token share the (cos, sin) of its position: a slot (the lanes that hold a row) reads what it needs of the table once, keeps it in
+// registers and goes through several heads of one token, a few rows in flight.  The first rows are asked for ahead of the table, so
+// that the way from the position to its (cos, sin) overlaps them.
 #include "intfa_rows.cuh"
 
 namespace intfa {
@@ -16,87 +16,87 @@ struct RotaryJob {
   long long xb[2], xh[2], xn[2], yb[2], yh[2], yn[2];
   int heads0, heads;                    // of the first tensor, of both
   long long tokens;
-  int N, rot, interleaved, inverse, pos64;
+  int N, rot, inverse, pos64;
   const float* table; long long rows;
   const void* pos; long long pos_b;
-  int tokens_cta;                       // a power of two
+  int lpr_log;                          // lanes of a row, D/16
+  int per_token;                        // slots that share a token
   int* status;
 };
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryJob p) {
-  constexpr int LPR = D / 8, SLOTS = kThreads / LPR, U = sizeof(T) == 4 ? 2 : 4;      // U: rows in flight
-  const int lane_e = threadIdx.x % LPR * 8, slot = threadIdx.x / LPR;
-  const int per_token = SLOTS / p.tokens_cta;
-  const long long token = (long long)blockIdx.x * p.tokens_cta + slot / per_token;
-  const int row0 = slot % per_token;
+template <typename T, int SPIN>
+__global__ void __launch_bounds__(kThreads, SPIN == kAny ? 2 : 3) rotary_kernel(const RotaryJob p) {
+  constexpr int U = sizeof(T) == 4 ? 1 : 2;                  // rows in flight
+  const int slot = threadIdx.x >> p.lpr_log, slots = kThreads >> p.lpr_log;
+  const int row0 = slot % p.per_token;
+  const long long token = (long long)blockIdx.x * (slots / p.per_token) + slot / p.per_token;
   pdl_wait();
   pdl_launch();
-  const bool token_ok = token < p.tokens;
-  const long long tok = token_ok ? token : 0;
-  const int b = (int)(tok / p.N), n = (int)(tok - (long long)b * p.N);
-  Raw<T> in[U];
-  auto src = [&](int r) {
-    const int w = r >= p.heads0, h = w ? r - p.heads0 : r;
-    return static_cast<const T*>(p.x[w]) + b * p.xb[w] + h * p.xh[w] + n * p.xn[w];
-  };
-  auto dst = [&](int r) {
-    const int w = r >= p.heads0, h = w ? r - p.heads0 : r;
-    return static_cast<T*>(p.y[w]) + b * p.yb[w] + h * p.yh[w] + n * p.yn[w];
-  };
+  if (token >= p.tokens || slot / p.per_token >= slots / p.per_token) return;
+  const int b = (int)(token / p.N), n = (int)(token - (long long)b * p.N);
+  Pieces at;
+  at.place<SPIN>(threadIdx.x & ((1 << p.lpr_log) - 1), p.rot);
+  const T* x0 = static_cast<const T*>(p.x[0]) + b * p.xb[0] + n * p.xn[0];
+  const T* x1 = static_cast<const T*>(p.x[1]) + b * p.xb[1] + n * p.xn[1] - p.heads0 * p.xh[1];
+  T* y0 = static_cast<T*>(p.y[0]) + b * p.yb[0] + n * p.yn[0];
+  T* y1 = static_cast<T*>(p.y[1]) + b * p.yb[1] + n * p.yn[1] - p.heads0 * p.yh[1];
+  auto src = [&](int r) { return r < p.heads0 ? x0 + r * p.xh[0] : x1 + r * p.xh[1]; };
+  auto dst = [&](int r) { return r < p.heads0 ? y0 + r * p.yh[0] : y1 + r * p.yh[1]; };
+  Row16<T> in[U];
   auto load = [&](int r) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      in[u].zero();
-      if (token_ok && r + u * per_token < p.heads) in[u].load(src(r + u * per_token) + lane_e);
-    }
+    for (int u = 0; u < U; ++u)
+      if (r + u * p.per_token < p.heads) in[u].load(src(r + u * p.per_token), at);
   };
   load(row0);
   const long long pi = b * p.pos_b + n;
-  const long long at = p.pos64 ? static_cast<const long long*>(p.pos)[pi] : static_cast<const int*>(p.pos)[pi];
-  const bool ok = at >= 0 && at < p.rows;
-  if (!ok && token_ok && p.status && lane_e == 0 && row0 == 0) atomicCAS(p.status, 0, kStatusBadIndex);
-  Turn turn;
-  turn.load(p.table, ok ? at : 0, p.rot, p.interleaved, p.inverse, lane_e);
-  // (every lane of a warp makes every round, for the shuffles)
-  const int rounds = (p.heads + per_token * U - 1) / (per_token * U);
+  const long long pos = p.pos64 ? static_cast<const long long*>(p.pos)[pi] : static_cast<const int*>(p.pos)[pi];
+  const bool ok = pos >= 0 && pos < p.rows;
+  if (!ok && p.status) atomicCAS(p.status, 0, kStatusBadIndex);
+  Turn<SPIN> turn;
+  turn.load(p.table, ok ? pos : 0, p.rot, p.inverse, at);
 #pragma unroll 1
-  for (int k = 0; k < rounds; ++k) {
-    const int r = row0 + k * per_token * U;
-    if (k > 0) load(r);
+  for (int r = row0; r < p.heads; r += U * p.per_token) {
+    if (r != row0) load(r);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int row = r + u * per_token;
-      const bool row_ok = token_ok && row < p.heads;
-      float x[8];
-      widen(in[u], x);
-      turn.apply(x, in[u], src(row_ok ? row : 0), row_ok, p.rot, p.interleaved, lane_e);
-      if (row_ok) {
-        Raw<T> out;
-        narrow(x, out);
-        if (lane_e >= p.rot) out = in[u];        // (as it is, a NaN's bits too)
-        if (!ok) out.zero();
-        out.store(dst(row) + lane_e);
+      const int row = r + u * p.per_token;
+      if (row >= p.heads) break;
+      float x[16];
+      widen16(in[u], x);
+      turn.apply(x, src(row), p.rot, at);
+      Raw<T> a, c;
+      narrow(reinterpret_cast<const float(&)[8]>(x[0]), a);
+      narrow(reinterpret_cast<const float(&)[8]>(x[8]), c);
+      // (what is not rotated as it is, a NaN's bits too)
+      if (at.a >= p.rot) a = in[u].a;
+      if (at.b >= p.rot) c = in[u].b;
+      if (!ok) {
+        a.zero();
+        c.zero();
       }
+      a.store(dst(row) + at.a);
+      c.store(dst(row) + at.b);
     }
   }
 }
 
 template <typename T>
-int run(const RotaryJob& job, int D, cudaStream_t stream) {
+int run(const RotaryJob& job, int D, bool interleaved, cudaStream_t stream) {
   RotaryJob p = job;
-  const int slots = kThreads / (D / 8);
-  p.tokens_cta = 1;
-  while (p.tokens_cta * 2 * p.heads <= slots) p.tokens_cta *= 2;
-  const long long grid = (p.tokens + p.tokens_cta - 1) / p.tokens_cta;
+  p.lpr_log = 0;
+  while ((16 << p.lpr_log) < D) ++p.lpr_log;
+  const int slots = kThreads >> p.lpr_log;
+  // Slots a token: one for about 8 heads, so that the table and the position are paid for by 8 rows, but as many as there are
+  // heads where that leaves SMs without work (a decode step)
+  p.per_token = (p.heads + 7) / 8;
+  while (p.per_token < p.heads && p.per_token < slots && p.tokens * p.per_token < 4LL * slots * sm_count_cached()) ++p.per_token;
+  if (p.per_token > slots) p.per_token = slots;
+  const int tokens_cta = slots / p.per_token;
+  const long long grid = (p.tokens + tokens_cta - 1) / tokens_cta;
   if (grid > 0x7fffffffLL) return set_error(INTFA_ERR_TOO_LARGE, "too many tokens");
-  switch (D) {
-    case 16: return launch_kernel("rotary", rotary_kernel<T, 16>, (unsigned)grid, kThreads, 0, stream, p);
-    case 32: return launch_kernel("rotary", rotary_kernel<T, 32>, (unsigned)grid, kThreads, 0, stream, p);
-    case 64: return launch_kernel("rotary", rotary_kernel<T, 64>, (unsigned)grid, kThreads, 0, stream, p);
-    case 128: return launch_kernel("rotary", rotary_kernel<T, 128>, (unsigned)grid, kThreads, 0, stream, p);
-    default: return launch_kernel("rotary", rotary_kernel<T, 256>, (unsigned)grid, kThreads, 0, stream, p);
-  }
+  auto go = [&](auto kernel) { return launch_kernel("rotary", kernel, (unsigned)grid, kThreads, 0, stream, p); };
+  return interleaved ? go(rotary_kernel<T, kPairs>) : p.rot % 16 == 0 ? go(rotary_kernel<T, kHalf>) : go(rotary_kernel<T, kAny>);
 }
 
 }  // namespace
@@ -117,7 +117,6 @@ int rotary(const IntfaRotaryParams* a, cudaStream_t stream) {
   p.N = a->N;
   p.tokens = (long long)a->B * a->N;
   p.rot = a->rot_dim;
-  p.interleaved = a->interleaved;
   p.inverse = a->inverse;
   p.pos64 = a->positions_i64;
   p.table = a->table;
@@ -125,8 +124,8 @@ int rotary(const IntfaRotaryParams* a, cudaStream_t stream) {
   p.pos = a->positions;
   p.pos_b = a->positions_stride;
   p.status = a->status;
-  return a->dtype == INTFA_TYPE_FP16 ? run<__half>(p, a->D, stream)
-         : a->dtype == INTFA_TYPE_BF16 ? run<__nv_bfloat16>(p, a->D, stream) : run<float>(p, a->D, stream);
+  return a->dtype == INTFA_TYPE_FP16 ? run<__half>(p, a->D, a->interleaved, stream)
+         : a->dtype == INTFA_TYPE_BF16 ? run<__nv_bfloat16>(p, a->D, a->interleaved, stream) : run<float>(p, a->D, a->interleaved, stream);
 }
 
 }  // namespace intfa

@@ -1,5 +1,5 @@
-// Rows of one head of one token: loading, rotating and quantising them, a lane holding 8 neighbouring channels
-// (so D/8 lanes, 2 to 32, hold a row).  Shared by the rotation and the paged cache's append.
+// Rows of one head of one token: loading, rotating and quantising them, a lane holding two pieces of 8 channels
+// (so D/16 lanes, 1 to 16, hold a row).  Shared by the rotation and the paged cache's append.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -72,88 +72,115 @@ __device__ __forceinline__ float widen1(T x) {
   else return __bfloat162float(x);
 }
 
-// The rotation of one lane's 8 channels at one position: pair j of the first rot channels, (a, b) = channels (j, j + rot/2), or
-// (2j, 2j + 1) interleaved, becomes (a c - b s, b c + a s) with (c, s) = table[position][j].  The products are rounded one by one (no
-// fma): the same bits as the same expression in single tensor operations.
-// What a lane needs of the table stays in registers for all heads of the token.
+// How a row is rotated.  kHalf: pair j is channels (j, j + rot/2), rot a multiple of 16; kAny: the same for other rot, element by element
+// with the partner read from memory once more; kPairs: channels (2j, 2j + 1).
+enum Spin { kNone, kHalf, kAny, kPairs };
+
+// Which 16 channels of a row lane j of D/16 holds, as two pieces of 8.  kHalf: both halves of the same pairs, so that a rotation stays
+// within the lane; the pieces that are not rotated two by two.  Else neighbours.
+struct Pieces {
+  int a, b;                          // first channel of each
+  template <int SPIN>
+  __device__ __forceinline__ void place(int j, int rot) {
+    const int h8 = rot >> 4;
+    if (SPIN == kHalf) {
+      a = j < h8 ? 8 * j : 16 * j;   // (16 h8 + 16 (j - h8))
+      b = j < h8 ? 8 * (j + h8) : a + 8;
+    } else {
+      a = 16 * j;
+      b = a + 8;
+    }
+  }
+};
+template <typename T>
+struct Row16 {
+  Raw<T> a, b;
+  __device__ __forceinline__ void load(const T* row, const Pieces& at) {
+    a.load(row + at.a);
+    b.load(row + at.b);
+  }
+  __device__ __forceinline__ void zero() {
+    a.zero();
+    b.zero();
+  }
+};
+template <typename T>
+__device__ __forceinline__ void widen16(const Row16<T>& r, float (&x)[16]) {
+  widen(r.a, reinterpret_cast<float(&)[8]>(x[0]));
+  widen(r.b, reinterpret_cast<float(&)[8]>(x[8]));
+}
+
+// The rotation of a lane's channels at one position: (a, b) of pair j becomes (a c - b s, b c + a s) with (c, s) = table[position][j].
+// The products are rounded one by one (no fma, and no packed pairs, which the compiler does contract): the same bits as the same expression
+// in single tensor operations.  What a lane needs of the table stays in registers for all heads of the token.
+template <int SPIN>
 struct Turn {
-  float c[8], s[8];                  // half layout: of the lane's channels; interleaved: of its 4 pairs (the first 4)
-  int kind;                          // 0: not rotated; 1, 2: half layout, the lane holds the a's, the b's; 3: interleaved; 4: half layout whose
-                                     // border lies inside a lane's 8 channels (rot no multiple of 16): element by element
-  __device__ __forceinline__ void load(const float* table, long long pos, int rot, bool interleaved, bool inverse, int e0) {
+  float c[SPIN == kAny ? 16 : 8], s[SPIN == kAny ? 16 : 8];      // kHalf: of the lane's 8 pairs; kPairs: 4 of each piece; kAny: of its channels
+  __device__ __forceinline__ void load(const float* table, long long pos, int rot, bool inverse, const Pieces& at) {
+    if constexpr (SPIN == kNone) return;
     const int half = rot >> 1;
     const float2* row = reinterpret_cast<const float2*>(table) + pos * half;
-    kind = 0;
+    auto put = [&](int i, float2 f) {
+      c[i] = f.x;
+      s[i] = inverse ? -f.y : f.y;
+    };
+    if constexpr (SPIN == kHalf) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = s[i] = 0.f;
-    if (e0 >= rot) {
-      if (!interleaved && (half & 7)) kind = 4;        // (its lanes all take the same way)
-    } else if (interleaved) {
-      kind = 3;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 f = e0 + 2 * i < rot ? row[(e0 >> 1) + i] : make_float2(1.f, 0.f);
-        c[i] = f.x;
-        s[i] = inverse ? -f.y : f.y;
-      }
-    } else if ((half & 7) == 0) {
-      kind = e0 < half ? 1 : 2;
-      const float4* r4 = reinterpret_cast<const float4*>(row + (e0 < half ? e0 : e0 - half));
+      for (int i = 0; i < 8; ++i) c[i] = s[i] = 0.f;
+      if (at.a >= half) return;
+      const float4* r4 = reinterpret_cast<const float4*>(row + at.a);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float4 f = r4[i];
-        c[2 * i] = f.x; s[2 * i] = inverse ? -f.y : f.y;
-        c[2 * i + 1] = f.z; s[2 * i + 1] = inverse ? -f.w : f.w;
+        put(2 * i, make_float2(f.x, f.y));
+        put(2 * i + 1, make_float2(f.z, f.w));
       }
-    } else {
-      kind = 4;
+    } else if constexpr (SPIN == kPairs) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int e = e0 + i;
-        const float2 f = e < rot ? row[e < half ? e : e - half] : make_float2(1.f, 0.f);
-        c[i] = f.x;
-        s[i] = inverse ? -f.y : f.y;
+        const int e = (i < 4 ? at.a : at.b) + 2 * (i & 3);
+        put(i, e < rot ? row[e >> 1] : make_float2(1.f, 0.f));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int e = (i < 8 ? at.a : at.b) + (i & 7);
+        put(i, e < rot ? row[e < half ? e : e - half] : make_float2(1.f, 0.f));
       }
     }
   }
-  // x: the lane's channels, r: as loaded, row: the row in memory, e0: the lane's first channel.  All lanes of the warp call this together;
-  // a row with turn = false is left alone.
+  // x: the lane's channels; row: the row in memory
   template <typename T>
-  __device__ __forceinline__ void apply(float (&x)[8], const Raw<T>& r, const T* row, bool row_ok, int rot, bool interleaved, int e0, bool turn = true) const {
-    const int kind = turn ? this->kind : 0;
-    if (interleaved) {
-      if (kind == 3) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (e0 + 2 * i >= rot) break;
-          const float a = x[2 * i], b = x[2 * i + 1];
-          x[2 * i] = __fsub_rn(__fmul_rn(a, c[i]), __fmul_rn(b, s[i]));
-          x[2 * i + 1] = __fadd_rn(__fmul_rn(b, c[i]), __fmul_rn(a, s[i]));
-        }
-      }
-      return;
-    }
+  __device__ __forceinline__ void apply(float (&x)[16], const T* row, int rot, const Pieces& at) const {
     const int half = rot >> 1;
-    float y[8];
-    if ((half & 7) == 0) {
-      const int lane = threadIdx.x & 31, other = kind == 1 ? lane + (half >> 3) : kind == 2 ? lane - (half >> 3) : lane;
-      Raw<T> o;
-#pragma unroll
-      for (int i = 0; i < Raw<T>::W; ++i) o.w[i] = __shfl_sync(0xffffffffu, r.w[i], other);
-      widen(o, y);
-    } else {
+    if constexpr (SPIN == kHalf) {
+      if (at.a >= half) return;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int e = e0 + i;
-        y[i] = row_ok && e < rot ? widen1(row[e < half ? e + half : e - half]) : 0.f;
+        const float a = x[i], b = x[8 + i];
+        x[i] = __fsub_rn(__fmul_rn(a, c[i]), __fmul_rn(b, s[i]));
+        x[8 + i] = __fadd_rn(__fmul_rn(b, c[i]), __fmul_rn(a, s[i]));
       }
-    }
+    } else if constexpr (SPIN == kPairs) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float p = __fmul_rn(x[i], c[i]), q = __fmul_rn(y[i], s[i]);
-      if (kind == 1) x[i] = __fsub_rn(p, q);
-      else if (kind == 2) x[i] = __fadd_rn(p, q);
-      else if (kind == 4 && e0 + i < rot) x[i] = e0 + i < half ? __fsub_rn(p, q) : __fadd_rn(p, q);
+      for (int i = 0; i < 8; ++i) {
+        const int e = (i < 4 ? at.a : at.b) + 2 * (i & 3), k = 2 * i;
+        if (e < rot) {
+          const float a = x[k], b = x[k + 1];
+          x[k] = __fsub_rn(__fmul_rn(a, c[i]), __fmul_rn(b, s[i]));
+          x[k + 1] = __fadd_rn(__fmul_rn(b, c[i]), __fmul_rn(a, s[i]));
+        }
+      }
+    } else if constexpr (SPIN == kAny) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int e = (i < 8 ? at.a : at.b) + (i & 7);
+        if (e < rot) {
+          const float y = widen1(row[e < half ? e + half : e - half]);
+          const float u = __fmul_rn(x[i], c[i]), v = __fmul_rn(y, s[i]);
+          x[i] = e < half ? __fsub_rn(u, v) : __fadd_rn(u, v);
+        }
+      }
     }
   }
 };
@@ -164,11 +191,14 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-__device__ __forceinline__ float absmax8(const float (&x)[8]) {
-  float m = fabsf(x[0]);
+__device__ __forceinline__ float absmax16(const float (&x)[16]) {
+  float m = fabsf(x[0]), n = fabsf(x[1]);
 #pragma unroll
-  for (int i = 1; i < 8; ++i) m = max_nan(m, fabsf(x[i]));
-  return m;
+  for (int i = 2; i < 16; i += 2) {
+    m = max_nan(m, fabsf(x[i]));
+    n = max_nan(n, fabsf(x[i + 1]));
+  }
+  return max_nan(m, n);
 }
 // ... of a row held by LPR neighbouring lanes
 template <int LPR>
@@ -180,29 +210,34 @@ __device__ __forceinline__ float row_max(float m) {
 // the scale of values up to `most`, rounded to fp32; 0, infinite or NaN where there is none
 __device__ __forceinline__ float scale_of(float most) { return __fdiv_rn(most, 127.0f); }
 
-// 8 values as int8 codes: x/scale, rounded to fp32 and then to the nearest whole number (ties to even); zeros where the scale is 0 or not
-// finite.  The quotient is formed with the reciprocal, whose error of less than 127 * 2^-22 decides nothing unless it is that near to
-// a border of two codes: then, which is once in 10 000 values, by a division.
-__device__ __forceinline__ uint2 codes8(const float (&x)[8], float scale, float inverse) {
+// Values as int8 codes: x/scale, rounded to fp32 and then to the nearest whole number (ties to even); zeros where the scale is 0 or not
+// finite.  The quotient is formed with an approximate reciprocal, whose error of less than 127 * 2^-21 decides nothing unless it
+// is that near to a border of two codes: then, which is once in 5 000 values, by a division.
+template <int N>
+__device__ __forceinline__ void codes(const float (&x)[N], float scale, uint32_t (&out)[N / 4]) {
   constexpr float kMagic = 12582912.0f;               // 1.5 * 2^23: the sum's low byte is the whole number
-  if (!(scale > 0.f && scale <= 3.402823466e38f)) return make_uint2(0u, 0u);
-  uint32_t b[8];
+  const bool ok = scale > 0.f && scale <= 3.402823466e38f;
+  float inverse;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(inverse) : "f"(scale));
+  const uint64_t inv2 = f2_pack(inverse, inverse), magic2 = f2_pack(kMagic, kMagic), minus2 = f2_pack(-kMagic, -kMagic), one2 = f2_pack(-1.f, -1.f);
+  uint32_t b[N];
   float off = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float q = __fmul_rn(x[i], inverse), t = __fadd_rn(q, kMagic);
-    off = fmaxf(off, fabsf(__fsub_rn(q, __fsub_rn(t, kMagic))));
-    b[i] = __float_as_uint(t);
+  for (int i = 0; i < N; i += 2) {
+    const uint64_t q = f2_mul(f2_pack(x[i], x[i + 1]), inv2), t = f2_add(q, magic2);
+    float d0, d1;
+    f2_unpack(f2_fma(q, one2, f2_add(t, minus2)), d0, d1);             // whole number - quotient
+    off = fmaxf(off, fmaxf(fabsf(d0), fabsf(d1)));
+    f2_unpacku(t, b[i], b[i + 1]);
   }
-  // (a scale whose reciprocal overflows or is rounded as a subnormal, an `off` that is not small: the careful way)
-  if (!(off < 0.4999f && scale > 1e-37f && inverse > 1e-37f)) {
+  // (an `off` that is not small, a scale whose reciprocal is not a normal number: the careful way)
+  if (ok && !(off < 0.4998f && scale > 1e-37f && scale < 1e37f)) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) b[i] = __float_as_uint(__fadd_rn(fminf(fmaxf(__fdiv_rn(x[i], scale), -127.f), 127.f), kMagic));
+    for (int i = 0; i < N; ++i) b[i] = __float_as_uint(__fadd_rn(fminf(fmaxf(__fdiv_rn(x[i], scale), -127.f), 127.f), kMagic));
   }
-  uint2 r;
-  r.x = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
-  r.y = __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410);
-  return r;
+#pragma unroll
+  for (int i = 0; i < N / 4; ++i)
+    out[i] = ok ? __byte_perm(__byte_perm(b[4 * i], b[4 * i + 1], 0x0040), __byte_perm(b[4 * i + 2], b[4 * i + 3], 0x0040), 0x5410) : 0u;
 }
 
 // largest i in [0, n) with f(i) <= x, by the lanes of a warp together (f grows, f(0) <= x)
