@@ -74,47 +74,32 @@ __device__ __forceinline__ Place place_of(const AppendJob& p, long long t) {
   return r;
 }
 
-// Rows of the tensors from FIRST on, tokens_cta tokens a CTA; each row has its own scale.  A slot (the lanes of a row) goes through several
-// rows of one token, two in flight; what it needs of the rotary table stays in registers for all of them.
-template <typename T, int D, int SPIN, int FIRST, int COUNT>
+// Rows that each have a scale of their own, tokens_cta tokens a CTA: q's, and with KV those of K and V.  A slot (the lanes of a row) goes
+// through several rows of one token, two in flight; what it needs of the rotary table stays in registers for all of them.
+template <typename T, int D, int SPIN, bool KV>
 __device__ __forceinline__ void token_rows(const AppendJob& p, long long cta, int tokens_cta, int per_token, Place* place) {
-  constexpr int LPR = D / 16, U = 2;
+  constexpr int LPR = D / 16;
   const int slot = threadIdx.x / LPR, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int mine = slot / per_token, row0 = slot % per_token;
   const long long token = cta * tokens_cta + mine;
   const bool in = token < p.tokens && mine < tokens_cta;
-  const int h0 = p.heads[FIRST], h1 = COUNT > 1 ? p.heads[FIRST + 1] : 0, rows = h0 + h1 + (COUNT > 2 ? p.heads[FIRST + 2] : 0);
   Pieces at;
   at.place<SPIN>(threadIdx.x % LPR, p.rot);
-  Row16<T> raw[U];
-  auto split = [&](int r, int& w, int& h) {
-    w = FIRST;
-    h = r;
-    if (COUNT > 1 && r >= h0) {
-      w = FIRST + 1;
-      h = r - h0;
-      if (COUNT > 2 && h >= h1) {
-        w = FIRST + 2;
-        h -= h1;
-      }
-    }
-  };
-  const T* base[3];
-#pragma unroll
-  for (int i = 0; i < 3; ++i) base[i] = i >= FIRST && i < FIRST + COUNT ? static_cast<const T*>(p.x[i]) + (in ? token : 0) * p.xn[i] : nullptr;
-  auto src = [&](int w, int h) { return (w == 0 ? base[0] : w == 1 ? base[1] : base[2]) + h * (w == 0 ? p.xh[0] : w == 1 ? p.xh[1] : p.xh[2]); };
-  auto load = [&](int r) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      raw[u].zero();
-      if (in && r + u * per_token < rows) {
-        int w, h;
-        split(r + u * per_token, w, h);
-        raw[u].load(src(w, h), at);
-      }
-    }
-  };
-  load(row0);
+  Row16<T> r0, r1;
+  r0.zero();
+  r1.zero();
+  auto row_of = [&](int w) { return static_cast<const T*>(p.x[w]) + (in ? token : 0) * p.xn[w] + row0 * p.xh[w]; };
+  // the first rows are asked for ahead of where they go
+  const T* xq = p.q8 ? row_of(0) : nullptr;
+  const long long sq = per_token * p.xh[0];
+  const int hq = p.heads[0], hk = p.heads[1];
+  if (hq > 0) {
+    if (in && row0 < hq) r0.load(xq, at);
+    if (in && row0 + per_token < hq) r1.load(xq + sq, at);
+  } else if (KV && in && row0 < hk) {
+    r0.load(row_of(1), at);
+    r1.load(row_of(2), at);
+  }
   for (int i = warp; i < tokens_cta; i += kThreads / 32) {
     const Place x = place_of(p, cta * tokens_cta + i);
     if (lane == 0) place[i] = x;
@@ -129,31 +114,54 @@ __device__ __forceinline__ void token_rows(const AppendJob& p, long long cta, in
     if (!pos_ok && in && to.own && threadIdx.x % LPR == 0 && row0 == 0) report(p);
     goes = goes && pos_ok;
   }
+  auto row = [&](const Row16<T>& raw, const T* src, bool ok, bool spin, int8_t* out, float* scale) {
+    float x[16];
+    widen16(raw, x);
+    if (spin && ok) turn.apply(x, src, p.rot, at);
+    const float s = scale_of(row_max<LPR>(absmax16(x)));
+    uint32_t c[4];
+    codes(x, s, c);
+    if (ok) {
+      *reinterpret_cast<uint2*>(out + at.a) = make_uint2(c[0], c[1]);
+      *reinterpret_cast<uint2*>(out + at.b) = make_uint2(c[2], c[3]);
+      if (threadIdx.x % LPR == 0) *scale = s;
+    }
+  };
   // (every lane of a warp makes every round, for the shuffles)
-  const int rounds = (rows + per_token * U - 1) / (per_token * U);
+  int8_t* q8 = p.q8 + (token * hq + row0) * D;
+  float* qs = p.qs + token * hq + row0;
 #pragma unroll 1
-  for (int k = 0; k < rounds; ++k) {
-    const int r = row0 + k * per_token * U;
-    if (k > 0) load(r);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int row = r + u * per_token;
-      const bool row_ok = goes && row < rows;
-      int w, h;
-      split(row < rows ? row : 0, w, h);
-      float x[16];
-      widen16(raw[u], x);
-      if (w < 2 && row_ok) turn.apply(x, src(w, h), p.rot, at);
-      const float s = scale_of(row_max<LPR>(absmax16(x)));
-      uint32_t c[4];
-      codes(x, s, c);
-      if (row_ok) {
-        int8_t* out = w == 0 ? p.q8 + (token * p.heads[0] + h) * D : p.cache[w - 1] + to.page * p.cp[w - 1] + h * p.ch[w - 1] + to.slot * p.cn[w - 1];
-        float* sc = w == 0 ? p.qs + token * p.heads[0] + h : p.scale[w - 1] + to.page * p.sp[w - 1] + h * p.sh[w - 1] + to.slot * p.sb[w - 1];
-        *reinterpret_cast<uint2*>(out + at.a) = make_uint2(c[0], c[1]);
-        *reinterpret_cast<uint2*>(out + at.b) = make_uint2(c[2], c[3]);
-        if (threadIdx.x % LPR == 0) *sc = s;
+  for (int h = 0; h < hq; h += 2 * per_token) {
+    if (h > 0) {
+      if (in && h + row0 < hq) r0.load(xq, at);
+      if (in && h + row0 + per_token < hq) r1.load(xq + sq, at);
+    }
+    row(r0, xq, goes && h + row0 < hq, true, q8, qs);
+    row(r1, xq + sq, goes && h + row0 + per_token < hq, true, q8 + per_token * D, qs + per_token);
+    xq += 2 * sq;
+    q8 += 2 * per_token * D;
+    qs += 2 * per_token;
+  }
+  if constexpr (KV) {
+    const T *xk = row_of(1), *xv = row_of(2);
+    const long long page = goes ? to.page : 0;
+    int8_t *ck = p.cache[0] + page * p.cp[0] + to.slot * p.cn[0] + row0 * p.ch[0], *cv = p.cache[1] + page * p.cp[1] + to.slot * p.cn[1] + row0 * p.ch[1];
+    float *ak = p.scale[0] + page * p.sp[0] + to.slot * p.sb[0] + row0 * p.sh[0], *av = p.scale[1] + page * p.sp[1] + to.slot * p.sb[1] + row0 * p.sh[1];
+#pragma unroll 1
+    for (int h = 0; h < hk; h += per_token) {
+      const bool have = h + row0 < hk;
+      if ((h > 0 || hq > 0) && in && have) {
+        r0.load(xk, at);
+        r1.load(xv, at);
       }
+      row(r0, xk, goes && have, true, ck, ak);
+      row(r1, xv, goes && have, false, cv, av);
+      xk += per_token * p.xh[1];
+      xv += per_token * p.xh[2];
+      ck += per_token * p.ch[0];
+      cv += per_token * p.ch[1];
+      ak += per_token * p.sh[0];
+      av += per_token * p.sh[1];
     }
   }
 }
@@ -164,7 +172,7 @@ __global__ void __launch_bounds__(kThreads, SPIN == kAny ? 2 : 3) append_tokens_
   __shared__ Place place[kMaxTokens];
   pdl_wait();
   pdl_launch();
-  token_rows<T, D, SPIN, 0, 3>(p, blockIdx.x, tokens_cta, per_token, place);
+  token_rows<T, D, SPIN, true>(p, blockIdx.x, tokens_cta, per_token, place);
 }
 
 // block > 1.  CTAs 0 .. units * groups - 1: what one sequence adds to one block, `heads_cta` heads of K and V; the rest: q.
@@ -178,7 +186,7 @@ __global__ void __launch_bounds__(kThreads, 2) append_blocks_kernel(const Append
   pdl_wait();
   pdl_launch();
   if ((long long)blockIdx.x >= (long long)units * groups) {
-    token_rows<T, D, SPIN, 0, 1>(p, (long long)blockIdx.x - (long long)units * groups, tokens_cta, per_token, place);
+    token_rows<T, D, SPIN, false>(p, (long long)blockIdx.x - (long long)units * groups, tokens_cta, per_token, place);
     return;
   }
   const int u = blockIdx.x / groups, head0 = (blockIdx.x - u * groups) * heads_cta;
@@ -282,15 +290,15 @@ __global__ void __launch_bounds__(kThreads, 2) append_blocks_kernel(const Append
 template <typename T, int D, int SPIN>
 int run(const AppendJob& p, cudaStream_t stream) {
   constexpr int SLOTS = kThreads / (D / 16);
-  // Slots a token: one for about 6 rows, but as many as there are rows where that leaves SMs without work (a decode step)
+  // Slots a token: one for about 12 rows, but as many as there are rows where that leaves SMs without work (a decode step)
   auto slots_of = [&](int heads) {
-    int n = (heads + 5) / 6;
-    while (n < heads && n < SLOTS && p.tokens * n < 3LL * SLOTS * sm_count_cached()) ++n;
-    if (n < (SLOTS + kMaxTokens - 1) / kMaxTokens) n = (SLOTS + kMaxTokens - 1) / kMaxTokens;
+    int n = 1;
+    while (n * 12 < heads || (n < heads && p.tokens * n < 3LL * SLOTS * sm_count_cached())) n *= 2;
+    if (n < SLOTS / kMaxTokens) n = SLOTS / kMaxTokens;
     return n < SLOTS ? n : SLOTS;
   };
   if (p.block_log == 0) {
-    const int per = slots_of(p.heads[0] + p.heads[1] + p.heads[2]), n = SLOTS / per;
+    const int per = slots_of(p.heads[0] > 0 ? p.heads[0] + 2 * p.heads[1] : 2 * p.heads[1]), n = SLOTS / per;
     const long long grid = (p.tokens + n - 1) / n;
     if (grid > 0x7fffffffLL) return set_error(INTFA_ERR_TOO_LARGE, "too many tokens");
     return launch_kernel("append", append_tokens_kernel<T, D, SPIN>, (unsigned)grid, kThreads, 0, stream, p, n, per);

@@ -40,13 +40,27 @@ constexpr int kChunk = 32;                        // keys
 constexpr float kMagicF = 12582912.0f;            // 1.5*2^23: added to an int32 below 2^22 as a bit pattern, it reads as fp32 1.5*2^23 + value
 constexpr int kMagicI = 0x4B400000;
 
-// a unit as combine_kernel sees it
-struct UnitPart {
-  long long chunk0, chunk1;                       // its chunks among all
-  int s, unit;                                    // sequence, unit in it
+// A unit as combine_kernel sees it (one load tells it all): where the parts are and which query rows it has.
+struct __align__(16) UnitPart {
   int open;                                       // 1: its parts are in scratch
-  int pad;
+  int first;                                      // warp that began it
+  int n0, n1, n2;                                 // parts of single warps first, first+1 ..; of whole CTAs; of single warps again
+  int cta;                                        // the first of those CTAs
+  int token, tokens;                              // its first token among all, its tokens
+  int row, head;                                  // row of that token that it begins with; K/V head
+  int pad[2];
 };
+static_assert(sizeof(UnitPart) == 48, "unit");
+// the parts of chunks chunk0 .. chunk1-1 in shares of `share`: CTAs that lie in the unit as a whole leave one part each, in their first warp's slot
+__device__ inline void set_parts(UnitPart& u, long long chunk0, long long chunk1, long long share, long long total, int cta_warps) {
+  const long long cs = share * cta_warps, a = chunk0 / share, b = (chunk1 - 1) / share;
+  const long long ka = (chunk0 + cs - 1) / cs, kb = chunk1 == total ? (total - 1) / cs : chunk1 / cs - 1;
+  u.first = (int)a;
+  u.cta = (int)ka;
+  u.n0 = (int)(ka <= kb ? ka * cta_warps - a : b - a + 1);
+  u.n1 = (int)(ka <= kb ? kb - ka + 1 : 0);
+  u.n2 = (int)(ka <= kb && b >= (kb + 1) * cta_warps ? b - (kb + 1) * cta_warps + 1 : 0);
+}
 
 struct PParams {
   const int8_t* q; const float* qs; void* o; float* lse;
@@ -64,7 +78,7 @@ struct PParams {
   int tile_tokens;                                // 128-row tiles: whole tokens in one; 0: packed RT rows
   float* part; float* part_ml;                    // [2*workers][RT][D]; [2*workers][RT]{m, mw, l, -}
   UnitPart* units; long long max_units;           // [max_units]
-  long long* head;                                // {units, share, chunks}
+  int* head;                                      // {units}
   int* status;
 };
 
@@ -461,30 +475,31 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_const
     }
     if (p.cu && threadIdx.x == 0) bad |= p.cu[p.S] > p.T;
     if (bad && p.status && blockIdx.x == 0) atomicCAS(p.status, 0, kStatusBadIndex);
+    // sums up to and with each thread: within the warps, then on top of the warps before
+    const long long most = p.max_units;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long x = __shfl_up_sync(0xffffffffu, c, o), y = __shfl_up_sync(0xffffffffu, u, o);
+      if (lane >= o) {
+        c += x;
+        u += y;
+      }
+    }
+    long long* sums = reinterpret_cast<long long*>(smem);      // (the ring is not in use yet)
+    if (lane == 31) {
+      sums[2 * warp] = c;
+      sums[2 * warp + 1] = u;
+    }
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) {
+      c += sums[2 * w];
+      u += sums[2 * w + 1];
+    }
     pre_c[threadIdx.x + 1] = c;
-    pre_u[threadIdx.x + 1] = (int)(u < p.max_units ? u : p.max_units);       // (more of them only where cu_seqlens overlap)
+    pre_u[threadIdx.x + 1] = (int)(u < most ? u : most);       // (more of them only where cu_seqlens overlap)
     if (threadIdx.x == 0) {
       pre_c[0] = 0;
       pre_u[0] = 0;
-    }
-  }
-  __syncthreads();
-  if (warp == 0) {
-    long long c0 = 0, u0 = 0;
-    for (int w = 0; w < WARPS; ++w) {
-      long long c = pre_c[w * 32 + lane + 1], u = pre_u[w * 32 + lane + 1];
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long x = __shfl_up_sync(0xffffffffu, c, o), y = __shfl_up_sync(0xffffffffu, u, o);
-        if (lane >= o) {
-          c += x;
-          u += y;
-        }
-      }
-      pre_c[w * 32 + lane + 1] = c + c0;
-      pre_u[w * 32 + lane + 1] = (int)(u + u0 < p.max_units ? u + u0 : p.max_units);
-      c0 += __shfl_sync(0xffffffffu, c, 31);
-      u0 += __shfl_sync(0xffffffffu, u, 31);
     }
   }
   __syncthreads();
@@ -493,8 +508,6 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_const
   if (share < p.least) share = p.least;
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     p.head[0] = pre_u[THREADS];
-    p.head[1] = share;
-    p.head[2] = total;
   }
   const int worker = blockIdx.x * WARPS + warp;
   const long long begin = worker * share;
@@ -659,12 +672,12 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_const
         if (p.status && lane == 0) atomicCAS(p.status, 0, kStatusBadIndex);            // (cu_seqlens that overlap)
       } else if (starts && lane == 0) {
         UnitPart u;
-        u.chunk0 = unit0;
-        u.chunk1 = unit1;
-        u.s = at.s;
-        u.unit = at.unit;
         u.open = !(ends || (cta0 == unit0 && cta1 == unit1));
-        u.pad = 0;
+        if (u.open) set_parts(u, unit0, unit1, share, total, WARPS);
+        u.token = at.q.t0 + tile * RT / p.ratio;
+        u.tokens = at.q.t0 + at.q.n - u.token;
+        u.row = tile * RT % p.ratio;
+        u.head = head;
         p.units[unit_id] = u;
       }
       if (starts && ends) {
@@ -725,34 +738,22 @@ __global__ void __launch_bounds__(GROUPS * (D / 4)) combine_kernel(const PParams
   const int grp = threadIdx.x / C4, ch = threadIdx.x % C4 * 4;
   pdl_wait();
   pdl_launch();
-  if (u >= p.head[0]) return;
-  const UnitPart up = p.units[u];
-  if (!up.open) return;
-  const long long share = p.head[1], total = p.head[2], cs = share * cta_warps;
-  const Seq q = seq_of(p, up.s);
-  const int tiles = p.tile_tokens ? (q.n + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens) : q.tiles;
-  const int head = up.unit / tiles, tile = up.unit - head * tiles;
-  // row r of the unit: query row (token n of the sequence, head h of the K/V head's)
+  const int units = p.head[0];
+  const UnitPart up = p.units[u];                 // (the two loads do not wait for one another)
+  if (u >= units || !up.open) return;
+  // row r of the unit: query row (token n, head h of the K/V head's)
   auto row_of = [&](int r, int& n, int& h) {
-    if (p.tile_tokens) {
-      const int rr = r & 127;
-      n = (2 * tile + (r >> 7)) * p.tile_tokens + rr / p.ratio;
-      h = rr % p.ratio;
-      return rr < p.tile_tokens * p.ratio && n < q.n;
-    }
-    n = (tile * p.rows_tile + r) / p.ratio;
-    h = (tile * p.rows_tile + r) % p.ratio;
-    return n < q.n;
+    const int rr = p.tile_tokens ? r & 127 : up.row + r;
+    n = rr / p.ratio;
+    h = rr - n * p.ratio;
+    if (p.tile_tokens && n >= p.tile_tokens) return false;
+    if (p.tile_tokens) n += (r >> 7) * p.tile_tokens;
+    return n < up.tokens;
   };
-  const long long a = up.chunk0 / share, b = (up.chunk1 - 1) / share;
-  // CTAs ka .. kb lie in the unit as a whole and have left one part each, in their first warp's slot
-  const long long ka = (up.chunk0 + cs - 1) / cs, kb = up.chunk1 == total ? (total - 1) / cs : up.chunk1 / cs - 1;
-  const long long n0 = ka <= kb ? ka * cta_warps - a : b - a + 1, n1 = ka <= kb ? kb - ka + 1 : 0;
-  const long long n2 = ka <= kb && b >= (kb + 1) * cta_warps ? b - (kb + 1) * cta_warps + 1 : 0;
-  const int parts = (int)(n0 + n1 + n2);
+  const int parts = up.n0 + up.n1 + up.n2;
   auto slot_of = [&](int i) {
-    const long long w = i < n0 ? a + i : i < n0 + n1 ? (ka + (i - n0)) * cta_warps : (kb + 1) * cta_warps + (i - n0 - n1);
-    return 2 * w + (w == a ? 1 : 0);
+    const int w = i < up.n0 ? up.first + i : i < up.n0 + up.n1 ? (up.cta + (i - up.n0)) * cta_warps : (up.cta + up.n1) * cta_warps + (i - up.n0 - up.n1);
+    return 2LL * w + (w == up.first ? 1 : 0);
   };
   const int first_row = (int)(blockIdx.x % per_unit) * rows_cta;
   const int row_step = rows_cta == 1 ? 1 : GROUPS, part_step = rows_cta == 1 ? GROUPS : 1;
@@ -773,7 +774,7 @@ __global__ void __launch_bounds__(GROUPS * (D / 4)) combine_kernel(const PParams
       if (grp > 0) return;
       for (int i = 1; i < GROUPS; ++i) x.add(red_ml[i], red[i][ch / 4]);
     }
-    write_sum(p, q.t0 + n, head * p.ratio + h, ch, x);
+    write_sum(p, up.token + n, up.head * p.ratio + h, ch, x);
   }
 }
 
@@ -927,13 +928,13 @@ int paged_attention(const IntfaPagedParams* a, cudaStream_t stream) {
   p.part_ml = reinterpret_cast<float*>(ws + pl.off_ml);
   p.units = reinterpret_cast<UnitPart*>(ws + pl.off_units);
   p.max_units = pl.max_units;
-  p.head = reinterpret_cast<long long*>(ws + pl.off_head);
+  p.head = reinterpret_cast<int*>(ws + pl.off_head);
   p.status = a->status;
   p.tile_tokens = 0;
   if (pl.tiles) {
     p.rows_tile = 2 * kTileRows;
     p.tile_tokens = kTileRows / p.ratio;
-    p.box_log = c.page_size < kTileKeys ? p.page_log : log2_of(kTileKeys);
+    p.box_log = c.page_size < tile_keys(c.D) ? p.page_log : log2_of(tile_keys(c.D));
     p.least = 2;
     return c.D == 64 ? run_tiles<64>(a, pl, p, stream) : run_tiles<128>(a, pl, p, stream);
   }

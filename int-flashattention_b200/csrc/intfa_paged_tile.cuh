@@ -2,27 +2,29 @@
 // (Included by intfa_paged_attn.cu inside namespace intfa, after the shared helpers.)
 //
 // A unit is (sequence, K/V head, 256 rows): two tiles of 128 rows, each the rows of as many whole tokens as fit, all query heads of the
-// K/V head packed.  The units' chunks of 128 keys (those that the last row of a unit sees) are dealt out to the CTAs, one an SM, in equal
+// K/V head packed.  The units' chunks of 64 or 128 keys (those that the last row of a unit sees) are dealt out to the CTAs, one an SM, in equal
 // contiguous shares; parts of units that are cut go to scratch and combine_kernel adds them up, as in the kernel for few rows.
 //
 // 512 threads:
-//   warp 0       TMA: Q once per unit (heads x tokens boxes), K and V pages of 8 to 128 rows each
+//   warp 0       TMA: Q once per unit (heads x tokens boxes), K and V pages of 8 rows and more each
 //   warp 1       MMA issuer.  For each tile in turn: P V of the last chunk, S = Q K^T of the next
 //   warp 2       TMEM; K scales, log2 and reciprocal of the V scales of a chunk into a ring
 //   warp 3       goes through the units and publishes them
 //   warps 4-7    V from int8 (as TMA left it) to fp16 in the MN-major tiles that P V takes
 //   warps 8-11, 12-15   softmax of tile 0 and of tile 1, one thread a row: while one tile is in the tensor core the other is here
-// TMEM: S of both tiles (128 columns each; P, fp16, over the first half of its own S), two accumulators of D columns.
+// TMEM: S of both tiles, their P (fp16), two accumulators of D columns.  S of the next chunk is there before P V of this one is done.
 //
-// The arithmetic is that of the kernel for few rows: w = p v_scale relative to a running maximum of w, P = fp16(w), l = sum p relative to a
-// reference of its own.  Both references follow their maxima only where these get 2^8 ahead: the accumulator is rescaled in a few
-// chunks of a unit, and w <= 2^8 loses no bits in fp16.  Where a chunk's V scales are within 2^60 of what the references differ by (nearly
+// The arithmetic is that of the kernel for few rows: w = p v_scale relative to a reference near its running maximum, P = fp16(w), l = sum p
+// relative to a reference of its own.  The references follow only where w gets 2^8 ahead: the accumulator is rescaled in a few chunks of
+// a unit, and w <= 2^8 loses no bits in fp16.  Where a chunk's V scales are within 2^60 of what the references differ by (nearly
 // always: the general way is for zeros and for scales of very different sizes) p = w / v_scale needs no exp2 of its own.
 // S starts from the bit pattern of 1.5*2^23, written by a small fp16 MMA, and reads as fp32 1.5*2^23 + dot.
 #pragma once
 
-constexpr int kTileRows = 128, kTileKeys = 128;
-constexpr int kTileService = 40, kTileConvert = 72, kTileSoftmax = 200;          // registers
+constexpr int kTileRows = 128;
+// Keys of a chunk.  S and P of both tiles and the accumulators share the 512 columns of TMEM.
+__host__ __device__ constexpr int tile_keys(int D) { return D == 64 ? 128 : 64; }
+constexpr int kTileService = 56, kTileConvert = 72, kTileSoftmax = 192;          // registers
 static_assert(128 * (kTileService + kTileConvert) + 256 * kTileSoftmax <= 65536, "setmaxnreg budget");
 
 // a unit, or the part of it that a CTA does
@@ -51,13 +53,14 @@ __device__ __forceinline__ TileSeq tile_seq_of(const PParams& p, int s) {
   w.uniform = !p.causal || w.first < 0 || q.len > q.keys;        // every unit goes over all keys (for the odd lengths, masked)
   return w;
 }
+template <int G>
 __device__ __forceinline__ int tile_chunks(const PParams& p, const TileSeq& q, int tile) {
   long long vis = q.keys;
   if (!q.uniform) vis = min(vis, q.first + (long long)(tile + 1) * 2 * p.tile_tokens);
-  return vis > kTileKeys ? (int)((vis + kTileKeys - 1) / kTileKeys) : 1;
+  return vis > G ? (int)((vis + G - 1) / G) : 1;
 }
 // sum of floor((a t + b) / m), t = 0 .. n-1 (a, b >= 0)
-__device__ inline long long floor_sum(long long n, long long m, long long a, long long b) {
+__device__ __noinline__ long long floor_sum(long long n, long long m, long long a, long long b) {
   long long sum = 0;
   while (n > 0) {
     sum += n * (n - 1) / 2 * (a / m) + n * (b / m);
@@ -74,19 +77,20 @@ __device__ inline long long floor_sum(long long n, long long m, long long a, lon
   return sum;
 }
 // chunks of the first k units of a K/V head
+template <int G>
 __device__ inline long long tile_chunks_before(const PParams& p, const TileSeq& q, int k) {
   if (k <= 0) return 0;
-  if (q.uniform) return (long long)k * tile_chunks(p, q, 0);
+  if (q.uniform) return (long long)k * tile_chunks<G>(p, q, 0);
   const int full = k < q.tiles ? k : q.tiles - 1;
   const long long step = 2 * p.tile_tokens;
-  return floor_sum(full, kTileKeys, step, q.first + step + kTileKeys - 1) + (k == q.tiles ? tile_chunks(p, q, q.tiles - 1) : 0);
+  return floor_sum(full, G, step, q.first + step + G - 1) + (k == q.tiles ? tile_chunks<G>(p, q, q.tiles - 1) : 0);
 }
 
 template <int D>
 struct TileCfg {
-  static constexpr int THREADS = 512, NK = 3, NV8 = 2, NV = 2, NSC = 4, NU = 4;
-  static constexpr int Q_BYTES = kTileRows * D, K_BYTES = kTileKeys * D, V_BYTES = kTileKeys * D * 2;
-  static constexpr int SC_FLOATS = 3 * kTileKeys + 4;
+  static constexpr int G = tile_keys(D), THREADS = 512, NK = D == 64 ? 4 : 5, NV8 = 4, NV = D == 64 ? 3 : 3, NSC = 8, NU = 4;
+  static constexpr int Q_BYTES = kTileRows * D, K_BYTES = G * D, V_BYTES = G * D * 2;
+  static constexpr int SC_FLOATS = 3 * G + 4;
   static constexpr int OFF_Q = 0, OFF_K = OFF_Q + 2 * Q_BYTES, OFF_V8 = OFF_K + NK * K_BYTES, OFF_V = OFF_V8 + NV8 * K_BYTES;
   static constexpr int OFF_ARM = OFF_V + NV * V_BYTES;
   static constexpr int OFF_SC = OFF_ARM + 4096;
@@ -98,12 +102,12 @@ struct TileCfg {
   static constexpr int SMEM = OFF_MISC + 32 + 1024;
   static_assert(SMEM <= 227 * 1024, "shared memory");
   static_assert(OFF_UNIT % 16 == 0 && OFF_SC % 16 == 0 && OFF_PRE % 8 == 0, "alignment");
-  static constexpr int COL_S = 0, COL_O = 2 * kTileKeys;
+  static constexpr int COL_S = 0, COL_P = 2 * G, COL_O = 3 * G;
   static_assert(COL_O + 2 * D <= 512, "TMEM columns");
   static constexpr uint64_t SWZ_QK = D == 128 ? kSwz128 : kSwz64;
-  static constexpr uint32_t IDESC_QK = make_idesc(2, 1, 1, 0, 0, kTileRows, kTileKeys);
+  static constexpr uint32_t IDESC_QK = make_idesc(2, 1, 1, 0, 0, kTileRows, G);
   static constexpr uint32_t IDESC_PV = make_idesc(1, 0, 0, 0, 1, kTileRows, D);
-  static constexpr uint32_t IDESC_ARM = make_idesc(1, 0, 0, 0, 0, kTileRows, kTileKeys);
+  static constexpr uint32_t IDESC_ARM = make_idesc(1, 0, 0, 0, 0, kTileRows, G);
 };
 
 enum TileWait { TW_UNIT = 65, TW_UEMPTY, TW_QE, TW_KE, TW_V8E, TW_QF, TW_KF, TW_VF, TW_P, TW_SCE, TW_V8F, TW_VE, TW_SC, TW_S, TW_O };
@@ -112,6 +116,7 @@ template <int D>
 __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                                                             const __grid_constant__ CUtensorMap tmV, const PParams p) {
   using C = TileCfg<D>;
+  constexpr int G = C::G;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((0u - smem_u32(smem_raw)) & 1023u);
   const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -123,7 +128,7 @@ __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constan
   constexpr int B_VF = B_V8E + C::NV8, B_VE = B_VF + C::NV;      // converting warps (4); commit
   constexpr int B_SCF = B_VE + C::NV, B_SCE = B_SCF + C::NSC;    // scale loader; softmax warps (8)
   constexpr int B_UF = B_SCE + C::NSC, B_UE = B_UF + C::NU;      // unit published; taken over by TMA, MMA, scale, converting, softmax warps (15)
-  constexpr int B_S = B_UE + C::NU, B_P = B_S + 2, B_O = B_P + 2;        // [2] commit: S; softmax warps of the tile (4): P; commit: last P V
+  constexpr int B_S = B_UE + C::NU, B_P = B_S + 2, B_O = B_P + 2;        // [2] commit: S; softmax warps of the tile (4): S read, P written; commit: P V
   static_assert(B_O + 2 == C::NBARS, "barriers");
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 8);
@@ -182,7 +187,7 @@ __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constan
     bool bad = false;
     for (int s = threadIdx.x * seg; s < (threadIdx.x + 1) * seg && s < p.S; ++s) {
       const TileSeq q = tile_seq_of(p, s);
-      if (q.n > 0) c += tile_chunks_before(p, q, q.tiles) * p.Hkv;
+      if (q.n > 0) c += tile_chunks_before<G>(p, q, q.tiles) * p.Hkv;
       bad |= q.n > 0 && q.first + q.n > q.keys;
     }
     if (p.cu && threadIdx.x == 0) bad |= p.cu[p.S] > p.T;
@@ -251,20 +256,20 @@ __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constan
         long long off = begin - pre[i];
         for (s = i * seg;; ++s) {
           q = tile_seq_of(p, s);
-          const long long c = q.n > 0 ? tile_chunks_before(p, q, q.tiles) * p.Hkv : 0;
+          const long long c = q.n > 0 ? tile_chunks_before<G>(p, q, q.tiles) * p.Hkv : 0;
           if (off < c || s + 1 >= p.S) break;
           off -= c;
         }
-        const long long per_head = tile_chunks_before(p, q, q.tiles);
+        const long long per_head = tile_chunks_before<G>(p, q, q.tiles);
         head = (int)(off / per_head);
         off -= head * per_head;
         int lo = 0, hi = q.tiles;                              // the last tile whose chunks begin at or before `off`
         while (hi - lo > 1) {
           const int mid = (lo + hi) / 2;
-          if (tile_chunks_before(p, q, mid) <= off) lo = mid; else hi = mid;
+          if (tile_chunks_before<G>(p, q, mid) <= off) lo = mid; else hi = mid;
         }
         tile = lo;
-        pos = begin - (off - tile_chunks_before(p, q, tile));  // where the first unit begins
+        pos = begin - (off - tile_chunks_before<G>(p, q, tile));  // where the first unit begins
       }
       bool ok = true;
       uint32_t seq = 0;
@@ -272,7 +277,7 @@ __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constan
       while (ok) {
         TileUnit u = none;
         if (pos < end) {
-          const int n = tile_chunks(p, q, tile), token = tile * 2 * p.tile_tokens;
+          const int n = tile_chunks<G>(p, q, tile), token = tile * 2 * p.tile_tokens;
           u.lim0 = p.causal ? q.first + token : (long long)q.keys;
           u.t0 = q.t0 + token;
           u.tokens = min(2 * p.tile_tokens, q.n - token);
@@ -284,12 +289,12 @@ __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constan
           const bool starts = pos >= begin, ends = pos + n <= end;
           u.slot = starts && ends ? -1 : 2 * (int)blockIdx.x + (starts ? 1 : 0);
           if (starts && !ends) {
-            part.chunk0 = pos;
-            part.chunk1 = pos + n;
-            part.s = s;
-            part.unit = head * q.tiles + tile;
             part.open = 1;
-            part.pad = 0;
+            set_parts(part, pos, pos + n, share, total, 1);
+            part.token = u.t0;
+            part.tokens = u.tokens;
+            part.row = 0;
+            part.head = head;
           }
           pos += n;
           if (++tile == q.tiles) {
@@ -314,17 +319,13 @@ __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constan
       }
       if (lane == 0) {
         p.units[blockIdx.x] = part;
-        if (blockIdx.x == 0) {
-          p.head[0] = gridDim.x;
-          p.head[1] = share;
-          p.head[2] = total;
-        }
+        if (blockIdx.x == 0) p.head[0] = gridDim.x;
       }
     } else if (warp == 0) {
       // ------------------------------------------------------------------ TMA
       uint32_t kit = 0, uit = 0;                               // chunks, units so far
       uint32_t qit1 = 0;                                       // units with a second tile
-      const int box_rows = 1 << p.box_log, boxes = kTileKeys >> p.box_log;
+      const int box_rows = 1 << p.box_log, boxes = G >> p.box_log;
       const uint32_t sQ = smem_u32(smem + C::OFF_Q), sK = smem_u32(smem + C::OFF_K), sV8 = smem_u32(smem + C::OFF_V8);
       const uint32_t q_box = (uint32_t)(p.tile_tokens * p.ratio * D);
       TileUnit u;
@@ -345,7 +346,7 @@ __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constan
         qit1 += two;
         // lane j: the page of box j of the next chunk
         auto look_up = [&](int c) {
-          const int key = c * kTileKeys + lane * box_rows;
+          const int key = c * G + lane * box_rows;
           return lane < boxes && c < u.c1 && key < u.keys ? table[key >> p.page_log] : 0;
         };
         int next = look_up(u.c0);
@@ -356,7 +357,7 @@ __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constan
             if (p.status) atomicCAS(p.status, 0, kStatusBadIndex);
             page = 0;
           }
-          const int key0 = c * kTileKeys, full = max(0, min(boxes, (u.keys - key0 + box_rows - 1) >> p.box_log));
+          const int key0 = c * G, full = max(0, min(boxes, (u.keys - key0 + box_rows - 1) >> p.box_log));
           const int slot = (key0 + lane * box_rows) & page_mask;
           const uint32_t bytes = (uint32_t)full * box_rows * D;
           const uint32_t k = kit % C::NK, v = kit % C::NV8;
@@ -378,9 +379,9 @@ __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constan
       // ------------------------------------------------------------------ MMA
       const uint32_t sQ = smem_u32(smem + C::OFF_Q), sK = smem_u32(smem + C::OFF_K), sV = smem_u32(smem + C::OFF_V);
       const uint64_t descQ = make_smem_desc(sQ, 16, 8 * D, C::SWZ_QK), descK = make_smem_desc(sK, 16, 8 * D, C::SWZ_QK);
-      const uint64_t descV = make_smem_desc(sV, D > 64 ? kTileKeys * 128 : 16, 8 * 128, kSwz128);
+      const uint64_t descV = make_smem_desc(sV, D > 64 ? G * 128 : 16, 8 * 128, kSwz128);
       const uint64_t descArm = make_smem_desc(smem_u32(smem + C::OFF_ARM), 128, 256, 0);
-      uint32_t kit = 0, vit = 0, uit[2] = {0, 0}, pit[2] = {0, 0};       // chunks of K, of V; units, P tiles
+      uint32_t kit = 0, vit = 0, uit = 0, pit = 0;             // chunks of K, of V; bit i: units, P tiles of tile i mod 2
       TileUnit u;
       bool ok = true;
       while (ok && next_unit(u)) {
@@ -389,23 +390,16 @@ __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constan
           const uint32_t k = kit % C::NK, v = vit % C::NV;
           if (j < n) ok = wait(B_KF + k, (kit / C::NK) & 1u, TW_KF);
           if (ok && j > 0) ok = wait(B_VF + v, (vit / C::NV) & 1u, TW_VF);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if (!ok || i > two) continue;
-            const uint32_t tS = tmem + C::COL_S + i * kTileKeys, tO = tmem + C::COL_O + i * D;
-            if (j == 0) ok = wait(B_QF + i, uit[i] & 1u, TW_QF);
-            else ok = wait(B_P + i, pit[i] & 1u, TW_P);
-            if (!ok) continue;
-            if (j > 0) ++pit[i];
+#pragma unroll 1
+          for (int i = 0; i <= two && ok; ++i) {
+            const uint32_t tS = tmem + C::COL_S + i * G, tP = tmem + C::COL_P + i * (G / 2), tO = tmem + C::COL_O + i * D;
+            if (j == 0) ok = wait(B_QF + i, uit >> i & 1u, TW_QF);
+            else ok = wait(B_P + i, pit >> i & 1u, TW_P);
+            if (!ok) break;
+            if (j > 0) pit ^= 1u << i;
             tc_fence_after();
             if (elect_one()) {
-              // (the tensor core takes them in this order: S of the next chunk comes over P when the P V that reads it is done)
-              if (j > 0) {
-                const uint64_t vd = descV + (uint64_t)(v * (C::V_BYTES >> 4));
-#pragma unroll
-                for (int kk = 0; kk < kTileKeys / 16; ++kk)
-                  umma_f16_ts(tO, tS + kk * 8, vd + (uint64_t)(kk * ((16 * 128) >> 4)), C::IDESC_PV, j > 1 || kk > 0 ? 1u : 0u);
-              }
+              // (the tile's softmax warps are done with S and have written P; S of the next chunk first, they wait for it)
               if (j < n) {
                 umma_f16(tS, descArm, descArm, C::IDESC_ARM, 0);
 #pragma unroll
@@ -413,7 +407,12 @@ __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constan
                   umma_i8(tS, descQ + (uint64_t)(i * (C::Q_BYTES >> 4) + 2 * kk), descK + (uint64_t)(k * (C::K_BYTES >> 4) + 2 * kk), C::IDESC_QK, 1);
                 umma_commit(BAR(B_S + i));
                 if (j + 1 == n) umma_commit(BAR(B_QE + i));
-              } else {
+              }
+              if (j > 0) {
+                const uint64_t vd = descV + (uint64_t)(v * (C::V_BYTES >> 4));
+#pragma unroll
+                for (int kk = 0; kk < G / 16; ++kk)
+                  umma_f16_ts(tO, tP + kk * 8, vd + (uint64_t)(kk * ((16 * 128) >> 4)), C::IDESC_PV, j > 1 || kk > 0 ? 1u : 0u);
                 umma_commit(BAR(B_O + i));
               }
               if (i == two) {
@@ -426,8 +425,7 @@ __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constan
           if (j < n) ++kit;
           if (j > 0) ++vit;
         }
-        ++uit[0];
-        uit[1] += two;
+        uit ^= two ? 3u : 1u;
       }
     } else {
       // ------------------------------------------------------------------ scales
@@ -438,24 +436,25 @@ __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constan
         const int* table = p.table + (long long)u.s * p.table_stride;
         const float* ks = p.ks + u.head * p.ksH;
         const float* vs = p.vs + u.head * p.vsH;
-        int page[4];
+        constexpr int N = G / 32;
+        int page[N];
         auto look_up = [&](int c) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int key = c * kTileKeys + i * 32 + lane;
+          for (int i = 0; i < N; ++i) {
+            const int key = c * G + i * 32 + lane;
             page[i] = c < u.c1 && key < u.keys ? table[key >> p.page_log] : -1;
           }
         };
         look_up(u.c0);
         for (int c = u.c0; c < u.c1 && ok; ++c, ++it) {
-          float a[4], b[4];
+          float a[N], b[N];
           unsigned in = 0;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int blk = ((c * kTileKeys + i * 32 + lane) & page_mask) >> p.block_log;
+          for (int i = 0; i < N; ++i) {
+            const int blk = ((c * G + i * 32 + lane) & page_mask) >> p.block_log;
             a[i] = 0.f;
             b[i] = 1.f;
-            if (c * kTileKeys + i * 32 + lane < u.keys) {
+            if (c * G + i * 32 + lane < u.keys) {
               const long long pg = bad_page(page[i]) ? 0 : page[i];
               a[i] = ks[pg * p.ksP + blk * p.ksB];
               b[i] = vs[pg * p.vsP + blk * p.vsB];
@@ -469,11 +468,11 @@ __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constan
           if (!ok) break;
           float lo = INFINITY, hi = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < N; ++i) {
             const float l = log2_approx(b[i]);
             sc[i * 32 + lane] = a[i];
-            sc[kTileKeys + i * 32 + lane] = l;
-            sc[2 * kTileKeys + i * 32 + lane] = 1.0f / b[i];
+            sc[G + i * 32 + lane] = l;
+            sc[2 * G + i * 32 + lane] = 1.0f / b[i];
             if (in >> i & 1u) {
               const bool odd = !(fabsf(l) < INFINITY);         // zero, infinite, NaN: the general way
               lo = fminf(lo, odd ? -INFINITY : l);
@@ -486,8 +485,8 @@ __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constan
             hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
           }
           if (lane == 0) {
-            sc[3 * kTileKeys] = lo;
-            sc[3 * kTileKeys + 1] = hi;
+            sc[3 * G] = lo;
+            sc[3 * G + 1] = hi;
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(BAR(B_SCF + slot));
@@ -510,8 +509,8 @@ __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constan
         ok = wait(B_V8F + a, (it / C::NV8) & 1u, TW_V8F) && wait(B_VE + b, ((it / C::NV) & 1u) ^ 1u, TW_VE);
         if (!ok) break;
         const uint32_t src = sV8 + a * C::K_BYTES, dst = sV + b * C::V_BYTES;
-#pragma unroll 2
-        for (int i = tid; i < kTileKeys * PIECES; i += 128) {
+#pragma unroll 1
+        for (int i = tid; i < G * PIECES; i += 128) {
           const int key = i / PIECES, pc = i % PIECES;
           const int sw = D == 128 ? key & 7 : (key >> 1) & 3;
           const uint4 x = lds16(src + key * D + ((pc ^ sw) << 4));
@@ -526,7 +525,7 @@ __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constan
           // channels pc*16 .. +15: chunks 2 (pc % 4) and the next of box pc / 4; the lanes of the second box begin with the other one, so
           // that a row's eight stores lie in different banks
           const int swap = (pc >> 2) & 1;
-          const uint32_t row = dst + (pc >> 2) * (kTileKeys * 128) + key * 128;
+          const uint32_t row = dst + (pc >> 2) * (G * 128) + key * 128;
           const int ch = (pc & 3) * 2;
           const uint4 y0 = make_uint4(h[0], h[1], h[2], h[3]), y1 = make_uint4(h[4], h[5], h[6], h[7]);
           const uint4 f = swap ? y1 : y0, g = swap ? y0 : y1;
@@ -547,24 +546,32 @@ __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constan
     // -------------------------------------------------------------------- softmax, one thread a row
     const int tile = (warp - 8) >> 2, rr = threadIdx.x & 127;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;         // (lane 32 * (warp % 4) in bits 16 and up)
-    const uint32_t tS = tmem + C::COL_S + tile * kTileKeys + lanes, tO = tmem + C::COL_O + tile * D + lanes;
+    const uint32_t tS = tmem + C::COL_S + tile * G + lanes, tP = tmem + C::COL_P + tile * (G / 2) + lanes, tO = tmem + C::COL_O + tile * D + lanes;
     const int tok = tile * p.tile_tokens + rr / p.ratio, hr = rr % p.ratio;
     uint32_t sit = 0, it = 0, oit = 0;                         // S tiles, chunks, units of this tile so far
+    // what a row needs of its unit; the scale of its query is asked for here and used a while later
     TileUnit u;
-    bool ok = true;
-    while (ok && next_unit(u)) {
-      const bool work = tile == 0 || u.tokens > p.tile_tokens;
-      if (!work) {
+    float qs_raw = 0.f;
+    bool mine = false;
+    auto take = [&]() {
+      if (!next_unit(u)) return false;
+      mine = tok < u.tokens && rr < p.tile_tokens * p.ratio;
+      qs_raw = 0.f;
+      if (mine) qs_raw = p.qs[(long long)(u.t0 + tok) * p.qsn + (u.head * p.ratio + hr) * p.qsh];
+      return true;
+    };
+    bool ok = true, have = take();
+    while (have) {
+      if (tile > 0 && u.tokens <= p.tile_tokens) {             // no rows in this tile
         for (int c = u.c0; c < u.c1 && ok; ++c, ++it) {
           ok = wait(B_SCF + it % C::NSC, (it / C::NSC) & 1u, TW_SC);
           if (lane == 0) mbar_arrive(BAR(B_SCE + it % C::NSC));
         }
+        have = ok && take();
         continue;
       }
-      const bool mine = tok < u.tokens && rr < p.tile_tokens * p.ratio;
-      const int h = u.head * p.ratio + hr;
-      float qs = 0.f;
-      if (mine) qs = p.qs[(long long)(u.t0 + tok) * p.qsn + h * p.qsh] * p.c;
+      const float qs = qs_raw * p.c;
+      const uint64_t qs2 = f2_pack(qs, qs), magic2 = f2_pack(-kMagicF, -kMagicF);
       long long lim = u.keys - 1;
       if (p.causal && mine) lim = min(lim, u.lim0 + tok);
       float mref = -INFINITY, ref = -INFINITY, l = 0.f;        // references of p and of w (of the accumulator)
@@ -573,78 +580,128 @@ __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constan
         ok = wait(B_SCF + slot, (it / C::NSC) & 1u, TW_SC) && wait(B_S + tile, sit & 1u, TW_S);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t sc = smem_u32(smem + C::OFF_SC) + slot * (C::SC_FLOATS * 4);
-        const uint64_t qs2 = f2_pack(qs, qs), magic2 = f2_pack(-kMagicF, -kMagicF);
-        const long long rel64 = lim - (long long)c * kTileKeys;
-        const int rel = rel64 < -1 ? -1 : rel64 > kTileKeys ? kTileKeys : (int)rel64;        // the last column that the row sees
-        const bool masked = __any_sync(0xffffffffu, rel < kTileKeys - 1);
-        // ---- exponents of w: x + log2 v_scale
-        uint64_t xw[kTileKeys / 2];
-        float mx = -INFINITY;
-        uint32_t buf[2][32];
-        tmem_ld32(tS, buf[0]);
+        const float* sc = reinterpret_cast<const float*>(smem + C::OFF_SC) + slot * C::SC_FLOATS;
+        const float lo = sc[3 * G], hi = sc[3 * G + 1];
+        const long long rel64 = lim - (long long)c * G;
+        const int rel = rel64 < -1 ? -1 : rel64 > G ? G : (int)rel64;        // the last column that the row sees
+        const int rel_least = (int)__reduce_min_sync(0xffffffffu, rel), rel_most = (int)__reduce_max_sync(0xffffffffu, rel);
+        // exponents of w, x + log2 v_scale - off, of 16 columns, in place of the scores
+        auto exponents = [&](int b, uint32_t (&r)[16], float off) {
+          const uint64_t off2 = f2_pack(-off, -off);
+          const float4* ks = reinterpret_cast<const float4*>(sc + b * 16);
+          const float4* lv = reinterpret_cast<const float4*>(sc + G + b * 16);
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          tmem_ld_wait(buf[b & 1]);
-          if (b < 3) tmem_ld32(tS + (b + 1) * 32, buf[(b + 1) & 1]);
-#pragma unroll
-          for (int k = 0; k < 32; k += 4) {
-            const uint4 a = lds16(sc + (b * 32 + k) * 4), v = lds16(sc + (kTileKeys + b * 32 + k) * 4);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const uint64_t t = f2_add(f2_packu(buf[b & 1][k + 2 * e], buf[b & 1][k + 2 * e + 1]), magic2);
-              const uint64_t x = f2_fma(t, f2_mul(e ? f2_packu(a.z, a.w) : f2_packu(a.x, a.y), qs2), e ? f2_packu(v.z, v.w) : f2_packu(v.x, v.y));
-              xw[(b * 32 + k) / 2 + e] = x;
-              float x0, x1;
-              f2_unpack(x, x0, x1);
-              mx = max3(mx, x0, x1);
-            }
+          for (int k = 0; k < 16; k += 4) {
+            const float4 a = ks[k / 4], v = lv[k / 4];
+            f2_unpacku(f2_fma(f2_add(f2_packu(r[k], r[k + 1]), magic2), f2_mul(f2_pack(a.x, a.y), qs2), f2_add(f2_pack(v.x, v.y), off2)), r[k], r[k + 1]);
+            f2_unpacku(f2_fma(f2_add(f2_packu(r[k + 2], r[k + 3]), magic2), f2_mul(f2_pack(a.z, a.w), qs2), f2_add(f2_pack(v.z, v.w), off2)), r[k + 2], r[k + 3]);
           }
-        }
-        if (masked) {
-          mx = -INFINITY;
+          if (b * 16 + 15 > rel_least) {
+            const int last = rel - b * 16;
 #pragma unroll
-          for (int k = 0; k < kTileKeys / 2; ++k) {
-            float x0, x1;
-            f2_unpack(xw[k], x0, x1);
-            x0 = 2 * k <= rel ? x0 : -INFINITY;
-            x1 = 2 * k + 1 <= rel ? x1 : -INFINITY;
-            mx = max3(mx, x0, x1);
-            xw[k] = f2_pack(x0, x1);
+            for (int k = 0; k < 16; ++k) r[k] = k <= last ? r[k] : __float_as_uint(-INFINITY);
           }
-        }
-        // ---- references
-        const bool up = mx > ref + 8.f || (ref == -INFINITY && mx > -INFINITY);
-        if (__any_sync(0xffffffffu, up)) {
-          const float to = up ? mx : ref, f = ref == -INFINITY ? 0.f : ex2_approx(ref - to);
-          if (up && ref > -INFINITY) {
-            mref += to - ref;
-            l *= f;
+        };
+        auto largest = [&](const uint32_t (&r)[16], float (&mx)[2]) {
+#pragma unroll
+          for (int k = 0; k < 16; k += 4) {
+            mx[0] = max3(mx[0], __uint_as_float(r[k]), __uint_as_float(r[k + 1]));
+            mx[1] = max3(mx[1], __uint_as_float(r[k + 2]), __uint_as_float(r[k + 3]));
           }
-          ref = to;
-          if (c > u.c0) {                        // (the first P V does not look at what is there)
-            const uint64_t f2 = f2_pack(up ? f : 1.f, up ? f : 1.f);
+        };
+        // The references are taken over as they are, and P is made with them in one go; only where some w comes out above 2^8 (or a row
+        // has no reference yet: in a unit's first chunk) the maxima are found first.
+        uint64_t sum2;
+        bool find = c == u.c0, settled = c == u.c0;            // settled: P V of the chunk before is done
+        for (;;) {
+          if (find) {
+            float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll 1
-            for (int b = 0; b < D / 32; ++b) {
-              uint32_t o[32];
-              tmem_ld32(tO + b * 32, o);
-              tmem_ld_wait(o);
+            for (int b = 0; b * 16 <= rel_most && b < G / 16; ++b) {
+              uint32_t r[16];
+              tmem_ld16(tS + b * 16, r);
+              tmem_ld_wait16(r);
+              exponents(b, r, 0.f);
+              largest(r, mx);
+            }
+            const float top = fmaxf(mx[0], mx[1]);
+            const float to = top > ref ? top : ref, f = ref == -INFINITY ? 0.f : ex2_approx(ref - to);
+            // (the reference of p as far from the largest p as a middling V scale is from 1; it stays until `easy` does not hold)
+            if (to > -INFINITY && mref == -INFINITY && hi - lo < 60.f) mref = to - 0.5f * (lo + hi);
+            ref = to;
+            if (!settled) {
+              ok = wait(B_O + tile, oit & 1u, TW_O);
+              if (!ok) break;
+              ++oit;
+              settled = true;
+              tc_fence_after();
+            }
+            if (c > u.c0) {                                    // (the first P V does not look at what is there)
+              const uint64_t f2 = f2_pack(f, f);
+#pragma unroll 1
+              for (int b = 0; b < D / 16; ++b) {
+                uint32_t o[16];
+                tmem_ld16(tO + b * 16, o);
+                tmem_ld_wait16(o);
 #pragma unroll
-              for (int k = 0; k < 32; k += 2) f2_unpacku(f2_mul(f2_packu(o[k], o[k + 1]), f2), o[k], o[k + 1]);
-              tmem_st32(tO + b * 32, o);
+                for (int k = 0; k < 16; k += 2) f2_unpacku(f2_mul(f2_packu(o[k], o[k + 1]), f2), o[k], o[k + 1]);
+                tmem_st16(tO + b * 16, o);
+              }
             }
           }
+          const float base = safe(ref);
+          float mx[2] = {-INFINITY, -INFINITY};
+          sum2 = 0;
+          // (two buffers of 16 columns in a rolled loop: the instruction cache has to hold the loops of all roles)
+          uint32_t buf[2][16];
+          tmem_ld16(tS, buf[0]);
+#pragma unroll 1
+          for (int b2 = 0; b2 < G / 16; b2 += 2) {
+#pragma unroll
+            for (int e2 = 0; e2 < 2; ++e2) {
+              const int b = b2 + e2;
+              uint32_t(&r)[16] = buf[e2];
+              tmem_ld_wait16(r);
+              if (e2 == 0 || b2 + 2 < G / 16) tmem_ld16(tS + (b + 1) * 16, buf[e2 ^ 1]);
+              exponents(b, r, base);
+              largest(r, mx);
+              uint32_t pk[8];
+              const float4* iv = reinterpret_cast<const float4*>(sc + 2 * G + b * 16);
+#pragma unroll
+              for (int k = 0; k < 16; k += 4) {
+                const float4 v = iv[k / 4];
+                const float w0 = ex2_approx(__uint_as_float(r[k])), w1 = ex2_approx(__uint_as_float(r[k + 1]));
+                const float w2 = ex2_approx(__uint_as_float(r[k + 2])), w3 = ex2_approx(__uint_as_float(r[k + 3]));
+                sum2 = f2_fma(f2_pack(w0, w1), f2_pack(v.x, v.y), sum2);
+                sum2 = f2_fma(f2_pack(w2, w3), f2_pack(v.z, v.w), sum2);
+                const __half2 y0 = __floats2half2_rn(w0, w1), y1 = __floats2half2_rn(w2, w3);
+                pk[k / 2] = *reinterpret_cast<const uint32_t*>(&y0);
+                pk[k / 2 + 1] = *reinterpret_cast<const uint32_t*>(&y1);
+              }
+              if (e2 == 0 && !settled) {         // (P and the accumulator are the P V's of the chunk before until then)
+                ok = wait(B_O + tile, oit & 1u, TW_O);
+                ++oit;
+                settled = true;
+                tc_fence_after();
+              }
+              tmem_st8(tP + b * 8, pk);
+            }
+          }
+          if (!ok) break;
+          const float top = fmaxf(mx[0], mx[1]);
+          if (!__any_sync(0xffffffffu, top > 8.f || (ref == -INFINITY && top > -INFINITY))) break;
+          find = true;
         }
-        float lo, hi;
-        {
-          const float2 r = lds_f2(sc + 3 * kTileKeys * 4);
-          lo = r.x;
-          hi = r.y;
-        }
+        if (!ok) break;
         const float d = ref - mref;
         const bool easy = ref == -INFINITY ? mref == -INFINITY && lo > -INFINITY : lo >= d - 60.f && hi <= d + 60.f;
-        const bool general = !__all_sync(0xffffffffu, easy);
-        if (general) {
+        if (__all_sync(0xffffffffu, easy)) {
+          if (ref > -INFINITY) {
+            float s0, s1;
+            f2_unpack(sum2, s0, s1);
+            l = fmaf(s0 + s1, ex2_approx(d), l);
+          }
+        } else {
           // p by itself: the scores once more
           float top = -INFINITY;
 #pragma unroll 1
@@ -652,18 +709,19 @@ __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constan
             float sum = 0.f;
             const float base = safe(mref);
 #pragma unroll 1
-            for (int b = 0; b < 4; ++b) {
-              uint32_t o[32];
-              tmem_ld32(tS + b * 32, o);
-              tmem_ld_wait(o);
+            for (int b = 0; b < G / 16; ++b) {
+              uint32_t o[16];
+              tmem_ld16(tS + b * 16, o);
+              tmem_ld_wait16(o);
+              const float4* ks = reinterpret_cast<const float4*>(sc + b * 16);
 #pragma unroll
-              for (int k = 0; k < 32; k += 4) {
-                const uint4 a = lds16(sc + (b * 32 + k) * 4);
-                const uint32_t aa[4] = {a.x, a.y, a.z, a.w};
+              for (int k = 0; k < 16; k += 4) {
+                const float4 a = ks[k / 4];
+                const float aa[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                  float x = (__uint_as_float(o[k + e]) - kMagicF) * (__uint_as_float(aa[e]) * qs);
-                  if (b * 32 + k + e > rel) x = -INFINITY;
+                  float x = (__uint_as_float(o[k + e]) - kMagicF) * (aa[e] * qs);
+                  if (b * 16 + k + e > rel) x = -INFINITY;
                   if (pass == 0) top = fmaxf(top, x);
                   else sum += ex2_approx(x - base);
                 }
@@ -679,34 +737,6 @@ __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constan
             }
           }
         }
-        // ---- w, its sum over v_scale, P
-        const float base = safe(ref);
-        const uint64_t nb = f2_pack(-base, -base);
-        uint64_t sum = 0;
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int k = 0; k < 16; k += 2) {
-            const uint4 iv = lds16(sc + (2 * kTileKeys + b * 32 + 2 * k) * 4);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float x0, x1;
-              f2_unpack(f2_add(xw[b * 16 + k + e], nb), x0, x1);
-              x0 = ex2_approx(x0);
-              x1 = ex2_approx(x1);
-              sum = f2_fma(f2_pack(x0, x1), e ? f2_packu(iv.z, iv.w) : f2_packu(iv.x, iv.y), sum);
-              const __half2 y = __floats2half2_rn(x0, x1);
-              pk[k + e] = *reinterpret_cast<const uint32_t*>(&y);
-            }
-          }
-          tmem_st16(tS + b * 16, pk);
-        }
-        if (!general && ref > -INFINITY) {
-          float s0, s1;
-          f2_unpack(sum, s0, s1);
-          l += (s0 + s1) * ex2_approx(ref - mref);
-        }
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
@@ -716,45 +746,45 @@ __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constan
         }
       }
       if (!ok) break;
-      // ---- the unit's rows
+      // ---- the unit's rows (and the scale of the row's next query on its way)
+      const TileUnit done = u;
+      const bool write = mine;
+      have = take();
       ok = wait(B_O + tile, oit & 1u, TW_O);
       ++oit;
       if (!ok) break;
       tc_fence_after();
-      const float f = u.slot < 0 ? row_factor(mref, ref, l) : 1.f;
-      const long long row = (long long)u.slot * (2 * kTileRows) + tile * kTileRows + rr;
-      uint16_t* o16 = static_cast<uint16_t*>(p.o) + (long long)(u.t0 + tok) * p.on + h * p.oh;
+      const float f = done.slot < 0 ? row_factor(mref, ref, l) : 1.f;
+      const int h = done.head * p.ratio + hr;
+      const long long row = (long long)done.slot * (2 * kTileRows) + tile * kTileRows + rr;
+      uint16_t* o16 = static_cast<uint16_t*>(p.o) + (long long)(done.t0 + tok) * p.on + h * p.oh;
 #pragma unroll 1
-      for (int b = 0; b < D / 32; ++b) {
-        uint32_t o[32];
-        tmem_ld32(tO + b * 32, o);
-        tmem_ld_wait(o);
-        if (mine && u.slot < 0) {
+      for (int b = 0; b < D / 16; ++b) {
+        uint32_t o[16];
+        tmem_ld16(tO + b * 16, o);
+        tmem_ld_wait16(o);
+        if (write && done.slot < 0) {
 #pragma unroll
-          for (int k = 0; k < 32; k += 8) {
+          for (int k = 0; k < 16; k += 8) {
             uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float x0 = __uint_as_float(o[k + 2 * e]) * f, x1 = __uint_as_float(o[k + 2 * e + 1]) * f;
-              if (p.o_bf16) {
-                const __nv_bfloat162 y = __floats2bfloat162_rn(x0, x1);
-                w[e] = *reinterpret_cast<const uint32_t*>(&y);
-              } else {
-                const __half2 y = __floats2half2_rn(x0, x1);
-                w[e] = *reinterpret_cast<const uint32_t*>(&y);
-              }
+              const __nv_bfloat162 y = __floats2bfloat162_rn(x0, x1);
+              const __half2 z = __floats2half2_rn(x0, x1);
+              w[e] = p.o_bf16 ? *reinterpret_cast<const uint32_t*>(&y) : *reinterpret_cast<const uint32_t*>(&z);
             }
-            *reinterpret_cast<uint4*>(o16 + b * 32 + k) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(o16 + b * 16 + k) = make_uint4(w[0], w[1], w[2], w[3]);
           }
-        } else if (mine) {
+        } else if (write) {
 #pragma unroll
-          for (int k = 0; k < 32; k += 4) *reinterpret_cast<uint4*>(p.part + row * D + b * 32 + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+          for (int k = 0; k < 16; k += 4) *reinterpret_cast<uint4*>(p.part + row * D + b * 16 + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
         }
         __syncwarp();
       }
-      if (mine) {
-        if (u.slot >= 0) *reinterpret_cast<float4*>(p.part_ml + row * 4) = make_float4(mref, ref, l, 0.f);
-        else if (p.lse) p.lse[(long long)(u.t0 + tok) * p.H + h] = mref + log2f(l);
+      if (write) {
+        if (done.slot >= 0) *reinterpret_cast<float4*>(p.part_ml + row * 4) = make_float4(mref, ref, l, 0.f);
+        else if (p.lse) p.lse[(long long)(done.t0 + tok) * p.H + h] = mref + log2f(l);
       }
       tc_fence_before();
     }

@@ -36,19 +36,27 @@ __global__ void __launch_bounds__(kThreads, SPIN == kAny ? 2 : 3) rotary_kernel(
   const int b = (int)(token / p.N), n = (int)(token - (long long)b * p.N);
   Pieces at;
   at.place<SPIN>(threadIdx.x & ((1 << p.lpr_log) - 1), p.rot);
-  const T* x0 = static_cast<const T*>(p.x[0]) + b * p.xb[0] + n * p.xn[0];
-  const T* x1 = static_cast<const T*>(p.x[1]) + b * p.xb[1] + n * p.xn[1] - p.heads0 * p.xh[1];
-  T* y0 = static_cast<T*>(p.y[0]) + b * p.yb[0] + n * p.yn[0];
-  T* y1 = static_cast<T*>(p.y[1]) + b * p.yb[1] + n * p.yn[1] - p.heads0 * p.yh[1];
-  auto src = [&](int r) { return r < p.heads0 ? x0 + r * p.xh[0] : x1 + r * p.xh[1]; };
-  auto dst = [&](int r) { return r < p.heads0 ? y0 + r * p.yh[0] : y1 + r * p.yh[1]; };
+  // rows of one tensor at a time, so that a row's address is one addition
+  const T* x = nullptr;
+  T* y = nullptr;
+  long long xs = 0, ys = 0;
+  int left = 0;                                              // heads from this slot's next row on
+  auto tensor = [&](int w) {
+    const int heads = w ? p.heads - p.heads0 : p.heads0;
+    x = static_cast<const T*>(p.x[w]) + b * p.xb[w] + n * p.xn[w] + row0 * p.xh[w];
+    y = static_cast<T*>(p.y[w]) + b * p.yb[w] + n * p.yn[w] + row0 * p.yh[w];
+    xs = p.per_token * p.xh[w];
+    ys = p.per_token * p.yh[w];
+    left = heads - row0;
+  };
   Row16<T> in[U];
-  auto load = [&](int r) {
+  auto load = [&]() {
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (r + u * p.per_token < p.heads) in[u].load(src(r + u * p.per_token), at);
+      if (u * p.per_token < left) in[u].load(x + u * xs, at);
   };
-  load(row0);
+  tensor(0);
+  load();
   const long long pi = b * p.pos_b + n;
   const long long pos = p.pos64 ? static_cast<const long long*>(p.pos)[pi] : static_cast<const int*>(p.pos)[pi];
   const bool ok = pos >= 0 && pos < p.rows;
@@ -56,27 +64,37 @@ __global__ void __launch_bounds__(kThreads, SPIN == kAny ? 2 : 3) rotary_kernel(
   Turn<SPIN> turn;
   turn.load(p.table, ok ? pos : 0, p.rot, p.inverse, at);
 #pragma unroll 1
-  for (int r = row0; r < p.heads; r += U * p.per_token) {
-    if (r != row0) load(r);
+  for (int w = 0; w < 2; ++w) {
+    if (w == 1) {
+      if (p.heads == p.heads0) return;
+      tensor(1);
+      load();
+    }
+#pragma unroll 1
+    while (left > 0) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int row = r + u * p.per_token;
-      if (row >= p.heads) break;
-      float x[16];
-      widen16(in[u], x);
-      turn.apply(x, src(row), p.rot, at);
-      Raw<T> a, c;
-      narrow(reinterpret_cast<const float(&)[8]>(x[0]), a);
-      narrow(reinterpret_cast<const float(&)[8]>(x[8]), c);
-      // (what is not rotated as it is, a NaN's bits too)
-      if (at.a >= p.rot) a = in[u].a;
-      if (at.b >= p.rot) c = in[u].b;
-      if (!ok) {
-        a.zero();
-        c.zero();
+      for (int u = 0; u < U; ++u) {
+        if (u * p.per_token >= left) break;
+        float v[16];
+        widen16(in[u], v);
+        turn.apply(v, x + u * xs, p.rot, at);
+        Raw<T> a, c;
+        narrow(reinterpret_cast<const float(&)[8]>(v[0]), a);
+        narrow(reinterpret_cast<const float(&)[8]>(v[8]), c);
+        // (what is not rotated as it is, a NaN's bits too)
+        if (at.a >= p.rot) a = in[u].a;
+        if (at.b >= p.rot) c = in[u].b;
+        if (!ok) {
+          a.zero();
+          c.zero();
+        }
+        a.store(y + u * ys + at.a);
+        c.store(y + u * ys + at.b);
       }
-      a.store(dst(row) + at.a);
-      c.store(dst(row) + at.b);
+      x += U * xs;
+      y += U * ys;
+      left -= U * p.per_token;
+      load();
     }
   }
 }
@@ -87,9 +105,9 @@ int run(const RotaryJob& job, int D, bool interleaved, cudaStream_t stream) {
   p.lpr_log = 0;
   while ((16 << p.lpr_log) < D) ++p.lpr_log;
   const int slots = kThreads >> p.lpr_log;
-  // Slots a token: one for about 8 heads, so that the table and the position are paid for by 8 rows, but as many as there are
+  // Slots a token: one for about 16 heads, so that the table and the position are paid for by 16 rows, but as many as there are
   // heads where that leaves SMs without work (a decode step)
-  p.per_token = (p.heads + 7) / 8;
+  p.per_token = (p.heads + 15) / 16;
   while (p.per_token < p.heads && p.per_token < slots && p.tokens * p.per_token < 4LL * slots * sm_count_cached()) ++p.per_token;
   if (p.per_token > slots) p.per_token = slots;
   const int tokens_cta = slots / p.per_token;

@@ -191,14 +191,19 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+__device__ __forceinline__ float max_nan3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 __device__ __forceinline__ float absmax16(const float (&x)[16]) {
   float m = fabsf(x[0]), n = fabsf(x[1]);
 #pragma unroll
-  for (int i = 2; i < 16; i += 2) {
-    m = max_nan(m, fabsf(x[i]));
-    n = max_nan(n, fabsf(x[i + 1]));
+  for (int i = 2; i < 14; i += 4) {
+    m = max_nan3(m, fabsf(x[i]), fabsf(x[i + 1]));
+    n = max_nan3(n, fabsf(x[i + 2]), fabsf(x[i + 3]));
   }
-  return max_nan(m, n);
+  return max_nan3(max_nan(m, n), fabsf(x[14]), fabsf(x[15]));
 }
 // ... of a row held by LPR neighbouring lanes
 template <int LPR>
@@ -211,8 +216,9 @@ __device__ __forceinline__ float row_max(float m) {
 __device__ __forceinline__ float scale_of(float most) { return __fdiv_rn(most, 127.0f); }
 
 // Values as int8 codes: x/scale, rounded to fp32 and then to the nearest whole number (ties to even); zeros where the scale is 0 or not
-// finite.  The quotient is formed with an approximate reciprocal, whose error of less than 127 * 2^-21 decides nothing unless it
-// is that near to a border of two codes: then, which is once in 5 000 values, by a division.
+// finite.  The quotient is formed with an approximate reciprocal, whose error (2^-23 of up to 127, and as much for
+// the two products' rounding: less than 4e-5) decides nothing unless it is that near to a border of two codes: then, which is once in
+// 12 000 values, by a division.
 template <int N>
 __device__ __forceinline__ void codes(const float (&x)[N], float scale, uint32_t (&out)[N / 4]) {
   constexpr float kMagic = 12582912.0f;               // 1.5 * 2^23: the sum's low byte is the whole number
@@ -227,11 +233,11 @@ __device__ __forceinline__ void codes(const float (&x)[N], float scale, uint32_t
     const uint64_t q = f2_mul(f2_pack(x[i], x[i + 1]), inv2), t = f2_add(q, magic2);
     float d0, d1;
     f2_unpack(f2_fma(q, one2, f2_add(t, minus2)), d0, d1);             // whole number - quotient
-    off = fmaxf(off, fmaxf(fabsf(d0), fabsf(d1)));
+    off = max3(off, fabsf(d0), fabsf(d1));
     f2_unpacku(t, b[i], b[i + 1]);
   }
   // (an `off` that is not small, a scale whose reciprocal is not a normal number: the careful way)
-  if (ok && !(off < 0.4998f && scale > 1e-37f && scale < 1e37f)) {
+  if (ok && !(off < 0.49996f && scale > 1e-37f && scale < 1e37f)) {
 #pragma unroll
     for (int i = 0; i < N; ++i) b[i] = __float_as_uint(__fadd_rn(fminf(fmaxf(__fdiv_rn(x[i], scale), -127.f), 127.f), kMagic));
   }
