@@ -934,7 +934,7 @@ int paged_attention(const IntfaPagedParams* a, cudaStream_t stream) {
   if (pl.tiles) {
     p.rows_tile = 2 * kTileRows;
     p.tile_tokens = kTileRows / p.ratio;
-    p.box_log = c.page_size < tile_keys(c.D) ? p.page_log : log2_of(tile_keys(c.D));
+    p.box_log = c.page_size < kTileKeys ? p.page_log : log2_of(kTileKeys);
     p.least = 2;
     return c.D == 64 ? run_tiles<64>(a, pl, p, stream) : run_tiles<128>(a, pl, p, stream);
   }

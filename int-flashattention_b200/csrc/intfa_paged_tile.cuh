@@ -2,17 +2,17 @@
 // (Included by intfa_paged_attn.cu inside namespace intfa, after the shared helpers.)
 //
 // A unit is (sequence, K/V head, 256 rows): two tiles of 128 rows, each the rows of as many whole tokens as fit, all query heads of the
-// K/V head packed.  The units' chunks of 64 or 128 keys (those that the last row of a unit sees) are dealt out to the CTAs, one an SM, in equal
+// K/V head packed.  The units' chunks of 64 keys (those that the last row of a unit sees) are dealt out to the CTAs, one an SM, in equal
 // contiguous shares; parts of units that are cut go to scratch and combine_kernel adds them up, as in the kernel for few rows.
 //
 // 512 threads:
 //   warp 0       TMA: Q once per unit (heads x tokens boxes), K and V pages of 8 rows and more each
-//   warp 1       MMA issuer.  For each tile in turn: P V of the last chunk, S = Q K^T of the next
+//   warp 1       MMA issuer.  For each tile in turn: P V of a chunk, S = Q K^T of the one after the next
 //   warp 2       TMEM; K scales, log2 and reciprocal of the V scales of a chunk into a ring
 //   warp 3       goes through the units and publishes them
 //   warps 4-7    V from int8 (as TMA left it) to fp16 in the MN-major tiles that P V takes
-//   warps 8-11, 12-15   softmax of tile 0 and of tile 1, one thread a row: while one tile is in the tensor core the other is here
-// TMEM: S of both tiles, their P (fp16), two accumulators of D columns.  S of the next chunk is there before P V of this one is done.
+//   warps 8-11, 12-15   softmax of tile 0 and of tile 1, one thread a row
+// TMEM: two S buffers of each tile, P (fp16) over the scores it was made of, two accumulators of D columns.  S is two chunks ahead of P V.
 //
 // The arithmetic is that of the kernel for few rows: w = p v_scale relative to a reference near its running maximum, P = fp16(w), l = sum p
 // relative to a reference of its own.  The references follow only where w gets 2^8 ahead: the accumulator is rescaled in a few chunks of
@@ -22,10 +22,9 @@
 #pragma once
 
 constexpr int kTileRows = 128;
-// Keys of a chunk.  S and P of both tiles and the accumulators share the 512 columns of TMEM.
-__host__ __device__ constexpr int tile_keys(int D) { return D == 64 ? 128 : 64; }
-constexpr int kTileService = 56, kTileConvert = 72, kTileSoftmax = 192;          // registers
-static_assert(128 * (kTileService + kTileConvert) + 256 * kTileSoftmax <= 65536, "setmaxnreg budget");
+constexpr int kTileKeys = 64;                     // keys of a chunk: two S buffers of two tiles and two accumulators of 128 fill TMEM
+constexpr int kTileThreads = 512, kTileLaunch = 128, kTileService = 56, kTileConvert = 72, kTileSoftmax = 192;        // registers
+static_assert(128 * (kTileService + kTileConvert) + 256 * kTileSoftmax <= kTileThreads * kTileLaunch, "setmaxnreg budget");
 
 // a unit, or the part of it that a CTA does
 struct __align__(16) TileUnit {
@@ -88,7 +87,7 @@ __device__ inline long long tile_chunks_before(const PParams& p, const TileSeq& 
 
 template <int D>
 struct TileCfg {
-  static constexpr int G = tile_keys(D), THREADS = 512, NK = D == 64 ? 4 : 5, NV8 = 4, NV = D == 64 ? 3 : 3, NSC = 8, NU = 4;
+  static constexpr int G = kTileKeys, THREADS = kTileThreads, NK = 5, NV8 = 4, NV = 3, NSC = 8, NU = 4;
   static constexpr int Q_BYTES = kTileRows * D, K_BYTES = G * D, V_BYTES = G * D * 2;
   static constexpr int SC_FLOATS = 3 * G + 4;
   static constexpr int OFF_Q = 0, OFF_K = OFF_Q + 2 * Q_BYTES, OFF_V8 = OFF_K + NK * K_BYTES, OFF_V = OFF_V8 + NV8 * K_BYTES;
@@ -96,13 +95,13 @@ struct TileCfg {
   static constexpr int OFF_SC = OFF_ARM + 4096;
   static constexpr int OFF_UNIT = OFF_SC + NSC * SC_FLOATS * 4;
   static constexpr int OFF_PRE = OFF_UNIT + NU * (int)sizeof(TileUnit);
-  static constexpr int NBARS = 4 + 2 * NK + 2 * NV8 + 2 * NV + 2 * NSC + 2 * NU + 6;
+  static constexpr int NBARS = 4 + 2 * NK + 2 * NV8 + 2 * NV + 2 * NSC + 2 * NU + 12;
   static constexpr int OFF_BAR = OFF_PRE + (THREADS + 2) * 8;
   static constexpr int OFF_MISC = OFF_BAR + NBARS * 8;
   static constexpr int SMEM = OFF_MISC + 32 + 1024;
   static_assert(SMEM <= 227 * 1024, "shared memory");
   static_assert(OFF_UNIT % 16 == 0 && OFF_SC % 16 == 0 && OFF_PRE % 8 == 0, "alignment");
-  static constexpr int COL_S = 0, COL_P = 2 * G, COL_O = 3 * G;
+  static constexpr int COL_S = 0, COL_O = 4 * G;
   static_assert(COL_O + 2 * D <= 512, "TMEM columns");
   static constexpr uint64_t SWZ_QK = D == 128 ? kSwz128 : kSwz64;
   static constexpr uint32_t IDESC_QK = make_idesc(2, 1, 1, 0, 0, kTileRows, G);
@@ -113,7 +112,7 @@ struct TileCfg {
 enum TileWait { TW_UNIT = 65, TW_UEMPTY, TW_QE, TW_KE, TW_V8E, TW_QF, TW_KF, TW_VF, TW_P, TW_SCE, TW_V8F, TW_VE, TW_SC, TW_S, TW_O };
 
 template <int D>
-__global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+__global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                                                             const __grid_constant__ CUtensorMap tmV, const PParams p) {
   using C = TileCfg<D>;
   constexpr int G = C::G;
@@ -128,8 +127,8 @@ __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constan
   constexpr int B_VF = B_V8E + C::NV8, B_VE = B_VF + C::NV;      // converting warps (4); commit
   constexpr int B_SCF = B_VE + C::NV, B_SCE = B_SCF + C::NSC;    // scale loader; softmax warps (8)
   constexpr int B_UF = B_SCE + C::NSC, B_UE = B_UF + C::NU;      // unit published; taken over by TMA, MMA, scale, converting, softmax warps (15)
-  constexpr int B_S = B_UE + C::NU, B_P = B_S + 2, B_O = B_P + 2;        // [2] commit: S; softmax warps of the tile (4): S read, P written; commit: P V
-  static_assert(B_O + 2 == C::NBARS, "barriers");
+  constexpr int B_S = B_UE + C::NU, B_P = B_S + 4, B_O = B_P + 4;        // [tile][buffer of the chunk] commit: S; softmax warps of the tile (4): S read, P written; commit: P V
+  static_assert(B_O + 4 == C::NBARS, "barriers");
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 8);
   TileUnit* units = reinterpret_cast<TileUnit*>(smem + C::OFF_UNIT);
@@ -139,9 +138,12 @@ __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constan
     for (int i = 0; i < 2; ++i) {
       mbar_init(BAR(B_QF + i), 1);
       mbar_init(BAR(B_QE + i), 1);
-      mbar_init(BAR(B_S + i), 1);
-      mbar_init(BAR(B_P + i), 4);
-      mbar_init(BAR(B_O + i), 1);
+      mbar_init(BAR(B_S + 2 * i), 1);
+      mbar_init(BAR(B_S + 2 * i + 1), 1);
+      mbar_init(BAR(B_P + 2 * i), 4);
+      mbar_init(BAR(B_P + 2 * i + 1), 4);
+      mbar_init(BAR(B_O + 2 * i), 1);
+      mbar_init(BAR(B_O + 2 * i + 1), 1);
     }
     for (int i = 0; i < C::NK; ++i) {
       mbar_init(BAR(B_KF + i), 1);
@@ -381,51 +383,75 @@ __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constan
       const uint64_t descQ = make_smem_desc(sQ, 16, 8 * D, C::SWZ_QK), descK = make_smem_desc(sK, 16, 8 * D, C::SWZ_QK);
       const uint64_t descV = make_smem_desc(sV, D > 64 ? G * 128 : 16, 8 * 128, kSwz128);
       const uint64_t descArm = make_smem_desc(smem_u32(smem + C::OFF_ARM), 128, 256, 0);
-      uint32_t kit = 0, vit = 0, uit = 0, pit = 0;             // chunks of K, of V; bit i: units, P tiles of tile i mod 2
+      uint32_t kit = 0, vit = 0;                               // chunks of K, of V
+      uint32_t uit = 0, sit = 0, pit = 0;                      // bit i: units, S tiles of tile i mod 2; bits 2i, 2i + 1: P tiles mod 4
       TileUnit u;
       bool ok = true;
+      // S of a chunk of tile i into its buffer `buf`
+      auto scores = [&](int i, uint32_t buf, uint32_t k, bool last) {
+        const uint32_t tS = tmem + C::COL_S + (2 * i + buf) * G;
+        umma_f16(tS, descArm, descArm, C::IDESC_ARM, 0);
+#pragma unroll
+        for (int kk = 0; kk < D / 32; ++kk)
+          umma_i8(tS, descQ + (uint64_t)(i * (C::Q_BYTES >> 4) + 2 * kk), descK + (uint64_t)(k * (C::K_BYTES >> 4) + 2 * kk), C::IDESC_QK, 1);
+        umma_commit(BAR(B_S + 2 * i + buf));
+        if (last) umma_commit(BAR(B_QE + i));
+      };
       while (ok && next_unit(u)) {
         const int n = u.c1 - u.c0, two = u.tokens > p.tile_tokens;
-        for (int j = 0; j <= n && ok; ++j) {
-          const uint32_t k = kit % C::NK, v = vit % C::NV;
-          if (j < n) ok = wait(B_KF + k, (kit / C::NK) & 1u, TW_KF);
-          if (ok && j > 0) ok = wait(B_VF + v, (vit / C::NV) & 1u, TW_VF);
+#pragma unroll 1
+        for (int j = 0; j < 2 && j < n && ok; ++j) {
+          const uint32_t k = kit % C::NK;
+          ok = wait(B_KF + k, (kit / C::NK) & 1u, TW_KF);
 #pragma unroll 1
           for (int i = 0; i <= two && ok; ++i) {
-            const uint32_t tS = tmem + C::COL_S + i * G, tP = tmem + C::COL_P + i * (G / 2), tO = tmem + C::COL_O + i * D;
             if (j == 0) ok = wait(B_QF + i, uit >> i & 1u, TW_QF);
-            else ok = wait(B_P + i, pit >> i & 1u, TW_P);
             if (!ok) break;
-            if (j > 0) pit ^= 1u << i;
             tc_fence_after();
             if (elect_one()) {
-              // (the tile's softmax warps are done with S and have written P; S of the next chunk first, they wait for it)
-              if (j < n) {
-                umma_f16(tS, descArm, descArm, C::IDESC_ARM, 0);
+              scores(i, sit >> i & 1u, k, j + 1 == n);
+              if (i == two) umma_commit(BAR(B_KE + k));
+            }
+            __syncwarp();
+            sit ^= 1u << i;
+          }
+          ++kit;
+        }
+        uit ^= two ? 3u : 1u;
+#pragma unroll 1
+        for (int j = 0; j < n && ok; ++j) {
+          const uint32_t k = kit % C::NK, v = vit % C::NV;
+          const bool more = j + 2 < n;
+          ok = wait(B_VF + v, (vit / C::NV) & 1u, TW_VF);
+          if (ok && more) ok = wait(B_KF + k, (kit / C::NK) & 1u, TW_KF);
+#pragma unroll 1
+          for (int i = 0; i <= two && ok; ++i) {
+            // (a buffer's barrier: warps whose S is there may be a chunk ahead of the others)
+            const uint32_t buf = pit >> (2 * i) & 1u;
+            ok = wait(B_P + 2 * i + buf, pit >> (2 * i + 1) & 1u, TW_P);
+            if (!ok) break;
+            pit = (pit & ~(3u << (2 * i))) | (((pit >> (2 * i)) + 1u & 3u) << (2 * i));
+            tc_fence_after();
+            const uint32_t tP = tmem + C::COL_S + (2 * i + buf) * G, tO = tmem + C::COL_O + i * D;
+            if (elect_one()) {
+              const uint64_t vd = descV + (uint64_t)(v * (C::V_BYTES >> 4));
 #pragma unroll
-                for (int kk = 0; kk < D / 32; ++kk)
-                  umma_i8(tS, descQ + (uint64_t)(i * (C::Q_BYTES >> 4) + 2 * kk), descK + (uint64_t)(k * (C::K_BYTES >> 4) + 2 * kk), C::IDESC_QK, 1);
-                umma_commit(BAR(B_S + i));
-                if (j + 1 == n) umma_commit(BAR(B_QE + i));
-              }
-              if (j > 0) {
-                const uint64_t vd = descV + (uint64_t)(v * (C::V_BYTES >> 4));
-#pragma unroll
-                for (int kk = 0; kk < G / 16; ++kk)
-                  umma_f16_ts(tO, tP + kk * 8, vd + (uint64_t)(kk * ((16 * 128) >> 4)), C::IDESC_PV, j > 1 || kk > 0 ? 1u : 0u);
-                umma_commit(BAR(B_O + i));
-              }
+              for (int kk = 0; kk < G / 16; ++kk)
+                umma_f16_ts(tO, tP + kk * 16, vd + (uint64_t)(kk * ((16 * 128) >> 4)), C::IDESC_PV, j > 0 || kk > 0 ? 1u : 0u);
+              umma_commit(BAR(B_O + 2 * i + buf));
+              // (the tensor core takes them in this order: S of the chunk after the next comes over P when the P V that reads it is done)
+              if (more) scores(i, buf, k, j + 3 == n);
               if (i == two) {
-                if (j < n) umma_commit(BAR(B_KE + k));
-                if (j > 0) umma_commit(BAR(B_VE + v));
+                umma_commit(BAR(B_VE + v));
+                if (more) umma_commit(BAR(B_KE + k));
               }
             }
             __syncwarp();
+            if (more) sit ^= 1u << i;
           }
-          if (j < n) ++kit;
-          if (j > 0) ++vit;
+          ++vit;
+          if (more) ++kit;
         }
-        uit ^= two ? 3u : 1u;
       }
     } else {
       // ------------------------------------------------------------------ scales
@@ -544,11 +570,12 @@ __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constan
   } else {
     reg_alloc<kTileSoftmax>();
     // -------------------------------------------------------------------- softmax, one thread a row
+    constexpr int NB = G / 16;                                 // blocks of 16 columns
     const int tile = (warp - 8) >> 2, rr = threadIdx.x & 127;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;         // (lane 32 * (warp % 4) in bits 16 and up)
-    const uint32_t tS = tmem + C::COL_S + tile * G + lanes, tP = tmem + C::COL_P + tile * (G / 2) + lanes, tO = tmem + C::COL_O + tile * D + lanes;
+    const uint32_t tS0 = tmem + C::COL_S + tile * 2 * G + lanes, tO = tmem + C::COL_O + tile * D + lanes;
     const int tok = tile * p.tile_tokens + rr / p.ratio, hr = rr % p.ratio;
-    uint32_t sit = 0, it = 0, oit = 0;                         // S tiles, chunks, units of this tile so far
+    uint32_t sit = 0, it = 0;                                  // chunks of this tile, of all so far
     // what a row needs of its unit; the scale of its query is asked for here and used a while later
     TileUnit u;
     float qs_raw = 0.f;
@@ -577,24 +604,25 @@ __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constan
       float mref = -INFINITY, ref = -INFINITY, l = 0.f;        // references of p and of w (of the accumulator)
       for (int c = u.c0; c < u.c1; ++c, ++it, ++sit) {
         const uint32_t slot = it % C::NSC;
-        ok = wait(B_SCF + slot, (it / C::NSC) & 1u, TW_SC) && wait(B_S + tile, sit & 1u, TW_S);
+        ok = wait(B_SCF + slot, (it / C::NSC) & 1u, TW_SC) && wait(B_S + 2 * tile + (sit & 1u), sit >> 1 & 1u, TW_S);
         if (!ok) break;
         tc_fence_after();
+        const uint32_t tS = tS0 + (sit & 1u) * G;
         const float* sc = reinterpret_cast<const float*>(smem + C::OFF_SC) + slot * C::SC_FLOATS;
         const float lo = sc[3 * G], hi = sc[3 * G + 1];
         const long long rel64 = lim - (long long)c * G;
-        const int rel = rel64 < -1 ? -1 : rel64 > G ? G : (int)rel64;        // the last column that the row sees
+        const int rel = rel64 < -1 ? -1 : rel64 > G ? G : (int)rel64;      // the last column that the row sees
         const int rel_least = (int)__reduce_min_sync(0xffffffffu, rel), rel_most = (int)__reduce_max_sync(0xffffffffu, rel);
         // exponents of w, x + log2 v_scale - off, of 16 columns, in place of the scores
         auto exponents = [&](int b, uint32_t (&r)[16], float off) {
           const uint64_t off2 = f2_pack(-off, -off);
-          const float4* ks = reinterpret_cast<const float4*>(sc + b * 16);
-          const float4* lv = reinterpret_cast<const float4*>(sc + G + b * 16);
+          const ulonglong2* ks = reinterpret_cast<const ulonglong2*>(sc + b * 16);
+          const ulonglong2* lv = reinterpret_cast<const ulonglong2*>(sc + G + b * 16);
 #pragma unroll
           for (int k = 0; k < 16; k += 4) {
-            const float4 a = ks[k / 4], v = lv[k / 4];
-            f2_unpacku(f2_fma(f2_add(f2_packu(r[k], r[k + 1]), magic2), f2_mul(f2_pack(a.x, a.y), qs2), f2_add(f2_pack(v.x, v.y), off2)), r[k], r[k + 1]);
-            f2_unpacku(f2_fma(f2_add(f2_packu(r[k + 2], r[k + 3]), magic2), f2_mul(f2_pack(a.z, a.w), qs2), f2_add(f2_pack(v.z, v.w), off2)), r[k + 2], r[k + 3]);
+            const ulonglong2 a = ks[k / 4], v = lv[k / 4];
+            f2_unpacku(f2_fma(f2_add(f2_packu(r[k], r[k + 1]), magic2), f2_mul(a.x, qs2), f2_add(v.x, off2)), r[k], r[k + 1]);
+            f2_unpacku(f2_fma(f2_add(f2_packu(r[k + 2], r[k + 3]), magic2), f2_mul(a.y, qs2), f2_add(v.y, off2)), r[k + 2], r[k + 3]);
           }
           if (b * 16 + 15 > rel_least) {
             const int last = rel - b * 16;
@@ -602,41 +630,38 @@ __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constan
             for (int k = 0; k < 16; ++k) r[k] = k <= last ? r[k] : __float_as_uint(-INFINITY);
           }
         };
-        auto largest = [&](const uint32_t (&r)[16], float (&mx)[2]) {
-#pragma unroll
-          for (int k = 0; k < 16; k += 4) {
-            mx[0] = max3(mx[0], __uint_as_float(r[k]), __uint_as_float(r[k + 1]));
-            mx[1] = max3(mx[1], __uint_as_float(r[k + 2]), __uint_as_float(r[k + 3]));
-          }
-        };
-        // The references are taken over as they are, and P is made with them in one go; only where some w comes out above 2^8 (or a row
-        // has no reference yet: in a unit's first chunk) the maxima are found first.
+        // The references are taken over as they are, and P is made with them in one go.  The sum of p = w / v_scale bounds every w (w <= sum p
+        // times the largest v_scale); where that does not say that all w are below 2^15, or a row has no reference yet, the reference is
+        // looked for: in a unit's first chunk in 16 columns, then, if need be, in all.
         uint64_t sum2;
-        bool find = c == u.c0, settled = c == u.c0;            // settled: P V of the chunk before is done
+        uint32_t pk[8 * NB];
+        float total = 0.f;
+        int find = c == u.c0 ? 1 : 0;                          // columns to look at: none, 16, all
+        const float most = hi < 100.f ? ex2_approx(15.f - hi) : 0.f;
         for (;;) {
           if (find) {
-            float mx[2] = {-INFINITY, -INFINITY};
+            float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll 1
-            for (int b = 0; b * 16 <= rel_most && b < G / 16; ++b) {
+            for (int b = 0; b * 16 <= rel_most && b < (find == 1 ? 1 : NB); ++b) {
               uint32_t r[16];
               tmem_ld16(tS + b * 16, r);
               tmem_ld_wait16(r);
               exponents(b, r, 0.f);
-              largest(r, mx);
+#pragma unroll
+              for (int k = 0; k < 16; k += 4) {
+                mx0 = max3(mx0, __uint_as_float(r[k]), __uint_as_float(r[k + 1]));
+                mx1 = max3(mx1, __uint_as_float(r[k + 2]), __uint_as_float(r[k + 3]));
+              }
             }
-            const float top = fmaxf(mx[0], mx[1]);
+            const float top = fmaxf(mx0, mx1);
             const float to = top > ref ? top : ref, f = ref == -INFINITY ? 0.f : ex2_approx(ref - to);
             // (the reference of p as far from the largest p as a middling V scale is from 1; it stays until `easy` does not hold)
             if (to > -INFINITY && mref == -INFINITY && hi - lo < 60.f) mref = to - 0.5f * (lo + hi);
             ref = to;
-            if (!settled) {
-              ok = wait(B_O + tile, oit & 1u, TW_O);
-              if (!ok) break;
-              ++oit;
-              settled = true;
-              tc_fence_after();
-            }
             if (c > u.c0) {                                    // (the first P V does not look at what is there)
+              ok = wait(B_O + 2 * tile + ((sit - 1u) & 1u), (sit - 1u) >> 1 & 1u, TW_O);       // P V of the chunk before is done
+              if (!ok) break;
+              tc_fence_after();
               const uint64_t f2 = f2_pack(f, f);
 #pragma unroll 1
               for (int b = 0; b < D / 16; ++b) {
@@ -650,57 +675,41 @@ __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constan
             }
           }
           const float base = safe(ref);
-          float mx[2] = {-INFINITY, -INFINITY};
           sum2 = 0;
-          // (two buffers of 16 columns in a rolled loop: the instruction cache has to hold the loops of all roles)
           uint32_t buf[2][16];
           tmem_ld16(tS, buf[0]);
-#pragma unroll 1
-          for (int b2 = 0; b2 < G / 16; b2 += 2) {
 #pragma unroll
-            for (int e2 = 0; e2 < 2; ++e2) {
-              const int b = b2 + e2;
-              uint32_t(&r)[16] = buf[e2];
-              tmem_ld_wait16(r);
-              if (e2 == 0 || b2 + 2 < G / 16) tmem_ld16(tS + (b + 1) * 16, buf[e2 ^ 1]);
-              exponents(b, r, base);
-              largest(r, mx);
-              uint32_t pk[8];
-              const float4* iv = reinterpret_cast<const float4*>(sc + 2 * G + b * 16);
+          for (int b = 0; b < NB; ++b) {
+            uint32_t(&r)[16] = buf[b & 1];
+            tmem_ld_wait16(r);
+            if (b + 1 < NB) tmem_ld16(tS + (b + 1) * 16, buf[(b + 1) & 1]);
+            exponents(b, r, base);
+            const ulonglong2* iv = reinterpret_cast<const ulonglong2*>(sc + 2 * G + b * 16);
 #pragma unroll
-              for (int k = 0; k < 16; k += 4) {
-                const float4 v = iv[k / 4];
-                const float w0 = ex2_approx(__uint_as_float(r[k])), w1 = ex2_approx(__uint_as_float(r[k + 1]));
-                const float w2 = ex2_approx(__uint_as_float(r[k + 2])), w3 = ex2_approx(__uint_as_float(r[k + 3]));
-                sum2 = f2_fma(f2_pack(w0, w1), f2_pack(v.x, v.y), sum2);
-                sum2 = f2_fma(f2_pack(w2, w3), f2_pack(v.z, v.w), sum2);
-                const __half2 y0 = __floats2half2_rn(w0, w1), y1 = __floats2half2_rn(w2, w3);
-                pk[k / 2] = *reinterpret_cast<const uint32_t*>(&y0);
-                pk[k / 2 + 1] = *reinterpret_cast<const uint32_t*>(&y1);
-              }
-              if (e2 == 0 && !settled) {         // (P and the accumulator are the P V's of the chunk before until then)
-                ok = wait(B_O + tile, oit & 1u, TW_O);
-                ++oit;
-                settled = true;
-                tc_fence_after();
-              }
-              tmem_st8(tP + b * 8, pk);
+            for (int k = 0; k < 16; k += 4) {
+              const ulonglong2 v = iv[k / 4];
+              const float w0 = ex2_approx(__uint_as_float(r[k])), w1 = ex2_approx(__uint_as_float(r[k + 1]));
+              const float w2 = ex2_approx(__uint_as_float(r[k + 2])), w3 = ex2_approx(__uint_as_float(r[k + 3]));
+              sum2 = f2_fma(f2_pack(w0, w1), v.x, sum2);
+              sum2 = f2_fma(f2_pack(w2, w3), v.y, sum2);
+              const __half2 y0 = __floats2half2_rn(w0, w1), y1 = __floats2half2_rn(w2, w3);
+              pk[b * 8 + k / 2] = *reinterpret_cast<const uint32_t*>(&y0);
+              pk[b * 8 + k / 2 + 1] = *reinterpret_cast<const uint32_t*>(&y1);
             }
           }
-          if (!ok) break;
-          const float top = fmaxf(mx[0], mx[1]);
-          if (!__any_sync(0xffffffffu, top > 8.f || (ref == -INFINITY && top > -INFINITY))) break;
-          find = true;
+          {
+            float s0, s1;
+            f2_unpack(sum2, s0, s1);
+            total = s0 + s1;
+          }
+          if (find == 2 || !__any_sync(0xffffffffu, !(total < most) || (ref == -INFINITY && total > 0.f))) break;
+          find = 2;
         }
         if (!ok) break;
         const float d = ref - mref;
         const bool easy = ref == -INFINITY ? mref == -INFINITY && lo > -INFINITY : lo >= d - 60.f && hi <= d + 60.f;
         if (__all_sync(0xffffffffu, easy)) {
-          if (ref > -INFINITY) {
-            float s0, s1;
-            f2_unpack(sum2, s0, s1);
-            l = fmaf(s0 + s1, ex2_approx(d), l);
-          }
+          if (ref > -INFINITY) l = fmaf(total, ex2_approx(d), l);
         } else {
           // p by itself: the scores once more
           float top = -INFINITY;
@@ -709,7 +718,7 @@ __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constan
             float sum = 0.f;
             const float base = safe(mref);
 #pragma unroll 1
-            for (int b = 0; b < G / 16; ++b) {
+            for (int b = 0; b < NB; ++b) {
               uint32_t o[16];
               tmem_ld16(tS + b * 16, o);
               tmem_ld_wait16(o);
@@ -737,11 +746,14 @@ __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constan
             }
           }
         }
+        // P over the scores it was made of: 16 keys in the first 8 of their 16 columns
+#pragma unroll
+        for (int b = 0; b < NB; ++b) tmem_st8(tS + b * 16, reinterpret_cast<const uint32_t(&)[8]>(pk[b * 8]));
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(BAR(B_P + tile));
+          mbar_arrive(BAR(B_P + 2 * tile + (sit & 1u)));
           mbar_arrive(BAR(B_SCE + slot));
         }
       }
@@ -750,8 +762,7 @@ __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constan
       const TileUnit done = u;
       const bool write = mine;
       have = take();
-      ok = wait(B_O + tile, oit & 1u, TW_O);
-      ++oit;
+      ok = wait(B_O + 2 * tile + ((sit - 1u) & 1u), (sit - 1u) >> 1 & 1u, TW_O);
       if (!ok) break;
       tc_fence_after();
       const float f = done.slot < 0 ? row_factor(mref, ref, l) : 1.f;
@@ -764,18 +775,17 @@ __global__ void __launch_bounds__(512, 1) paged_tile_kernel(const __grid_constan
         tmem_ld16(tO + b * 16, o);
         tmem_ld_wait16(o);
         if (write && done.slot < 0) {
+          uint32_t w[8];
 #pragma unroll
-          for (int k = 0; k < 16; k += 8) {
-            uint32_t w[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float x0 = __uint_as_float(o[k + 2 * e]) * f, x1 = __uint_as_float(o[k + 2 * e + 1]) * f;
-              const __nv_bfloat162 y = __floats2bfloat162_rn(x0, x1);
-              const __half2 z = __floats2half2_rn(x0, x1);
-              w[e] = p.o_bf16 ? *reinterpret_cast<const uint32_t*>(&y) : *reinterpret_cast<const uint32_t*>(&z);
-            }
-            *reinterpret_cast<uint4*>(o16 + b * 16 + k) = make_uint4(w[0], w[1], w[2], w[3]);
+          for (int e = 0; e < 8; ++e) {
+            const float x0 = __uint_as_float(o[2 * e]) * f, x1 = __uint_as_float(o[2 * e + 1]) * f;
+            const __nv_bfloat162 y = __floats2bfloat162_rn(x0, x1);
+            const __half2 z = __floats2half2_rn(x0, x1);
+            w[e] = p.o_bf16 ? *reinterpret_cast<const uint32_t*>(&y) : *reinterpret_cast<const uint32_t*>(&z);
           }
+          uint4* to = reinterpret_cast<uint4*>(o16 + b * 16);
+          to[0] = make_uint4(w[0], w[1], w[2], w[3]);
+          to[1] = make_uint4(w[4], w[5], w[6], w[7]);
         } else if (write) {
 #pragma unroll
           for (int k = 0; k < 16; k += 4) *reinterpret_cast<uint4*>(p.part + row * D + b * 16 + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);

@@ -54,11 +54,14 @@ class Setup:
     def args(self, causal=True):
         return (self.q8, self.kc, self.vc, self.qs, self.ks, self.vs, self.table, self.lens, self.cu, causal, self.scale)
 
+    def tolerance(self, want, A, B, out_dtype=torch.float16, more=0.0):
+        n = int(self.lens.max())
+        return (2.0 ** -11 + 2.0 ** -16 + more + (n / 8 + 64) * 2.0 ** -24) * A + n * 2.0 ** -25 * 2 * B[..., None] + EPS[out_dtype] * want.abs() + 2.0 ** -25
+
     def check(self, pkg, causal=True, out_dtype=torch.float16, got=None, more=0.0):
         o, lse = pkg.attention_int8_paged(*self.args(causal), out_dtype=out_dtype, return_lse=True) if got is None else got
         want, wlse, A, B = O.attention(self.q8, self.qs, self.kc, self.vc, self.ks, self.vs, self.table, self.lens, self.cu, causal, self.scale)
-        n = int(self.lens.max())
-        tol = (2.0 ** -11 + 2.0 ** -16 + more + (n / 8 + 64) * 2.0 ** -24) * A + n * 2.0 ** -25 * 2 * B[..., None] + EPS[out_dtype] * want.abs() + 2.0 ** -25
+        tol = self.tolerance(want, A, B, out_dtype, more)
         assert o.dtype == out_dtype
         off = (o.double() - want).abs()
         assert (off <= tol).all(), (float((off / tol).max()), torch.nonzero(~(off <= tol))[:5].tolist())
