@@ -37,6 +37,11 @@ struct __align__(16) TileUnit {
 };
 static_assert(sizeof(TileUnit) == 48, "unit");
 
+template <bool B>
+struct Flag {
+  static constexpr bool value = B;
+};
+
 struct TileSeq {
   int t0, n, keys, tiles, uniform;
   long long first;
@@ -614,7 +619,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         const int rel = rel64 < -1 ? -1 : rel64 > G ? G : (int)rel64;      // the last column that the row sees
         const int rel_least = (int)__reduce_min_sync(0xffffffffu, rel), rel_most = (int)__reduce_max_sync(0xffffffffu, rel);
         // exponents of w, x + log2 v_scale - off, of 16 columns, in place of the scores
-        auto exponents = [&](int b, uint32_t (&r)[16], float off) {
+        auto exponents = [&](int b, uint32_t* r, float off, bool mask) {
           const uint64_t off2 = f2_pack(-off, -off);
           const ulonglong2* ks = reinterpret_cast<const ulonglong2*>(sc + b * 16);
           const ulonglong2* lv = reinterpret_cast<const ulonglong2*>(sc + G + b * 16);
@@ -624,7 +629,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
             f2_unpacku(f2_fma(f2_add(f2_packu(r[k], r[k + 1]), magic2), f2_mul(a.x, qs2), f2_add(v.x, off2)), r[k], r[k + 1]);
             f2_unpacku(f2_fma(f2_add(f2_packu(r[k + 2], r[k + 3]), magic2), f2_mul(a.y, qs2), f2_add(v.y, off2)), r[k + 2], r[k + 3]);
           }
-          if (b * 16 + 15 > rel_least) {
+          if (mask) {
             const int last = rel - b * 16;
 #pragma unroll
             for (int k = 0; k < 16; ++k) r[k] = k <= last ? r[k] : __float_as_uint(-INFINITY);
@@ -633,7 +638,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         // The references are taken over as they are, and P is made with them in one go.  The sum of p = w / v_scale bounds every w (w <= sum p
         // times the largest v_scale); where that does not say that all w are below 2^15, or a row has no reference yet, the reference is
         // looked for: in a unit's first chunk in 16 columns, then, if need be, in all.
-        uint64_t sum2;
+        uint64_t sum2, sum3;
         uint32_t pk[8 * NB];
         float total = 0.f;
         int find = c == u.c0 ? 1 : 0;                          // columns to look at: none, 16, all
@@ -646,7 +651,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
               uint32_t r[16];
               tmem_ld16(tS + b * 16, r);
               tmem_ld_wait16(r);
-              exponents(b, r, 0.f);
+              exponents(b, r, 0.f, true);
 #pragma unroll
               for (int k = 0; k < 16; k += 4) {
                 mx0 = max3(mx0, __uint_as_float(r[k]), __uint_as_float(r[k + 1]));
@@ -675,32 +680,40 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
             }
           }
           const float base = safe(ref);
-          sum2 = 0;
-          uint32_t buf[2][16];
-          tmem_ld16(tS, buf[0]);
+          sum2 = sum3 = 0;
+          // (all columns of a chunk at once, in a straight line: there are two such warps a scheduler, and only what is independent within one
+          // hides the latencies)
+          auto make_p = [&](auto mask) {
+            uint32_t r[G];
 #pragma unroll
-          for (int b = 0; b < NB; ++b) {
-            uint32_t(&r)[16] = buf[b & 1];
-            tmem_ld_wait16(r);
-            if (b + 1 < NB) tmem_ld16(tS + (b + 1) * 16, buf[(b + 1) & 1]);
-            exponents(b, r, base);
-            const ulonglong2* iv = reinterpret_cast<const ulonglong2*>(sc + 2 * G + b * 16);
+            for (int b = 0; b < G; b += 32) tmem_ld32(tS + b, *reinterpret_cast<uint32_t(*)[32]>(r + b));
 #pragma unroll
-            for (int k = 0; k < 16; k += 4) {
-              const ulonglong2 v = iv[k / 4];
-              const float w0 = ex2_approx(__uint_as_float(r[k])), w1 = ex2_approx(__uint_as_float(r[k + 1]));
-              const float w2 = ex2_approx(__uint_as_float(r[k + 2])), w3 = ex2_approx(__uint_as_float(r[k + 3]));
-              sum2 = f2_fma(f2_pack(w0, w1), v.x, sum2);
-              sum2 = f2_fma(f2_pack(w2, w3), v.y, sum2);
-              const __half2 y0 = __floats2half2_rn(w0, w1), y1 = __floats2half2_rn(w2, w3);
-              pk[b * 8 + k / 2] = *reinterpret_cast<const uint32_t*>(&y0);
-              pk[b * 8 + k / 2 + 1] = *reinterpret_cast<const uint32_t*>(&y1);
+            for (int b = 0; b < G; b += 32) tmem_ld_wait(*reinterpret_cast<uint32_t(*)[32]>(r + b));
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+              exponents(b, r + b * 16, base, decltype(mask)::value);
+              const ulonglong2* iv = reinterpret_cast<const ulonglong2*>(sc + 2 * G + b * 16);
+#pragma unroll
+              for (int k = 0; k < 16; k += 4) {
+                const ulonglong2 v = iv[k / 4];
+                const uint32_t* x = r + b * 16 + k;
+                const float w0 = ex2_approx(__uint_as_float(x[0])), w1 = ex2_approx(__uint_as_float(x[1]));
+                const float w2 = ex2_approx(__uint_as_float(x[2])), w3 = ex2_approx(__uint_as_float(x[3]));
+                sum2 = f2_fma(f2_pack(w0, w1), v.x, sum2);
+                sum3 = f2_fma(f2_pack(w2, w3), v.y, sum3);
+                const __half2 y0 = __floats2half2_rn(w0, w1), y1 = __floats2half2_rn(w2, w3);
+                pk[b * 8 + k / 2] = *reinterpret_cast<const uint32_t*>(&y0);
+                pk[b * 8 + k / 2 + 1] = *reinterpret_cast<const uint32_t*>(&y1);
+              }
             }
-          }
+          };
+          if (rel_least >= G - 1) make_p(Flag<false>());
+          else make_p(Flag<true>());
           {
-            float s0, s1;
+            float s0, s1, s2, s3;
             f2_unpack(sum2, s0, s1);
-            total = s0 + s1;
+            f2_unpack(sum3, s2, s3);
+            total = (s0 + s1) + (s2 + s3);
           }
           if (find == 2 || !__any_sync(0xffffffffu, !(total < most) || (ref == -INFINITY && total > 0.f))) break;
           find = 2;
