@@ -103,7 +103,8 @@ struct TileCfg {
   static constexpr int NBARS = 4 + 2 * NK + 2 * NV8 + 2 * NV + 2 * NSC + 2 * NU + 12;
   static constexpr int OFF_BAR = OFF_PRE + (THREADS + 2) * 8;
   static constexpr int OFF_MISC = OFF_BAR + NBARS * 8;
-  static constexpr int SMEM = OFF_MISC + 32 + 1024;
+  static constexpr int OFF_OUT = (OFF_MISC + 32 + 127) / 128 * 128;      // 32 rows x 64 channels of each softmax warp, on their way out
+  static constexpr int SMEM = OFF_OUT + 8 * 4096 + 1024;
   static_assert(SMEM <= 227 * 1024, "shared memory");
   static_assert(OFF_UNIT % 16 == 0 && OFF_SC % 16 == 0 && OFF_PRE % 8 == 0, "alignment");
   static constexpr int COL_S = 0, COL_O = 4 * G;
@@ -468,7 +469,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         const float* ks = p.ks + u.head * p.ksH;
         const float* vs = p.vs + u.head * p.vsH;
         constexpr int N = G / 32;
+        // pages two chunks ahead, scales one chunk ahead of what is written
         int page[N];
+        float a[N], b[N], na[N], nb[N];
         auto look_up = [&](int c) {
 #pragma unroll
           for (int i = 0; i < N; ++i) {
@@ -476,23 +479,30 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
             page[i] = c < u.c1 && key < u.keys ? table[key >> p.page_log] : -1;
           }
         };
-        look_up(u.c0);
-        for (int c = u.c0; c < u.c1 && ok; ++c, ++it) {
-          float a[N], b[N];
-          unsigned in = 0;
+        auto fetch = [&](int c) {
 #pragma unroll
           for (int i = 0; i < N; ++i) {
-            const int blk = ((c * G + i * 32 + lane) & page_mask) >> p.block_log;
-            a[i] = 0.f;
-            b[i] = 1.f;
-            if (c * G + i * 32 + lane < u.keys) {
+            const int key = c * G + i * 32 + lane, blk = (key & page_mask) >> p.block_log;
+            na[i] = 0.f;
+            nb[i] = 1.f;
+            if (c < u.c1 && key < u.keys) {
               const long long pg = bad_page(page[i]) ? 0 : page[i];
-              a[i] = ks[pg * p.ksP + blk * p.ksB];
-              b[i] = vs[pg * p.vsP + blk * p.vsB];
-              in |= 1u << i;
+              na[i] = ks[pg * p.ksP + blk * p.ksB];
+              nb[i] = vs[pg * p.vsP + blk * p.vsB];
             }
           }
-          look_up(c + 1);
+        };
+        look_up(u.c0);
+        fetch(u.c0);
+        look_up(u.c0 + 1);
+        for (int c = u.c0; c < u.c1 && ok; ++c, ++it) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            a[i] = na[i];
+            b[i] = nb[i];
+          }
+          fetch(c + 1);
+          look_up(c + 2);
           const uint32_t slot = it % C::NSC;
           float* sc = reinterpret_cast<float*>(smem + C::OFF_SC) + slot * C::SC_FLOATS;
           ok = wait(B_SCE + slot, ((it / C::NSC) & 1u) ^ 1u, TW_SCE);
@@ -504,7 +514,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
             sc[i * 32 + lane] = a[i];
             sc[G + i * 32 + lane] = l;
             sc[2 * G + i * 32 + lane] = 1.0f / b[i];
-            if (in >> i & 1u) {
+            if (c * G + i * 32 + lane < u.keys) {
               const bool odd = !(fabsf(l) < INFINITY);         // zero, infinite, NaN: the general way
               lo = fminf(lo, odd ? -INFINITY : l);
               hi = fmaxf(hi, odd ? INFINITY : l);
@@ -528,9 +538,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
   } else if (warp < 8) {
     reg_dealloc<kTileConvert>();
     // -------------------------------------------------------------------- V: int8 -> fp16
-    constexpr int PIECES = D / 16;                             // 16-byte pieces of a key's int8 channels
-    const int tid = threadIdx.x - 128;
+    // A warp takes 8 keys x 64 channels at a time: lane = 4 pieces of 16 channels x 2 keys x 4.  The two keys of 8 lanes are k and k ^ 5, which lie
+    // in different banks in both tiles, the int8 one (pieces ^ key) and the fp16 one (pieces 2 pc ^ key).
+    constexpr int BOXES = D / 64;
+    const int key = ((lane >> 3) ^ ((lane >> 2 & 1) * 5)), pc = lane & 3, w0 = warp - 4;
     const uint32_t sV8 = smem_u32(smem + C::OFF_V8), sV = smem_u32(smem + C::OFF_V);
+    const uint32_t at0 = key * 128 + (((2 * pc) ^ key) << 4), at1 = key * 128 + (((2 * pc + 1) ^ key) << 4);
     uint32_t it = 0;
     TileUnit u;
     bool ok = true;
@@ -540,11 +553,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         ok = wait(B_V8F + a, (it / C::NV8) & 1u, TW_V8F) && wait(B_VE + b, ((it / C::NV) & 1u) ^ 1u, TW_VE);
         if (!ok) break;
         const uint32_t src = sV8 + a * C::K_BYTES, dst = sV + b * C::V_BYTES;
-#pragma unroll 1
-        for (int i = tid; i < G * PIECES; i += 128) {
-          const int key = i / PIECES, pc = i % PIECES;
-          const int sw = D == 128 ? key & 7 : (key >> 1) & 3;
-          const uint4 x = lds16(src + key * D + ((pc ^ sw) << 4));
+#pragma unroll 2
+        for (int i = w0; i < G / 8 * BOXES; i += 4) {
+          const int blk = i / BOXES, box = i % BOXES;
+          const int row = blk * 8 + key, piece = box * 4 + pc;
+          const uint4 x = lds16(src + row * D + ((piece ^ (D == 128 ? key : (row >> 1) & 3)) << 4));
           const uint32_t w[4] = {x.x ^ 0x80808080u, x.y ^ 0x80808080u, x.z ^ 0x80808080u, x.w ^ 0x80808080u};
           uint32_t h[8];
 #pragma unroll
@@ -553,15 +566,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
             const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&r), __half2half2(__ushort_as_half(0x6480)));
             h[k] = *reinterpret_cast<const uint32_t*>(&y);
           }
-          // channels pc*16 .. +15: chunks 2 (pc % 4) and the next of box pc / 4; the lanes of the second box begin with the other one, so
-          // that a row's eight stores lie in different banks
-          const int swap = (pc >> 2) & 1;
-          const uint32_t row = dst + (pc >> 2) * (G * 128) + key * 128;
-          const int ch = (pc & 3) * 2;
-          const uint4 y0 = make_uint4(h[0], h[1], h[2], h[3]), y1 = make_uint4(h[4], h[5], h[6], h[7]);
-          const uint4 f = swap ? y1 : y0, g = swap ? y0 : y1;
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(row + (((ch + swap) ^ (key & 7)) << 4)), "r"(f.x), "r"(f.y), "r"(f.z), "r"(f.w) : "memory");
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(row + (((ch + 1 - swap) ^ (key & 7)) << 4)), "r"(g.x), "r"(g.y), "r"(g.z), "r"(g.w) : "memory");
+          const uint32_t to = dst + box * (G * 128) + blk * 1024;
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + at0), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + at1), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7]) : "memory");
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -604,20 +611,22 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
       }
       const float qs = qs_raw * p.c;
       const uint64_t qs2 = f2_pack(qs, qs), magic2 = f2_pack(-kMagicF, -kMagicF);
-      long long lim = u.keys - 1;
-      if (p.causal && mine) lim = min(lim, u.lim0 + tok);
+      // the last key that the row sees; the least and the most of the warp
+      int lim = u.keys - 1;
+      if (p.causal && mine && u.lim0 + tok < lim) lim = u.lim0 + tok < -1 ? -1 : (int)(u.lim0 + tok);
+      const int lim_least = __reduce_min_sync(0xffffffffu, lim), lim_most = __reduce_max_sync(0xffffffffu, lim);
       float mref = -INFINITY, ref = -INFINITY, l = 0.f;        // references of p and of w (of the accumulator)
       for (int c = u.c0; c < u.c1; ++c, ++it, ++sit) {
         const uint32_t slot = it % C::NSC;
-        ok = wait(B_SCF + slot, (it / C::NSC) & 1u, TW_SC) && wait(B_S + 2 * tile + (sit & 1u), sit >> 1 & 1u, TW_S);
+        ok = mbar_wait2_warp(BAR(B_SCF + slot), (it / C::NSC) & 1u, code_hi | TW_SC, BAR(B_S + 2 * tile + (sit & 1u)), sit >> 1 & 1u, code_hi | TW_S, abort_flag,
+                             p.status);
         if (!ok) break;
         tc_fence_after();
         const uint32_t tS = tS0 + (sit & 1u) * G;
         const float* sc = reinterpret_cast<const float*>(smem + C::OFF_SC) + slot * C::SC_FLOATS;
         const float lo = sc[3 * G], hi = sc[3 * G + 1];
-        const long long rel64 = lim - (long long)c * G;
-        const int rel = rel64 < -1 ? -1 : rel64 > G ? G : (int)rel64;      // the last column that the row sees
-        const int rel_least = (int)__reduce_min_sync(0xffffffffu, rel), rel_most = (int)__reduce_max_sync(0xffffffffu, rel);
+        const int key0 = c * G, rel = lim - key0;              // (the last column that the row sees)
+        const bool whole = lim_least - key0 >= G - 1;
         // exponents of w, x + log2 v_scale - off, of 16 columns, in place of the scores
         auto exponents = [&](int b, uint32_t* r, float off, bool mask) {
           const uint64_t off2 = f2_pack(-off, -off);
@@ -647,7 +656,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
           if (find) {
             float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll 1
-            for (int b = 0; b * 16 <= rel_most && b < (find == 1 ? 1 : NB); ++b) {
+            for (int b = 0; b * 16 <= lim_most - key0 && b < (find == 1 ? 1 : NB); ++b) {
               uint32_t r[16];
               tmem_ld16(tS + b * 16, r);
               tmem_ld_wait16(r);
@@ -707,7 +716,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
               }
             }
           };
-          if (rel_least >= G - 1) make_p(Flag<false>());
+          if (whole) make_p(Flag<false>());
           else make_p(Flag<true>());
           {
             float s0, s1, s2, s3;
@@ -782,28 +791,51 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
       const int h = done.head * p.ratio + hr;
       const long long row = (long long)done.slot * (2 * kTileRows) + tile * kTileRows + rr;
       uint16_t* o16 = static_cast<uint16_t*>(p.o) + (long long)(done.t0 + tok) * p.on + h * p.oh;
+      if (done.slot < 0) {
+        // 64 channels at a time: the warp's 32 rows through shared memory (16-byte pieces ^ row: no bank conflicts), then out as 128-byte lines
+        uint8_t* stage = smem + C::OFF_OUT + (warp - 8) * 4096;
+        const int piece = lane & 7;
 #pragma unroll 1
-      for (int b = 0; b < D / 16; ++b) {
-        uint32_t o[16];
-        tmem_ld16(tO + b * 16, o);
-        tmem_ld_wait16(o);
-        if (write && done.slot < 0) {
-          uint32_t w[8];
+        for (int b = 0; b < D / 64; ++b) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float x0 = __uint_as_float(o[2 * e]) * f, x1 = __uint_as_float(o[2 * e + 1]) * f;
-            const __nv_bfloat162 y = __floats2bfloat162_rn(x0, x1);
-            const __half2 z = __floats2half2_rn(x0, x1);
-            w[e] = p.o_bf16 ? *reinterpret_cast<const uint32_t*>(&y) : *reinterpret_cast<const uint32_t*>(&z);
+          for (int e = 0; e < 2; ++e) {
+            uint32_t o[32];
+            tmem_ld32(tO + b * 64 + e * 32, o);
+            tmem_ld_wait(o);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              uint32_t w[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float x0 = __uint_as_float(o[8 * k + 2 * i]) * f, x1 = __uint_as_float(o[8 * k + 2 * i + 1]) * f;
+                const __nv_bfloat162 y = __floats2bfloat162_rn(x0, x1);
+                const __half2 z = __floats2half2_rn(x0, x1);
+                w[i] = p.o_bf16 ? *reinterpret_cast<const uint32_t*>(&y) : *reinterpret_cast<const uint32_t*>(&z);
+              }
+              *reinterpret_cast<uint4*>(stage + lane * 128 + (((e * 4 + k) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
           }
-          uint4* to = reinterpret_cast<uint4*>(o16 + b * 16);
-          to[0] = make_uint4(w[0], w[1], w[2], w[3]);
-          to[1] = make_uint4(w[4], w[5], w[6], w[7]);
-        } else if (write) {
-#pragma unroll
-          for (int k = 0; k < 16; k += 4) *reinterpret_cast<uint4*>(p.part + row * D + b * 16 + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+          __syncwarp();
+#pragma unroll 2
+          for (int i = lane >> 3; i < 32; i += 4) {
+            const long long to = __shfl_sync(0xffffffffu, (long long)(write ? o16 - static_cast<uint16_t*>(p.o) : -1), i);
+            const uint4 w = *reinterpret_cast<const uint4*>(stage + i * 128 + ((piece ^ (i & 7)) << 4));
+            if (to >= 0) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.o) + to + b * 64 + piece * 8) = w;
+          }
+          __syncwarp();
         }
-        __syncwarp();
+      } else {
+#pragma unroll 1
+        for (int b = 0; b < D / 16; ++b) {
+          uint32_t o[16];
+          tmem_ld16(tO + b * 16, o);
+          tmem_ld_wait16(o);
+          if (write) {
+#pragma unroll
+            for (int k = 0; k < 16; k += 4) *reinterpret_cast<uint4*>(p.part + row * D + b * 16 + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+          }
+          __syncwarp();
+        }
       }
       if (write) {
         if (done.slot >= 0) *reinterpret_cast<float4*>(p.part_ml + row * 4) = make_float4(mref, ref, l, 0.f);
