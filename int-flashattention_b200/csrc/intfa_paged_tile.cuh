@@ -790,52 +790,56 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
       const float f = done.slot < 0 ? row_factor(mref, ref, l) : 1.f;
       const int h = done.head * p.ratio + hr;
       const long long row = (long long)done.slot * (2 * kTileRows) + tile * kTileRows + rr;
-      uint16_t* o16 = static_cast<uint16_t*>(p.o) + (long long)(done.t0 + tok) * p.on + h * p.oh;
-      if (done.slot < 0) {
-        // 64 channels at a time: the warp's 32 rows through shared memory (16-byte pieces ^ row: no bank conflicts), then out as 128-byte lines
-        uint8_t* stage = smem + C::OFF_OUT + (warp - 8) * 4096;
-        const int piece = lane & 7;
+      const long long out_at = write ? (long long)(done.t0 + tok) * p.on + h * p.oh : -1;
+      // 64 channels at a time: the warp's 32 rows through shared memory (16-byte pieces ^ row: no bank conflicts), then out as 128-byte lines;
+      // a unit's part goes to scratch as it is.
+      uint8_t* stage = smem + C::OFF_OUT + (warp - 8) * 4096 + lane * 128;
+      const uint8_t* staged = smem + C::OFF_OUT + (warp - 8) * 4096 + (lane >> 3) * 128;
+      float* part = p.part + row * D;
 #pragma unroll 1
-        for (int b = 0; b < D / 64; ++b) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            uint32_t o[32];
-            tmem_ld32(tO + b * 64 + e * 32, o);
-            tmem_ld_wait(o);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              uint32_t w[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float x0 = __uint_as_float(o[8 * k + 2 * i]) * f, x1 = __uint_as_float(o[8 * k + 2 * i + 1]) * f;
-                const __nv_bfloat162 y = __floats2bfloat162_rn(x0, x1);
-                const __half2 z = __floats2half2_rn(x0, x1);
-                w[i] = p.o_bf16 ? *reinterpret_cast<const uint32_t*>(&y) : *reinterpret_cast<const uint32_t*>(&z);
-              }
-              *reinterpret_cast<uint4*>(stage + lane * 128 + (((e * 4 + k) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-          }
-          __syncwarp();
-#pragma unroll 2
-          for (int i = lane >> 3; i < 32; i += 4) {
-            const long long to = __shfl_sync(0xffffffffu, (long long)(write ? o16 - static_cast<uint16_t*>(p.o) : -1), i);
-            const uint4 w = *reinterpret_cast<const uint4*>(stage + i * 128 + ((piece ^ (i & 7)) << 4));
-            if (to >= 0) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.o) + to + b * 64 + piece * 8) = w;
-          }
-          __syncwarp();
-        }
-      } else {
-#pragma unroll 1
-        for (int b = 0; b < D / 16; ++b) {
-          uint32_t o[16];
-          tmem_ld16(tO + b * 16, o);
-          tmem_ld_wait16(o);
+      for (int b = 0; b < D; b += 64) {
+        uint32_t o[64];
+        tmem_ld32(tO + b, reinterpret_cast<uint32_t(&)[32]>(o[0]));
+        tmem_ld32(tO + b + 32, reinterpret_cast<uint32_t(&)[32]>(o[32]));
+        tmem_ld_wait(reinterpret_cast<uint32_t(&)[32]>(o[0]));
+        tmem_ld_wait(reinterpret_cast<uint32_t(&)[32]>(o[32]));
+        if (done.slot >= 0) {
           if (write) {
 #pragma unroll
-            for (int k = 0; k < 16; k += 4) *reinterpret_cast<uint4*>(p.part + row * D + b * 16 + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+            for (int k = 0; k < 64; k += 4) *reinterpret_cast<uint4*>(part + b + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
           }
           __syncwarp();
+          continue;
         }
+        if (p.o_bf16) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const __nv_bfloat162 y = __floats2bfloat162_rn(__uint_as_float(o[2 * i]) * f, __uint_as_float(o[2 * i + 1]) * f);
+            o[i] = *reinterpret_cast<const uint32_t*>(&y);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const __half2 y = __floats2half2_rn(__uint_as_float(o[2 * i]) * f, __uint_as_float(o[2 * i + 1]) * f);
+            o[i] = *reinterpret_cast<const uint32_t*>(&y);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          *reinterpret_cast<uint4*>(stage + ((k ^ (lane & 7)) << 4)) = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+        __syncwarp();
+        uint4 y[8];
+        long long to[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int from = 4 * i + (lane >> 3);
+          y[i] = *reinterpret_cast<const uint4*>(staged + i * 512 + (((lane & 7) ^ (from & 7)) << 4));
+          to[i] = __shfl_sync(0xffffffffu, out_at, from);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (to[i] >= 0) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.o) + to[i] + b + (lane & 7) * 8) = y[i];
+        __syncwarp();
       }
       if (write) {
         if (done.slot >= 0) *reinterpret_cast<float4*>(p.part_ml + row * 4) = make_float4(mref, ref, l, 0.f);
