@@ -725,6 +725,21 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_const
   }
 }
 
+// row r of a unit: query row (token n among the unit's, head h of the K/V head's), or false
+__device__ __forceinline__ bool row_of(const PParams& p, const UnitPart& up, int r, int& n, int& h) {
+  const int rr = p.tile_tokens ? r & 127 : up.row + r;
+  n = rr / p.ratio;
+  h = rr - n * p.ratio;
+  if (p.tile_tokens && n >= p.tile_tokens) return false;
+  if (p.tile_tokens) n += (r >> 7) * p.tile_tokens;
+  return n < up.tokens;
+}
+// the i-th part's place in scratch
+__device__ __forceinline__ long long slot_of(const UnitPart& up, int i, int cta_warps) {
+  const int w = i < up.n0 ? up.first + i : i < up.n0 + up.n1 ? (up.cta + (i - up.n0)) * cta_warps : (up.cta + up.n1) * cta_warps + (i - up.n0 - up.n1);
+  return 2LL * w + (w == up.first ? 1 : 0);
+}
+
 // Sum of the parts of the units that lie in several warps' shares.  GROUPS groups of D/4 threads a row take the parts in turn; the groups'
 // sums are added in order, so a call repeats itself bit for bit.  A chain of L2 latencies: with few units, and so many parts each, one
 // row a CTA and all groups on it; else one unit a CTA.
@@ -741,30 +756,17 @@ __global__ void __launch_bounds__(GROUPS * (D / 4)) combine_kernel(const PParams
   const int units = p.head[0];
   const UnitPart up = p.units[u];                 // (the two loads do not wait for one another)
   if (u >= units || !up.open) return;
-  // row r of the unit: query row (token n, head h of the K/V head's)
-  auto row_of = [&](int r, int& n, int& h) {
-    const int rr = p.tile_tokens ? r & 127 : up.row + r;
-    n = rr / p.ratio;
-    h = rr - n * p.ratio;
-    if (p.tile_tokens && n >= p.tile_tokens) return false;
-    if (p.tile_tokens) n += (r >> 7) * p.tile_tokens;
-    return n < up.tokens;
-  };
   const int parts = up.n0 + up.n1 + up.n2;
-  auto slot_of = [&](int i) {
-    const int w = i < up.n0 ? up.first + i : i < up.n0 + up.n1 ? (up.cta + (i - up.n0)) * cta_warps : (up.cta + up.n1) * cta_warps + (i - up.n0 - up.n1);
-    return 2LL * w + (w == up.first ? 1 : 0);
-  };
   const int first_row = (int)(blockIdx.x % per_unit) * rows_cta;
   const int row_step = rows_cta == 1 ? 1 : GROUPS, part_step = rows_cta == 1 ? GROUPS : 1;
   for (int r = first_row + (rows_cta == 1 ? 0 : grp); r < first_row + rows_cta; r += row_step) {
     int n, h;
-    if (!row_of(r, n, h)) continue;
+    if (!row_of(p, up, r, n, h)) continue;
     Sum x;
     x.clear();
 #pragma unroll 4
     for (int i = rows_cta == 1 ? grp : 0; i < parts; i += part_step) {
-      const long long s = slot_of(i) * p.rows_tile + r;
+      const long long s = slot_of(up, i, cta_warps) * p.rows_tile + r;
       x.add(*reinterpret_cast<const float4*>(p.part_ml + s * 4), *reinterpret_cast<const float4*>(p.part + s * D + ch));
     }
     if (rows_cta == 1) {
@@ -773,6 +775,47 @@ __global__ void __launch_bounds__(GROUPS * (D / 4)) combine_kernel(const PParams
       __syncthreads();
       if (grp > 0) return;
       for (int i = 1; i < GROUPS; ++i) x.add(red_ml[i], red[i][ch / 4]);
+    }
+    write_sum(p, up.token + n, up.head * p.ratio + h, ch, x);
+  }
+}
+
+// The same for the 128-row tiles: at most one unit a CTA is open, and which are is known on the device alone.  Every CTA lists them; their
+// rows are dealt out to all groups of D/4 threads of the grid.
+template <int D>
+__global__ void __launch_bounds__(256) combine_tiles_kernel(const PParams p, int entries) {
+  constexpr int C4 = D / 4, GROUPS = 256 / C4;
+  extern __shared__ int list[];
+  __shared__ int counts[8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, grp = threadIdx.x / C4, ch = threadIdx.x % C4 * 4;
+  pdl_wait();
+  pdl_launch();
+  int open_units = 0;
+  for (int e0 = 0; e0 < entries; e0 += 256) {
+    const int e = e0 + threadIdx.x;
+    const bool open = e < entries && p.units[e].open;
+    const unsigned votes = __ballot_sync(0xffffffffu, open);
+    if (lane == 0) counts[warp] = __popc(votes);
+    __syncthreads();
+    int at = open_units;
+    for (int w = 0; w < 8; ++w) {
+      if (w < warp) at += counts[w];
+      open_units += counts[w];
+    }
+    if (open) list[at + __popc(votes & ((1u << lane) - 1u))] = e;
+    __syncthreads();
+  }
+  for (int i = blockIdx.x * GROUPS + grp; i < open_units * p.rows_tile; i += gridDim.x * GROUPS) {
+    const UnitPart up = p.units[list[i / p.rows_tile]];
+    const int r = i % p.rows_tile, parts = up.n0 + up.n1 + up.n2;
+    int n, h;
+    if (!row_of(p, up, r, n, h)) continue;
+    Sum x;
+    x.clear();
+#pragma unroll 4
+    for (int k = 0; k < parts; ++k) {
+      const long long s = slot_of(up, k, 1) * p.rows_tile + r;
+      x.add(*reinterpret_cast<const float4*>(p.part_ml + s * 4), *reinterpret_cast<const float4*>(p.part + s * D + ch));
     }
     write_sum(p, up.token + n, up.head * p.ratio + h, ch, x);
   }
@@ -789,8 +832,15 @@ struct Plan {
   long long max_units = 0;
   size_t off_ml = 0, off_units = 0, off_head = 0, bytes = 0;
 };
-// An average sequence with more rows a K/V head than this takes 128-row tiles
-constexpr double kFewRows = 32;
+// 128-row tiles, or packed rows of 8 or 16?  A tile costs the same however many of its rows there are, and a unit on tiles takes longer to
+// begin, to end and to be put together.  The lengths of the sequences are not known here; timed on both with 600 and 4000 keys: at 128 channels
+// 16 sequences of 8 K/V heads, 64 rows each a head, 26.0 / 74.0 us packed, 30.6 / 63.7 on tiles, of 32 rows 23.3 / 49.1 and 29.8 / 56.7; one
+// sequence, 256 rows, 24.2 / 51.4 and 28.5 / 29.1, 128 rows 15.7 / 31.3 and 17.9 / 29.3; at 64 channels 16 sequences, 128 rows, 27.9 / 81.9 and
+// 30.6 / 60.5, 64 rows 19.6 / 46.4 and 26.9 / 61.7.
+bool takes_tiles(const IntfaPagedParams* a) {
+  const double rows = (double)a->tokens * (a->H / a->cache.H_kv) / a->cache.S;          // of an average sequence and K/V head
+  return a->cache.D <= 128 && a->H / a->cache.H_kv <= kTileRows && rows >= (a->cache.D == 64 ? 112 : 64) && rows * a->cache.S * a->cache.H_kv >= 2048;
+}
 Plan make_plan(const IntfaPagedParams* a, int sms) {
   Plan pl;
   const IntfaPagedCache& c = a->cache;
@@ -801,7 +851,7 @@ Plan make_plan(const IntfaPagedParams* a, int sms) {
     pl.bytes += (bytes + 255) / 256 * 256;
     return r;
   };
-  pl.tiles = c.D <= 128 && ratio <= kTileRows && (double)a->tokens * ratio > kFewRows * c.S;
+  pl.tiles = takes_tiles(a);
   if (pl.tiles) {
     pl.warps = 1;
     pl.max_units = pl.ctas;
@@ -872,8 +922,7 @@ int run_tiles(const IntfaPagedParams* a, const Plan& pl, PParams p, cudaStream_t
     attr_done[dev].store(true, std::memory_order_release);
   }
   if ((rc = launch_kernel("paged attention", kern, pl.ctas, C::THREADS, C::SMEM, stream, tmQ, tmK, tmV, p))) return rc;
-  constexpr int GROUPS = 1024 / D, ROWS = 32;
-  return launch_kernel("paged combine", combine_kernel<D, GROUPS>, (unsigned)(pl.ctas * (2 * kTileRows / ROWS)), GROUPS * (D / 4), 0, stream, p, 1, ROWS);
+  return launch_kernel("paged combine", combine_tiles_kernel<D>, 4 * pl.ctas, 256, pl.ctas * sizeof(int), stream, p, pl.ctas);
 }
 
 int log2_of(long long n) {
