@@ -93,7 +93,7 @@ class IntfaPagedParams(ctypes.Structure):
         ("lse_out", ctypes.c_void_p), ("q_stride", _i64x2), ("qs_stride", _i64x2), ("o_stride", _i64x2),
         ("tokens", ctypes.c_int64), ("H", ctypes.c_int32), ("o_dtype", ctypes.c_int32), ("cu_seqlens", ctypes.c_void_p),
         ("causal", ctypes.c_int32), ("sm_scale", ctypes.c_float), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64),
-        ("status", ctypes.c_void_p),
+        ("status", ctypes.c_void_p), ("debug_path", ctypes.c_int32),
     ]
 
 

@@ -838,6 +838,7 @@ struct Plan {
 // sequence, 256 rows, 24.2 / 51.4 and 28.5 / 29.1, 128 rows 15.7 / 31.3 and 17.9 / 29.3; at 64 channels 16 sequences, 128 rows, 27.9 / 81.9 and
 // 30.6 / 60.5, 64 rows 19.6 / 46.4 and 26.9 / 61.7.
 bool takes_tiles(const IntfaPagedParams* a) {
+  if (a->debug_path) return a->debug_path == 2;
   const double rows = (double)a->tokens * (a->H / a->cache.H_kv) / a->cache.S;          // of an average sequence and K/V head
   return a->cache.D <= 128 && a->H / a->cache.H_kv <= kTileRows && rows >= (a->cache.D == 64 ? 112 : 64) && rows * a->cache.S * a->cache.H_kv >= 2048;
 }

@@ -865,11 +865,11 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // paged(q, k_cache, v_cache, q_scale, k_scale, v_scale, block_table, seq_lens, cu_seqlens | None, causal, sm_scale, out_dtype | None, out | None,
-//       return_lse)
+//       return_lse, debug_path)
 PyObject* paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   try {
-    if (n != 14) raise(PyExc_TypeError, "paged takes 14 arguments");
+    if (n != 15) raise(PyExc_TypeError, "paged takes 15 arguments");
     const at::Tensor &q0 = tensor(a[0], "q"), &kc = tensor(a[1], "k_cache"), &vc = tensor(a[2], "v_cache"), &qs = tensor(a[3], "q_scale");
     const at::Tensor &ks = tensor(a[4], "k_scale"), &vs = tensor(a[5], "v_scale"), &bt = tensor(a[6], "block_table"), &sl = tensor(a[7], "seq_lens");
     if (!is(q0, at::kChar)) raise(PyExc_TypeError, "q must be int8");
@@ -902,6 +902,7 @@ PyObject* paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
       out = empty({T, H, D}, o.out, dev);
     }
     const bool want_lse = truth(a[13]);
+    P.debug_path = static_cast<int>(as_long(a[14]));
     at::Tensor lse = want_lse ? empty({T, H}, at::kFloat, dev) : at::Tensor();
     if (T > 0) {
       if (P.cache.table_width < 1) raise(PyExc_ValueError, "block_table has no columns");
@@ -924,6 +925,7 @@ PyObject* paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
       P.causal = truth(a[9]);
       P.sm_scale = static_cast<float>(as_double(a[10]));
       const size_t bytes = intfa_paged_workspace_bytes(&P);
+      if (bytes == 0) check(intfa_paged_attention(&P, nullptr));          // (refused: says why)
       at::Tensor ws = empty({static_cast<int64_t>(bytes)}, at::kByte, dev);
       P.workspace = ws.data_ptr();
       P.workspace_bytes = bytes;

@@ -51,6 +51,11 @@ class Setup:
         self.qs = torch.rand(T, H, device="cuda", generator=g) * 0.02 + 0.005
         self.scale = D ** -0.5
 
+    path = 0                              # (debug_path: the rule on sizes)
+
+    def call(self, pkg, causal=True, **kw):
+        return pkg.attention_int8_paged(*self.args(causal), debug_path=self.path, **kw)
+
     def args(self, causal=True):
         return (self.q8, self.kc, self.vc, self.qs, self.ks, self.vs, self.table, self.lens, self.cu, causal, self.scale)
 
@@ -59,7 +64,7 @@ class Setup:
         return (2.0 ** -11 + 2.0 ** -16 + more + (n / 8 + 64) * 2.0 ** -24) * A + n * 2.0 ** -25 * 2 * B[..., None] + EPS[out_dtype] * want.abs() + 2.0 ** -25
 
     def check(self, pkg, causal=True, out_dtype=torch.float16, got=None, more=0.0):
-        o, lse = pkg.attention_int8_paged(*self.args(causal), out_dtype=out_dtype, return_lse=True) if got is None else got
+        o, lse = self.call(pkg, causal, out_dtype=out_dtype, return_lse=True) if got is None else got
         want, wlse, A, B = O.attention(self.q8, self.qs, self.kc, self.vc, self.ks, self.vs, self.table, self.lens, self.cu, causal, self.scale)
         tol = self.tolerance(want, A, B, out_dtype, more)
         assert o.dtype == out_dtype
@@ -87,7 +92,9 @@ def test_decode(D, page, block, ratio, pkg):
 @pytest.mark.parametrize("out_dtype", [torch.float16, torch.bfloat16])
 def test_several_rows(D, causal, ratio, news, out_dtype, pkg):
     lens = [n + old for n, old in zip(news, [0, 1, 300, 50, 29, 0])]
-    Setup(news, lens, 2 * ratio, 2, D, 16, 4, seed=D + ratio).check(pkg, causal, out_dtype)
+    s = Setup(news, lens, 2 * ratio, 2, D, 16, 4, seed=D + ratio)
+    s.path = 1
+    s.check(pkg, causal, out_dtype)
 
 
 @pytest.mark.parametrize("S,n,Hkv,ratio,D", [(1, 5000, 1, 1, 128), (1, 40000, 1, 8, 64), (1, 20001, 8, 4, 128), (2, 9999, 1, 16, 256), (1, 120, 1, 2, 128),
@@ -97,7 +104,7 @@ def test_shares(S, n, Hkv, ratio, D, pkg):
     lens = [max(1, n - 37 * s % n) for s in range(S)]
     s = Setup([1] * S, lens, Hkv * ratio, Hkv, D, 32, 8, one=True, seed=S)
     a = s.check(pkg)
-    assert torch.equal(a, pkg.attention_int8_paged(*s.args()))           # repeats itself
+    assert torch.equal(a, s.call(pkg))           # repeats itself
 
 
 @pytest.mark.parametrize("layout", ["heads", "tokens"])
@@ -114,7 +121,7 @@ def test_query_and_output_views(pkg):
     s.qs = s.qs.t().contiguous().t()
     base = torch.full((5, 6, 256), 7.0, device="cuda", dtype=torch.bfloat16)
     out = base[..., :128]
-    o, lse = pkg.attention_int8_paged(*s.args(), out=out, return_lse=True)
+    o, lse = s.call(pkg, out=out, return_lse=True)
     assert o.data_ptr() == out.data_ptr() and (base[..., 128:] == 7).all()
     s.check(pkg, got=(o, lse), out_dtype=torch.bfloat16)
 
@@ -132,7 +139,7 @@ def test_small_values(pkg):
     s = Setup([1, 1], [300, 40], 4, 2, 128, 16, 1, garbage=False)
     s.vs.mul_(1e-30)
     s.check(pkg, out_dtype=torch.bfloat16)
-    o = pkg.attention_int8_paged(*s.args(), out_dtype=torch.bfloat16)
+    o = s.call(pkg, out_dtype=torch.bfloat16)
     assert (o.float().abs() > 1e-32).float().mean() > 0.9
     s.vs.zero_()
     s.check(pkg)
@@ -153,10 +160,10 @@ def test_sharp_and_negative_scores(pkg):
 
 def test_nan_reaches_its_rows_only(pkg):
     s = Setup([1, 1, 2], [100, 64, 33], 4, 2, 64, 16, 1)
-    clean = pkg.attention_int8_paged(*s.args())
+    clean = s.call(pkg)
     s.ks[s.table[0, 2].long(), 1, 3] = float("nan")
     s.vs[s.table[2, 2].long(), 0, 0] = float("nan")       # the last token: seen by the last row alone
-    o = pkg.attention_int8_paged(*s.args())
+    o = s.call(pkg)
     bad = torch.zeros(4, 4, 1, dtype=torch.bool, device="cuda")
     bad[0, 2:] = True
     bad[3, :2] = True
@@ -167,7 +174,7 @@ def test_nan_reaches_its_rows_only(pkg):
 def test_rows_that_see_nothing(pkg):
     """Causal rows ahead of their sequence's first token, and sequences without tokens."""
     s = Setup([5, 2, 1], [3, 0, 40], 4, 2, 128, 16, 1)
-    o, lse = pkg.attention_int8_paged(*s.args(), return_lse=True)
+    o, lse = s.call(pkg, return_lse=True)
     assert (o[:2] == 0).all() and (o[5:7] == 0).all() and torch.isinf(lse[:2]).all() and torch.isinf(lse[5:7]).all()
     s.check(pkg)
     s.check(pkg, causal=False)
@@ -176,45 +183,45 @@ def test_rows_that_see_nothing(pkg):
 @pytest.mark.parametrize("news", [[1, 1, 1], [3, 20, 9]])
 def test_rows_behind_the_last_sequence_stay(news, pkg):
     s = Setup(news, [50, 60, 70], 4, 2, 64, 16, 1)
-    want = pkg.attention_int8_paged(*s.args())
+    want = s.call(pkg)
     T = sum(news)
     pad = lambda x: torch.cat([x, x[:2]])
     s.q8, s.qs = pad(s.q8), pad(s.qs)
     out = torch.full((T + 2, 4, 64), 9.0, device="cuda", dtype=torch.float16)
-    pkg.attention_int8_paged(*s.args(), out=out)
+    s.call(pkg, out=out)
     assert torch.equal(out[:T], want) and (out[T:] == 9).all()
     s.cu[0] = 1                           # rows ahead of the first sequence, too
     out[:] = 9
-    pkg.attention_int8_paged(*s.args(), out=out)
+    s.call(pkg, out=out)
     assert (out[0] == 9).all() and torch.equal(out[news[0]:T], want[news[0]:]) and (out[T:] == 9).all()
     assert pkg.check_status() == 0
 
 
 def test_bad_indices(pkg):
     s = Setup([1, 1], [100, 40], 4, 2, 64, 16, 1)
-    good = pkg.attention_int8_paged(*s.args())
+    good = s.call(pkg)
     assert pkg.check_status() == 0
     for bad in (s.kc.shape[0], -1, 1 << 30):
         was = s.table[0, 3].clone()
         s.table[0, 3] = bad
-        o = pkg.attention_int8_paged(*s.args())
+        o = s.call(pkg)
         with pytest.raises(pkg.IntfaError, match="outside its table"):
             pkg.check_status()
         assert torch.equal(o[1], good[1])
         s.table[0, 3] = was
     s.lens[0] = s.table.shape[1] * 16 + 1
     s.table[0] = 0
-    o = pkg.attention_int8_paged(*s.args())
+    o = s.call(pkg)
     with pytest.raises(pkg.IntfaError, match="outside its table"):
         pkg.check_status()
     assert torch.equal(o[1], good[1])
     s.lens[0] = -3                        # no tokens
-    assert (pkg.attention_int8_paged(*s.args())[0] == 0).all()
+    assert (s.call(pkg)[0] == 0).all()
     # ends that run backwards or past the rows: nothing is read or written outside
     for cu in ([0, 2, 1], [0, 1, 9], [-4, 1, 2], [1, 0, 2], [2, 2, 2]):
         s.cu = torch.tensor(cu, dtype=torch.int32, device="cuda")
         s.lens[:] = 20
-        pkg.attention_int8_paged(*s.args())
+        s.call(pkg)
         try:
             pkg.check_status()
         except pkg.IntfaError:
@@ -223,13 +230,13 @@ def test_bad_indices(pkg):
 
 def test_no_rows(pkg):
     s = Setup([0, 0], [5, 0], 4, 2, 64, 16, 1)
-    o, lse = pkg.attention_int8_paged(*s.args(), return_lse=True)
+    o, lse = s.call(pkg, return_lse=True)
     assert o.shape == (0, 4, 64) and lse.shape == (0, 4)
 
 
 def test_two_streams_at_once_and_a_replayed_graph(pkg):
     a, b = Setup([1] * 4, [900, 33, 500, 8], 8, 2, 128, 16, 1, one=True), Setup([3, 60], [1000, 200], 8, 2, 128, 16, 4, seed=5)
-    wa, wb = pkg.attention_int8_paged(*a.args()), pkg.attention_int8_paged(*b.args())
+    wa, wb = a.call(pkg), b.call(pkg)
     sa, sb = torch.cuda.Stream(), torch.cuda.Stream()
     for s in (sa, sb):
         s.wait_stream(torch.cuda.current_stream())
@@ -237,17 +244,17 @@ def test_two_streams_at_once_and_a_replayed_graph(pkg):
     for _ in range(10):
         for s, x, w in ((sa, a, wa), (sb, b, wb)):
             with torch.cuda.stream(s):
-                got.append((pkg.attention_int8_paged(*x.args()), w))
+                got.append((x.call(pkg), w))
     torch.cuda.synchronize()
     assert all(torch.equal(x, w) for x, w in got)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        outs = [pkg.attention_int8_paged(*a.args()) for _ in range(2)]
+        outs = [a.call(pkg) for _ in range(2)]
     lens = a.lens.clone()
     for new in ([900, 33, 500, 8], [1, 20, 499, 0], [640, 33, 0, 8]):      # other lengths, other shares
         a.lens.copy_(torch.tensor(new, device="cuda"))
         graph.replay()
-        want = pkg.attention_int8_paged(*a.args())
+        want = a.call(pkg)
         assert all(torch.equal(o, want) for o in outs)
     a.lens.copy_(lens)
     graph.replay()
@@ -262,14 +269,14 @@ def test_pages_past_32_bits(pkg):
     s = Setup([1], [150], 8, Hkv, D, page, 1)
     small_k, small_v, small_t = s.kc, s.vc, s.table.clone()
     ks, vs = s.ks, s.vs
-    want = pkg.attention_int8_paged(*s.args())
+    want = s.call(pkg)
     s.kc, s.vc = (torch.zeros(pages, Hkv, page, D, dtype=torch.int8, device="cuda") for _ in range(2))
     s.ks, s.vs = (torch.ones(pages, Hkv, page, device="cuda") for _ in range(2))
     for i in range(3):
         to, frm = pages - 1 - i, int(small_t[0, i])
         s.kc[to], s.vc[to], s.ks[to], s.vs[to] = small_k[frm], small_v[frm], ks[frm], vs[frm]
         s.table[0, i] = to
-    assert torch.equal(pkg.attention_int8_paged(*s.args()), want)
+    assert torch.equal(s.call(pkg), want)
     k = torch.randn(1, Hkv, D, device="cuda").half()
     before = s.kc[:5].clone()
     pkg.append_int8_paged(k, k, s.kc, s.vc, s.ks, s.vs, s.table, s.lens)

@@ -5,9 +5,29 @@ import pytest
 import torch
 
 import test_gpu_paged_attention as base
-from test_gpu_paged_attention import Setup
 
 pytestmark = pytest.mark.gpu
+
+
+class Setup(base.Setup):
+    path = 2                              # 128-row tiles, also where the rule on sizes takes packed rows
+
+
+def test_the_rule_takes_either_path(pkg):
+    """Prompts on tiles, drafts and single tokens packed: what the rule gives is bit for bit what one of the two gives."""
+    for news, lens, path in (([300, 500, 200], [300, 900, 201], 2), ([4, 3, 5], [400, 900, 201], 1), ([1, 1], [1, 700], 1)):
+        s = Setup(news, lens, 32, 8, 128, 16, 1)
+        want = s.call(pkg)
+        s.path = path
+        got = s.call(pkg)
+        s.path = 0
+        assert torch.equal(s.call(pkg), got)
+        if path == 1:
+            assert not torch.equal(want, got)          # (the two round differently)
+    for D, ratio in ((256, 2), (64, 129)):
+        s = Setup([3], [30], ratio, 1, D, 16, 1)
+        with pytest.raises(pkg.IntfaError, match="debug_path"):
+            s.call(pkg)
 
 
 @pytest.mark.parametrize("D", [64, 128])
@@ -37,7 +57,7 @@ def test_shares(S, n, length, H, Hkv, D, pkg):
     news = [max(1, n - 3 * s % 29) for s in range(S)]
     s = Setup(news, [length - 7 * i % 31 if length > n else m for i, m in enumerate(news)], H, Hkv, D, 64, 1, seed=S + n)
     a = s.check(pkg)
-    assert torch.equal(a, pkg.attention_int8_paged(*s.args()))
+    assert torch.equal(a, s.call(pkg))
 
 
 @pytest.mark.parametrize("spread", [3.0, 12.0, 40.0])
@@ -86,7 +106,7 @@ def test_nan_reaches_its_rows_only(pkg):
     s.ks[s.table[0, 2].long(), 1, 3] = float("nan")               # key 35 of all rows of the first sequence
     s.vs[s.table[1, 2].long(), 0, 0] = float("nan")               # key 32: seen from row 32 on
     s.vs[s.table[1, 3].long(), 1, 15] = float("inf")              # the last key
-    o = pkg.attention_int8_paged(*s.args())
+    o = s.call(pkg)
     bad = torch.zeros(164, 4, 1, dtype=torch.bool, device="cuda")
     bad[:100, 2:] = True
     bad[132:, :2] = True
@@ -100,7 +120,7 @@ def test_nan_reaches_its_rows_only(pkg):
 
 def test_rows_that_see_nothing(pkg):
     s = Setup([90, 50, 40], [30, 0, 300], 4, 2, 128, 16, 1)
-    o, lse = pkg.attention_int8_paged(*s.args(), return_lse=True)
+    o, lse = s.call(pkg, return_lse=True)
     assert (o[:60] == 0).all() and (o[90:140] == 0).all() and torch.isinf(lse[:60]).all() and torch.isinf(lse[90:140]).all()
     s.check(pkg)
     s.check(pkg, causal=False)
@@ -108,11 +128,11 @@ def test_rows_that_see_nothing(pkg):
 
 def test_rows_behind_the_last_sequence_stay(pkg):
     s = Setup([70, 50], [70, 99], 4, 2, 64, 16, 1)
-    want, T = pkg.attention_int8_paged(*s.args()), 120
+    want, T = s.call(pkg), 120
     pad = lambda x: torch.cat([x, x[:9]])
     s.q8, s.qs = pad(s.q8), pad(s.qs)
     out = torch.full((T + 9, 4, 64), 9.0, device="cuda", dtype=torch.float16)
-    pkg.attention_int8_paged(*s.args(), out=out)
+    s.call(pkg, out=out)
     assert torch.equal(out[:T], want) and (out[T:] == 9).all()
 
 
@@ -122,7 +142,7 @@ def test_query_and_output_views(pkg):
     wide[:, 2:8, 128:] = s.q8
     s.q8 = wide[:, 2:8, 128:]
     base_ = torch.full((141, 6, 256), 7.0, device="cuda", dtype=torch.float16)
-    o, lse = pkg.attention_int8_paged(*s.args(), out=base_[..., :128], return_lse=True)
+    o, lse = s.call(pkg, out=base_[..., :128], return_lse=True)
     assert (base_[..., 128:] == 7).all()
     s.check(pkg, got=(o, lse))
     s.q8 = s.q8[:, :1].expand(141, 6, 128)                        # one head's rows for all
@@ -131,19 +151,19 @@ def test_query_and_output_views(pkg):
 
 def test_bad_indices(pkg):
     s = Setup([100, 60], [100, 200], 4, 2, 64, 16, 1)
-    good = pkg.attention_int8_paged(*s.args())
+    good = s.call(pkg)
     assert pkg.check_status() == 0
     for bad in (s.kc.shape[0], -1, 1 << 30):
         was = s.table[0, 3].clone()
         s.table[0, 3] = bad
-        o = pkg.attention_int8_paged(*s.args())
+        o = s.call(pkg)
         with pytest.raises(pkg.IntfaError, match="outside its table"):
             pkg.check_status()
         assert torch.equal(o[100:], good[100:])
         s.table[0, 3] = was
     s.table[0] = 0
     s.lens[0] = s.table.shape[1] * 16 + 1
-    o = pkg.attention_int8_paged(*s.args())
+    o = s.call(pkg)
     with pytest.raises(pkg.IntfaError, match="outside its table"):
         pkg.check_status()
     assert torch.equal(o[100:], good[100:])
@@ -151,7 +171,7 @@ def test_bad_indices(pkg):
     for cu in ([0, 160, 100], [0, 100, 200], [-4, 1, 160], [100, 0, 160], [160, 160, 160], [0, 0, 160]):
         s.cu = torch.tensor(cu, dtype=torch.int32, device="cuda")
         s.lens[:] = 200
-        pkg.attention_int8_paged(*s.args())
+        s.call(pkg)
         try:
             pkg.check_status()
         except pkg.IntfaError:
@@ -160,7 +180,7 @@ def test_bad_indices(pkg):
 
 def test_two_streams_at_once_and_a_replayed_graph(pkg):
     a, b = Setup([100, 300, 8], [900, 300, 500], 8, 2, 128, 16, 1), Setup([3, 160], [1000, 200], 8, 2, 64, 16, 4, seed=5)
-    wa, wb = pkg.attention_int8_paged(*a.args()), pkg.attention_int8_paged(*b.args())
+    wa, wb = a.call(pkg), b.call(pkg)
     sa, sb = torch.cuda.Stream(), torch.cuda.Stream()
     for s in (sa, sb):
         s.wait_stream(torch.cuda.current_stream())
@@ -168,19 +188,19 @@ def test_two_streams_at_once_and_a_replayed_graph(pkg):
     for _ in range(10):
         for s, x, w in ((sa, a, wa), (sb, b, wb)):
             with torch.cuda.stream(s):
-                got.append((pkg.attention_int8_paged(*x.args()), w))
+                got.append((x.call(pkg), w))
     torch.cuda.synchronize()
     assert all(torch.equal(x, w) for x, w in got)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        outs = [pkg.attention_int8_paged(*a.args()) for _ in range(2)]
+        outs = [a.call(pkg) for _ in range(2)]
     cu, lens = a.cu.clone(), a.lens.clone()
     for news, ls in (([100, 300, 8], [900, 300, 500]), ([1, 407, 0], [33, 407, 0]), ([200, 8, 200], [200, 8, 511])):
         a.cu[1:] = torch.tensor(news, device="cuda").cumsum(0).int()
         a.lens.copy_(torch.tensor(ls, device="cuda"))
         a.table.clamp_(max=a.kc.shape[0] - 1)
         graph.replay()
-        want = pkg.attention_int8_paged(*a.args())
+        want = a.call(pkg)
         # (bit by bit: the longer ones run into pages whose scales are NaN)
         assert all(torch.equal(o.view(torch.int16), want.view(torch.int16)) for o in outs)
     pkg.check_status()
@@ -191,8 +211,8 @@ def test_after_and_before_the_other_kernels(pkg, oracle):
     a, b = Setup([100, 300, 8], [900, 300, 500], 8, 2, 128, 16, 1), Setup([1, 1], [700, 90], 8, 2, 128, 16, 1, seed=3)
     g = torch.Generator(device="cuda").manual_seed(1)
     q, k, v = (torch.randn(1, 4, 512, 128, device="cuda", generator=g).half() for _ in range(3))
-    calls = [lambda: pkg.attention_int8_paged(*a.args()), lambda: pkg.int_flash_attention(q, k, v, True, 0.09), lambda: pkg.attention_int8_paged(*b.args()),
-             lambda: pkg.int_flash_attention(q, k, v, False, 0.09, variant="half"), lambda: pkg.attention_int8_paged(*a.args())]
+    calls = [lambda: a.call(pkg), lambda: pkg.int_flash_attention(q, k, v, True, 0.09), lambda: b.call(pkg),
+             lambda: pkg.int_flash_attention(q, k, v, False, 0.09, variant="half"), lambda: a.call(pkg)]
     want = []
     for f in calls:
         want.append(f())
