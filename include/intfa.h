@@ -323,7 +323,7 @@ typedef struct IntfaPagedParams {
   int32_t causal; float sm_scale;
   void* workspace; uint64_t workspace_bytes;
   int32_t* status;
-  int32_t debug_path;                   /* test hook: 0 the rule on sizes, 1 packed rows, 2 128-row tiles (D <= 128, H/H_kv <= 128) */
+  int32_t debug_path;                   /* test hook: 0 the rule on sizes, 1 packed rows, 2 128-row tiles (H/H_kv <= 128) */
 } IntfaPagedParams;
 int intfa_paged_attention(const IntfaPagedParams* p, void* stream);
 size_t intfa_paged_workspace_bytes(const IntfaPagedParams* p);

@@ -308,8 +308,8 @@ static int check_paged(const IntfaPagedParams* p) {
   if (!p->cu_seqlens && p->tokens != p->cache.S) return set_error(INTFA_ERR_INVALID_ARG, "without cu_seqlens there is one row a sequence: %lld rows, %d sequences", (long long)p->tokens, p->cache.S);
   if (p->tokens * p->H > 0x7fffffffLL) return set_error(INTFA_ERR_TOO_LARGE, "too many query rows");
   if (p->o_dtype != INTFA_OUT_FP16 && p->o_dtype != INTFA_OUT_BF16) return set_error(INTFA_ERR_INVALID_ARG, "o_dtype must be INTFA_OUT_FP16 or INTFA_OUT_BF16");
-  if (p->debug_path < 0 || p->debug_path > 2 || (p->debug_path == 2 && (p->cache.D > 128 || p->H / p->cache.H_kv > 128)))
-    return set_error(INTFA_ERR_UNSUPPORTED, "debug_path %d: 0, 1, or 2 for head dims up to 128 and up to 128 query heads a K/V head", p->debug_path);
+  if (p->debug_path < 0 || p->debug_path > 2 || (p->debug_path == 2 && p->H / p->cache.H_kv > 128))
+    return set_error(INTFA_ERR_UNSUPPORTED, "debug_path %d: 0, 1, or 2 for up to 128 query heads a K/V head", p->debug_path);
   return INTFA_OK;
 }
 size_t intfa_paged_workspace_bytes(const IntfaPagedParams* p) { return p && check_paged(p) == INTFA_OK ? paged_workspace_bytes(p) : 0; }

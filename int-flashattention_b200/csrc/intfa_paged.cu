@@ -4,7 +4,7 @@
 // Reads 2 bytes a value, writes 1 (10 000 tokens of 32 + 8 + 8 heads x 128: 345 MB, 53 us at the measured copy rate): bound by HBM, and
 // by launch and latency for the few tokens of a decode step.
 //   block = 1   a row (one head of one token) is quantised by the lanes that loaded it; a CTA takes one token, or a few of few heads
-//   block > 1   a CTA takes what a sequence adds to one block, for some heads: the largest magnitudes first, then the codes.  A block that
+//   block > 1   a warp (short blocks) or a CTA takes what a sequence adds to one block, for some heads: the largest magnitudes first, then the codes.  A block that
 //               began in an earlier call keeps the larger of its old scale and the new tokens'; where that grew its older codes become
 //               rint(code * (old / new)).  So a block's codes depend on how its tokens were handed over, as its scale must.
 #include "intfa_rows.cuh"
@@ -175,8 +175,112 @@ __global__ void __launch_bounds__(kThreads, SPIN == kAny ? 2 : 3) append_tokens_
   token_rows<T, D, SPIN, true>(p, blockIdx.x, tokens_cta, per_token, place);
 }
 
-// block > 1.  CTAs 0 .. units * groups - 1: what one sequence adds to one block, `heads_cta` heads of K and V; the rest: q.
-// Unit u of sequence s: u = cu[s] / block + 2 s + i for the i-th block that the sequence touches (it touches at most n / block + 2).
+// What one sequence adds to one block.  Unit u of sequence s: u = cu[s] / block + 2 s + i for the i-th block that the sequence touches (it
+// touches at most n / block + 2).  Called by a warp.
+struct BlockRun {
+  long long first, b0, n0, n1;           // the sequence's first new token; the block's first token; its new ones (positions)
+  int t0, page, slot0;                   // row of the sequence's first new token; page; slot of b0 in it
+};
+__device__ __forceinline__ bool block_run(const AppendJob& p, int u, bool report_bad, BlockRun& r) {
+  const int s = p.cu ? find_last(p.S, u, [&](int i) { return (long long)(p.cu[i] >> p.block_log) + 2 * i; })
+                     : find_last(p.S, u, [&](int i) { return (long long)(i >> p.block_log) + 2 * i; });
+  const int t1 = cu_at(p, s + 1), block = 1 << p.block_log;
+  r.t0 = cu_at(p, s);
+  const long long len = p.lens[s];
+  r.first = len - (t1 - r.t0);
+  if (r.t0 < 0 || t1 <= r.t0 || len == 0) return false;
+  const long long bi = (r.first >> p.block_log) + (u - ((r.t0 >> p.block_log) + 2 * s));
+  r.b0 = bi << p.block_log;
+  r.n0 = r.b0 > r.first ? r.b0 : r.first;
+  r.n1 = r.b0 + block < len ? r.b0 + block : len;
+  const long long col = r.b0 >> p.page_log;
+  const bool bad = r.first < 0 || t1 > p.tokens;
+  if (!bad && r.n0 >= r.n1) return false;
+  r.page = !bad && col < p.width ? p.table[s * p.table_stride + col] : -1;
+  if (r.page < 0 || r.page >= p.pages || (p.rot_table && r.n1 > p.rot_rows)) {
+    if (report_bad) report(p);
+    return false;
+  }
+  r.slot0 = (int)(r.b0 & ((1 << p.page_log) - 1));
+  return true;
+}
+// 16 codes of an older token under a scale that grew
+__device__ __forceinline__ void follow(int8_t* at, float was, float now) {
+  const uint4 c = *reinterpret_cast<const uint4*>(at);
+  const uint32_t cw[4] = {c.x, c.y, c.z, c.w};
+  const float ratio = now > 0.f && now <= 3.402823466e38f ? __fdiv_rn(was, now) : 0.f;
+  uint32_t b[16], o[4];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) b[j] = __float_as_uint(__fadd_rn(__fmul_rn((float)(int8_t)(cw[j / 4] >> (8 * (j & 3))), ratio), 12582912.0f));
+#pragma unroll
+  for (int j = 0; j < 4; ++j) o[j] = __byte_perm(__byte_perm(b[4 * j], b[4 * j + 1], 0x0040), __byte_perm(b[4 * j + 2], b[4 * j + 3], 0x0040), 0x5410);
+  *reinterpret_cast<uint4*>(at) = make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+// Short blocks: a warp takes what a sequence adds to one block, `pairs` of the (head, K or V) one after the other, and keeps the values of one in
+// registers from the maximum to the codes: nothing but shuffles between them.  CTAs from `ctas` on: q.
+constexpr int kRounds = 4;               // rows a slot holds: blocks of up to 4 * 32 / (D/16) tokens
+template <typename T, int D, int SPIN>
+__global__ void __launch_bounds__(kThreads, 2) append_runs_kernel(const AppendJob p, int units, int groups, int pairs, int ctas, int tokens_cta, int per_token) {
+  constexpr int LPR = D / 16, SLOTS = 32 / LPR;
+  __shared__ Place place[kMaxTokens];
+  pdl_wait();
+  pdl_launch();
+  if ((int)blockIdx.x >= ctas) {
+    token_rows<T, D, SPIN, false>(p, (int)blockIdx.x - ctas, tokens_cta, per_token, place);
+    return;
+  }
+  const int lane = threadIdx.x & 31, id = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), u = id / groups, g = id - u * groups;
+  BlockRun r;
+  if (u >= units || !block_run(p, u, lane == 0, r)) return;
+  const int slot = lane / LPR, nt = (int)(r.n1 - r.n0), older = (int)(r.n0 - r.b0), blk = r.slot0 >> p.block_log;
+  Pieces at;
+  at.place<SPIN>(lane % LPR, p.rot);
+  const int end = min((g + 1) * pairs, 2 * p.heads[1]);
+#pragma unroll 1
+  for (int pair = g * pairs; pair < end; ++pair) {
+    const int w = pair & 1, h = pair >> 1;
+    const T* row = static_cast<const T*>(p.x[1 + w]) + (r.t0 + (r.n0 - r.first) + slot) * p.xn[1 + w] + h * p.xh[1 + w];
+    float* sc = p.scale[w] + r.page * p.sp[w] + h * p.sh[w] + blk * p.sb[w];
+    int8_t* out = p.cache[w] + r.page * p.cp[w] + h * p.ch[w] + r.slot0 * p.cn[w];
+    Row16<T> raw[kRounds];
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k) {
+      raw[k].zero();
+      if (k * SLOTS + slot < nt) raw[k].load(row + k * SLOTS * p.xn[1 + w], at);
+    }
+    const float was = older > 0 ? *sc : 0.f;
+    float x[kRounds][16], m = 0.f;
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k) {
+      if (k * SLOTS >= nt) break;
+      widen16(raw[k], x[k]);
+      if (SPIN != kNone && w == 0 && k * SLOTS + slot < nt) {
+        Turn<SPIN> turn;
+        turn.load(p.rot_table, r.n0 + k * SLOTS + slot, p.rot, false, at);
+        turn.apply(x[k], row + k * SLOTS * p.xn[1 + w], p.rot, at);
+      }
+      m = max_nan(m, absmax16(x[k]));
+    }
+    const float now = max_nan(was, scale_of(row_max<32>(m)));
+    if (lane == 0) *sc = now;
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k) {
+      if (k * SLOTS >= nt) break;
+      uint32_t c[4];
+      codes(x[k], now, c);
+      if (k * SLOTS + slot < nt) {
+        int8_t* o = out + (older + k * SLOTS + slot) * p.cn[w];
+        *reinterpret_cast<uint2*>(o + at.a) = make_uint2(c[0], c[1]);
+        *reinterpret_cast<uint2*>(o + at.b) = make_uint2(c[2], c[3]);
+      }
+    }
+    if (__float_as_uint(was) != __float_as_uint(now))
+      for (int i = slot; i < older; i += SLOTS) follow(out + i * p.cn[w] + lane % LPR * 16, was, now);
+  }
+}
+
+// Longer blocks: a CTA takes them, some heads at a time; maxima first, then the rows once more for the codes.  CTAs from units * groups on: q.
 template <typename T, int D, int SPIN>
 __global__ void __launch_bounds__(kThreads, 2) append_blocks_kernel(const AppendJob p, int units, int groups, int heads_cta, int tokens_cta, int per_token) {
   constexpr int LPR = D / 16, SLOTS = kThreads / LPR;
@@ -189,35 +293,16 @@ __global__ void __launch_bounds__(kThreads, 2) append_blocks_kernel(const Append
     token_rows<T, D, SPIN, false>(p, (long long)blockIdx.x - (long long)units * groups, tokens_cta, per_token, place);
     return;
   }
-  const int u = blockIdx.x / groups, head0 = (blockIdx.x - u * groups) * heads_cta;
-  const int nh = min(heads_cta, p.heads[1] - head0), block = 1 << p.block_log;
-  const int s = p.cu ? find_last(p.S, u, [&](int i) { return (long long)(p.cu[i] >> p.block_log) + 2 * i; })
-                     : find_last(p.S, u, [&](int i) { return (long long)(i >> p.block_log) + 2 * i; });
-  const int t0 = cu_at(p, s), t1 = cu_at(p, s + 1);
-  const long long len = p.lens[s], first = len - (t1 - t0);
-  if (t0 < 0 || t1 <= t0 || len == 0) return;
-  if (first < 0 || t1 > p.tokens) {
-    if (threadIdx.x == 0) report(p);
-    return;
-  }
-  // the block, its new tokens [n0, n1) (positions) and where its older ones begin
-  const long long bi = (first >> p.block_log) + (u - ((t0 >> p.block_log) + 2 * s)), b0 = bi << p.block_log;
-  const long long n0 = b0 > first ? b0 : first, n1 = b0 + block < len ? b0 + block : len;
-  if (n0 >= n1) return;
-  const bool began = b0 < n0;
-  const long long col = b0 >> p.page_log;
-  const int page = col < p.width ? p.table[s * p.table_stride + col] : -1;
-  if (page < 0 || page >= p.pages || (p.rot_table && n1 > p.rot_rows)) {
-    if (threadIdx.x == 0) report(p);
-    return;
-  }
-  const int slot0 = (int)(b0 & ((1 << p.page_log) - 1)), blk = slot0 >> p.block_log;
+  const int u = blockIdx.x / groups, head0 = (blockIdx.x - u * groups) * heads_cta, nh = min(heads_cta, p.heads[1] - head0);
+  BlockRun run;
+  if (!block_run(p, u, threadIdx.x == 0, run)) return;
+  const int slot0 = run.slot0, blk = slot0 >> p.block_log, page = run.page, older = (int)(run.n0 - run.b0);
   const int slot = threadIdx.x / LPR;
   Pieces at;
   at.place<SPIN>(threadIdx.x % LPR, p.rot);
   for (int i = threadIdx.x; i < 2 * nh; i += kThreads) most[i] = 0u;
   __syncthreads();
-  const int nt = (int)(n1 - n0), rows = nt * nh * 2, rounds = (rows + SLOTS - 1) / SLOTS;
+  const int nt = (int)(run.n1 - run.n0), rows = nt * nh * 2, rounds = (rows + SLOTS - 1) / SLOTS;
   // row r: token r / (2 nh), then K's heads and V's
   float x[16];
   auto fetch = [&](int k, int& token, int& wh) {
@@ -226,14 +311,14 @@ __global__ void __launch_bounds__(kThreads, 2) append_blocks_kernel(const Append
     token = ok ? r / (2 * nh) : 0;
     wh = ok ? r - token * 2 * nh : 0;
     const int w = wh >= nh ? 1 : 0, h = head0 + wh - (w ? nh : 0);
-    const T* row = static_cast<const T*>(p.x[1 + w]) + (t0 + (n0 - first) + token) * p.xn[1 + w] + h * p.xh[1 + w];
+    const T* row = static_cast<const T*>(p.x[1 + w]) + (run.t0 + (run.n0 - run.first) + token) * p.xn[1 + w] + h * p.xh[1 + w];
     Row16<T> raw;
     raw.zero();
     if (ok) raw.load(row, at);
     widen16(raw, x);
     if (SPIN != kNone && ok && w == 0) {
       Turn<SPIN> turn;
-      turn.load(p.rot_table, n0 + token, p.rot, false, at);
+      turn.load(p.rot_table, run.n0 + token, p.rot, false, at);
       turn.apply(x, row, p.rot, at);
     }
     return ok;
@@ -249,11 +334,11 @@ __global__ void __launch_bounds__(kThreads, 2) append_blocks_kernel(const Append
   __syncthreads();
   for (int i = threadIdx.x; i < 2 * nh; i += kThreads) {
     const int w = i >= nh ? 1 : 0, h = head0 + i - (w ? nh : 0);
-    float* at = p.scale[w] + page * p.sp[w] + h * p.sh[w] + blk * p.sb[w];
-    const float old = began ? *at : 0.f, now = max_nan(old, scale_of(__uint_as_float(most[i])));
+    float* sc = p.scale[w] + page * p.sp[w] + h * p.sh[w] + blk * p.sb[w];
+    const float old = older > 0 ? *sc : 0.f, now = max_nan(old, scale_of(__uint_as_float(most[i])));
     s_old[i] = old;
     s_new[i] = now;
-    *at = now;
+    *sc = now;
   }
   __syncthreads();
 #pragma unroll 1
@@ -263,27 +348,15 @@ __global__ void __launch_bounds__(kThreads, 2) append_blocks_kernel(const Append
     const int w = wh >= nh ? 1 : 0, h = head0 + wh - (w ? nh : 0);
     uint32_t c[4];
     codes(x, s_new[wh], c);
-    int8_t* out = p.cache[w] + page * p.cp[w] + h * p.ch[w] + (slot0 + (int)(n0 - b0) + token) * p.cn[w];
+    int8_t* out = p.cache[w] + page * p.cp[w] + h * p.ch[w] + (slot0 + older + token) * p.cn[w];
     *reinterpret_cast<uint2*>(out + at.a) = make_uint2(c[0], c[1]);
     *reinterpret_cast<uint2*>(out + at.b) = make_uint2(c[2], c[3]);
   }
-  if (!began) return;
-  const int older = (int)(n0 - b0) * nh * 2;
 #pragma unroll 1
-  for (int r = slot; r < older; r += SLOTS) {
+  for (int r = slot; r < older * nh * 2; r += SLOTS) {
     const int tk = r / (2 * nh), i = r - tk * 2 * nh, w = i >= nh ? 1 : 0, h = head0 + i - (w ? nh : 0);
-    const float was = s_old[i], now = s_new[i];
-    if (__float_as_uint(was) == __float_as_uint(now)) continue;
-    uint4* out = reinterpret_cast<uint4*>(p.cache[w] + page * p.cp[w] + h * p.ch[w] + (slot0 + tk) * p.cn[w] + threadIdx.x % LPR * 16);
-    const uint4 c = *out;
-    const uint32_t cw[4] = {c.x, c.y, c.z, c.w};
-    const float ratio = now > 0.f && now <= 3.402823466e38f ? __fdiv_rn(was, now) : 0.f;
-    uint32_t b[16], o[4];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) b[j] = __float_as_uint(__fadd_rn(__fmul_rn((float)(int8_t)(cw[j / 4] >> (8 * (j & 3))), ratio), 12582912.0f));
-#pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = __byte_perm(__byte_perm(b[4 * j], b[4 * j + 1], 0x0040), __byte_perm(b[4 * j + 2], b[4 * j + 3], 0x0040), 0x5410);
-    *out = make_uint4(o[0], o[1], o[2], o[3]);
+    if (__float_as_uint(s_old[i]) == __float_as_uint(s_new[i])) continue;
+    follow(p.cache[w] + page * p.cp[w] + h * p.ch[w] + (slot0 + tk) * p.cn[w] + threadIdx.x % LPR * 16, s_old[i], s_new[i]);
   }
 }
 
@@ -303,15 +376,26 @@ int run(const AppendJob& p, cudaStream_t stream) {
     if (grid > 0x7fffffffLL) return set_error(INTFA_ERR_TOO_LARGE, "too many tokens");
     return launch_kernel("append", append_tokens_kernel<T, D, SPIN>, (unsigned)grid, kThreads, 0, stream, p, n, per);
   }
-  // Heads a CTA: one or two rounds of rows, so that a step of one token has all its heads in one CTA
+  const int per = p.q8 ? slots_of(p.heads[0]) : SLOTS, n = SLOTS / per;
+  const long long units = (p.tokens >> p.block_log) + 2LL * p.S, q_ctas = p.q8 ? (p.tokens + n - 1) / n : 0;
+  if constexpr (SPIN != kAny)             // (whose element-wise way has no registers for it)
+  if ((1 << p.block_log) <= kRounds * 32 / (D / 16)) {
+    // (head, K or V) pairs a warp: so many that all warps are there at once, eight at most
+    long long pairs = units * 2 * p.heads[1] / (16LL * sm_count_cached());
+    pairs = pairs < 1 ? 1 : pairs > 8 ? 8 : pairs;
+    const long long groups = (2 * p.heads[1] + pairs - 1) / pairs, ctas = (units * groups + kThreads / 32 - 1) / (kThreads / 32);
+    if (units * groups > 0x7fffffffLL || ctas + q_ctas > 0x7fffffffLL) return set_error(INTFA_ERR_TOO_LARGE, "too many tokens");
+    return launch_kernel("append", append_runs_kernel<T, D, SPIN>, (unsigned)(ctas + q_ctas), kThreads, 0, stream, p, (int)units, (int)groups, (int)pairs, (int)ctas, n,
+                         per);
+  }
+  // Heads a CTA: one or two rounds of rows
   int heads_cta = 2 * SLOTS / (2 << p.block_log);
   if (heads_cta < 1) heads_cta = 1;
   if (heads_cta > p.heads[1]) heads_cta = p.heads[1];
   if (heads_cta > kThreads) heads_cta = kThreads;
-  const int groups = (p.heads[1] + heads_cta - 1) / heads_cta, per = p.q8 ? slots_of(p.heads[0]) : SLOTS, n = SLOTS / per;
-  const long long units = (p.tokens >> p.block_log) + 2LL * p.S, grid = units * groups + (p.q8 ? (p.tokens + n - 1) / n : 0);
-  if (grid > 0x7fffffffLL) return set_error(INTFA_ERR_TOO_LARGE, "too many tokens");
-  return launch_kernel("append", append_blocks_kernel<T, D, SPIN>, (unsigned)grid, kThreads, 0, stream, p, (int)units, groups, heads_cta, n, per);
+  const int groups = (p.heads[1] + heads_cta - 1) / heads_cta;
+  if (units * groups + q_ctas > 0x7fffffffLL) return set_error(INTFA_ERR_TOO_LARGE, "too many tokens");
+  return launch_kernel("append", append_blocks_kernel<T, D, SPIN>, (unsigned)(units * groups + q_ctas), kThreads, 0, stream, p, (int)units, groups, heads_cta, n, per);
 }
 template <typename T, int D>
 int run_spin(const AppendJob& p, bool interleaved, cudaStream_t stream) {

@@ -74,8 +74,8 @@ struct PParams {
   int causal, o_bf16;
   float c;                                        // sm_scale * log2(e)
   int workers, least;                             // warps of the grid; fewest chunks a warp takes
-  int rows_tile;                                  // rows of a unit: RT, or 256 on the 128-row tiles
-  int tile_tokens;                                // 128-row tiles: whole tokens in one; 0: packed RT rows
+  int rows_tile;                                  // rows of a unit: RT, or those of one or two 128-row tiles
+  int tile_tokens, unit_tokens;                   // 128-row tiles: whole tokens in one, in a unit; 0: packed RT rows
   float* part; float* part_ml;                    // [2*workers][RT][D]; [2*workers][RT]{m, mw, l, -}
   UnitPart* units; long long max_units;           // [max_units]
   int* head;                                      // {units}
@@ -836,11 +836,13 @@ struct Plan {
 // begin, to end and to be put together.  The lengths of the sequences are not known here; timed on both with 600 and 4000 keys: at 128 channels
 // 16 sequences of 8 K/V heads, 64 rows each a head, 26.0 / 74.0 us packed, 30.6 / 63.7 on tiles, of 32 rows 23.3 / 49.1 and 29.8 / 56.7; one
 // sequence, 256 rows, 24.2 / 51.4 and 28.5 / 29.1, 128 rows 15.7 / 31.3 and 17.9 / 29.3; at 64 channels 16 sequences, 128 rows, 27.9 / 81.9 and
-// 30.6 / 60.5, 64 rows 19.6 / 46.4 and 26.9 / 61.7.
+// 30.6 / 60.5, 64 rows 19.6 / 46.4 and 26.9 / 61.7; at 256 channels 32 rows 40.1 / 93.1 and 36.0 / 69.7, one sequence, 128 rows, 25.9 / 50.0 and
+// 21.9 / 37.0, 64 rows 17.3 / 30.3 and 18.7 / 31.3.
 bool takes_tiles(const IntfaPagedParams* a) {
   if (a->debug_path) return a->debug_path == 2;
   const double rows = (double)a->tokens * (a->H / a->cache.H_kv) / a->cache.S;          // of an average sequence and K/V head
-  return a->cache.D <= 128 && a->H / a->cache.H_kv <= kTileRows && rows >= (a->cache.D == 64 ? 112 : 64) && rows * a->cache.S * a->cache.H_kv >= 2048;
+  return a->H / a->cache.H_kv <= kTileRows && rows >= (a->cache.D == 64 ? 112 : a->cache.D == 128 ? 64 : 32) &&
+         rows * a->cache.S * a->cache.H_kv >= (a->cache.D == 256 ? 1024 : 2048);
 }
 Plan make_plan(const IntfaPagedParams* a, int sms) {
   Plan pl;
@@ -856,8 +858,9 @@ Plan make_plan(const IntfaPagedParams* a, int sms) {
   if (pl.tiles) {
     pl.warps = 1;
     pl.max_units = pl.ctas;
-    take((size_t)2 * pl.ctas * 2 * kTileRows * c.D * 4);
-    pl.off_ml = take((size_t)2 * pl.ctas * 2 * kTileRows * 16);
+    const int rows = c.D == 256 ? kTileRows : 2 * kTileRows;
+    take((size_t)2 * pl.ctas * rows * c.D * 4);
+    pl.off_ml = take((size_t)2 * pl.ctas * rows * 16);
     pl.off_units = take((size_t)pl.max_units * sizeof(UnitPart));
     pl.off_head = take(32);
     return pl;
@@ -907,12 +910,12 @@ int run_tiles(const IntfaPagedParams* a, const Plan& pl, PParams p, cudaStream_t
   using C = TileCfg<D>;
   const IntfaPagedCache& c = a->cache;
   CUtensorMap tmQ, tmK, tmV;
-  const CUtensorMapSwizzle swz = D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+  const CUtensorMapSwizzle swz = C::PANEL == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
   const int64_t qst[3] = {(int64_t)p.T * p.qn, p.qn, p.qh};
   int rc;
-  if ((rc = make_tmap(&tmQ, a->q, 1, qst, 1, (int)p.T, a->H, D, D, p.ratio, swz, p.tile_tokens))) return rc;
-  if ((rc = make_tmap(&tmK, c.k, 1, c.k_stride, c.pages, c.H_kv, c.page_size, D, D, 1 << p.box_log, swz))) return rc;
-  if ((rc = make_tmap(&tmV, c.v, 1, c.v_stride, c.pages, c.H_kv, c.page_size, D, D, 1 << p.box_log, swz))) return rc;
+  if ((rc = make_tmap(&tmQ, a->q, 1, qst, 1, (int)p.T, a->H, D, C::PANEL, p.ratio, swz, p.tile_tokens))) return rc;
+  if ((rc = make_tmap(&tmK, c.k, 1, c.k_stride, c.pages, c.H_kv, c.page_size, D, C::PANEL, 1 << p.box_log, swz))) return rc;
+  if ((rc = make_tmap(&tmV, c.v, 1, c.v_stride, c.pages, c.H_kv, c.page_size, D, C::PANEL, 1 << p.box_log, swz))) return rc;
   auto kern = paged_tile_kernel<D>;
   static std::atomic<bool> attr_done[64];
   int dev = 0;
@@ -982,11 +985,12 @@ int paged_attention(const IntfaPagedParams* a, cudaStream_t stream) {
   p.status = a->status;
   p.tile_tokens = 0;
   if (pl.tiles) {
-    p.rows_tile = 2 * kTileRows;
+    p.rows_tile = c.D == 256 ? kTileRows : 2 * kTileRows;
     p.tile_tokens = kTileRows / p.ratio;
+    p.unit_tokens = p.tile_tokens * (p.rows_tile / kTileRows);
     p.box_log = c.page_size < kTileKeys ? p.page_log : log2_of(kTileKeys);
     p.least = 2;
-    return c.D == 64 ? run_tiles<64>(a, pl, p, stream) : run_tiles<128>(a, pl, p, stream);
+    return c.D == 64 ? run_tiles<64>(a, pl, p, stream) : c.D == 128 ? run_tiles<128>(a, pl, p, stream) : run_tiles<256>(a, pl, p, stream);
   }
   switch (c.D) {
     case 64: return pl.NT == 2 ? run<64, 2, 8, 4>(a, pl, p, stream) : run<64, 1, 8, 5>(a, pl, p, stream);

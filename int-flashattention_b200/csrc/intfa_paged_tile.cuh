@@ -53,14 +53,14 @@ __device__ __forceinline__ TileSeq tile_seq_of(const PParams& p, int s) {
   w.n = q.n;
   w.keys = q.keys;
   w.first = q.len - q.n;
-  w.tiles = (q.n + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
+  w.tiles = (q.n + p.unit_tokens - 1) / p.unit_tokens;
   w.uniform = !p.causal || w.first < 0 || q.len > q.keys;        // every unit goes over all keys (for the odd lengths, masked)
   return w;
 }
 template <int G>
 __device__ __forceinline__ int tile_chunks(const PParams& p, const TileSeq& q, int tile) {
   long long vis = q.keys;
-  if (!q.uniform) vis = min(vis, q.first + (long long)(tile + 1) * 2 * p.tile_tokens);
+  if (!q.uniform) vis = min(vis, q.first + (long long)(tile + 1) * p.unit_tokens);
   return vis > G ? (int)((vis + G - 1) / G) : 1;
 }
 // sum of floor((a t + b) / m), t = 0 .. n-1 (a, b >= 0)
@@ -86,16 +86,21 @@ __device__ inline long long tile_chunks_before(const PParams& p, const TileSeq& 
   if (k <= 0) return 0;
   if (q.uniform) return (long long)k * tile_chunks<G>(p, q, 0);
   const int full = k < q.tiles ? k : q.tiles - 1;
-  const long long step = 2 * p.tile_tokens;
+  const long long step = p.unit_tokens;
   return floor_sum(full, G, step, q.first + step + G - 1) + (k == q.tiles ? tile_chunks<G>(p, q, q.tiles - 1) : 0);
 }
 
 template <int D>
 struct TileCfg {
-  static constexpr int G = kTileKeys, THREADS = kTileThreads, NK = 5, NV8 = 4, NV = 3, NSC = 8, NU = 4;
+  // (256 channels: an accumulator of 256 columns, so one tile of rows, and half of the buffers)
+  static constexpr bool WIDE = D == 256;
+  static constexpr int G = kTileKeys, THREADS = kTileThreads, TILES = WIDE ? 1 : 2, NK = WIDE ? 3 : 5, NV8 = WIDE ? 2 : 4, NV = WIDE ? 2 : 3, NSC = 8, NU = 4;
+  static constexpr int PANEL = D < 128 ? D : 128, PANELS = D / PANEL;   // Q, K and the int8 V lie in panels of at most 128 bytes a row
+  // start-address offset (16-byte units) of the kk-th 32-byte slice of an operand of so many rows
+  __host__ __device__ static constexpr uint32_t slice(int kk, int rows) { return (uint32_t)((kk / 4) * ((rows * PANEL) >> 4) + 2 * (kk % 4)); }
   static constexpr int Q_BYTES = kTileRows * D, K_BYTES = G * D, V_BYTES = G * D * 2;
   static constexpr int SC_FLOATS = 3 * G + 4;
-  static constexpr int OFF_Q = 0, OFF_K = OFF_Q + 2 * Q_BYTES, OFF_V8 = OFF_K + NK * K_BYTES, OFF_V = OFF_V8 + NV8 * K_BYTES;
+  static constexpr int OFF_Q = 0, OFF_K = OFF_Q + TILES * Q_BYTES, OFF_V8 = OFF_K + NK * K_BYTES, OFF_V = OFF_V8 + NV8 * K_BYTES;
   static constexpr int OFF_ARM = OFF_V + NV * V_BYTES;
   static constexpr int OFF_SC = OFF_ARM + 4096;
   static constexpr int OFF_UNIT = OFF_SC + NSC * SC_FLOATS * 4;
@@ -108,8 +113,8 @@ struct TileCfg {
   static_assert(SMEM <= 227 * 1024, "shared memory");
   static_assert(OFF_UNIT % 16 == 0 && OFF_SC % 16 == 0 && OFF_PRE % 8 == 0, "alignment");
   static constexpr int COL_S = 0, COL_O = 4 * G;
-  static_assert(COL_O + 2 * D <= 512, "TMEM columns");
-  static constexpr uint64_t SWZ_QK = D == 128 ? kSwz128 : kSwz64;
+  static_assert(COL_O + TILES * D <= 512, "TMEM columns");
+  static constexpr uint64_t SWZ_QK = PANEL == 128 ? kSwz128 : kSwz64;
   static constexpr uint32_t IDESC_QK = make_idesc(2, 1, 1, 0, 0, kTileRows, G);
   static constexpr uint32_t IDESC_PV = make_idesc(1, 0, 0, 0, 1, kTileRows, D);
   static constexpr uint32_t IDESC_ARM = make_idesc(1, 0, 0, 0, 0, kTileRows, G);
@@ -285,10 +290,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
       while (ok) {
         TileUnit u = none;
         if (pos < end) {
-          const int n = tile_chunks<G>(p, q, tile), token = tile * 2 * p.tile_tokens;
+          const int n = tile_chunks<G>(p, q, tile), token = tile * p.unit_tokens;
           u.lim0 = p.causal ? q.first + token : (long long)q.keys;
           u.t0 = q.t0 + token;
-          u.tokens = min(2 * p.tile_tokens, q.n - token);
+          u.tokens = min(p.unit_tokens, q.n - token);
           u.head = head;
           u.s = s;
           u.keys = q.keys;
@@ -346,7 +351,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
           ok = wait(B_QE + i, (n & 1u) ^ 1u, TW_QE);
           if (ok && lane == 0) {
             mbar_expect_tx(BAR(B_QF + i), q_box);
-            tma_load_4d(sQ + i * C::Q_BYTES, &tmQ, BAR(B_QF + i), 0, u.head * p.ratio, u.t0 + i * p.tile_tokens, 0);
+            for (int pn = 0; pn < C::PANELS; ++pn)
+              tma_load_4d(sQ + i * C::Q_BYTES + pn * (kTileRows * C::PANEL), &tmQ, BAR(B_QF + i), pn * C::PANEL, u.head * p.ratio, u.t0 + i * p.tile_tokens, 0);
           }
           __syncwarp();
         }
@@ -373,20 +379,24 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
           if (!ok) break;
           if (lane == 0) mbar_expect_tx(BAR(B_KF + k), bytes);
           __syncwarp();
-          if (lane < full) tma_load_4d(sK + k * C::K_BYTES + lane * box_rows * D, &tmK, BAR(B_KF + k), 0, slot, u.head, page);
+          if (lane < full)
+            for (int pn = 0; pn < C::PANELS; ++pn)
+              tma_load_4d(sK + k * C::K_BYTES + (pn * G + lane * box_rows) * C::PANEL, &tmK, BAR(B_KF + k), pn * C::PANEL, slot, u.head, page);
           __syncwarp();
           ok = wait(B_V8E + v, ((kit / C::NV8) & 1u) ^ 1u, TW_V8E);
           if (!ok) break;
           if (lane == 0) mbar_expect_tx(BAR(B_V8F + v), bytes);
           __syncwarp();
-          if (lane < full) tma_load_4d(sV8 + v * C::K_BYTES + lane * box_rows * D, &tmV, BAR(B_V8F + v), 0, slot, u.head, page);
+          if (lane < full)
+            for (int pn = 0; pn < C::PANELS; ++pn)
+              tma_load_4d(sV8 + v * C::K_BYTES + (pn * G + lane * box_rows) * C::PANEL, &tmV, BAR(B_V8F + v), pn * C::PANEL, slot, u.head, page);
           __syncwarp();
         }
       }
     } else if (warp == 1) {
       // ------------------------------------------------------------------ MMA
       const uint32_t sQ = smem_u32(smem + C::OFF_Q), sK = smem_u32(smem + C::OFF_K), sV = smem_u32(smem + C::OFF_V);
-      const uint64_t descQ = make_smem_desc(sQ, 16, 8 * D, C::SWZ_QK), descK = make_smem_desc(sK, 16, 8 * D, C::SWZ_QK);
+      const uint64_t descQ = make_smem_desc(sQ, 16, 8 * C::PANEL, C::SWZ_QK), descK = make_smem_desc(sK, 16, 8 * C::PANEL, C::SWZ_QK);
       const uint64_t descV = make_smem_desc(sV, D > 64 ? G * 128 : 16, 8 * 128, kSwz128);
       const uint64_t descArm = make_smem_desc(smem_u32(smem + C::OFF_ARM), 128, 256, 0);
       uint32_t kit = 0, vit = 0;                               // chunks of K, of V
@@ -399,7 +409,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         umma_f16(tS, descArm, descArm, C::IDESC_ARM, 0);
 #pragma unroll
         for (int kk = 0; kk < D / 32; ++kk)
-          umma_i8(tS, descQ + (uint64_t)(i * (C::Q_BYTES >> 4) + 2 * kk), descK + (uint64_t)(k * (C::K_BYTES >> 4) + 2 * kk), C::IDESC_QK, 1);
+          umma_i8(tS, descQ + (uint64_t)(i * (C::Q_BYTES >> 4) + C::slice(kk, kTileRows)), descK + (uint64_t)(k * (C::K_BYTES >> 4) + C::slice(kk, G)), C::IDESC_QK,
+                  1);
         umma_commit(BAR(B_S + 2 * i + buf));
         if (last) umma_commit(BAR(B_QE + i));
       };
@@ -556,8 +567,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
 #pragma unroll 2
         for (int i = w0; i < G / 8 * BOXES; i += 4) {
           const int blk = i / BOXES, box = i % BOXES;
-          const int row = blk * 8 + key, piece = box * 4 + pc;
-          const uint4 x = lds16(src + row * D + ((piece ^ (D == 128 ? key : (row >> 1) & 3)) << 4));
+          const int row = blk * 8 + key;
+          const uint32_t from = D == 64 ? row * 64 + ((pc ^ ((row >> 1) & 3)) << 4) : (box >> 1) * (G * 128) + row * 128 + ((((box & 1) * 4 + pc) ^ key) << 4);
+          const uint4 x = lds16(src + from);
           const uint32_t w[4] = {x.x ^ 0x80808080u, x.y ^ 0x80808080u, x.z ^ 0x80808080u, x.w ^ 0x80808080u};
           uint32_t h[8];
 #pragma unroll
@@ -789,7 +801,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
       tc_fence_after();
       const float f = done.slot < 0 ? row_factor(mref, ref, l) : 1.f;
       const int h = done.head * p.ratio + hr;
-      const long long row = (long long)done.slot * (2 * kTileRows) + tile * kTileRows + rr;
+      const long long row = (long long)done.slot * p.rows_tile + tile * kTileRows + rr;
       const long long out_at = write ? (long long)(done.t0 + tok) * p.on + h * p.oh : -1;
       // 64 channels at a time: the warp's 32 rows through shared memory (16-byte pieces ^ row: no bank conflicts), then out as 128-byte lines;
       // a unit's part goes to scratch as it is.

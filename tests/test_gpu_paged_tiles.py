@@ -24,13 +24,14 @@ def test_the_rule_takes_either_path(pkg):
         assert torch.equal(s.call(pkg), got)
         if path == 1:
             assert not torch.equal(want, got)          # (the two round differently)
-    for D, ratio in ((256, 2), (64, 129)):
-        s = Setup([3], [30], ratio, 1, D, 16, 1)
-        with pytest.raises(pkg.IntfaError, match="debug_path"):
-            s.call(pkg)
+    s = Setup([3], [30], 129, 1, 64, 16, 1)            # more query heads a K/V head than a tile has rows
+    with pytest.raises(pkg.IntfaError, match="debug_path"):
+        s.call(pkg)
+    s.path = 0
+    s.check(pkg)
 
 
-@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("ratio,Hkv", [(1, 3), (4, 2), (5, 2), (8, 1), (48, 1), (128, 1)])
 def test_prompts(D, causal, ratio, Hkv, pkg):
@@ -39,7 +40,7 @@ def test_prompts(D, causal, ratio, Hkv, pkg):
 
 
 @pytest.mark.parametrize("page,block", [(8, 1), (8, 8), (16, 2), (32, 32), (64, 1), (128, 16), (256, 1), (256, 256)])
-@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("D", [64, 128, 256])
 def test_pages(page, block, D, pkg):
     s = Setup([150, 70], [150, 427], 8, 2, D, page, block, seed=page, layout="tokens" if block == 2 else "heads")
     s.check(pkg)
@@ -47,12 +48,13 @@ def test_pages(page, block, D, pkg):
 
 @pytest.mark.parametrize("n", [33, 63, 64, 65, 127, 128, 129, 255, 256, 257, 383])
 def test_lengths(n, pkg):
-    for ratio in (1, 2):
-        Setup([n, n + 1], [n, n + 130], 2 * ratio, 2, 64, 32, 1, seed=n).check(pkg)
+    for ratio, D in ((1, 64), (2, 64), (1, 128), (1, 256)):
+        Setup([n, n + 1], [n, n + 130], 2 * ratio, 2, D, 32, 1, seed=n).check(pkg)
 
 
 @pytest.mark.parametrize("S,n,length,H,Hkv,D", [(1, 40, 30000, 8, 1, 128), (1, 9, 5000, 8, 2, 64), (1, 256, 256, 1, 1, 128), (40, 30, 500, 8, 2, 64), (200, 33, 40, 2, 1, 128),
-                                                (1, 2000, 2000, 16, 4, 128), (3, 700, 3001, 32, 8, 64), (600, 33, 33, 1, 1, 64)])
+                                                (1, 2000, 2000, 16, 4, 128), (3, 700, 3001, 32, 8, 64), (600, 33, 33, 1, 1, 64), (2, 300, 9000, 8, 2, 256),
+                                                (1, 700, 700, 6, 2, 256)])
 def test_shares(S, n, length, H, Hkv, D, pkg):
     news = [max(1, n - 3 * s % 29) for s in range(S)]
     s = Setup(news, [length - 7 * i % 31 if length > n else m for i, m in enumerate(news)], H, Hkv, D, 64, 1, seed=S + n)
@@ -84,7 +86,12 @@ def test_scales_of_zero(pkg):
 
 def test_rising_and_falling_scores(pkg):
     """The largest score in the last keys, in the first, and far apart."""
-    s = Setup([64, 40], [1200, 900], 4, 2, 128, 16, 1, garbage=False)
+    for D in (128, 256):
+        rising_and_falling(D, pkg)
+
+
+def rising_and_falling(D, pkg):
+    s = Setup([64, 40], [1200, 900], 4, 2, D, 16, 1, garbage=False)
     order = torch.linspace(0.2, 3, 1200, device="cuda")
     for slope in (order, order.flip(0)):
         for b in range(2):
@@ -92,12 +99,12 @@ def test_rising_and_falling_scores(pkg):
             pos = torch.arange(n, device="cuda")
             s.ks[s.table[b, :-(-n // 16)].long()] = 0.02
             s.ks[s.table[b].long()[pos // 16], :, pos % 16] = (0.02 * slope[:n])[:, None]
-        # exponents up to 127 * 127 * 128 * 0.025 * 0.06 / sqrt(128) * 1.4427 = 395: 4 * 395 * 2^-24 * ln 2 * 2 = 1.3e-4
+        # exponents up to 127 * 127 * D * 0.025 * 0.06 / sqrt(D) * 1.4427 = 35 sqrt(D), 558 at D = 256: 4 * 558 * 2^-24 * ln 2 * 2 = 1.9e-4
         s.check(pkg, more=2.0 ** -12)
     s.scale = -0.05
     s.check(pkg, more=2.0 ** -12)
     s.scale = 1.0
-    s.check(pkg, more=2.0 ** -8)                     # 4469 (11.3 times as much): 1.5e-3
+    s.check(pkg, more=2.0 ** -8)                     # sqrt(D) times as much: 8939, 3.0e-3
 
 
 def test_nan_reaches_its_rows_only(pkg):
