@@ -263,6 +263,7 @@ static int check_cache(const IntfaPagedCache* c) {
   if (!power_of_two(c->block) || c->block > c->page_size)
     return set_error(INTFA_ERR_UNSUPPORTED, "block %d unsupported: a power of two up to page_size = %d", c->block, c->page_size);
   if (c->S <= 0 || c->pages <= 0 || c->H_kv <= 0 || c->table_width <= 0) return set_error(INTFA_ERR_INVALID_ARG, "S, pages, H_kv and table_width must be positive");
+  if ((int64_t)c->table_width * c->page_size > 1 << 30) return set_error(INTFA_ERR_TOO_LARGE, "block_table: more than 2^30 tokens a sequence");
   if ((rc = check_tma_tensor("k_cache", c->k, c->k_stride, 1)) || (rc = check_tma_tensor("v_cache", c->v, c->v_stride, 1))) return rc;
   if (!c->k_scale || !c->v_scale) return set_error(INTFA_ERR_INVALID_ARG, "k_scale / v_scale is NULL");
   if (!c->block_table || !c->seq_lens) return set_error(INTFA_ERR_INVALID_ARG, "block_table / seq_lens is NULL");
@@ -290,7 +291,7 @@ int intfa_paged_append(const IntfaAppendParams* p, void* stream) {
   if (p->tokens <= 0 || (p->q && p->H <= 0)) return set_error(INTFA_ERR_INVALID_ARG, "tokens and H must be positive");
   if (!p->cu_seqlens && p->tokens != p->cache.S) return set_error(INTFA_ERR_INVALID_ARG, "without cu_seqlens there is one token a sequence: %lld tokens, %d sequences", (long long)p->tokens, p->cache.S);
   if (p->dtype != INTFA_TYPE_FP16 && p->dtype != INTFA_TYPE_BF16) return set_error(INTFA_ERR_INVALID_ARG, "dtype must be INTFA_TYPE_FP16 or INTFA_TYPE_BF16");
-  if (p->tokens > 0x7fffffffLL) return set_error(INTFA_ERR_TOO_LARGE, "too many tokens");
+  if (p->tokens > 1 << 30 || p->cache.S > 1 << 28) return set_error(INTFA_ERR_TOO_LARGE, "too many tokens or sequences");
   if ((rc = check_rows("k", p->k, p->k_stride, 2, 2)) || (rc = check_rows("v", p->v, p->v_stride, 2, 2))) return rc;
   if (p->q) {
     if ((rc = check_rows("q", p->q, p->q_stride, 2, 2))) return rc;
@@ -306,7 +307,7 @@ static int check_paged(const IntfaPagedParams* p) {
   if (p->tokens <= 0 || p->H <= 0) return set_error(INTFA_ERR_INVALID_ARG, "tokens and H must be positive");
   if (p->H % p->cache.H_kv) return set_error(INTFA_ERR_INVALID_ARG, "H=%d must be a multiple of H_kv=%d", p->H, p->cache.H_kv);
   if (!p->cu_seqlens && p->tokens != p->cache.S) return set_error(INTFA_ERR_INVALID_ARG, "without cu_seqlens there is one row a sequence: %lld rows, %d sequences", (long long)p->tokens, p->cache.S);
-  if (p->tokens * p->H > 0x7fffffffLL) return set_error(INTFA_ERR_TOO_LARGE, "too many query rows");
+  if (p->tokens > 1 << 30 || p->tokens * p->H > 1 << 30) return set_error(INTFA_ERR_TOO_LARGE, "too many query rows");
   if (p->o_dtype != INTFA_OUT_FP16 && p->o_dtype != INTFA_OUT_BF16) return set_error(INTFA_ERR_INVALID_ARG, "o_dtype must be INTFA_OUT_FP16 or INTFA_OUT_BF16");
   if (p->debug_path < 0 || p->debug_path > 2 || (p->debug_path == 2 && p->H / p->cache.H_kv > 128))
     return set_error(INTFA_ERR_UNSUPPORTED, "debug_path %d: 0, 1, or 2 for up to 128 query heads a K/V head", p->debug_path);

@@ -188,7 +188,11 @@ __device__ __forceinline__ bool block_run(const AppendJob& p, int u, bool report
   r.t0 = cu_at(p, s);
   const long long len = p.lens[s];
   r.first = len - (t1 - r.t0);
-  if (r.t0 < 0 || t1 <= r.t0 || len == 0) return false;
+  if (r.t0 < 0 || t1 < r.t0) {
+    if (report_bad) report(p);
+    return false;
+  }
+  if (t1 == r.t0 || len == 0) return false;
   const long long bi = (r.first >> p.block_log) + (u - ((r.t0 >> p.block_log) + 2 * s));
   r.b0 = bi << p.block_log;
   r.n0 = r.b0 > r.first ? r.b0 : r.first;

@@ -131,6 +131,7 @@ struct Seq {
   int keys;                  // that are looked at
   long long len;
   int tiles, chunks;         // row tiles and chunks of each K/V head
+  bool bad;                  // its rows or its tokens are not where they can be
 };
 __device__ __forceinline__ Seq seq_of(const PParams& p, int s) {
   Seq q;
@@ -140,6 +141,7 @@ __device__ __forceinline__ Seq seq_of(const PParams& p, int s) {
   q.len = p.lens[s];
   const long long most = (long long)p.width << p.page_log;
   q.keys = (int)(q.len < 0 ? 0 : q.len < most ? q.len : most);
+  q.bad = t0 < 0 || t1 < t0 || t1 > p.T || (q.n > 0 && q.len != q.keys);
   q.tiles = (int)(((long long)q.n * p.ratio + p.rows_tile - 1) / p.rows_tile);
   q.chunks = q.keys > kChunk ? (q.keys + kChunk - 1) / kChunk : 1;      // (a row without keys is written, too)
   return q;
@@ -215,8 +217,10 @@ __device__ __forceinline__ int channel_of(int i, int g) {
 __device__ __forceinline__ float safe(float m) { return m == -INFINITY ? 0.f : m; }
 
 // what the sum of a row is multiplied by: 2^(mw - m) / l.  A row that sees nothing has l = 0, one whose values are all zero mw = -inf.
+// (The power in two halves: V scales below 2^-126 leave one that exp2 would flush to zero.)
 __device__ __forceinline__ float row_factor(float m, float mw, float l) {
-  return l == 0.f ? 0.f : mw == -INFINITY ? l * 0.f : ex2_approx(mw - safe(m)) / l;
+  const float half = ex2_approx(0.5f * (mw - safe(m)));
+  return l == 0.f ? 0.f : mw == -INFINITY ? l * 0.f : half / l * half;
 }
 
 template <int D, int NT>
@@ -471,9 +475,8 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_const
       const long long units = (long long)q.tiles * p.Hkv;
       c += units * q.chunks;
       u += units;
-      bad |= q.n > 0 && q.len > q.keys;
+      bad |= q.bad;
     }
-    if (p.cu && threadIdx.x == 0) bad |= p.cu[p.S] > p.T;
     if (bad && p.status && blockIdx.x == 0) atomicCAS(p.status, 0, kStatusBadIndex);
     // sums up to and with each thread: within the warps, then on top of the warps before
     const long long most = p.max_units;
@@ -700,6 +703,23 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_const
       ++unit_id;
     }
     at.next(p);
+  }
+  if (!ok) {
+    // A wait ran out.  The units that this share begins and that were not reached are no parts for combine_kernel; what this warp asked for comes
+    // before it goes, or does not come at all.
+    for (long long i = left - to_load; i > 0; --i) {
+      mbar_drain(bar0 + 8 * stage, parity);
+      if (++stage == NS) {
+        stage = 0;
+        parity ^= 1;
+      }
+    }
+    for (bool begins = open ? unit0 >= begin : at.chunk == 0; left > 0; --left) {
+      if (begins && lane == 0 && unit_id < p.max_units) p.units[unit_id].open = 0;
+      if (at.chunk + 1 == at.q.chunks) ++unit_id;
+      at.next(p);
+      begins = at.chunk == 0;
+    }
   }
   if (!__syncthreads_or(merge)) return;
   // (every warp is done with its ring: what it asked for has come)

@@ -45,6 +45,7 @@ struct Flag {
 struct TileSeq {
   int t0, n, keys, tiles, uniform;
   long long first;
+  bool bad;
 };
 __device__ __forceinline__ TileSeq tile_seq_of(const PParams& p, int s) {
   const Seq q = seq_of(p, s);
@@ -52,6 +53,7 @@ __device__ __forceinline__ TileSeq tile_seq_of(const PParams& p, int s) {
   w.t0 = q.t0;
   w.n = q.n;
   w.keys = q.keys;
+  w.bad = q.bad;
   w.first = q.len - q.n;
   w.tiles = (q.n + p.unit_tokens - 1) / p.unit_tokens;
   w.uniform = !p.causal || w.first < 0 || q.len > q.keys;        // every unit goes over all keys (for the odd lengths, masked)
@@ -201,9 +203,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
     for (int s = threadIdx.x * seg; s < (threadIdx.x + 1) * seg && s < p.S; ++s) {
       const TileSeq q = tile_seq_of(p, s);
       if (q.n > 0) c += tile_chunks_before<G>(p, q, q.tiles) * p.Hkv;
-      bad |= q.n > 0 && q.first + q.n > q.keys;
+      bad |= q.bad;
     }
-    if (p.cu && threadIdx.x == 0) bad |= p.cu[p.S] > p.T;
     if (bad && p.status && blockIdx.x == 0) atomicCAS(p.status, 0, kStatusBadIndex);
     pre[threadIdx.x + 1] = c;
     if (threadIdx.x == 0) pre[0] = 0;
@@ -336,7 +337,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
       }
     } else if (warp == 0) {
       // ------------------------------------------------------------------ TMA
-      uint32_t kit = 0, uit = 0;                               // chunks, units so far
+      uint32_t kit = 0, vit = 0, uit = 0;                      // chunks of K, of V, units so far
       uint32_t qit1 = 0;                                       // units with a second tile
       const int box_rows = 1 << p.box_log, boxes = G >> p.box_log;
       const uint32_t sQ = smem_u32(smem + C::OFF_Q), sK = smem_u32(smem + C::OFF_K), sV8 = smem_u32(smem + C::OFF_V8);
@@ -355,16 +356,16 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
               tma_load_4d(sQ + i * C::Q_BYTES + pn * (kTileRows * C::PANEL), &tmQ, BAR(B_QF + i), pn * C::PANEL, u.head * p.ratio, u.t0 + i * p.tile_tokens, 0);
           }
           __syncwarp();
+          if (ok && i == 0) ++uit;
+          if (ok && i == 1) ++qit1;
         }
-        ++uit;
-        qit1 += two;
         // lane j: the page of box j of the next chunk
         auto look_up = [&](int c) {
           const int key = c * G + lane * box_rows;
           return lane < boxes && c < u.c1 && key < u.keys ? table[key >> p.page_log] : 0;
         };
         int next = look_up(u.c0);
-        for (int c = u.c0; c < u.c1 && ok; ++c, ++kit) {
+        for (int c = u.c0; c < u.c1 && ok; ++c) {
           int page = next;
           next = look_up(c + 1);
           if (bad_page(page)) {
@@ -374,7 +375,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
           const int key0 = c * G, full = max(0, min(boxes, (u.keys - key0 + box_rows - 1) >> p.box_log));
           const int slot = (key0 + lane * box_rows) & page_mask;
           const uint32_t bytes = (uint32_t)full * box_rows * D;
-          const uint32_t k = kit % C::NK, v = kit % C::NV8;
+          const uint32_t k = kit % C::NK, v = vit % C::NV8;
           ok = wait(B_KE + k, ((kit / C::NK) & 1u) ^ 1u, TW_KE);
           if (!ok) break;
           if (lane == 0) mbar_expect_tx(BAR(B_KF + k), bytes);
@@ -383,7 +384,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
             for (int pn = 0; pn < C::PANELS; ++pn)
               tma_load_4d(sK + k * C::K_BYTES + (pn * G + lane * box_rows) * C::PANEL, &tmK, BAR(B_KF + k), pn * C::PANEL, slot, u.head, page);
           __syncwarp();
-          ok = wait(B_V8E + v, ((kit / C::NV8) & 1u) ^ 1u, TW_V8E);
+          ++kit;
+          ok = wait(B_V8E + v, ((vit / C::NV8) & 1u) ^ 1u, TW_V8E);
           if (!ok) break;
           if (lane == 0) mbar_expect_tx(BAR(B_V8F + v), bytes);
           __syncwarp();
@@ -391,7 +393,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
             for (int pn = 0; pn < C::PANELS; ++pn)
               tma_load_4d(sV8 + v * C::K_BYTES + (pn * G + lane * box_rows) * C::PANEL, &tmV, BAR(B_V8F + v), pn * C::PANEL, slot, u.head, page);
           __syncwarp();
+          ++vit;
         }
+      }
+      if (*abort_flag) {                                       // a wait ran out: what was asked for comes before the CTA goes, or not at all
+        for (uint32_t i = kit > C::NK ? kit - C::NK : 0; i < kit; ++i) mbar_drain(BAR(B_KF + i % C::NK), (i / C::NK) & 1u);
+        for (uint32_t i = vit > C::NV8 ? vit - C::NV8 : 0; i < vit; ++i) mbar_drain(BAR(B_V8F + i % C::NV8), (i / C::NV8) & 1u);
+        if (uit > 0) mbar_drain(BAR(B_QF), (uit - 1) & 1u);
+        if (qit1 > 0) mbar_drain(BAR(B_QF + 1), (qit1 - 1) & 1u);
       }
     } else if (warp == 1) {
       // ------------------------------------------------------------------ MMA
@@ -526,7 +535,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
             sc[G + i * 32 + lane] = l;
             sc[2 * G + i * 32 + lane] = 1.0f / b[i];
             if (c * G + i * 32 + lane < u.keys) {
-              const bool odd = !(fabsf(l) < INFINITY);         // zero, infinite, NaN: the general way
+              const bool odd = !(fabsf(l) < 120.f);            // zero, infinite, NaN, next to them (1/b is not normal): the general way
               lo = fminf(lo, odd ? -INFINITY : l);
               hi = fmaxf(hi, odd ? INFINITY : l);
             }

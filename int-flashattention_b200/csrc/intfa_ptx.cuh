@@ -92,6 +92,14 @@ __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, vo
   return true;
 }
 
+// until a phase is complete, or 2^20 cycles: what was asked for ahead of a wait that ran out
+__device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
+  const uint32_t t0 = (uint32_t)clock();
+#pragma unroll 1
+  while (!mbar_try_wait(bar, parity) && (uint32_t)clock() - t0 < 1u << 20) {
+  }
+}
+
 // N instructions (16 bytes each) that do nothing: filler to move the code behind it in the instruction cache.
 // Placed on a path that is never taken.
 template <int N>

@@ -627,9 +627,11 @@ int dtype_of(const at::Tensor& t, const char* what, bool fp32) {
 // rows that 16-byte loads can take
 at::Tensor rows_ready(const at::Tensor& t) {
   bool ok = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
-  for (int64_t i = 0; ok && i + 1 < t.dim(); ++i) ok = t.stride(i) >= 0 && t.stride(i) * t.element_size() % 16 == 0;
-  return ok ? t : t.is_contiguous() ? t.clone() : t.contiguous();
+  for (int64_t i = 0; ok && i + 1 < t.dim(); ++i) ok = t.size(i) == 1 || (t.stride(i) >= 0 && t.stride(i) * t.element_size() % 16 == 0);
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
+// ... of dimension i, whatever a dimension of one says
+int64_t step(const at::Tensor& t, int64_t i) { return t.size(i) == 1 ? t.size(-1) : t.stride(i); }
 at::Tensor rotary_table(const at::Tensor& t, int64_t D) {
   if (!is(t, at::kFloat)) raise(PyExc_TypeError, "table must be float32");
   if (t.dim() != 3 || t.size(2) != 2 || t.size(0) < 1) bad_shape("table", "[n, rot_dim/2, 2] with n > 0", t);
@@ -676,9 +678,9 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
       if (none) raise(PyExc_ValueError, "q has no rows, k has some");
       const at::Tensor q = rows_ready(q0), k = no_k ? at::Tensor() : rows_ready(k0), table = aligned16(t0), pos = p0.contiguous();
       auto strides = [&](int64_t (&d)[3], const at::Tensor& t) {
-        d[0] = packed ? 0 : t.stride(0);
-        d[1] = t.stride(1);
-        d[2] = packed ? t.stride(0) : t.stride(2);
+        d[0] = packed ? 0 : step(t, 0);
+        d[1] = step(t, 1);
+        d[2] = packed ? step(t, 0) : step(t, 2);
       };
       P.q = q.data_ptr();
       P.q_out = qo.data_ptr();
@@ -758,7 +760,7 @@ CacheArgs cache_in(IntfaPagedCache& C, const at::Tensor& k, const at::Tensor& v,
   }
   for (const at::Tensor* c : {&k, &v}) {
     bool ok = c->stride(3) == 1 && reinterpret_cast<uintptr_t>(c->data_ptr()) % 16 == 0;
-    for (int i = 0; i < 3; ++i) ok = ok && (c->stride(i) > 0 || c->size(i) == 1) && c->stride(i) % 16 == 0;
+    for (int i = 0; i < 3; ++i) ok = ok && (c->size(i) == 1 || (c->stride(i) > 0 && c->stride(i) % 16 == 0));
     if (!ok) raise(PyExc_ValueError, "k_cache and v_cache must have a contiguous last dim and lie, with every stride, on 16-byte boundaries");
   }
   x.k = k;
@@ -773,8 +775,8 @@ CacheArgs cache_in(IntfaPagedCache& C, const at::Tensor& k, const at::Tensor& v,
   C.k_scale = ks.data_ptr<float>();
   C.v_scale = vs.data_ptr<float>();
   for (int i = 0; i < 3; ++i) {
-    C.k_stride[i] = k.size(i) == 1 && k.stride(i) <= 0 ? D : k.stride(i);
-    C.v_stride[i] = v.size(i) == 1 && v.stride(i) <= 0 ? D : v.stride(i);
+    C.k_stride[i] = step(k, i);
+    C.v_stride[i] = step(v, i);
     C.ks_stride[i] = ks.stride(i);
     C.vs_stride[i] = vs.stride(i);
   }
@@ -828,13 +830,13 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
       P.k = k.data_ptr();
       P.v = v.data_ptr();
       for (int i = 0; i < 2; ++i) {
-        P.k_stride[i] = k.stride(i);
-        P.v_stride[i] = v.stride(i);
+        P.k_stride[i] = step(k, i);
+        P.v_stride[i] = step(v, i);
       }
       if (q.defined()) {
         P.q = q.data_ptr();
-        P.q_stride[0] = q.stride(0);
-        P.q_stride[1] = q.stride(1);
+        P.q_stride[0] = step(q, 0);
+        P.q_stride[1] = step(q, 1);
         P.q8 = q8.data_ptr();
         P.q_scale = qs.data_ptr<float>();
         P.H = q.size(1);
@@ -896,7 +898,7 @@ PyObject* paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
     c10::cuda::CUDAGuard guard(dev);
     if (out.defined()) {
       bool ok = out.stride(2) == 1 && reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0;
-      for (int i = 0; i < 2; ++i) ok = ok && (out.stride(i) > 0 || out.size(i) <= 1) && out.stride(i) % 8 == 0;
+      for (int i = 0; i < 2; ++i) ok = ok && (out.size(i) <= 1 || (out.stride(i) > 0 && out.stride(i) % 8 == 0));
       if (!ok) raise(PyExc_ValueError, "out must have a contiguous last dim and lie, with every stride, on 16-byte boundaries");
     } else {
       out = empty({T, H, D}, o.out, dev);
@@ -907,16 +909,16 @@ PyObject* paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (T > 0) {
       if (P.cache.table_width < 1) raise(PyExc_ValueError, "block_table has no columns");
       at::Tensor q = rows_ready(q0);
-      if (q.stride(0) <= 0 || q.stride(1) <= 0) q = q.contiguous();
+      if (step(q, 0) <= 0 || step(q, 1) <= 0) q = q.clone(at::MemoryFormat::Contiguous);
       const at::Tensor s = qs.stride(0) >= 0 && qs.stride(1) >= 0 ? qs : qs.contiguous();
       P.q = q.data_ptr();
       P.q_scale = s.data_ptr<float>();
       P.o = out.data_ptr();
       P.lse_out = want_lse ? lse.data_ptr<float>() : nullptr;
       for (int i = 0; i < 2; ++i) {
-        P.q_stride[i] = q.size(i) == 1 && q.stride(i) <= 0 ? H * D : q.stride(i);
+        P.q_stride[i] = step(q, i);
         P.qs_stride[i] = s.stride(i);
-        P.o_stride[i] = out.size(i) <= 1 ? H * D : out.stride(i);
+        P.o_stride[i] = step(out, i);
       }
       P.tokens = T;
       P.H = H;

@@ -197,6 +197,15 @@ def test_bad_indices_write_nothing(what, block, pkg):
         assert not torch.equal(s.kc, before[0])            # the second sequence was appended
 
 
+def test_ends_that_run_backwards(pkg):
+    s = Setup([3, 2], [3, 18], 2, 2, 64, 16, 8)
+    for cu in ([0, 3, 1], [-2, 3, 5]):
+        s.cu.copy_(torch.tensor(cu))
+        s.run(pkg, None)
+        with pytest.raises(pkg.IntfaError, match="outside its table"):
+            pkg.check_status()
+
+
 def test_a_replayed_graph_appends_the_next_tokens(pkg):
     s = Setup([1, 1, 1], [40, 9, 64], 4, 2, 64, 16, 1, extra=9)
     cs = pkg.rotary_table(128, 64, device="cuda")

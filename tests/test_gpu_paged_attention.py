@@ -59,9 +59,9 @@ class Setup:
     def args(self, causal=True):
         return (self.q8, self.kc, self.vc, self.qs, self.ks, self.vs, self.table, self.lens, self.cu, causal, self.scale)
 
-    def tolerance(self, want, A, B, out_dtype=torch.float16, more=0.0):
+    def tolerance(self, want, A, B, out_dtype=torch.float16, more=0.0, least=2.0 ** -25):
         n = int(self.lens.max())
-        return (2.0 ** -11 + 2.0 ** -16 + more + (n / 8 + 64) * 2.0 ** -24) * A + n * 2.0 ** -25 * 2 * B[..., None] + EPS[out_dtype] * want.abs() + 2.0 ** -25
+        return (2.0 ** -11 + 2.0 ** -16 + more + (n / 8 + 64) * 2.0 ** -24) * A + n * 2.0 ** -25 * 2 * B[..., None] + EPS[out_dtype] * want.abs() + least
 
     def check(self, pkg, causal=True, out_dtype=torch.float16, got=None, more=0.0):
         o, lse = self.call(pkg, causal, out_dtype=out_dtype, return_lse=True) if got is None else got
@@ -147,6 +147,70 @@ def test_small_values(pkg):
     s.check(pkg)
 
 
+@pytest.mark.parametrize("path", [1, 2])
+def test_value_scales_below_the_normal_numbers(path, pkg):
+    """2^-146 .. 2^-122, as single ones and next to larger ones: the outputs are bf16 numbers.  No absolute term but half a step of its smallest."""
+    s = Setup([3, 70], [200, 90], 4, 2, 128, 16, 1, garbage=False)
+    s.path = path
+    g = torch.Generator(device="cuda").manual_seed(3)
+    exponents = torch.rand(s.vs.shape, device="cuda", generator=g).double() * 24 - 146
+    small = torch.exp2(exponents).float()
+    for vs in (small, torch.full_like(small, 2.0 ** -130), torch.where(torch.rand(s.vs.shape, device="cuda", generator=g) < 0.5, small, s.vs)):
+        s.vs = vs
+        o = s.call(pkg, out_dtype=torch.bfloat16)
+        want, _, A, B = O.attention(*s.args()[:1], s.qs, s.kc, s.vc, s.ks, s.vs, s.table, s.lens, s.cu, True, s.scale)
+        tol = s.tolerance(want, A, B, torch.bfloat16, least=2.0 ** -134)
+        assert ((o.double() - want).abs() <= tol).all()
+    pkg.check_status()
+
+
+@pytest.mark.parametrize("path", [1, 2])
+def test_sequences_that_share_pages(path, pkg):
+    """A common prefix: the pages of one sequence in the tables of others."""
+    s = Setup([4, 40, 1], [200, 200, 70], 8, 2, 128, 16, 4, garbage=False)
+    s.path = path
+    s.table[1, :9] = s.table[0, :9]
+    s.table[2, :4] = s.table[0, :4]
+    s.check(pkg)
+
+
+@pytest.mark.parametrize("path", [1, 2])
+def test_padding(path, pkg):
+    """Rows of sequences without tokens may hold anything."""
+    s = Setup([1, 1, 1, 1], [40, 0, 0, 7], 4, 2, 64, 16, 1, one=True)
+    s.path = path
+    s.table[1:3] = -1
+    want = s.call(pkg)
+    s.qs[1], s.qs[2] = float("nan"), float("inf")
+    o, lse = s.call(pkg, return_lse=True)
+    assert torch.equal(o, want) and (o[1:3] == 0).all() and (lse[1:3] == -float("inf")).all()
+    assert pkg.check_status() == 0
+
+
+def test_strides_of_dimensions_of_one(pkg):
+    """What a dimension of size one gives as its stride has no meaning."""
+    odd = lambda x, i: x.as_strided(x.shape, [7 if j == i else st for j, st in enumerate(x.stride())], x.storage_offset())
+    s = Setup([1], [20], 1, 1, 64, 32, 1, one=True, garbage=False)
+    want = s.call(pkg)
+    page = int(s.table[0, 0])
+    s.kc, s.vc, s.ks, s.vs = (odd(x[page:page + 1].contiguous(), 0) for x in (s.kc, s.vc, s.ks, s.vs))
+    s.table[0, 0] = 0
+    out = odd(odd(torch.empty_like(want), 0), 1)
+    s.q8, s.qs = odd(odd(s.q8, 0), 1), odd(odd(s.qs, 0), 1)
+    for path in (1, 2):
+        s.path = path
+        s.call(pkg, out=out)
+        assert (out.float() - want.float()).abs().max() < 2e-3 * want.float().abs().max()
+    k = torch.randn(1, 1, 64, device="cuda").half()
+    ready, torn = [x.clone() for x in (s.kc, s.vc, s.ks, s.vs)], [s.kc, s.vc, s.ks, s.vs]
+    a = pkg.append_int8_paged(k, k, *ready, s.table, s.lens, q=k)
+    b = pkg.append_int8_paged(odd(odd(k, 0), 1), odd(k, 1), *torn, s.table, s.lens, q=odd(k, 0))
+    assert all(torch.equal(x, y) for x, y in zip([*ready, *a], [*torn, *b]))
+    cs = pkg.rotary_table(30, 64, device="cuda")
+    assert torch.equal(pkg.rotary(odd(odd(k, 0), 1), odd(k, 1), cs, s.lens)[0], pkg.rotary(k, None, cs, s.lens))
+    pkg.check_status()
+
+
 def test_sharp_and_negative_scores(pkg):
     s = Setup([1, 2], [700, 90], 4, 2, 128, 16, 1)
     for scale in (-0.03, 0.0):
@@ -217,15 +281,20 @@ def test_bad_indices(pkg):
     assert torch.equal(o[1], good[1])
     s.lens[0] = -3                        # no tokens
     assert (s.call(pkg)[0] == 0).all()
+    with pytest.raises(pkg.IntfaError, match="outside its table"):
+        pkg.check_status()
     # ends that run backwards or past the rows: nothing is read or written outside
-    for cu in ([0, 2, 1], [0, 1, 9], [-4, 1, 2], [1, 0, 2], [2, 2, 2]):
-        s.cu = torch.tensor(cu, dtype=torch.int32, device="cuda")
-        s.lens[:] = 20
+    s.lens[:] = 20
+    for path in (1, 2):
+        s.path = path
+        for cu in ([0, 2, 1], [0, 1, 9], [-4, 1, 2], [1, 0, 2]):
+            s.cu = torch.tensor(cu, dtype=torch.int32, device="cuda")
+            s.call(pkg)
+            with pytest.raises(pkg.IntfaError, match="outside its table"):
+                pkg.check_status()
+        s.cu = torch.tensor([2, 2, 2], dtype=torch.int32, device="cuda")
         s.call(pkg)
-        try:
-            pkg.check_status()
-        except pkg.IntfaError:
-            pass
+        assert pkg.check_status() == 0
 
 
 def test_no_rows(pkg):

@@ -63,6 +63,18 @@ def test_c_abi_refuses_bad_caches(lib, change, word):
     assert h.intfa_paged_workspace_bytes(ctypes.byref(P)) == 0
 
 
+def test_c_abi_refuses_sizes_past_its_counters(lib):
+    h = lib.load()
+    A, P = lib.IntfaAppendParams(), lib.IntfaPagedParams()
+    for X, f in ((A, h.intfa_paged_append), (P, h.intfa_paged_attention)):
+        X.cache, X.tokens, X.H = cache(lib, table_width=(1 << 26) + 1), 3, 4
+        assert f(ctypes.byref(X), None) == lib.ERR_TOO_LARGE and "block_table" in lib.last_error()
+        X.cache, X.cu_seqlens, X.tokens = cache(lib), 1 << 20, (1 << 30) + 1
+        assert f(ctypes.byref(X), None) == lib.ERR_TOO_LARGE and "too many" in lib.last_error()
+    P.tokens = (1 << 28) + 1                          # (4 heads of them)
+    assert h.intfa_paged_attention(ctypes.byref(P), None) == lib.ERR_TOO_LARGE and "too many" in lib.last_error()
+
+
 def test_c_abi_refuses_bad_arguments(lib):
     h = lib.load()
     for f in (h.intfa_rotary, h.intfa_paged_append, h.intfa_paged_attention):
