@@ -82,9 +82,10 @@ struct PParams {
   int* status;
 };
 
-__device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, const int (&c)[4]) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+               : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
 }
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -100,9 +101,9 @@ __device__ __forceinline__ uint2 lds8(uint32_t a) {
   asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
   return v;
 }
-__device__ __forceinline__ float2 lds_f2(uint32_t a) {
-  float2 v;
-  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+__device__ __forceinline__ uint64_t lds_u64(uint32_t a) {
+  uint64_t v;
+  asm volatile("ld.shared.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
   return v;
 }
 __device__ __forceinline__ float lds_f(uint32_t a) {
@@ -150,12 +151,14 @@ __device__ __forceinline__ Seq seq_of(const PParams& p, int s) {
 // a place in the row of all chunks
 struct Cursor {
   Seq q;
-  int s, unit, chunk;        // sequence; unit in it (K/V head * tiles + tile); chunk in that
+  int s, head, tile, chunk;  // sequence; unit in it: K/V head and tile; chunk in that
   __device__ __forceinline__ void next(const PParams& p) {
     if (++chunk < q.chunks) return;
     chunk = 0;
-    if (++unit < q.tiles * p.Hkv) return;
-    unit = 0;
+    if (++tile < q.tiles) return;
+    tile = 0;
+    if (++head < p.Hkv) return;
+    head = 0;
     next_seq(p);
   }
   // to the next sequence with query rows, if there is one
@@ -314,18 +317,18 @@ __device__ __forceinline__ void write_part(float* part, float* ml, int stride, c
   }
 }
 
-// One chunk.  sK, sV: its rows in shared memory; sS: its K scales, then its V scales; last[n]: the last key of the chunk that row n*8 + g sees.
+// One chunk.  sK, sV: its rows in shared memory; sS: its K scales, then the logarithms of its V scales; last[n]: the last key of the chunk that row n*8 + g sees.
 template <int D, int NT, bool MASKED>
 __device__ __forceinline__ void chunk_step(RowState<D, NT>& st, const uint32_t (&q)[D / 64][NT][4], const float (&qs)[NT], const int (&last)[NT],
                                            uint32_t sK, uint32_t sV, uint32_t sS) {
+  const int magic[4] = {kMagicI, kMagicI, kMagicI, kMagicI};
+  const uint64_t less = f2_pack(-kMagicF, -kMagicF);
   constexpr int CH = D / 64, AT = (NT + 1) / 2, W = RowState<D, NT>::W, PANELS = RowState<D, NT>::PANELS, PANEL = D < 128 ? D : 128;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  float x[NT][4][2], lv[4][2];
+  uint64_t x[NT][4], lv[4];                       // keys 2t, 2t + 1 of each tile of 8
 #pragma unroll
   for (int kt = 0; kt < 4; ++kt) {
     int d[AT][4];
-#pragma unroll
-    for (int a = 0; a < AT; ++a) d[a][0] = d[a][1] = d[a][2] = d[a][3] = kMagicI;
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch) {
       // row kt*8 + g; piece 2t + (ch & 1) of a 128-byte panel, or t of a 64-byte one
@@ -339,33 +342,38 @@ __device__ __forceinline__ void chunk_step(RowState<D, NT>& st, const uint32_t (
         const bool two = 2 * i + 1 < NT;
         const uint32_t(&lo)[4] = q[ch][2 * i];
         const uint32_t(&hi)[4] = q[ch][two ? 2 * i + 1 : 2 * i];
-        mma_s8(d[i], lo[0], two ? hi[0] : 0u, lo[1], two ? hi[1] : 0u, kw.x, kw.y);
-        mma_s8(d[i], lo[2], two ? hi[2] : 0u, lo[3], two ? hi[3] : 0u, kw.z, kw.w);
+        if (ch == 0) mma_s8(d[i], lo[0], two ? hi[0] : 0u, lo[1], two ? hi[1] : 0u, kw.x, kw.y, magic);
+        else mma_s8(d[i], lo[0], two ? hi[0] : 0u, lo[1], two ? hi[1] : 0u, kw.x, kw.y, d[i]);
+        mma_s8(d[i], lo[2], two ? hi[2] : 0u, lo[3], two ? hi[3] : 0u, kw.z, kw.w, d[i]);
       }
     }
-    const float2 ks = lds_f2(sS + (kt * 8 + 2 * t) * 4), vs = lds_f2(sS + (kChunk + kt * 8 + 2 * t) * 4);
-    lv[kt][0] = log2_approx(vs.x);
-    lv[kt][1] = log2_approx(vs.y);
+    const uint64_t ks = lds_u64(sS + (kt * 8 + 2 * t) * 4);
+    lv[kt] = lds_u64(sS + (kChunk + kt * 8 + 2 * t) * 4);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      x[n][kt][0] = (__int_as_float(d[n / 2][(n & 1) * 2]) - kMagicF) * qs[n] * ks.x;
-      x[n][kt][1] = (__int_as_float(d[n / 2][(n & 1) * 2 + 1]) - kMagicF) * qs[n] * ks.y;
-    }
+    for (int n = 0; n < NT; ++n)
+      x[n][kt] = f2_mul(f2_add(f2_packu(d[n / 2][(n & 1) * 2], d[n / 2][(n & 1) * 2 + 1]), less), f2_mul(ks, f2_pack(qs[n], qs[n])));
   }
   uint32_t b[NT][4];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    float w[4][2], mx = -INFINITY, mw = -INFINITY;
+    uint64_t w[4];
+    float mx = -INFINITY, mw = -INFINITY;
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        w[kt][e] = x[n][kt][e] + lv[kt][e];
-        // (chosen, not added: what lies in a place that is not looked at may be anything)
-        if (MASKED && kt * 8 + 2 * t + e > last[n]) x[n][kt][e] = w[kt][e] = -INFINITY;
-        mx = fmaxf(mx, x[n][kt][e]);
-        mw = fmaxf(mw, w[kt][e]);
+    for (int kt = 0; kt < 4; ++kt) {
+      w[kt] = f2_add(x[n][kt], lv[kt]);
+      float x0, x1, w0, w1;
+      f2_unpack(x[n][kt], x0, x1);
+      f2_unpack(w[kt], w0, w1);
+      // (chosen, not added: what lies in a place that is not looked at may be anything)
+      if (MASKED) {
+        if (kt * 8 + 2 * t > last[n]) x0 = w0 = -INFINITY;
+        if (kt * 8 + 2 * t + 1 > last[n]) x1 = w1 = -INFINITY;
+        x[n][kt] = f2_pack(x0, x1);
+        w[kt] = f2_pack(w0, w1);
       }
+      mx = max3(mx, x0, x1);
+      mw = max3(mw, w0, w1);
+    }
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
@@ -379,14 +387,19 @@ __device__ __forceinline__ void chunk_step(RowState<D, NT>& st, const uint32_t (
     const float f = ex2_approx(st.mw[n] - mws);
     st.m[n] = mx;
     st.mw[n] = mw;
-    float sum = 0.f;
+    uint64_t sum = 0;
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt) {
-      sum += ex2_approx(x[n][kt][0] - ms) + ex2_approx(x[n][kt][1] - ms);
-      const __half2 h = __floats2half2_rn(ex2_approx(w[kt][0] - mws), ex2_approx(w[kt][1] - mws));
+      float x0, x1, w0, w1;
+      f2_unpack(f2_add(x[n][kt], f2_pack(-ms, -ms)), x0, x1);
+      f2_unpack(f2_add(w[kt], f2_pack(-mws, -mws)), w0, w1);
+      sum = f2_add(sum, f2_pack(ex2_approx(x0), ex2_approx(x1)));
+      const __half2 h = __floats2half2_rn(ex2_approx(w0), ex2_approx(w1));
       b[n][kt] = *reinterpret_cast<const uint32_t*>(&h);
     }
-    st.l[n] += sum;
+    float s0, s1;
+    f2_unpack(sum, s0, s1);
+    st.l[n] += s0 + s1;
     if (__any_sync(0xffffffffu, moved)) {
       const float f0 = __shfl_sync(0xffffffffu, f, 8 * t), f1 = __shfl_sync(0xffffffffu, f, 8 * t + 4);
 #pragma unroll
@@ -530,9 +543,11 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_const
       off -= c;
       unit_id += units;
     } while (at.s < p.S);
-    at.unit = (int)(off / at.q.chunks);
-    at.chunk = (int)(off - (long long)at.unit * at.q.chunks);
-    unit_id += at.unit;
+    const int unit = (int)(off / at.q.chunks);
+    at.chunk = (int)(off - (long long)unit * at.q.chunks);
+    at.head = unit / at.q.tiles;
+    at.tile = unit - at.head * at.q.tiles;
+    unit_id += unit;
   }
   // ---- loads
   const uint32_t sKV = smem_u32(smem) + warp * NS * 2 * C::KV;
@@ -549,7 +564,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_const
   const int rows_box = 1 << p.box_log, boxes = kChunk >> p.box_log;
   auto load = [&](int stage) {
     if (to_load > 0) {
-      const int key0 = ahead.chunk * kChunk, key = key0 + lane, head = ahead.unit / ahead.q.tiles, tile = ahead.unit - head * ahead.q.tiles;
+      const int key0 = ahead.chunk * kChunk, key = key0 + lane, head = ahead.head, tile = ahead.tile;
       const bool in = key < ahead.q.keys;
       if (page < 0 || page >= p.pages) {
         if (p.status) atomicCAS(p.status, 0, kStatusBadIndex);
@@ -591,9 +606,8 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_const
         }
       }
       --to_load;
-      const int unit = ahead.unit, s = ahead.s;
       ahead.next(p);
-      fresh = ahead.unit != unit || ahead.s != s;
+      fresh = ahead.chunk == 0;
       look_up();
     }
     cp_async_commit();
@@ -621,12 +635,15 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_const
     ok = mbar_wait_warp(bar0 + 8 * stage, parity, abort_flag, p.status, (int)(blockIdx.x << 8) | kWaitChunk);
     if (!ok) break;
     const uint32_t kv = sKV + stage * 2 * C::KV, x = sX + stage * C::EXTRA;
+    // the logarithms of the V scales, once for all rows
+    asm volatile("st.shared.f32 [%0], %1;" ::"r"(x + (kChunk + lane) * 4), "f"(log2_approx(lds_f(x + (kChunk + lane) * 4))) : "memory");
+    __syncwarp();
     if (!open) {
       open = true;
       unit0 = pos - at.chunk;
       unit1 = unit0 + at.q.chunks;
       st.clear();
-      const int tile = at.unit % at.q.tiles, R = at.q.n * p.ratio;
+      const int tile = at.tile, R = at.q.n * p.ratio;
       const uint32_t xq = x + 2 * kChunk * 4;
       full_keys = at.q.keys;
 #pragma unroll
@@ -669,7 +686,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_const
     ++pos;
     if (at.chunk + 1 == at.q.chunks || left == 0) {
       st.reduce_l();
-      const int head = at.unit / at.q.tiles, tile = at.unit - head * at.q.tiles;
+      const int head = at.head, tile = at.tile;
       const bool starts = unit0 >= begin, ends = unit1 <= pos;
       if (unit_id >= p.max_units) {
         if (p.status && lane == 0) atomicCAS(p.status, 0, kStatusBadIndex);            // (cu_seqlens that overlap)
