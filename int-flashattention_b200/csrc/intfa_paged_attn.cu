@@ -36,7 +36,6 @@
 namespace intfa {
 namespace {
 
-constexpr int kChunk = 32;                        // keys
 constexpr float kMagicF = 12582912.0f;            // 1.5*2^23: added to an int32 below 2^22 as a bit pattern, it reads as fp32 1.5*2^23 + value
 constexpr int kMagicI = 0x4B400000;
 
@@ -69,7 +68,7 @@ struct PParams {
   long long ksP, ksH, ksB, vsP, vsH, vsB;
   const int* table; long long table_stride; int width;
   const int* lens; const int* cu;
-  int S, H, Hkv, ratio, pages, page_log, block_log, box_log;
+  int S, H, Hkv, ratio, pages, page_log, block_log, box_log, chunk_log;
   long long T;
   int causal, o_bf16;
   float c;                                        // sm_scale * log2(e)
@@ -144,7 +143,7 @@ __device__ __forceinline__ Seq seq_of(const PParams& p, int s) {
   q.keys = (int)(q.len < 0 ? 0 : q.len < most ? q.len : most);
   q.bad = t0 < 0 || t1 < t0 || t1 > p.T || (q.n > 0 && q.len != q.keys);
   q.tiles = (int)(((long long)q.n * p.ratio + p.rows_tile - 1) / p.rows_tile);
-  q.chunks = q.keys > kChunk ? (q.keys + kChunk - 1) / kChunk : 1;      // (a row without keys is written, too)
+  q.chunks = q.keys > 0 ? ((q.keys - 1) >> p.chunk_log) + 1 : 1;        // (a row without keys is written, too)
   return q;
 }
 
@@ -171,11 +170,12 @@ struct Cursor {
   }
 };
 
-template <int D, int NT, int WARPS, int NS>
+// G: keys of a chunk
+template <int D, int NT, int WARPS, int NS, int G>
 struct DecodeCfg {
-  static constexpr int RT = 8 * NT, KV = kChunk * D;                    // rows of a tile; bytes of K or V of a chunk
+  static constexpr int RT = 8 * NT, KV = G * D;                         // rows of a tile; bytes of K or V of a chunk
   static constexpr int PANEL = D < 128 ? D : 128, PANELS = D / PANEL;   // a row lies in panels of at most 128 bytes
-  static constexpr int EXTRA = 2 * kChunk * 4 + RT * D + RT * 4;        // scales, query rows and their scales
+  static constexpr int EXTRA = 2 * G * 4 + RT * D + RT * 4;             // scales, query rows and their scales
   static constexpr int OFF_EXTRA = WARPS * NS * 2 * KV;
   static constexpr int OFF_BAR = OFF_EXTRA + WARPS * NS * EXTRA;
   static constexpr int OFF_PRE = OFF_BAR + WARPS * NS * 8;              // [threads + 1] chunks (long long) and units (int) before a thread's sequences
@@ -318,23 +318,24 @@ __device__ __forceinline__ void write_part(float* part, float* ml, int stride, c
 }
 
 // One chunk.  sK, sV: its rows in shared memory; sS: its K scales, then the logarithms of its V scales; last[n]: the last key of the chunk that row n*8 + g sees.
-template <int D, int NT, bool MASKED>
+template <int D, int NT, int G, bool MASKED>
 __device__ __forceinline__ void chunk_step(RowState<D, NT>& st, const uint32_t (&q)[D / 64][NT][4], const float (&qs)[NT], const int (&last)[NT],
                                            uint32_t sK, uint32_t sV, uint32_t sS) {
   const int magic[4] = {kMagicI, kMagicI, kMagicI, kMagicI};
   const uint64_t less = f2_pack(-kMagicF, -kMagicF);
   constexpr int CH = D / 64, AT = (NT + 1) / 2, W = RowState<D, NT>::W, PANELS = RowState<D, NT>::PANELS, PANEL = D < 128 ? D : 128;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  uint64_t x[NT][4], lv[4];                       // keys 2t, 2t + 1 of each tile of 8
+  constexpr int KT = G / 8;
+  uint64_t x[NT][KT], lv[KT];                     // keys 2t, 2t + 1 of each tile of 8
 #pragma unroll
-  for (int kt = 0; kt < 4; ++kt) {
+  for (int kt = 0; kt < KT; ++kt) {
     int d[AT][4];
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch) {
       // row kt*8 + g; piece 2t + (ch & 1) of a 128-byte panel, or t of a 64-byte one
       const int row = kt * 8 + g;
       uint32_t a;
-      if constexpr (PANEL == 128) a = sK + (ch / 2) * (kChunk * 128) + row * 128 + (((2 * t + (ch & 1)) ^ g) << 4);
+      if constexpr (PANEL == 128) a = sK + (ch / 2) * (G * 128) + row * 128 + (((2 * t + (ch & 1)) ^ g) << 4);
       else a = sK + row * 64 + ((t ^ ((g >> 1) & 3)) << 4);
       const uint4 kw = lds16(a);
 #pragma unroll
@@ -348,18 +349,18 @@ __device__ __forceinline__ void chunk_step(RowState<D, NT>& st, const uint32_t (
       }
     }
     const uint64_t ks = lds_u64(sS + (kt * 8 + 2 * t) * 4);
-    lv[kt] = lds_u64(sS + (kChunk + kt * 8 + 2 * t) * 4);
+    lv[kt] = lds_u64(sS + (G + kt * 8 + 2 * t) * 4);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
       x[n][kt] = f2_mul(f2_add(f2_packu(d[n / 2][(n & 1) * 2], d[n / 2][(n & 1) * 2 + 1]), less), f2_mul(ks, f2_pack(qs[n], qs[n])));
   }
-  uint32_t b[NT][4];
+  uint32_t b[NT][KT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    uint64_t w[4];
+    uint64_t w[KT];
     float mx = -INFINITY, mw = -INFINITY;
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
+    for (int kt = 0; kt < KT; ++kt) {
       w[kt] = f2_add(x[n][kt], lv[kt]);
       float x0, x1, w0, w1;
       f2_unpack(x[n][kt], x0, x1);
@@ -389,7 +390,7 @@ __device__ __forceinline__ void chunk_step(RowState<D, NT>& st, const uint32_t (
     st.mw[n] = mw;
     uint64_t sum = 0;
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
+    for (int kt = 0; kt < KT; ++kt) {
       float x0, x1, w0, w1;
       f2_unpack(f2_add(x[n][kt], f2_pack(-ms, -ms)), x0, x1);
       f2_unpack(f2_add(w[kt], f2_pack(-mws, -mws)), w0, w1);
@@ -413,7 +414,7 @@ __device__ __forceinline__ void chunk_step(RowState<D, NT>& st, const uint32_t (
   }
   // O^T (channels x rows) += V^T P^T, 16 keys at a time: two 8-key tiles, of which the lane holds keys 2t and 2t + 1
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < G / 16; ++h) {
 #pragma unroll
     for (int pn = 0; pn < PANELS; ++pn) {
       uint32_t v[4][W];
@@ -421,7 +422,7 @@ __device__ __forceinline__ void chunk_step(RowState<D, NT>& st, const uint32_t (
       for (int i = 0; i < 4; ++i) {
         const int row = h * 16 + (i >> 1) * 8 + 2 * t + (i & 1);
         if constexpr (W == 4) {
-          const uint4 y = lds16(sV + pn * (kChunk * 128) + row * 128 + ((g ^ (row & 7)) << 4));
+          const uint4 y = lds16(sV + pn * (G * 128) + row * 128 + ((g ^ (row & 7)) << 4));
           v[i][0] = y.x; v[i][1] = y.y; v[i][2] = y.z; v[i][3] = y.w;
         } else {
           const uint2 y = lds8(sV + row * 64 + (((g >> 1) ^ ((row >> 1) & 3)) << 4) + (g & 1) * 8);
@@ -455,10 +456,10 @@ __device__ __forceinline__ void chunk_step(RowState<D, NT>& st, const uint32_t (
 
 enum { kWaitChunk = 64 };
 
-template <int D, int NT, int WARPS, int NS>
+template <int D, int NT, int WARPS, int NS, int G>
 __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const PParams p) {
-  using C = DecodeCfg<D, NT, WARPS, NS>;
-  constexpr int RT = C::RT, THREADS = 32 * WARPS;
+  using C = DecodeCfg<D, NT, WARPS, NS, G>;
+  constexpr int RT = C::RT, THREADS = 32 * WARPS, M = G / 32;            // keys a lane
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((0u - smem_u32(smem_raw)) & 1023u);
   const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -555,24 +556,31 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_const
   Cursor ahead = at;
   long long to_load = left;
   bool fresh = true;                                         // the next chunk to load needs its query rows, too
-  int page = 0;                                              // of key `lane` of the next chunk to load
+  int page[M];                                               // of keys `lane`, `lane` + 32 .. of the next chunk to load
   auto look_up = [&]() {
-    const int key = ahead.chunk * kChunk + lane;
-    page = 0;
-    if (to_load > 0 && key < ahead.q.keys) page = p.table[ahead.s * p.table_stride + (key >> p.page_log)];
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      const int key = ahead.chunk * G + i * 32 + lane;
+      page[i] = 0;
+      if (to_load > 0 && key < ahead.q.keys) page[i] = p.table[ahead.s * p.table_stride + (key >> p.page_log)];
+    }
   };
-  const int rows_box = 1 << p.box_log, boxes = kChunk >> p.box_log;
+  const int rows_box = 1 << p.box_log, boxes = G >> p.box_log;
   auto load = [&](int stage) {
     if (to_load > 0) {
-      const int key0 = ahead.chunk * kChunk, key = key0 + lane, head = ahead.head, tile = ahead.tile;
-      const bool in = key < ahead.q.keys;
-      if (page < 0 || page >= p.pages) {
-        if (p.status) atomicCAS(p.status, 0, kStatusBadIndex);
-        page = 0;
+      const int key0 = ahead.chunk * G, head = ahead.head, tile = ahead.tile;
+      // the rows of a copy lie in one page; lane j issues copy j
+      int first_page = 0;
+#pragma unroll
+      for (int i = 0; i < M; ++i) {
+        if (page[i] < 0 || page[i] >= p.pages) {
+          if (p.status) atomicCAS(p.status, 0, kStatusBadIndex);
+          page[i] = 0;
+        }
+        const int pg = __shfl_sync(0xffffffffu, page[i], (lane << p.box_log) & 31);
+        if (M == 1 || (lane << p.box_log) >> 5 == i) first_page = pg;
       }
       const uint32_t bar = bar0 + 8 * stage, dst = sKV + stage * 2 * C::KV, x = sX + stage * C::EXTRA;
-      // the rows of a copy lie in one page; lane j issues copy j
-      const int first_page = __shfl_sync(0xffffffffu, page, (lane << p.box_log) & 31);
       const int full = min(boxes, (ahead.q.keys - key0 + rows_box - 1) >> p.box_log);
       if (lane == 0) mbar_expect_tx(bar, full > 0 ? full * rows_box * 2 * D : 0);
       __syncwarp();
@@ -580,16 +588,21 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_const
         const int slot = (key0 + (lane << p.box_log)) & ((1 << p.page_log) - 1);
 #pragma unroll
         for (int pn = 0; pn < C::PANELS; ++pn) {
-          const uint32_t d = dst + pn * (kChunk * C::PANEL) + (lane << p.box_log) * C::PANEL;
+          const uint32_t d = dst + pn * (G * C::PANEL) + (lane << p.box_log) * C::PANEL;
           tma_load_4d(d, &tmK, bar, pn * C::PANEL, slot, head, first_page);
           tma_load_4d(d + C::KV, &tmV, bar, pn * C::PANEL, slot, head, first_page);
         }
       }
-      const long long blk = (key & ((1 << p.page_log) - 1)) >> p.block_log;
-      cp_async4(x + lane * 4, p.ks + (in ? page * p.ksP + head * p.ksH + blk * p.ksB : 0), in);
-      cp_async4(x + (kChunk + lane) * 4, p.vs + (in ? page * p.vsP + head * p.vsH + blk * p.vsB : 0), in);
+#pragma unroll
+      for (int i = 0; i < M; ++i) {
+        const int key = key0 + i * 32 + lane;
+        const bool in = key < ahead.q.keys;
+        const long long blk = (key & ((1 << p.page_log) - 1)) >> p.block_log;
+        cp_async4(x + (i * 32 + lane) * 4, p.ks + (in ? page[i] * p.ksP + head * p.ksH + blk * p.ksB : 0), in);
+        cp_async4(x + (G + i * 32 + lane) * 4, p.vs + (in ? page[i] * p.vsP + head * p.vsH + blk * p.vsB : 0), in);
+      }
       if (fresh) {
-        const uint32_t xq = x + 2 * kChunk * 4;
+        const uint32_t xq = x + 2 * G * 4;
         const int R = ahead.q.n * p.ratio;
 #pragma unroll
         for (int i = lane; i < RT * (D / 16); i += 32) {
@@ -636,7 +649,11 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_const
     if (!ok) break;
     const uint32_t kv = sKV + stage * 2 * C::KV, x = sX + stage * C::EXTRA;
     // the logarithms of the V scales, once for all rows
-    asm volatile("st.shared.f32 [%0], %1;" ::"r"(x + (kChunk + lane) * 4), "f"(log2_approx(lds_f(x + (kChunk + lane) * 4))) : "memory");
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      const uint32_t at_v = x + (G + i * 32 + lane) * 4;
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(at_v), "f"(log2_approx(lds_f(at_v))) : "memory");
+    }
     __syncwarp();
     if (!open) {
       open = true;
@@ -644,7 +661,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_const
       unit1 = unit0 + at.q.chunks;
       st.clear();
       const int tile = at.tile, R = at.q.n * p.ratio;
-      const uint32_t xq = x + 2 * kChunk * 4;
+      const uint32_t xq = x + 2 * G * 4;
       full_keys = at.q.keys;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -667,14 +684,14 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_const
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) full_keys = min(full_keys, __shfl_xor_sync(0xffffffffu, full_keys, o));
     }
-    const int key0 = at.chunk * kChunk;
-    if (key0 + kChunk <= full_keys) {
-      chunk_step<D, NT, false>(st, q, qs, last, kv, kv + C::KV, x);
+    const int key0 = at.chunk * G;
+    if (key0 + G <= full_keys) {
+      chunk_step<D, NT, G, false>(st, q, qs, last, kv, kv + C::KV, x);
     } else {
       int rel[NT];
 #pragma unroll
       for (int n = 0; n < NT; ++n) rel[n] = last[n] - key0;
-      chunk_step<D, NT, true>(st, q, qs, rel, kv, kv + C::KV, x);
+      chunk_step<D, NT, G, true>(st, q, qs, rel, kv, kv + C::KV, x);
     }
     __syncwarp();
     load(stage);
@@ -916,16 +933,18 @@ Plan make_plan(const IntfaPagedParams* a, int sms) {
   return pl;
 }
 
-template <int D, int NT, int WARPS, int NS>
+template <int D, int NT, int WARPS, int NS, int G = 32>
 int run(const IntfaPagedParams* a, const Plan& pl, PParams p, cudaStream_t stream) {
-  using C = DecodeCfg<D, NT, WARPS, NS>;
+  using C = DecodeCfg<D, NT, WARPS, NS, G>;
   const IntfaPagedCache& c = a->cache;
+  p.chunk_log = G == 64 ? 6 : 5;
+  p.box_log = c.page_size < G ? p.page_log : p.chunk_log;
   CUtensorMap tmK, tmV;
   const CUtensorMapSwizzle swz = C::PANEL == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
   int rc;
   if ((rc = make_tmap(&tmK, c.k, 1, c.k_stride, c.pages, c.H_kv, c.page_size, D, C::PANEL, 1 << p.box_log, swz))) return rc;
   if ((rc = make_tmap(&tmV, c.v, 1, c.v_stride, c.pages, c.H_kv, c.page_size, D, C::PANEL, 1 << p.box_log, swz))) return rc;
-  auto kern = paged_kernel<D, NT, WARPS, NS>;
+  auto kern = paged_kernel<D, NT, WARPS, NS, G>;
   static std::atomic<bool> attr_done[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return set_error(INTFA_ERR_CUDA, "cannot query the current device");
@@ -1005,7 +1024,6 @@ int paged_attention(const IntfaPagedParams* a, cudaStream_t stream) {
   p.S = c.S; p.H = a->H; p.Hkv = c.H_kv; p.ratio = a->H / c.H_kv; p.pages = c.pages;
   p.page_log = log2_of(c.page_size);
   p.block_log = log2_of(c.block);
-  p.box_log = c.page_size < kChunk ? p.page_log : log2_of(kChunk);
   p.T = a->tokens;
   p.causal = a->causal ? 1 : 0;
   p.o_bf16 = a->o_dtype == INTFA_OUT_BF16;
@@ -1021,6 +1039,7 @@ int paged_attention(const IntfaPagedParams* a, cudaStream_t stream) {
   p.head = reinterpret_cast<int*>(ws + pl.off_head);
   p.status = a->status;
   p.tile_tokens = 0;
+  p.chunk_log = p.box_log = 5;
   if (pl.tiles) {
     p.rows_tile = c.D == 256 ? kTileRows : 2 * kTileRows;
     p.tile_tokens = kTileRows / p.ratio;
@@ -1030,7 +1049,7 @@ int paged_attention(const IntfaPagedParams* a, cudaStream_t stream) {
     return c.D == 64 ? run_tiles<64>(a, pl, p, stream) : c.D == 128 ? run_tiles<128>(a, pl, p, stream) : run_tiles<256>(a, pl, p, stream);
   }
   switch (c.D) {
-    case 64: return pl.NT == 2 ? run<64, 2, 8, 4>(a, pl, p, stream) : run<64, 1, 8, 5>(a, pl, p, stream);
+    case 64: return pl.NT == 2 ? run<64, 2, 8, 2, 64>(a, pl, p, stream) : run<64, 1, 8, 3, 64>(a, pl, p, stream);
     case 128: return pl.NT == 2 ? run<128, 2, 6, 3>(a, pl, p, stream) : run<128, 1, 8, 3>(a, pl, p, stream);
     default: return pl.NT == 2 ? run<256, 2, 4, 2>(a, pl, p, stream) : run<256, 1, 4, 3>(a, pl, p, stream);
   }
