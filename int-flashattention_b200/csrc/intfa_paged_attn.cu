@@ -921,7 +921,7 @@ Plan make_plan(const IntfaPagedParams* a, int sms) {
   }
   // Rows a tile: 16 where an average sequence has more than 8 rows a K/V head
   pl.NT = (double)a->tokens * ratio > 8.0 * c.S ? 2 : 1;
-  pl.warps = c.D == 256 ? 4 : c.D == 128 && pl.NT == 2 ? 6 : 8;
+  pl.warps = c.D == 256 ? 4 : 8;
   pl.max_units = (a->tokens * ratio / (8 * pl.NT) + c.S) * c.H_kv;
   if (pl.max_units > 0x7fffffffLL) return Plan();
   const int RT = 8 * pl.NT;
@@ -1050,7 +1050,7 @@ int paged_attention(const IntfaPagedParams* a, cudaStream_t stream) {
   }
   switch (c.D) {
     case 64: return pl.NT == 2 ? run<64, 2, 8, 2, 64>(a, pl, p, stream) : run<64, 1, 8, 3, 64>(a, pl, p, stream);
-    case 128: return pl.NT == 2 ? run<128, 2, 6, 3>(a, pl, p, stream) : run<128, 1, 8, 3>(a, pl, p, stream);
+    case 128: return pl.NT == 2 ? run<128, 2, 8, 2>(a, pl, p, stream) : run<128, 1, 8, 3>(a, pl, p, stream);
     default: return pl.NT == 2 ? run<256, 2, 4, 2>(a, pl, p, stream) : run<256, 1, 4, 3>(a, pl, p, stream);
   }
 }
