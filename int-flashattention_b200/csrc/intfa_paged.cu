@@ -75,31 +75,54 @@ __device__ __forceinline__ Place place_of(const AppendJob& p, long long t) {
 }
 
 // Rows that each have a scale of their own, tokens_cta tokens a CTA: q's, and with KV those of K and V.  A slot (the lanes of a row) goes
-// through several rows of one token, two in flight; what it needs of the rotary table stays in registers for all of them.
+// through the rows of one token in pairs, two of q or one of K and V.  Two pairs are on their way meanwhile, through shared memory, where they take
+// no registers (no thread reads another's, so nothing waits for the CTA); the first are asked for ahead of where the token goes.  What a slot
+// needs of the rotary table stays in registers for all rows.
+struct RowRing {
+  uint4 at[2][4][kThreads];              // [pair][row, piece][thread]
+};
 template <typename T, int D, int SPIN, bool KV>
-__device__ __forceinline__ void token_rows(const AppendJob& p, long long cta, int tokens_cta, int per_token, Place* place) {
+__device__ __forceinline__ void token_rows(const AppendJob& p, long long cta, int tokens_cta, int per_token, Place* place, RowRing& ring) {
   constexpr int LPR = D / 16;
   const int slot = threadIdx.x / LPR, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int mine = slot / per_token, row0 = slot % per_token;
   const long long token = cta * tokens_cta + mine;
   const bool in = token < p.tokens && mine < tokens_cta;
+  const int hq = p.heads[0], hk = p.heads[1];
+  const int pairs_q = (hq + 2 * per_token - 1) / (2 * per_token), pairs = pairs_q + (KV ? (hk + per_token - 1) / per_token : 0);
   Pieces at;
   at.place<SPIN>(threadIdx.x % LPR, p.rot);
-  Row16<T> r0, r1;
-  r0.zero();
-  r1.zero();
   auto row_of = [&](int w) { return static_cast<const T*>(p.x[w]) + (in ? token : 0) * p.xn[w] + row0 * p.xh[w]; };
-  // the first rows are asked for ahead of where they go
-  const T* xq = p.q8 ? row_of(0) : nullptr;
   const long long sq = per_token * p.xh[0];
-  const int hq = p.heads[0], hk = p.heads[1];
-  if (hq > 0) {
-    if (in && row0 < hq) r0.load(xq, at);
-    if (in && row0 + per_token < hq) r1.load(xq + sq, at);
-  } else if (KV && in && row0 < hk) {
-    r0.load(row_of(1), at);
-    r1.load(row_of(2), at);
-  }
+  const uint32_t mem = smem_u32(&ring.at[0][0][threadIdx.x]);
+  const T *la = hq > 0 ? row_of(0) : row_of(1), *lb = hq > 0 ? la + sq : row_of(2);          // the next pair to ask for
+  auto load = [&](int g) {
+    if (g < pairs) {
+      const bool q = g < pairs_q;
+      const int h = row0 + (q ? 2 * g : g - pairs_q) * per_token;
+      const uint32_t to = mem + (g & 1) * (4 * kThreads * 16);
+      if (in && h < (q ? hq : hk)) {
+        cp_async16(to, la + at.a);
+        cp_async16(to + kThreads * 16, la + at.b);
+      }
+      if (in && (q ? h + per_token < hq : h < hk)) {
+        cp_async16(to + 2 * kThreads * 16, lb + at.a);
+        cp_async16(to + 3 * kThreads * 16, lb + at.b);
+      }
+      if (q && g + 1 == pairs_q) {
+        if (KV) {
+          la = row_of(1);
+          lb = row_of(2);
+        }
+      } else {
+        la += q ? 2 * sq : per_token * p.xh[1];
+        lb += q ? 2 * sq : per_token * p.xh[2];
+      }
+    }
+    cp_async_commit();
+  };
+  load(0);
+  load(1);
   for (int i = warp; i < tokens_cta; i += kThreads / 32) {
     const Place x = place_of(p, cta * tokens_cta + i);
     if (lane == 0) place[i] = x;
@@ -114,6 +137,16 @@ __device__ __forceinline__ void token_rows(const AppendJob& p, long long cta, in
     if (!pos_ok && in && to.own && threadIdx.x % LPR == 0 && row0 == 0) report(p);
     goes = goes && pos_ok;
   }
+  auto take = [&](int g, Row16<T>& a, Row16<T>& b) {
+    cp_async_wait<1>();
+    Raw<T>* const r[4] = {&a.a, &a.b, &b.a, &b.b};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4 v = ring.at[g & 1][i][threadIdx.x];
+      r[i]->w[0] = v.x; r[i]->w[1] = v.y; r[i]->w[2] = v.z; r[i]->w[3] = v.w;
+    }
+    load(g + 2);
+  };
   auto row = [&](const Row16<T>& raw, const T* src, bool ok, bool spin, int8_t* out, float* scale) {
     float x[16];
     widen16(raw, x);
@@ -128,34 +161,35 @@ __device__ __forceinline__ void token_rows(const AppendJob& p, long long cta, in
     }
   };
   // (every lane of a warp makes every round, for the shuffles)
-  int8_t* q8 = p.q8 + (token * hq + row0) * D;
-  float* qs = p.qs + token * hq + row0;
+  Row16<T> r0, r1;
+  int g = 0, h = row0;
+  if (pairs_q > 0) {
+    const T* xq = row_of(0);
+    int8_t* q8 = p.q8 + (token * hq + row0) * D;
+    float* qs = p.qs + token * hq + row0;
 #pragma unroll 1
-  for (int h = 0; h < hq; h += 2 * per_token) {
-    if (h > 0) {
-      if (in && h + row0 < hq) r0.load(xq, at);
-      if (in && h + row0 + per_token < hq) r1.load(xq + sq, at);
+    for (; g < pairs_q; ++g) {
+      take(g, r0, r1);
+      row(r0, xq, goes && h < hq, true, q8, qs);
+      row(r1, xq + sq, goes && h + per_token < hq, true, q8 + per_token * D, qs + per_token);
+      h += 2 * per_token;
+      xq += 2 * sq;
+      q8 += 2 * per_token * D;
+      qs += 2 * per_token;
     }
-    row(r0, xq, goes && h + row0 < hq, true, q8, qs);
-    row(r1, xq + sq, goes && h + row0 + per_token < hq, true, q8 + per_token * D, qs + per_token);
-    xq += 2 * sq;
-    q8 += 2 * per_token * D;
-    qs += 2 * per_token;
   }
   if constexpr (KV) {
     const T *xk = row_of(1), *xv = row_of(2);
     const long long page = goes ? to.page : 0;
     int8_t *ck = p.cache[0] + page * p.cp[0] + to.slot * p.cn[0] + row0 * p.ch[0], *cv = p.cache[1] + page * p.cp[1] + to.slot * p.cn[1] + row0 * p.ch[1];
     float *ak = p.scale[0] + page * p.sp[0] + to.slot * p.sb[0] + row0 * p.sh[0], *av = p.scale[1] + page * p.sp[1] + to.slot * p.sb[1] + row0 * p.sh[1];
+    h = row0;
 #pragma unroll 1
-    for (int h = 0; h < hk; h += per_token) {
-      const bool have = h + row0 < hk;
-      if ((h > 0 || hq > 0) && in && have) {
-        r0.load(xk, at);
-        r1.load(xv, at);
-      }
-      row(r0, xk, goes && have, true, ck, ak);
-      row(r1, xv, goes && have, false, cv, av);
+    for (; g < pairs; ++g) {
+      take(g, r0, r1);
+      row(r0, xk, goes && h < hk, true, ck, ak);
+      row(r1, xv, goes && h < hk, false, cv, av);
+      h += per_token;
       xk += per_token * p.xh[1];
       xv += per_token * p.xh[2];
       ck += per_token * p.ch[0];
@@ -170,9 +204,10 @@ __device__ __forceinline__ void token_rows(const AppendJob& p, long long cta, in
 template <typename T, int D, int SPIN>
 __global__ void __launch_bounds__(kThreads, SPIN == kAny ? 2 : 3) append_tokens_kernel(const AppendJob p, int tokens_cta, int per_token) {
   __shared__ Place place[kMaxTokens];
+  __shared__ RowRing ring;
   pdl_wait();
   pdl_launch();
-  token_rows<T, D, SPIN, true>(p, blockIdx.x, tokens_cta, per_token, place);
+  token_rows<T, D, SPIN, true>(p, blockIdx.x, tokens_cta, per_token, place, ring);
 }
 
 // What one sequence adds to one block.  Unit u of sequence s: u = cu[s] / block + 2 s + i for the i-th block that the sequence touches (it
@@ -228,10 +263,11 @@ template <typename T, int D, int SPIN>
 __global__ void __launch_bounds__(kThreads, 2) append_runs_kernel(const AppendJob p, int units, int groups, int pairs, int ctas, int tokens_cta, int per_token) {
   constexpr int LPR = D / 16, SLOTS = 32 / LPR;
   __shared__ Place place[kMaxTokens];
+  __shared__ RowRing ring;
   pdl_wait();
   pdl_launch();
   if ((int)blockIdx.x >= ctas) {
-    token_rows<T, D, SPIN, false>(p, (int)blockIdx.x - ctas, tokens_cta, per_token, place);
+    token_rows<T, D, SPIN, false>(p, (int)blockIdx.x - ctas, tokens_cta, per_token, place, ring);
     return;
   }
   const int lane = threadIdx.x & 31, id = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), u = id / groups, g = id - u * groups;
@@ -289,12 +325,13 @@ template <typename T, int D, int SPIN>
 __global__ void __launch_bounds__(kThreads, 2) append_blocks_kernel(const AppendJob p, int units, int groups, int heads_cta, int tokens_cta, int per_token) {
   constexpr int LPR = D / 16, SLOTS = kThreads / LPR;
   __shared__ Place place[kMaxTokens];
+  __shared__ RowRing ring;
   __shared__ unsigned int most[2 * kThreads];        // [K, V][heads_cta]
   __shared__ float s_old[2 * kThreads], s_new[2 * kThreads];
   pdl_wait();
   pdl_launch();
   if ((long long)blockIdx.x >= (long long)units * groups) {
-    token_rows<T, D, SPIN, false>(p, (long long)blockIdx.x - (long long)units * groups, tokens_cta, per_token, place);
+    token_rows<T, D, SPIN, false>(p, (long long)blockIdx.x - (long long)units * groups, tokens_cta, per_token, place, ring);
     return;
   }
   const int u = blockIdx.x / groups, head0 = (blockIdx.x - u * groups) * heads_cta, nh = min(heads_cta, p.heads[1] - head0);

@@ -216,28 +216,29 @@ __device__ __forceinline__ float row_max(float m) {
 __device__ __forceinline__ float scale_of(float most) { return __fdiv_rn(most, 127.0f); }
 
 // Values as int8 codes: x/scale, rounded to fp32 and then to the nearest whole number (ties to even); zeros where the scale is 0 or not
-// finite.  The quotient is formed with an approximate reciprocal, whose error (2^-23 of up to 127, and as much for
-// the two products' rounding: less than 4e-5) decides nothing unless it is that near to a border of two codes: then, which is once in
-// 12 000 values, by a division.
+// finite.  Without a division: the reciprocal is approximate (2^-23), a little more and a little less of it (1 +- 2^-21, and 2^-24 of rounding)
+// are on either side of every quotient that the division could give.  Where both round to the same code it is that one; where they do not, once
+// in some 25 000 values, by a division.
 template <int N>
 __device__ __forceinline__ void codes(const float (&x)[N], float scale, uint32_t (&out)[N / 4]) {
   constexpr float kMagic = 12582912.0f;               // 1.5 * 2^23: the sum's low byte is the whole number
   const bool ok = scale > 0.f && scale <= 3.402823466e38f;
   float inverse;
   asm("rcp.approx.f32 %0, %1;" : "=f"(inverse) : "f"(scale));
-  const uint64_t inv2 = f2_pack(inverse, inverse), magic2 = f2_pack(kMagic, kMagic), minus2 = f2_pack(-kMagic, -kMagic), one2 = f2_pack(-1.f, -1.f);
-  uint32_t b[N];
-  float off = 0.f;
+  const float more = inverse * (1.f + 4.76837158e-7f), less = inverse * (1.f - 4.76837158e-7f);
+  const uint64_t more2 = f2_pack(more, more), less2 = f2_pack(less, less), magic2 = f2_pack(kMagic, kMagic);
+  uint32_t b[N], differ = 0u;
 #pragma unroll
   for (int i = 0; i < N; i += 2) {
-    const uint64_t q = f2_mul(f2_pack(x[i], x[i + 1]), inv2), t = f2_add(q, magic2);
-    float d0, d1;
-    f2_unpack(f2_fma(q, one2, f2_add(t, minus2)), d0, d1);             // whole number - quotient
-    off = max3(off, fabsf(d0), fabsf(d1));
-    f2_unpacku(t, b[i], b[i + 1]);
+    const uint64_t q = f2_pack(x[i], x[i + 1]);
+    uint32_t m0, m1;
+    f2_unpacku(f2_fma(q, more2, magic2), m0, m1);
+    f2_unpacku(f2_fma(q, less2, magic2), b[i], b[i + 1]);
+    differ |= m0 ^ b[i];
+    differ |= m1 ^ b[i + 1];
   }
-  // (an `off` that is not small, a scale whose reciprocal is not a normal number: the careful way)
-  if (ok && !(off < 0.49996f && scale > 1e-37f && scale < 1e37f)) {
+  // (a scale whose reciprocal is not a normal number: the careful way)
+  if (ok && !(differ == 0u && scale > 1e-37f && scale < 1e37f)) {
 #pragma unroll
     for (int i = 0; i < N; ++i) b[i] = __float_as_uint(__fadd_rn(fminf(fmaxf(__fdiv_rn(x[i], scale), -127.f), 127.f), kMagic));
   }
@@ -245,6 +246,14 @@ __device__ __forceinline__ void codes(const float (&x)[N], float scale, uint32_t
   for (int i = 0; i < N / 4; ++i)
     out[i] = ok ? __byte_perm(__byte_perm(b[4 * i], b[4 * i + 1], 0x0040), __byte_perm(b[4 * i + 2], b[4 * i + 3], 0x0040), 0x5410) : 0u;
 }
+
+// 16 bytes to shared memory, zeros unless ok
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok = true) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // largest i in [0, n) with f(i) <= x, by the lanes of a warp together (f grows, f(0) <= x)
 template <typename F>
