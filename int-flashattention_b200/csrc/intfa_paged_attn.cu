@@ -5,14 +5,14 @@
 // Reads K and V once (64 sequences of up to 8192 keys, 8 heads x 128: 703 MB, 109 us at the measured copy rate): bound by HBM.
 //
 // Work.  A unit is (sequence, K/V head, tile of RT = 8 NT rows); the rows of all query heads that share the K/V head are packed into it, so
-// that K and V are read once for all of them.  Its keys are cut into chunks of 32.  The chunks of all units in a row are dealt out to the
+// that K and V are read once for all of them.  Its keys are cut into chunks of G = 32, 64 at head dim 64.  The chunks of all units in a row are dealt out to the
 // warps of the GPU in equal contiguous shares, whatever the sequences' lengths are: the lengths are read on the device, so nothing waits for
 // the host and a captured graph takes other lengths at its next replay.  A warp keeps the softmax state and the output of the unit it is in
 // in registers.  A unit that lies within one warp's share is written at once; the parts of the others go to scratch and combine_kernel adds
 // them up, in the order of the keys.
 //
 // Loads.  Each warp has a ring of NS chunks of its own, filled by TMA (pages of any size and order, 8 to 32 rows a copy) and by cp.async (scales,
-// query rows), so no warp waits for another and NS - 1 chunks a warp (128 KB an SM) are in flight.  A chunk's rows are swizzled by the
+// query rows), so no warp waits for another and NS - 1 chunks a warp (64 to 128 KB an SM) are in flight.  A chunk's rows are swizzled by the
 // TMA such that the 16-byte reads below are free of bank conflicts.
 //
 // Arithmetic.  m16n8 warp-level MMAs straight from that ring: 8 or 16 rows are far below the smallest tcgen05 tile.  Q K^T is an int8
@@ -881,16 +881,18 @@ struct Plan {
   size_t off_ml = 0, off_units = 0, off_head = 0, bytes = 0;
 };
 // 128-row tiles, or packed rows of 8 or 16?  A tile costs the same however many of its rows there are, and a unit on tiles takes longer to
-// begin, to end and to be put together.  The lengths of the sequences are not known here; timed on both with 600 and 4000 keys: at 128 channels
-// 16 sequences of 8 K/V heads, 64 rows each a head, 26.0 / 74.0 us packed, 30.6 / 63.7 on tiles, of 32 rows 23.3 / 49.1 and 29.8 / 56.7; one
-// sequence, 256 rows, 24.2 / 51.4 and 28.5 / 29.1, 128 rows 15.7 / 31.3 and 17.9 / 29.3; at 64 channels 16 sequences, 128 rows, 27.9 / 81.9 and
-// 30.6 / 60.5, 64 rows 19.6 / 46.4 and 26.9 / 61.7; at 256 channels 32 rows 40.1 / 93.1 and 36.0 / 69.7, one sequence, 128 rows, 25.9 / 50.0 and
-// 21.9 / 37.0, 64 rows 17.3 / 30.3 and 18.7 / 31.3.
+// begin, to end and to be put together.  The lengths of the sequences are not known here; timed on both with up to 600 and 4000 keys, packed /
+// on tiles, in us.  16 sequences of 8 K/V heads: at 64 channels 64 rows a head 18.5 / 26.6 and 38.9 / 57.6, 128 rows 25.3 / 30.6 and
+// 63.1 / 56.3, 256 rows 39.0 / 33.9 and 125 / 77.5; at 128 channels 64 rows 25.6 / 31.0 and 58.5 / 62.9, 128 rows 35.2 / 35.8 and 100 / 63.1; at 256
+// channels 32 rows 39.1 / 36.4 and 96.9 / 71.3.  Few rows in all do not fill the GPU with tiles: one sequence of 8 heads, at 64 channels 256 rows
+// 20.4 / 21.7 and 31.3 / 25.8, four of one head and 512 rows 16.0 / 23.1 and 24.9 / 32.0; at 128 channels 128 rows 16.5 / 18.0 and 25.4 / 29.6, 256
+// rows 21.9 / 28.8 and 42.8 / 29.0; at 256 channels 64 rows 17.5 / 18.5 and 31.5 / 31.3, 128 rows 25.8 / 21.7 and 52.7 / 37.3.
 bool takes_tiles(const IntfaPagedParams* a) {
   if (a->debug_path) return a->debug_path == 2;
   const double rows = (double)a->tokens * (a->H / a->cache.H_kv) / a->cache.S;          // of an average sequence and K/V head
-  return a->H / a->cache.H_kv <= kTileRows && rows >= (a->cache.D == 64 ? 112 : a->cache.D == 128 ? 64 : 32) &&
-         rows * a->cache.S * a->cache.H_kv >= (a->cache.D == 256 ? 1024 : 2048);
+  const int D = a->cache.D;
+  return a->H / a->cache.H_kv <= kTileRows && rows >= (D == 64 ? 128 : D == 128 ? 96 : 32) &&
+         rows * a->cache.S * a->cache.H_kv >= (D == 64 ? 4096 : D == 128 ? 2048 : 1024);
 }
 Plan make_plan(const IntfaPagedParams* a, int sms) {
   Plan pl;
@@ -913,7 +915,7 @@ Plan make_plan(const IntfaPagedParams* a, int sms) {
     pl.off_head = take(32);
     return pl;
   }
-  // Rows a tile: 16 where an average sequence has more than 8 rows a K/V head
+  // Rows a tile: 16 where an average sequence has more than 8 rows a K/V head (up to 8 of them cost half in tiles of 8, more twice the bytes)
   pl.NT = (double)a->tokens * ratio > 8.0 * c.S ? 2 : 1;
   pl.warps = c.D == 256 ? 4 : 8;
   pl.max_units = (a->tokens * ratio / (8 * pl.NT) + c.S) * c.H_kv;
@@ -1042,6 +1044,10 @@ int paged_attention(const IntfaPagedParams* a, cudaStream_t stream) {
     p.least = 2;
     return c.D == 64 ? run_tiles<64>(a, pl, p, stream) : c.D == 128 ? run_tiles<128>(a, pl, p, stream) : run_tiles<256>(a, pl, p, stream);
   }
+  // Warps and chunks a ring, as timed with 64 sequences of one row and up to 8192 keys (NT 1), 32 of 4 rows, 4 query heads a K/V head, and
+  // up to 4097 (NT 2), in us.  64 channels: 71.3 (12 warps with 2 chunks 73.1; chunks of 32 keys, 8 with 5: 92.8), NT 2 33.5 (7 with 3 37.8, 6 with 3
+  // 39.4, 9 with 2 42; chunks of 32 keys, 8 with 4: 38.6).  128 channels: 118 (chunks of 64 keys, 6 with 2: 124, 4 with 3: 125), NT 2 49.8 (6 with 3
+  // 57.8, 4 with 5 63.7).  256 channels: what fits registers and shared memory.
   switch (c.D) {
     case 64: return pl.NT == 2 ? run<64, 2, 8, 2, 64>(a, pl, p, stream) : run<64, 1, 8, 3, 64>(a, pl, p, stream);
     case 128: return pl.NT == 2 ? run<128, 2, 8, 2>(a, pl, p, stream) : run<128, 1, 8, 3>(a, pl, p, stream);
