@@ -269,7 +269,8 @@ int intfa_rotary(const IntfaRotaryParams* p, void* stream);
 /*
  * A paged int8 K/V cache and which of its pages hold which tokens.  k, v: [pages, H_kv, page_size, D] int8, element strides for
  * (page, head, token) that are multiples of 16, last dim contiguous, 16-byte aligned.  k_scale, v_scale: fp32
- * [pages, H_kv, page_size/block], any positive strides: a value is its code times the scale of its block of `block` tokens and head.
+ * [pages, H_kv, page_size/block], any positive strides, not negative: a value is its code times the scale of its block of `block` tokens
+ * and head.  At most 2^30 tokens a sequence (table_width * page_size).
  * Token i of sequence s is in slot i % page_size of page block_table[s][i / page_size]; entries past the last token are not read.
  * seq_lens [S]: tokens in the cache, those of the call included (the new tokens of intfa_paged_append, the query rows of a causal
  * intfa_paged_attention are the last of them).
@@ -310,7 +311,8 @@ int intfa_paged_append(const IntfaAppendParams* p, void* stream);
  * cu_seqlens[s] .. cu_seqlens[s+1]-1 (NULL: one row a sequence); causal: row i of n sees the keys up to seq_lens[s] - n + i, else all.
  * Softmax, sums and the running output in fp32, p * v_scale rounded to fp16 for the product with v.  A row that sees nothing is zero
  * (lse -inf); rows behind the last sequence are not written.  o [tokens, H, D]: strides for (token, head), multiples of 8.
- * lse_out (or NULL): [tokens, H] fp32 contiguous, log2 domain, as intfa_fwd's.
+ * Sequences may share pages.  cu_seqlens must not fall; where it does, or a length does not fit its table row, nothing is read or written
+ * outside and `status` tells.  lse_out (or NULL): [tokens, H] fp32 contiguous, log2 domain, as intfa_fwd's.
  * workspace: device scratch of intfa_paged_workspace_bytes() bytes, 256-byte aligned, contents irrelevant.
  */
 typedef struct IntfaPagedParams {

@@ -1,10 +1,12 @@
 // New tokens into a paged int8 cache: keys rotated by their positions, keys and values quantised with one scale for each block of
 // `block` tokens and head, queries of the same tokens rotated and quantised per token, all in one launch.
 //
-// Reads 2 bytes a value, writes 1 (10 000 tokens of 32 + 8 + 8 heads x 128: 345 MB, 53 us at the measured copy rate): bound by HBM, and
-// by launch and latency for the few tokens of a decode step.
+// Reads 2 bytes a value, writes 1 (18 700 tokens of 32 + 8 + 8 heads x 128: 345 MB, 53 us at the measured copy rate): 85 us, bound by the issue of
+// instructions (72 % of the slots: 300 for a warp's 16 values a lane, of them 126 the rotation, whose products are rounded one by one, and 80 the
+// proof that the codes are those of a division).  The few tokens of a decode step: launch and latency, 5.4 us in a graph.
 //   block = 1   a row (one head of one token) is quantised by the lanes that loaded it; a CTA takes one token, or a few of few heads
-//   block > 1   a warp (short blocks) or a CTA takes what a sequence adds to one block, for some heads: the largest magnitudes first, then the codes.  A block that
+//   block > 1   a warp (short blocks: 12 us for 40 sequences of up to 200 tokens, where CTAs took 19) or a CTA takes what a sequence adds to one
+//               block, for some heads: the largest magnitudes first, then the codes.  A block that
 //               began in an earlier call keeps the larger of its old scale and the new tokens'; where that grew its older codes become
 //               rint(code * (old / new)).  So a block's codes depend on how its tokens were handed over, as its scale must.
 #include "intfa_rows.cuh"

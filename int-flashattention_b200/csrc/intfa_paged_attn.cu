@@ -2,16 +2,18 @@
 //
 //   s = dot(q8, k8) * (q_scale * sm_scale * log2 e) * k_scale[block],   p = exp2(s - max),   o = sum p v_scale[block] v8 / sum p
 //
-// Reads K and V once (64 sequences of up to 8192 keys, 8 heads x 128: 703 MB, 109 us at the measured copy rate): bound by HBM.
+// Reads K and V once (64 sequences of up to 8192 keys, 8 heads x 128: 703 MB, 109 us at the measured copy rate, 118 to 133 here): bound by HBM.  One
+// sequence of 131 072 keys 41.6 and 57: ten microseconds are the start, the end and the combination, which is all of a short call (513 keys: 10.5).
+// 16 rows a K/V head at 64 channels (91 MB) 14.1 and 33.6: the latency of two warps a scheduler, whose exp2 are per row and key.
 //
 // Work.  A unit is (sequence, K/V head, tile of RT = 8 NT rows); the rows of all query heads that share the K/V head are packed into it, so
-// that K and V are read once for all of them.  Its keys are cut into chunks of G = 32, 64 at head dim 64.  The chunks of all units in a row are dealt out to the
-// warps of the GPU in equal contiguous shares, whatever the sequences' lengths are: the lengths are read on the device, so nothing waits for
-// the host and a captured graph takes other lengths at its next replay.  A warp keeps the softmax state and the output of the unit it is in
+// that K and V are read once for all of them.  Its keys are cut into chunks of G = 32, 64 at head dim 64.  The chunks of all units in a row are
+// dealt out to the warps of the GPU in equal contiguous shares, whatever the sequences' lengths are: the lengths are read on the device, so
+// nothing waits for the host and a captured graph takes other lengths at its next replay.  A warp keeps the softmax state and the output of the unit it is in
 // in registers.  A unit that lies within one warp's share is written at once; the parts of the others go to scratch and combine_kernel adds
 // them up, in the order of the keys.
 //
-// Loads.  Each warp has a ring of NS chunks of its own, filled by TMA (pages of any size and order, 8 to 32 rows a copy) and by cp.async (scales,
+// Loads.  Each warp has a ring of NS chunks of its own, filled by TMA (pages of any size and order, 8 to G rows a copy) and by cp.async (scales,
 // query rows), so no warp waits for another and NS - 1 chunks a warp (64 to 128 KB an SM) are in flight.  A chunk's rows are swizzled by the
 // TMA such that the 16-byte reads below are free of bank conflicts.
 //

@@ -219,7 +219,7 @@ def append_int8_paged(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq
     position first where a `table` (rotary_table) is given, then both quantised with one scale for each block of tokens and head.
       k_cache, v_cache   int8 [pages, heads, page_size, D]: any page and head strides of 16 bytes, D 64, 128 or 256,
                          page_size a power of two from 8 to 256
-      k_scale, v_scale   float32 [pages, heads, page_size/block]; block 1 is one scale a token
+      k_scale, v_scale   float32 [pages, heads, page_size/block], not negative; block 1 is one scale a token
       block_table        int32 [S, columns]: the page of a sequence's tokens i*page_size ...
       seq_lens           int32 [S]: tokens in the cache with the new ones, which are the last
       cu_seqlens         int32 [S+1]: where each sequence's new tokens begin among `tokens`; None: one token a sequence
@@ -235,7 +235,7 @@ def attention_int8_paged(q, k_cache, v_cache, q_scale, k_scale, v_scale, block_t
     """Attention of packed int8 query rows q [tokens, query heads, D] over a paged int8 cache (append_int8_paged has the tensors):
     softmax(sm_scale * q k^T) v, with q = q8 * q_scale and the cache's values as codes times scales.  The rows of sequence s are
     cu_seqlens[s] .. cu_seqlens[s+1]-1 (None: one row each, decode); causal: they are its last tokens, row i of n sees keys up to
-    seq_lens[s] - n + i, else all keys.  Query heads share K/V heads in order, as in attention_int8.  A row that sees no key is
+    seq_lens[s] - n + i, else all keys.  Sequences may share pages.  Query heads share K/V heads in order, as in attention_int8.  A row that sees no key is
     zero.  Returns o [tokens, query heads, D] in out_dtype (torch.float16 unless given, or torch.bfloat16); with `out` it is written there,
     and rows behind the last sequence stay as they were (without it they are not set).  return_lse: and the log2-domain LSE
     [tokens, query heads].  (debug_path: test hook, 1 or 2 for one of the two kernels whatever the sizes.)"""
