@@ -3,7 +3,7 @@
 //   s = dot(q8, k8) * (q_scale * sm_scale * log2 e) * k_scale[block],   p = exp2(s - max),   o = sum p v_scale[block] v8 / sum p
 //
 // Reads K and V once (64 sequences of up to 8192 keys, 8 heads x 128: 703 MB, 109 us at the measured copy rate, 118 to 133 here): bound by HBM.  One
-// sequence of 131 072 keys 41.6 and 57: ten microseconds are the start, the end and the combination, which is all of a short call (513 keys: 10.5).
+// sequence of 131 072 keys 41.6 and 57: ten microseconds are the start, the end and the combination.  Short calls are all that, 6.4 in clusters.
 // 16 rows a K/V head at 64 channels (91 MB) 14.1 and 33.6: the latency of two warps a scheduler, whose exp2 are per row and key.
 //
 // Work.  A unit is (sequence, K/V head, tile of RT = 8 NT rows); the rows of all query heads that share the K/V head are packed into it, so
@@ -11,7 +11,8 @@
 // dealt out to the warps of the GPU in equal contiguous shares, whatever the sequences' lengths are: the lengths are read on the device, so
 // nothing waits for the host and a captured graph takes other lengths at its next replay.  A warp keeps the softmax state and the output of the unit it is in
 // in registers.  A unit that lies within one warp's share is written at once; the parts of the others go to scratch and combine_kernel adds
-// them up, in the order of the keys.
+// them up, in the order of the keys.  Few units of few keys: a unit is the work of a cluster of CTAs, whose parts are added up through their shared
+// memory, with no second launch.
 //
 // Loads.  Each warp has a ring of NS chunks of its own, filled by TMA (pages of any size and order, 8 to G rows a copy) and by cp.async (scales,
 // query rows), so no warp waits for another and NS - 1 chunks a warp (64 to 128 KB an SM) are in flight.  A chunk's rows are swizzled by the
@@ -177,7 +178,7 @@ struct DecodeCfg {
   static constexpr int OFF_PRE = OFF_BAR + WARPS * NS * 8;              // [threads + 1] chunks (long long) and units (int) before a thread's sequences
   static constexpr int OFF_MISC = OFF_PRE + ((32 * WARPS + 1) * 12 + 15) / 16 * 16;
   static constexpr int SMEM = OFF_MISC + 32 + 1024;
-  static constexpr int MERGE = WARPS * RT * ((D + 4) + 4) * 4;          // (over the ring, when it is done with)
+  static constexpr int MERGE = (WARPS + 1) * RT * ((D + 4) + 4) * 4;    // (over the ring, when it is done with)
   static_assert(MERGE <= OFF_EXTRA, "merge");
   static_assert(EXTRA % 16 == 0, "alignment");
   static_assert(SMEM <= 227 * 1024, "shared memory");
@@ -452,7 +453,8 @@ __device__ __forceinline__ void chunk_step(RowState<D, NT>& st, const uint32_t (
 
 enum { kWaitChunk = 64 };
 
-template <int D, int NT, int WARPS, int NS, int G>
+// CL: a unit is the work of a cluster of CTAs, whose warps share its chunks; the parts are added up through their shared memory
+template <int D, int NT, int WARPS, int NS, int G, bool CL>
 __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const PParams p) {
   using C = DecodeCfg<D, NT, WARPS, NS, G>;
   constexpr int RT = C::RT, THREADS = 32 * WARPS, M = G / 32;            // keys a lane
@@ -475,6 +477,21 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_const
   mbar_init_fence();
   pdl_wait();
   pdl_launch();
+  Cursor at;
+  long long total, share, begin, unit_id = 0;                // chunks, of a warp, before this warp; the unit among all
+  if constexpr (CL) {
+    const int size = (int)cluster_size(), rank = (int)cluster_rank(), unit = blockIdx.x / size, per_seq = (gridDim.x / size) / p.S;
+    at.s = unit / per_seq;
+    at.q = seq_of(p, at.s);
+    at.head = (unit - at.s * per_seq) / at.q.tiles;
+    at.tile = (unit - at.s * per_seq) - at.head * at.q.tiles;
+    if (at.q.bad && p.status && threadIdx.x == 0 && rank == 0) atomicCAS(p.status, 0, kStatusBadIndex);
+    total = at.q.chunks;
+    share = (total + size * WARPS - 1) / (size * WARPS);
+    begin = (warp * size + rank) * share;                    // (few chunks: on as many SMs as there are)
+    at.chunk = (int)begin;
+    __syncthreads();
+  } else {
   // ---- the row of all chunks: thread i counts the sequences i*seg .. (i+1)*seg - 1
   const int seg = (p.S + THREADS - 1) / THREADS;
   {
@@ -516,19 +533,14 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_const
     }
   }
   __syncthreads();
-  const long long total = pre_c[THREADS];
-  long long share = (total + p.workers - 1) / p.workers;
+  total = pre_c[THREADS];
+  share = (total + p.workers - 1) / p.workers;
   if (share < p.least) share = p.least;
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     p.head[0] = pre_u[THREADS];
   }
-  const int worker = blockIdx.x * WARPS + warp;
-  const long long begin = worker * share;
-  const long long left0 = total - begin < share ? total - begin : share;
-  long long left = left0 < 0 ? 0 : left0;                    // chunks to do
-  Cursor at;
-  long long unit_id = 0;                                     // of all units
-  if (left > 0) {
+  begin = (long long)(blockIdx.x * WARPS + warp) * share;
+  if (begin < total) {
     const int i = find_last(THREADS, begin, [&](int j) { return pre_c[j]; });
     long long off = begin - pre_c[i];
     unit_id = pre_u[i];
@@ -546,6 +558,14 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_const
     at.tile = unit - at.head * at.q.tiles;
     unit_id += unit;
   }
+  }
+  const int worker = blockIdx.x * WARPS + warp;
+  const long long left0 = total - begin < share ? total - begin : share;
+  long long left = left0 < 0 ? 0 : left0;                    // chunks to do
+  auto advance = [&](Cursor& c) {
+    if constexpr (CL) ++c.chunk;
+    else c.next(p);
+  };
   // ---- loads
   const uint32_t sKV = smem_u32(smem) + warp * NS * 2 * C::KV;
   const uint32_t sX = smem_u32(smem + C::OFF_EXTRA) + warp * NS * C::EXTRA;
@@ -615,7 +635,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_const
         }
       }
       --to_load;
-      ahead.next(p);
+      advance(ahead);
       fresh = ahead.chunk == 0;
       look_up();
     }
@@ -697,7 +717,9 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_const
     }
     --left;
     ++pos;
-    if (at.chunk + 1 == at.q.chunks || left == 0) {
+    if constexpr (CL) {
+      if (left == 0) st.reduce_l();
+    } else if (at.chunk + 1 == at.q.chunks || left == 0) {
       st.reduce_l();
       const int head = at.head, tile = at.tile;
       const bool starts = unit0 >= begin, ends = unit1 <= pos;
@@ -732,7 +754,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_const
       open = false;
       ++unit_id;
     }
-    at.next(p);
+    advance(at);
   }
   if (!ok) {
     // A wait ran out.  The units that this share begins and that were not reached are no parts for combine_kernel; what this warp asked for comes
@@ -744,20 +766,22 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_const
         parity ^= 1;
       }
     }
-    for (bool begins = open ? unit0 >= begin : at.chunk == 0; left > 0; --left) {
+    for (bool begins = open ? unit0 >= begin : at.chunk == 0; !CL && left > 0; --left) {
       if (begins && lane == 0 && unit_id < p.max_units) p.units[unit_id].open = 0;
       if (at.chunk + 1 == at.q.chunks) ++unit_id;
       at.next(p);
       begins = at.chunk == 0;
     }
   }
-  if (!__syncthreads_or(merge)) return;
+  if (!__syncthreads_or(merge || CL)) return;
   // (every warp is done with its ring: what it asked for has come)
   float* red = reinterpret_cast<float*>(smem);
   float* red_ml = red + WARPS * RT * (D + 4);
   write_part<D, NT>(red + warp * RT * (D + 4), red_ml + warp * RT * 4, D + 4, st);
   __syncthreads();
-  const long long slot = 2LL * blockIdx.x * WARPS + whole[1];
+  float* mine = red_ml + WARPS * RT * 4;                     // (CL) the CTA's sums, then their m, mw, l
+  float* mine_ml = mine + RT * (D + 4);
+  const long long slot = CL ? 0 : 2LL * blockIdx.x * WARPS + whole[1];
   for (int i = threadIdx.x; i < RT * (D / 4); i += THREADS) {
     const int r = i / (D / 4), ch = i % (D / 4) * 4;
     Sum x;
@@ -765,13 +789,32 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_const
 #pragma unroll
     for (int w = 0; w < WARPS; ++w)
       x.add(*reinterpret_cast<const float4*>(red_ml + (w * RT + r) * 4), *reinterpret_cast<const float4*>(red + (w * RT + r) * (D + 4) + ch));
-    if (!whole[0]) {
+    if constexpr (CL) {
+      *reinterpret_cast<float4*>(mine + r * (D + 4) + ch) = x.a;
+      if (ch == 0) *reinterpret_cast<float4*>(mine_ml + r * 4) = make_float4(x.m, x.mw, x.l, 0.f);
+    } else if (!whole[0]) {
       *reinterpret_cast<float4*>(p.part + (slot * RT + r) * D + ch) = x.a;
       if (ch == 0) *reinterpret_cast<float4*>(p.part_ml + (slot * RT + r) * 4) = make_float4(x.m, x.mw, x.l, 0.f);
     } else if (r < whole[3]) {
       const int row = whole[5] * RT + r;
       write_sum(p, whole[2] + row / p.ratio, whole[4] * p.ratio + row % p.ratio, ch, x);
     }
+  }
+  if constexpr (CL) {
+    const int size = (int)cluster_size(), rank = (int)cluster_rank();
+    cluster_arrive();
+    cluster_wait();
+    for (int i = rank + size * threadIdx.x; i < RT * (D / 4); i += size * THREADS) {
+      const int r = i / (D / 4), ch = i % (D / 4) * 4, row = at.tile * RT + r;
+      if (row >= at.q.n * p.ratio) continue;
+      Sum x;
+      x.clear();
+#pragma unroll 8
+      for (int c = 0; c < size; ++c) x.add(ld_peer4(mine_ml + r * 4, c), ld_peer4(mine + r * (D + 4) + ch, c));
+      write_sum(p, at.q.t0 + row / p.ratio, at.head * p.ratio + row % p.ratio, ch, x);
+    }
+    cluster_arrive();                                        // (no CTA ends while a peer reads from it)
+    cluster_wait();
   }
 }
 
@@ -931,6 +974,36 @@ Plan make_plan(const IntfaPagedParams* a, int sms) {
   return pl;
 }
 
+// Clusters of 2^n CTAs (up to 16) of paged_kernel that the current device holds at once, one CTA an SM; 0: none, or it cannot be asked.
+template <int D, int NT, int WARPS, int NS, int G>
+int cluster_places(int n) {
+  static std::atomic<int> cache[64][5];                       // number + 1; 0: not asked yet
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  std::atomic<int>& known = cache[dev][n];
+  if (const int k = known.load(std::memory_order_acquire)) return k - 1;
+  auto kern = paged_kernel<D, NT, WARPS, NS, G, true>;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(1 << n);
+  cfg.blockDim = dim3(32 * WARPS);
+  cfg.dynamicSmemBytes = DecodeCfg<D, NT, WARPS, NS, G>::SMEM;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 1u << n;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int clusters = 0;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes) != cudaSuccess ||
+      cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    clusters = 0;
+  }
+  known.store(clusters + 1, std::memory_order_release);
+  return clusters;
+}
+
 template <int D, int NT, int WARPS, int NS, int G = 32>
 int run(const IntfaPagedParams* a, const Plan& pl, PParams p, cudaStream_t stream) {
   using C = DecodeCfg<D, NT, WARPS, NS, G>;
@@ -942,7 +1015,19 @@ int run(const IntfaPagedParams* a, const Plan& pl, PParams p, cudaStream_t strea
   int rc;
   if ((rc = make_tmap(&tmK, c.k, 1, c.k_stride, c.pages, c.H_kv, c.page_size, D, C::PANEL, 1 << p.box_log, swz))) return rc;
   if ((rc = make_tmap(&tmV, c.v, 1, c.v_stride, c.pages, c.H_kv, c.page_size, D, C::PANEL, 1 << p.box_log, swz))) return rc;
-  auto kern = paged_kernel<D, NT, WARPS, NS, G>;
+  // Units whose number is known here (one row a sequence) and which are there all at once, a cluster each: one launch and no scratch, but each
+  // unit takes as long as its own keys.  Where the table has room for so few that a CTA reads 400 KB at most: measured against the shares, 32 / 8
+  // heads x 128, up to 513 keys 6.4 against 9.9 us (8 sequences 7.1 / 10.6), 2048 6.7 / 9.8 (10.3 / 14.3), 8192 in clusters of 8 (270 KB) 10.7 / 11.8,
+  // of 4 (540 KB) 16.0 / 15.6, 32768 26.1 / 20.1; at 64 channels 32768 (557 KB) 17.1 / 15.0, at 256 8192 (532 KB) 17.3 / 16.4.
+  const long long units = (long long)c.S * c.H_kv * ((p.ratio + C::RT - 1) / C::RT);
+  if (!a->cu_seqlens && units <= pl.ctas) {
+    int n = 4;
+    while (n >= 0 && units > cluster_places<D, NT, WARPS, NS, G>(n)) --n;
+    const int size = n < 0 ? 0 : 1 << n;
+    if ((long long)c.table_width * c.page_size * (2 * D + 8) <= 400000LL * size)
+      return launch_clusters("paged attention", paged_kernel<D, NT, WARPS, NS, G, true>, (unsigned)(units * size), size, 32 * WARPS, C::SMEM, stream, tmK, tmV, p);
+  }
+  auto kern = paged_kernel<D, NT, WARPS, NS, G, false>;
   static std::atomic<bool> attr_done[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return set_error(INTFA_ERR_CUDA, "cannot query the current device");

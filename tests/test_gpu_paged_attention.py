@@ -99,12 +99,24 @@ def test_several_rows(D, causal, ratio, news, out_dtype, pkg):
 
 @pytest.mark.parametrize("S,n,Hkv,ratio,D", [(1, 5000, 1, 1, 128), (1, 40000, 1, 8, 64), (1, 20001, 8, 4, 128), (2, 9999, 1, 16, 256), (1, 120, 1, 2, 128),
                                              (600, 40, 1, 1, 64), (300, 333, 2, 4, 128), (5, 2048, 16, 1, 64), (1, 1, 1, 1, 128)])
-def test_shares(S, n, Hkv, ratio, D, pkg):
-    """Units cut into many parts, a few, none; many units to a share."""
+@pytest.mark.parametrize("one", [True, False])
+def test_shares(S, n, Hkv, ratio, D, one, pkg):
+    """Units cut into many parts, a few, none; many units to a share.  One row a sequence by itself, or because cu_seqlens says so."""
     lens = [max(1, n - 37 * s % n) for s in range(S)]
-    s = Setup([1] * S, lens, Hkv * ratio, Hkv, D, 32, 8, one=True, seed=S)
+    s = Setup([1] * S, lens, Hkv * ratio, Hkv, D, 32, 8, one=one, seed=S)
+    s.path = 1
     a = s.check(pkg)
     assert torch.equal(a, s.call(pkg))           # repeats itself
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("S,Hkv,ratio", [(1, 1, 1), (1, 8, 4), (2, 8, 1), (1, 2, 16), (1, 2, 40), (3, 3, 7), (1, 17, 2), (1, 16, 9), (5, 3, 2)])
+def test_few_units(S, Hkv, ratio, D, pkg):
+    """One row a sequence, up to 16 (sequence, K/V head, tile) units and a few more: lengths from none to more chunks than there are warps."""
+    for n in (0, 1, 33, 64, 300, 2000, 9000):
+        s = Setup([1] * S, [max(0, n - 31 * i) for i in range(S)], Hkv * ratio, Hkv, D, 16, 1, one=True, seed=n + S)
+        o = s.check(pkg)
+        assert torch.equal(o, s.call(pkg))
 
 
 @pytest.mark.parametrize("layout", ["heads", "tokens"])
