@@ -421,15 +421,16 @@ int run(const AppendJob& p, cudaStream_t stream) {
   }
   const int per = p.q8 ? slots_of(p.heads[0]) : SLOTS, n = SLOTS / per;
   const long long units = (p.tokens >> p.block_log) + 2LL * p.S, q_ctas = p.q8 ? (p.tokens + n - 1) / n : 0;
-  if constexpr (SPIN != kAny)             // (whose element-wise way has no registers for it)
-  if ((1 << p.block_log) <= kRounds * 32 / (D / 16)) {
-    // (head, K or V) pairs a warp: so many that all warps are there at once, eight at most
-    long long pairs = units * 2 * p.heads[1] / (16LL * sm_count_cached());
-    pairs = pairs < 1 ? 1 : pairs > 8 ? 8 : pairs;
-    const long long groups = (2 * p.heads[1] + pairs - 1) / pairs, ctas = (units * groups + kThreads / 32 - 1) / (kThreads / 32);
-    if (units * groups > 0x7fffffffLL || ctas + q_ctas > 0x7fffffffLL) return set_error(INTFA_ERR_TOO_LARGE, "too many tokens");
-    return launch_kernel("append", append_runs_kernel<T, D, SPIN>, (unsigned)(ctas + q_ctas), kThreads, 0, stream, p, (int)units, (int)groups, (int)pairs, (int)ctas, n,
-                         per);
+  if constexpr (SPIN != kAny) {           // (whose element-wise way has no registers for it)
+    if ((1 << p.block_log) <= kRounds * 32 / (D / 16)) {
+      // (head, K or V) pairs a warp: so many that all warps are there at once, eight at most
+      long long pairs = units * 2 * p.heads[1] / (16LL * sm_count_cached());
+      pairs = pairs < 1 ? 1 : pairs > 8 ? 8 : pairs;
+      const long long groups = (2 * p.heads[1] + pairs - 1) / pairs, ctas = (units * groups + kThreads / 32 - 1) / (kThreads / 32);
+      if (units * groups > 0x7fffffffLL || ctas + q_ctas > 0x7fffffffLL) return set_error(INTFA_ERR_TOO_LARGE, "too many tokens");
+      return launch_kernel("append", append_runs_kernel<T, D, SPIN>, (unsigned)(ctas + q_ctas), kThreads, 0, stream, p, (int)units, (int)groups, (int)pairs, (int)ctas, n,
+                           per);
+    }
   }
   // Heads a CTA: one or two rounds of rows
   int heads_cta = 2 * SLOTS / (2 << p.block_log);

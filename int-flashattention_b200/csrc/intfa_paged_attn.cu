@@ -492,72 +492,72 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_const
     at.chunk = (int)begin;
     __syncthreads();
   } else {
-  // ---- the row of all chunks: thread i counts the sequences i*seg .. (i+1)*seg - 1
-  const int seg = (p.S + THREADS - 1) / THREADS;
-  {
-    long long c = 0, u = 0;
-    bool bad = false;
-    for (int s = threadIdx.x * seg; s < (threadIdx.x + 1) * seg && s < p.S; ++s) {
-      const Seq q = seq_of(p, s);
-      const long long units = (long long)q.tiles * p.Hkv;
-      c += units * q.chunks;
-      u += units;
-      bad |= q.bad;
-    }
-    if (bad && p.status && blockIdx.x == 0) atomicCAS(p.status, 0, kStatusBadIndex);
-    // sums up to and with each thread: within the warps, then on top of the warps before
-    const long long most = p.max_units;
+    // ---- the row of all chunks: thread i counts the sequences i*seg .. (i+1)*seg - 1
+    const int seg = (p.S + THREADS - 1) / THREADS;
+    {
+      long long c = 0, u = 0;
+      bool bad = false;
+      for (int s = threadIdx.x * seg; s < (threadIdx.x + 1) * seg && s < p.S; ++s) {
+        const Seq q = seq_of(p, s);
+        const long long units = (long long)q.tiles * p.Hkv;
+        c += units * q.chunks;
+        u += units;
+        bad |= q.bad;
+      }
+      if (bad && p.status && blockIdx.x == 0) atomicCAS(p.status, 0, kStatusBadIndex);
+      // sums up to and with each thread: within the warps, then on top of the warps before
+      const long long most = p.max_units;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long x = __shfl_up_sync(0xffffffffu, c, o), y = __shfl_up_sync(0xffffffffu, u, o);
-      if (lane >= o) {
-        c += x;
-        u += y;
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, c, o), y = __shfl_up_sync(0xffffffffu, u, o);
+        if (lane >= o) {
+          c += x;
+          u += y;
+        }
+      }
+      long long* sums = reinterpret_cast<long long*>(smem);      // (the ring is not in use yet)
+      if (lane == 31) {
+        sums[2 * warp] = c;
+        sums[2 * warp + 1] = u;
+      }
+      __syncthreads();
+      for (int w = 0; w < warp; ++w) {
+        c += sums[2 * w];
+        u += sums[2 * w + 1];
+      }
+      pre_c[threadIdx.x + 1] = c;
+      pre_u[threadIdx.x + 1] = (int)(u < most ? u : most);       // (more of them only where cu_seqlens overlap)
+      if (threadIdx.x == 0) {
+        pre_c[0] = 0;
+        pre_u[0] = 0;
       }
     }
-    long long* sums = reinterpret_cast<long long*>(smem);      // (the ring is not in use yet)
-    if (lane == 31) {
-      sums[2 * warp] = c;
-      sums[2 * warp + 1] = u;
-    }
     __syncthreads();
-    for (int w = 0; w < warp; ++w) {
-      c += sums[2 * w];
-      u += sums[2 * w + 1];
+    total = pre_c[THREADS];
+    share = (total + p.workers - 1) / p.workers;
+    if (share < p.least) share = p.least;
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+      p.head[0] = pre_u[THREADS];
     }
-    pre_c[threadIdx.x + 1] = c;
-    pre_u[threadIdx.x + 1] = (int)(u < most ? u : most);       // (more of them only where cu_seqlens overlap)
-    if (threadIdx.x == 0) {
-      pre_c[0] = 0;
-      pre_u[0] = 0;
+    begin = (long long)(blockIdx.x * WARPS + warp) * share;
+    if (begin < total) {
+      const int i = find_last(THREADS, begin, [&](int j) { return pre_c[j]; });
+      long long off = begin - pre_c[i];
+      unit_id = pre_u[i];
+      at.s = i * seg - 1;
+      do {
+        at.next_seq(p);
+        const long long units = (long long)at.q.tiles * p.Hkv, c = units * at.q.chunks;
+        if (off < c) break;
+        off -= c;
+        unit_id += units;
+      } while (at.s < p.S);
+      const int unit = (int)(off / at.q.chunks);
+      at.chunk = (int)(off - (long long)unit * at.q.chunks);
+      at.head = unit / at.q.tiles;
+      at.tile = unit - at.head * at.q.tiles;
+      unit_id += unit;
     }
-  }
-  __syncthreads();
-  total = pre_c[THREADS];
-  share = (total + p.workers - 1) / p.workers;
-  if (share < p.least) share = p.least;
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
-    p.head[0] = pre_u[THREADS];
-  }
-  begin = (long long)(blockIdx.x * WARPS + warp) * share;
-  if (begin < total) {
-    const int i = find_last(THREADS, begin, [&](int j) { return pre_c[j]; });
-    long long off = begin - pre_c[i];
-    unit_id = pre_u[i];
-    at.s = i * seg - 1;
-    do {
-      at.next_seq(p);
-      const long long units = (long long)at.q.tiles * p.Hkv, c = units * at.q.chunks;
-      if (off < c) break;
-      off -= c;
-      unit_id += units;
-    } while (at.s < p.S);
-    const int unit = (int)(off / at.q.chunks);
-    at.chunk = (int)(off - (long long)unit * at.q.chunks);
-    at.head = unit / at.q.tiles;
-    at.tile = unit - at.head * at.q.tiles;
-    unit_id += unit;
-  }
   }
   const int worker = blockIdx.x * WARPS + warp;
   const long long left0 = total - begin < share ? total - begin : share;
