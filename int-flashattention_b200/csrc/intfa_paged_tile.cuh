@@ -671,7 +671,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         };
         // The references are taken over as they are, and P is made with them in one go.  The sum of p = w / v_scale bounds every w (w <= sum p
         // times the largest v_scale); where that does not say that all w are below 2^15, or a row has no reference yet, the reference is
-        // looked for: in a unit's first chunk in 16 columns, then, if need be, in all.
+        // looked for: in a unit's first chunk in 16 columns, then, if need be, in all.  (A row without one is looked at whatever its sum says: all V
+        // scales so far were 0, and relative to nothing w may be too small for fp32.)
         uint64_t sum2, sum3;
         uint32_t pk[8 * NB];
         float total = 0.f;
@@ -749,7 +750,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
             f2_unpack(sum3, s2, s3);
             total = (s0 + s1) + (s2 + s3);
           }
-          if (find == 2 || !__any_sync(0xffffffffu, !(total < most) || (ref == -INFINITY && total > 0.f))) break;
+          if (find == 2 || !__any_sync(0xffffffffu, !(total < most) || (ref == -INFINITY && rel >= 0 && hi > -INFINITY))) break;
           find = 2;
         }
         if (!ok) break;
