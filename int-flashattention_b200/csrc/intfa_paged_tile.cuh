@@ -757,7 +757,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         const float d = ref - mref;
         const bool easy = ref == -INFINITY ? mref == -INFINITY && lo > -INFINITY : lo >= d - 60.f && hi <= d + 60.f;
         if (__all_sync(0xffffffffu, easy)) {
-          if (ref > -INFINITY) l = fmaf(total, ex2_approx(d), l);
+          l = ref > -INFINITY ? fmaf(total, ex2_approx(d), l) : l + total;       // (without a reference: 0, or NaN where no score is a number)
         } else {
           // p by itself: the scores once more
           float top = -INFINITY;
@@ -786,7 +786,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
             }
             if (pass == 0) {
               if (top > mref + 8.f || (mref == -INFINITY && top > -INFINITY)) {
-                l = mref == -INFINITY ? 0.f : l * ex2_approx(mref - top);
+                if (mref > -INFINITY) l *= ex2_approx(mref - top);         // (else 0, or NaN)
                 mref = top;
               }
             } else {

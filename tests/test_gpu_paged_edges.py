@@ -42,3 +42,37 @@ def test_values_of_zero_ahead_of_scores_far_below(D, zeros, path, pkg):
     for causal in (True, False):
         o = s.check(pkg, causal, torch.bfloat16, more=more)
         assert (o[:100].abs().amax(-1) > 0).all()
+
+
+@pytest.mark.parametrize("path", [1, 2])
+@pytest.mark.parametrize("v_zero", [False, True])
+@pytest.mark.parametrize("what", ["row", "chunks", "length"])
+def test_scores_that_are_not_numbers(what, v_zero, path, pkg):
+    """A query scale, or the K scales of a sequence's first tokens, are NaN: the rows that see them are, and so are their sums."""
+    s = base.Setup([100, 3, 70], [400, 303, 70], 8, 2, 128, 16, 1, seed=7)
+    s.path = path
+    bad = torch.zeros(173, 8, dtype=torch.bool, device="cuda")
+    if what == "row":
+        bad[[0, 5, 101, 110, 172], 3] = True
+        s.qs[bad] = float("nan")
+    else:
+        n = 64 if what == "chunks" else 400
+        for i in (0, 2):
+            for key in range(min(n, int(s.lens[i]))):
+                s.ks[int(s.table[i, key // 16]), 1, key % 16] = float("nan")
+        bad[:100, 4:] = True
+        bad[103:, 4:] = True
+    if v_zero:                               # zero V scales among them: the sums are made the general way
+        for i in (0, 2):
+            s.vs[int(s.table[i, 0]), :, 3:7] = 0
+            s.vs[int(s.table[i, 0]), :, 0] = 0
+    want, wlse, A, B = O.attention(s.q8, s.qs, s.kc, s.vc, s.ks, s.vs, s.table, s.lens, s.cu, True, s.scale)
+    o, lse = s.call(pkg, return_lse=True)
+    assert torch.equal(torch.isnan(wlse), bad) and torch.equal(torch.isnan(want).all(-1), bad)
+    assert torch.equal(torch.isnan(lse), bad)
+    assert torch.equal(torch.isnan(o), bad[..., None].expand_as(o))
+    # The others to the rounding of any row.  (Not bit for bit what they are without their neighbours' NaN: on tiles the 32 rows of a warp look for new
+    # references together, and w, relative to another one, is rounded elsewhere.)
+    assert ((o.double() - want).abs() <= s.tolerance(want, A, B))[~bad].all()
+    assert ((lse.double() - wlse).abs() <= 2.0 ** -16 * 64)[~bad].all()
+    pkg.check_status()
