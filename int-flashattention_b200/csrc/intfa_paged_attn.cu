@@ -315,6 +315,9 @@ __device__ __forceinline__ void write_part(float* part, float* ml, int stride, c
 }
 
 // One chunk.  sK, sV: its rows in shared memory; sS: its K scales, then the logarithms of its V scales; last[n]: the last key of the chunk that row n*8 + g sees.
+// MASKED: not all rows see all keys, or the K scales say kNoKey.
+constexpr float kNoKey = -INFINITY;               // in place of the K scale: no key, its page lies outside the cache (the V scale is 0)
+__device__ const float no_key = kNoKey;
 template <int D, int NT, int G, bool MASKED>
 __device__ __forceinline__ void chunk_step(RowState<D, NT>& st, const uint32_t (&q)[D / 64][NT][4], const float (&qs)[NT], const int (&last)[NT],
                                            uint32_t sK, uint32_t sV, uint32_t sS) {
@@ -348,8 +351,15 @@ __device__ __forceinline__ void chunk_step(RowState<D, NT>& st, const uint32_t (
     const uint64_t ks = lds_u64(sS + (kt * 8 + 2 * t) * 4);
     lv[kt] = lds_u64(sS + (G + kt * 8 + 2 * t) * 4);
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n) {
       x[n][kt] = f2_mul(f2_add(f2_packu(d[n / 2][(n & 1) * 2], d[n / 2][(n & 1) * 2 + 1]), less), f2_mul(ks, f2_pack(qs[n], qs[n])));
+      if (MASKED) {
+        float x0, x1, k0, k1;
+        f2_unpack(x[n][kt], x0, x1);
+        f2_unpack(ks, k0, k1);
+        x[n][kt] = f2_pack(k0 == kNoKey ? -INFINITY : x0, k1 == kNoKey ? -INFINITY : x1);
+      }
+    }
   }
   uint32_t b[NT][KT];
 #pragma unroll
@@ -591,7 +601,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_const
       for (int i = 0; i < M; ++i) {
         if (page[i] < 0 || page[i] >= p.pages) {
           if (p.status) atomicCAS(p.status, 0, kStatusBadIndex);
-          page[i] = 0;
+          page[i] = p.pages;                                 // (one past the last: the copies are zeros)
         }
         const int pg = __shfl_sync(0xffffffffu, page[i], (lane << p.box_log) & 31);
         if (M == 1 || (lane << p.box_log) >> 5 == i) first_page = pg;
@@ -612,9 +622,9 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_const
 #pragma unroll
       for (int i = 0; i < M; ++i) {
         const int key = key0 + i * 32 + lane;
-        const bool in = key < ahead.q.keys;
+        const bool in = key < ahead.q.keys && page[i] != p.pages;
         const long long blk = (key & ((1 << p.page_log) - 1)) >> p.block_log;
-        cp_async4(x + (i * 32 + lane) * 4, p.ks + (in ? page[i] * p.ksP + head * p.ksH + blk * p.ksB : 0), in);
+        cp_async4(x + (i * 32 + lane) * 4, in ? p.ks + (page[i] * p.ksP + head * p.ksH + blk * p.ksB) : &no_key, true);
         cp_async4(x + (G + i * 32 + lane) * 4, p.vs + (in ? page[i] * p.vsP + head * p.vsH + blk * p.vsB : 0), in);
       }
       if (fresh) {
@@ -665,11 +675,15 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_const
     if (!ok) break;
     const uint32_t kv = sKV + stage * 2 * C::KV, x = sX + stage * C::EXTRA;
     // the logarithms of the V scales, once for all rows
+    bool zero = false;
 #pragma unroll
     for (int i = 0; i < M; ++i) {
       const uint32_t at_v = x + (G + i * 32 + lane) * 4;
-      asm volatile("st.shared.f32 [%0], %1;" ::"r"(at_v), "f"(log2_approx(lds_f(at_v))) : "memory");
+      const float v = lds_f(at_v);
+      zero |= v == 0.f;
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(at_v), "f"(log2_approx(v)) : "memory");
     }
+    zero = __any_sync(0xffffffffu, zero);                    // (among them may be keys that are not there)
     __syncwarp();
     if (!open) {
       open = true;
@@ -701,7 +715,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_const
       for (int o = 16; o > 0; o >>= 1) full_keys = min(full_keys, __shfl_xor_sync(0xffffffffu, full_keys, o));
     }
     const int key0 = at.chunk * G;
-    if (key0 + G <= full_keys) {
+    if (key0 + G <= full_keys && !zero) {
       chunk_step<D, NT, G, false>(st, q, qs, last, kv, kv + C::KV, x);
     } else {
       int rel[NT];

@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
           next = look_up(c + 1);
           if (bad_page(page)) {
             if (p.status) atomicCAS(p.status, 0, kStatusBadIndex);
-            page = 0;
+            page = p.pages;                                    // (one past the last: the copies are zeros, and the scales leave them out)
           }
           const int key0 = c * G, full = max(0, min(boxes, (u.keys - key0 + box_rows - 1) >> p.box_log));
           const int slot = (key0 + lane * box_rows) & page_mask;
@@ -510,9 +510,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
             na[i] = 0.f;
             nb[i] = 1.f;
             if (c < u.c1 && key < u.keys) {
-              const long long pg = bad_page(page[i]) ? 0 : page[i];
-              na[i] = ks[pg * p.ksP + blk * p.ksB];
-              nb[i] = vs[pg * p.vsP + blk * p.vsB];
+              nb[i] = -INFINITY;                               // a page outside the cache: the key does not count
+              if (!bad_page(page[i])) {
+                na[i] = ks[page[i] * p.ksP + blk * p.ksB];
+                nb[i] = vs[page[i] * p.vsP + blk * p.vsB];
+              }
             }
           }
         };
@@ -534,11 +536,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
           float lo = INFINITY, hi = -INFINITY;
 #pragma unroll
           for (int i = 0; i < N; ++i) {
-            const float l = log2_approx(b[i]);
+            const bool gap = b[i] == -INFINITY;                // logarithm -inf, reciprocal 0: neither w nor p of it
+            const float l = gap ? -INFINITY : log2_approx(b[i]);
             sc[i * 32 + lane] = a[i];
             sc[G + i * 32 + lane] = l;
             sc[2 * G + i * 32 + lane] = 1.0f / b[i];
-            if (c * G + i * 32 + lane < u.keys) {
+            if (c * G + i * 32 + lane < u.keys && !gap) {
               const bool odd = !(fabsf(l) < 120.f);            // zero, infinite, NaN, next to them (1/b is not normal): the general way
               lo = fminf(lo, odd ? -INFINITY : l);
               hi = fmaxf(hi, odd ? INFINITY : l);
@@ -778,7 +781,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                   float x = (__uint_as_float(o[k + e]) - kMagicF) * (aa[e] * qs);
-                  if (b * 16 + k + e > rel) x = -INFINITY;
+                  const int at = b * 16 + k + e;
+                  if (at > rel || (sc[2 * G + at] == 0.f && sc[G + at] == -INFINITY)) x = -INFINITY;
                   if (pass == 0) top = fmaxf(top, x);
                   else sum += ex2_approx(x - base);
                 }

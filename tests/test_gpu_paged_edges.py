@@ -76,3 +76,75 @@ def test_scores_that_are_not_numbers(what, v_zero, path, pkg):
     assert ((o.double() - want).abs() <= s.tolerance(want, A, B))[~bad].all()
     assert ((lse.double() - wlse).abs() <= 2.0 ** -16 * 64)[~bad].all()
     pkg.check_status()
+
+
+def without(s, seq, columns):
+    """The same rows over a cache in which the tokens of those columns of a sequence's table are not there."""
+    t = base.Setup.__new__(base.Setup)
+    t.__dict__.update(s.__dict__)
+    t.table, t.lens = s.table.clone(), s.lens.clone()
+    page, width = s.kc.shape[2], s.table.shape[1]
+    keep = [c for c in range(width) if c not in columns]
+    t.table[seq, :len(keep)] = s.table[seq, keep]
+    t.lens[seq] -= page * len(columns)
+    return t
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("page,block", [(8, 1), (16, 4), (64, 64)])
+@pytest.mark.parametrize("news,one,path", [([1, 1, 1], True, 1), ([1, 1, 1], False, 1), ([3, 2, 4], False, 1), ([70, 3, 130], False, 2), ([3, 1, 2], False, 2)])
+def test_keys_of_pages_outside_the_cache_do_not_count(news, one, path, D, page, block, pkg):
+    lens = [6 * page + 5 + news[0], 0, 11 * page + news[2]]
+    s = base.Setup(news, lens, 8, 2, D, page, block, one=one, seed=page, garbage=False)
+    s.path = path
+    s.check(pkg)
+    for seq, columns, to in ((0, [0], -1), (0, [3], s.kc.shape[0]), (2, [1, 2, 7], 1 << 30), (2, [10], -(1 << 31)), (0, list(range(6)), s.kc.shape[0])):
+        want = without(s, seq, columns)
+        was = s.table.clone()
+        s.table[seq, columns] = to
+        for causal in (True, False):
+            got = s.call(pkg, causal, return_lse=True)
+            with pytest.raises(pkg.IntfaError, match="outside its table"):
+                pkg.check_status()
+            want.check(pkg, causal, got=got)
+        # nothing is taken from any page that is not in the tables
+        others = torch.ones(s.kc.shape[0], dtype=torch.bool, device="cuda")
+        others[s.table[(s.table >= 0) & (s.table < s.kc.shape[0])].long()] = False
+        keep = [x.clone() for x in (s.kc, s.vc, s.ks, s.vs)]
+        s.kc[others], s.vc[others], s.ks[others], s.vs[others] = 127, -127, float("nan"), float("inf")
+        again = s.call(pkg, False, return_lse=True)
+        assert torch.equal(again[0], got[0]) and torch.equal(again[1], got[1])
+        for x, y in zip((s.kc, s.vc, s.ks, s.vs), keep):
+            x.copy_(y)
+        with pytest.raises(pkg.IntfaError, match="outside its table"):
+            pkg.check_status()
+        s.table.copy_(was)
+
+
+@pytest.mark.parametrize("path", [1, 2])
+@pytest.mark.parametrize("one", [True, False])
+def test_a_sequence_without_a_page_in_the_cache(one, path, pkg):
+    """Rows that see no key that is there: zero, and no sum."""
+    s = base.Setup([1, 1], [100, 40], 8, 2, 128, 16, 1, one=one)
+    s.path = path
+    good = s.call(pkg)
+    s.table[0] = -1
+    o, lse = s.call(pkg, return_lse=True)
+    assert (o[0] == 0).all() and (lse[0] == -math.inf).all() and torch.equal(o[1], good[1])
+    with pytest.raises(pkg.IntfaError, match="outside its table"):
+        pkg.check_status()
+
+
+@pytest.mark.parametrize("path", [1, 2])
+def test_values_of_zero_next_to_a_page_outside_the_cache(path, pkg):
+    """Zero V scales, for which p is summed up by itself on tiles, in the chunk of a page that is not there: its keys count for nothing, the zeros' do."""
+    s = base.Setup([40, 2], [170, 50], 8, 2, 128, 16, 1, garbage=False)
+    s.path = path
+    for col in (0, 2, 5):
+        s.vs[int(s.table[0, col]), :, ::3] = 0
+    want = without(s, 0, [1, 6])
+    s.table[0, 1] = s.table[0, 6] = s.kc.shape[0]
+    got = s.call(pkg, return_lse=True)
+    with pytest.raises(pkg.IntfaError, match="outside its table"):
+        pkg.check_status()
+    want.check(pkg, got=got)
