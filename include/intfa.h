@@ -291,7 +291,8 @@ typedef struct IntfaPagedCache {
  * began before this call keeps the larger of its old scale and the new tokens', and where that grew its older codes become
  * rint(code * (old/new)).  Rows behind the last sequence, and those of a sequence with seq_lens 0
  * (padding), are left out.  Two sequences may not append to the same page in one call.
- * q [tokens, H, D] if not NULL: rotated alike and quantised per row into q8 [tokens, H, D], q_scale [tokens, H] (both contiguous).
+ * q [tokens, H, D] if not NULL: rotated alike and quantised per row into q8 [tokens, H, D], q_scale [tokens, H] (both contiguous); zeros for a
+ * token whose position or page is outside, rows that are left out stay as they were.
  */
 typedef struct IntfaAppendParams {
   IntfaPagedCache cache;

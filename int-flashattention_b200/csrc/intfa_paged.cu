@@ -169,6 +169,12 @@ __device__ __forceinline__ void token_rows(const AppendJob& p, long long cta, in
     const T* xq = row_of(0);
     int8_t* q8 = p.q8 + (token * hq + row0) * D;
     float* qs = p.qs + token * hq + row0;
+    if (in && to.own && !goes) {           // refused: zeros
+      for (int i = 0; row0 + i < hq; i += per_token) {
+        *reinterpret_cast<uint2*>(q8 + i * D + at.a) = *reinterpret_cast<uint2*>(q8 + i * D + at.b) = make_uint2(0u, 0u);
+        if (threadIdx.x % LPR == 0) qs[i] = 0.f;
+      }
+    }
 #pragma unroll 1
     for (; g < pairs_q; ++g) {
       take(g, r0, r1);

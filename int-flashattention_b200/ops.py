@@ -226,7 +226,8 @@ def append_int8_paged(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq
     Where a block began in an earlier call its scale becomes the larger of the old one and the new tokens', and the codes of its older
     tokens follow.  Tokens behind the last sequence, and those of a sequence with seq_lens 0 (padding), are left out.  Two sequences may
     not append to one page in a call.  With q [tokens, query heads, D]: the same tokens' queries,
-    rotated and quantised per token; returns (q8, q_scale [tokens, heads]) as attention_int8_paged takes them."""
+    rotated and quantised per token; returns (q8, q_scale [tokens, heads]) as attention_int8_paged takes them: zeros for a token whose position or page lies
+    outside its table or cache (check_status() tells), not set for one that is left out."""
     return (_native_mod or _native()).append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_seqlens, q, table, interleaved)
 
 

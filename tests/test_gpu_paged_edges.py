@@ -7,6 +7,7 @@ import math
 import pytest
 import torch
 
+import test_gpu_paged_append as append
 import test_gpu_paged_attention as base
 from oracle import paged_oracle as O
 
@@ -148,3 +149,37 @@ def test_values_of_zero_next_to_a_page_outside_the_cache(path, pkg):
     with pytest.raises(pkg.IntfaError, match="outside its table"):
         pkg.check_status()
     want.check(pkg, got=got)
+
+
+@pytest.mark.parametrize("block", [1, 8, 64])
+@pytest.mark.parametrize("H,Hkv,D", [(2, 2, 64), (40, 8, 128), (3, 1, 256)])
+@pytest.mark.parametrize("what", ["page", "width", "length", "rotation"])
+def test_queries_of_refused_tokens_are_zero(what, H, Hkv, D, block, pkg):
+    """With scale zero; the other sequences' as ever, and padding, which is left out."""
+    s = append.Setup([5, 2, 60], [70, 2, 70], H, Hkv, D, 64, block)
+    cs = pkg.rotary_table(100, D, device="cuda")
+    refused = torch.zeros(67, dtype=torch.bool, device="cuda")
+    if what == "page":                       # tokens 64 .. 69 of the last sequence
+        s.table[2, 1] = s.kc.shape[0]
+        refused[67 - 6:] = True
+    elif what == "width":
+        s.lens[0] = s.table.shape[1] * 64 + 5
+        refused[:5] = True
+    elif what == "length":
+        s.lens[0] = -4
+        refused[:5] = True
+    else:
+        cs = pkg.rotary_table(66, D, device="cuda")        # positions 65 .. 69 and 10 .. 69
+        refused[1:5] = True
+        refused[67 - 4:] = True
+    pos = torch.cat([torch.arange(65, 70), torch.arange(2), torch.arange(10, 70)]).cuda()
+    x = O.turn(s.q.float(), pkg.rotary_table(100, D, device="cuda")[pos][:, None], False)
+    qs = O.scale_of(O.absmax(x))
+    q8 = O.codes(x, qs[..., None])
+    q8[refused], qs[refused] = 0, 0.0
+    old = torch.full_like(q8, 77), torch.full_like(qs, 77.0)             # (what a new tensor is likely to hold)
+    del old
+    got = s.run(pkg, cs)
+    with pytest.raises(pkg.IntfaError, match="outside its table"):
+        pkg.check_status()
+    assert torch.equal(got[0], q8) and torch.equal(got[1], qs)
