@@ -177,10 +177,13 @@ struct DecodeCfg {
   static constexpr int OFF_BAR = OFF_EXTRA + WARPS * NS * EXTRA;
   static constexpr int OFF_PRE = OFF_BAR + WARPS * NS * 8;              // [threads + 1] chunks (long long) and units (int) before a thread's sequences
   static constexpr int OFF_MISC = OFF_PRE + ((32 * WARPS + 1) * 12 + 15) / 16 * 16;
+  static constexpr int OFF_SUMS = OFF_EXTRA;                            // [warps] chunks and units (long long) of a warp's sequences, ahead of the first load
+  static_assert(OFF_SUMS >= WARPS * NS * 2 * KV, "the sums lie outside the ring: the async proxy's copies into it know nothing of plain stores");
   static constexpr int SMEM = OFF_MISC + 32 + 1024;
   static constexpr int MERGE = (WARPS + 1) * RT * ((D + 4) + 4) * 4;    // (over the ring, when it is done with)
   static_assert(MERGE <= OFF_EXTRA, "merge");
   static_assert(EXTRA % 16 == 0, "alignment");
+  static_assert(WARPS * 16 <= WARPS * NS * EXTRA, "sums");
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
@@ -525,7 +528,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_const
           u += y;
         }
       }
-      long long* sums = reinterpret_cast<long long*>(smem);      // (the ring is not in use yet)
+      long long* sums = reinterpret_cast<long long*>(smem + C::OFF_SUMS);
       if (lane == 31) {
         sums[2 * warp] = c;
         sums[2 * warp + 1] = u;
