@@ -311,6 +311,7 @@ __global__ void __launch_bounds__(kThreads, 2) append_runs_kernel(const AppendJo
       m = max_nan(m, absmax16(x[k]));
     }
     const float now = max_nan(was, scale_of(row_max<32>(m)));
+    __syncwarp();                          // (all lanes have read the old scale)
     if (lane == 0) *sc = now;
 #pragma unroll
     for (int k = 0; k < kRounds; ++k) {

@@ -183,3 +183,18 @@ def test_queries_of_refused_tokens_are_zero(what, H, Hkv, D, block, pkg):
     with pytest.raises(pkg.IntfaError, match="outside its table"):
         pkg.check_status()
     assert torch.equal(got[0], q8) and torch.equal(got[1], qs)
+
+
+@pytest.mark.parametrize("D,block", [(64, 32), (128, 16), (256, 8), (128, 64)])
+def test_scales_that_grow_with_every_token(D, block, pkg):
+    """Each token is larger than all before it, so that every append reads its block's scale, raises it and moves all older codes."""
+    S, Hkv = 40, 3
+    s = append.Setup([1] * S, [1 + i % 5 for i in range(S)], 0, Hkv, D, 64, block)
+    s.table[s.table < 0] = 0
+    for i in range(block + 3):
+        s.k = (torch.randn(S, Hkv, D, device="cuda", generator=s.g) * 1.3 ** i).half()
+        s.v = (torch.randn(S, Hkv, D, device="cuda", generator=s.g) * 1.3 ** (i % 9)).half()
+        s.check(pkg, cu=None)
+        s.lens += 1
+        if int(s.lens.max()) > 64:             # (its only page is full)
+            break
