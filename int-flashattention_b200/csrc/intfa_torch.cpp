@@ -6,6 +6,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -667,6 +668,11 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const bool per_batch = p0.dim() == 2 && !packed;
     if (!(p0.dim() == 1 && p0.size(0) == N) && !(per_batch && p0.size(0) == B && p0.size(1) == N))
       bad_shape("positions", packed ? "[tokens]" : "[N] or [B,N]", p0);
+    if (c10::GradMode::is_enabled())
+      for (const at::Tensor* t : {&q0, &k0, &t0})
+        if (t->defined() && t->requires_grad())
+          raise(PyExc_ValueError, "rotary has no autograd and an input requires grad: call it under torch.no_grad(), or from a torch.autograd.Function "
+                                  "(the gradient of q and k is rotary of the other `inverse`)");
     same_device({&q0, &k0, &t0, &p0});
     const c10::Device dev = q0.device();
     c10::cuda::CUDAGuard guard(dev);

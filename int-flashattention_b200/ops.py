@@ -209,7 +209,8 @@ def rotary(q, k, table, positions, *, interleaved=False, inverse=False):
     (j, j + rot_dim/2), or (2j, 2j+1) where interleaved, becomes (a c - b s, b c + a s) with (c, s) = table[position, j]
     (rotary_table).  q [B,H,N,D] with positions [N] or [B,N], or packed [tokens, heads, D] with positions [tokens]; k likewise with
     heads of its own.  float16, bfloat16 or float32; computed in fp32 and rounded once.  inverse=True is the gradient of the call
-    with inverse=False (no autograd here): the rotation back.  Returns q', or (q', k')."""
+    with inverse=False: the rotation back.  No autograd: where gradients are recorded, inputs that require them are refused; call it under
+    torch.no_grad() or from the forward and backward of a torch.autograd.Function.  Returns q', or (q', k')."""
     return (_native_mod or _native()).rotary(q, k, table, positions, interleaved, inverse)
 
 
