@@ -80,7 +80,7 @@ struct PParams {
   int tile_tokens, unit_tokens;                   // 128-row tiles: whole tokens in one, in a unit; 0: packed RT rows
   float* part; float* part_ml;                    // [2*workers][RT][D]; [2*workers][RT]{m, mw, l, -}
   UnitPart* units; long long max_units;           // [max_units]
-  int* head;                                      // {units}
+  int* head;                                      // {units}; packed rows only
   int* status;
 };
 
@@ -974,7 +974,6 @@ Plan make_plan(const IntfaPagedParams* a, int sms) {
     take((size_t)2 * pl.ctas * rows * c.D * 4);
     pl.off_ml = take((size_t)2 * pl.ctas * rows * 16);
     pl.off_units = take((size_t)pl.max_units * sizeof(UnitPart));
-    pl.off_head = take(32);
     return pl;
   }
   // Rows a tile: 16 where an average sequence has more than 8 rows a K/V head (up to 8 of them cost half in tiles of 8, more twice the bytes)
@@ -1136,7 +1135,7 @@ int paged_attention(const IntfaPagedParams* a, cudaStream_t stream) {
   p.part_ml = reinterpret_cast<float*>(ws + pl.off_ml);
   p.units = reinterpret_cast<UnitPart*>(ws + pl.off_units);
   p.max_units = pl.max_units;
-  p.head = reinterpret_cast<int*>(ws + pl.off_head);
+  p.head = pl.tiles ? nullptr : reinterpret_cast<int*>(ws + pl.off_head);
   p.status = a->status;
   p.tile_tokens = 0;
   p.chunk_log = p.box_log = 5;

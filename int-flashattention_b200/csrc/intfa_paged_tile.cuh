@@ -335,10 +335,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         ++seq;
         if (u.c0 < 0) break;
       }
-      if (lane == 0) {
-        p.units[blockIdx.x] = part;
-        if (blockIdx.x == 0) p.head[0] = gridDim.x;
-      }
+      if (lane == 0) p.units[blockIdx.x] = part;
     } else if (warp == 0) {
       // ------------------------------------------------------------------ TMA
       uint32_t kit = 0, vit = 0, uit = 0;                      // chunks of K, of V, units so far
