@@ -198,3 +198,81 @@ def test_scales_that_grow_with_every_token(D, block, pkg):
         s.lens += 1
         if int(s.lens.max()) > 64:             # (its only page is full)
             break
+
+
+@pytest.mark.parametrize("path", [1, 2])
+@pytest.mark.parametrize("cu,valid", [([0, 160, 100], [0, 160, 160]), ([0, 100, 200], [0, 100, 100]), ([-4, 1, 160], [1, 1, 160]), ([100, 0, 160], [0, 0, 160]),
+                                      ([160, 160, 160], None), ([0, 0, 160], None), ([-9, -3, 70], [70, 70, 70]), ([1 << 30, 0, 0], [0, 0, 0])])
+def test_ends_that_cannot_be(cu, valid, path, pkg):
+    """Reported; the rows of the sequences whose ends can be are written as ever, no others."""
+    s = base.Setup([100, 60], [200, 200], 4, 2, 64, 16, 1, garbage=False)
+    s.path = path
+    s.cu = torch.tensor(cu, dtype=torch.int32, device="cuda")
+    whole = torch.full((170, 4, 64), 9.0, device="cuda", dtype=torch.float16)
+    out = whole[5:165]
+    _, lse = s.call(pkg, out=out, return_lse=True)
+    if valid is None:
+        assert pkg.check_status() == 0
+    else:
+        with pytest.raises(pkg.IntfaError, match="outside its table"):
+            pkg.check_status()
+        s.cu = torch.tensor(valid, dtype=torch.int32, device="cuda")
+    want, wlse, A, B = O.attention(s.q8, s.qs, s.kc, s.vc, s.ks, s.vs, s.table, s.lens, s.cu, True, s.scale)
+    rows = ~torch.isnan(wlse[:, 0])
+    assert int(rows.sum()) == int(s.cu[2] - s.cu[0])
+    assert ((out.double() - want).abs() <= s.tolerance(want, A, B))[rows].all()
+    assert ((lse.double() - wlse).abs() <= 2.0 ** -16 * 64)[rows].all()
+    assert (out[~rows] == 9).all() and (whole[:5] == 9).all() and (whole[165:] == 9).all()
+
+
+@pytest.mark.parametrize("block", [1, 8])
+@pytest.mark.parametrize("what", ["rotation", "ends"])
+def test_append_writes_only_what_it_may(what, block, pkg):
+    """Positions past the rotary table, and ends past the rows: with a scale a token the tokens that are inside are written, with longer blocks none of the
+    run that is not inside as a whole; every other slot and scale stays."""
+    s = append.Setup([3, 2], [3, 18], 2, 2, 64, 16, block)
+    cs = pkg.rotary_table(64, 64, device="cuda")
+    before = [x.clone() for x in s.state()]
+    if what == "rotation":
+        cs = pkg.rotary_table(1, 64, device="cuda")
+        s.lens[1] = 0
+        inside = [(0, 0)]                                    # (sequence, position): the first token
+    else:
+        s.cu[2], s.lens[1] = 9, 8                            # positions 2 .. 7, of which rows 3 and 4 are here
+        inside = [(0, 0), (0, 1), (0, 2), (1, 2), (1, 3)]
+    if block > 1:
+        inside = [x for x in inside if what == "ends" and x[0] == 0]
+    s.run(pkg, cs)
+    with pytest.raises(pkg.IntfaError, match="outside its table"):
+        pkg.check_status()
+    slots = torch.zeros(s.kc.shape[0], 16, dtype=torch.bool, device="cuda")
+    for seq, pos in inside:
+        slots[int(s.table[seq, pos // 16]), pos % 16] = True
+    scales = slots.view(-1, 16 // block, block).any(-1)
+    for now, was, there in zip(s.state(), before, (slots, slots, scales, scales)):
+        same = (now == was).flatten(3).all(-1) if now.dim() == 4 else now == was
+        assert same.transpose(1, 2)[~there].all()
+        assert not same.transpose(1, 2)[there].any() if now.dim() == 4 else True
+    rows = [0, 1, 2, 3, 4] if what == "ends" else [0]
+    x = s.v[rows[:len(inside)]].float()
+    if block == 1:
+        for i, (seq, pos) in enumerate(inside):
+            page = int(s.table[seq, pos // 16])
+            scale = O.scale_of(O.absmax(x[i]))
+            assert torch.equal(s.vs[page, :, pos % 16], scale) and torch.equal(s.vc[page, :, pos % 16], O.codes(x[i], scale[:, None]))
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("news,lens", [([1] * 15 + [300], [40 + 31 * i for i in range(15)] + [420]),          # a step: single tokens and a chunk of a prompt
+                                       ([500] + [1] * 3, [500, 900, 1, 33]), ([1, 2, 0, 1, 700, 1, 5, 1], [800, 2, 5, 0, 900, 64, 5, 129]),
+                                       ([1] * 60 + [90, 1], [1 + 17 * i for i in range(60)] + [90, 1])])
+def test_single_tokens_and_chunks_in_one_call(news, lens, D, pkg):
+    """Whatever path the rule on sizes takes: it is one of the two, bit for bit, and right."""
+    s = base.Setup(news, lens, 8, 2, D, 16, 4, seed=D)
+    for causal in (True, False):
+        o = s.check(pkg, causal)
+        both = []
+        for s.path in (1, 2):
+            both.append(s.check(pkg, causal))
+        s.path = 0
+        assert any(torch.equal(o, x) for x in both)
