@@ -625,9 +625,10 @@ __global__ void __launch_bounds__(32 * WARPS, 1) paged_kernel(const __grid_const
 #pragma unroll
       for (int i = 0; i < M; ++i) {
         const int key = key0 + i * 32 + lane;
-        const bool in = key < ahead.q.keys && page[i] != p.pages;
+        const bool gap = page[i] == p.pages, in = key < ahead.q.keys && !gap;
         const long long blk = (key & ((1 << p.page_log) - 1)) >> p.block_log;
-        cp_async4(x + (i * 32 + lane) * 4, in ? p.ks + (page[i] * p.ksP + head * p.ksH + blk * p.ksB) : &no_key, true);
+        const float* ks = p.ks + (in ? page[i] * p.ksP + head * p.ksH + blk * p.ksB : 0);
+        cp_async4(x + (i * 32 + lane) * 4, gap ? &no_key : ks, in || gap);
         cp_async4(x + (G + i * 32 + lane) * 4, p.vs + (in ? page[i] * p.vsP + head * p.vsH + blk * p.vsB : 0), in);
       }
       if (fresh) {
