@@ -1,9 +1,10 @@
 // New tokens into a paged int8 cache: keys rotated by their positions, keys and values quantised with one scale for each block of
 // `block` tokens and head, queries of the same tokens rotated and quantised per token, all in one launch.
 //
-// Reads 2 bytes a value, writes 1 (18 700 tokens of 32 + 8 + 8 heads x 128: 345 MB, 53 us at the measured copy rate): 85 us, bound by the issue of
-// instructions (72 % of the slots: 300 for a warp's 16 values a lane, of them 126 the rotation, whose products are rounded one by one, and 80 the
-// proof that the codes are those of a division).  The few tokens of a decode step: launch and latency, 5.4 us in a graph.
+// Reads 2 bytes a value, writes 1 (18 048 tokens of 32 + 8 + 8 heads x 128: 345 MB, 53 us at the measured copy rate): 85 us, bound by the issue of
+// instructions (72 % of the slots: 300 for a warp's 16 values a lane; 126 with the rotation, of which its products and sums, each rounded by
+// itself, are 48, and 80 with the proof that the codes are those of a division).  Three CTAs an SM leave 80 registers a thread, and 32 bytes
+// spill (40 where pairs are neighbours).  The few tokens of a decode step: launch and latency, 5.4 us in a graph.
 //   block = 1   a row (one head of one token) is quantised by the lanes that loaded it; a CTA takes one token, or a few of few heads
 //   block > 1   a warp (short blocks: 12 us for 40 sequences of up to 200 tokens, where CTAs took 19) or a CTA takes what a sequence adds to one
 //               block, for some heads: the largest magnitudes first, then the codes.  A block that
@@ -330,6 +331,7 @@ __global__ void __launch_bounds__(kThreads, 2) append_runs_kernel(const AppendJo
 }
 
 // Longer blocks: a CTA takes them, some heads at a time; maxima first, then the rows once more for the codes.  CTAs from units * groups on: q.
+// 40 sequences of up to 200 tokens, 32 + 8 + 8 heads x 128, blocks of 64: 50 us (short blocks of 16: 34; 97 MB, 15 us): rows are read and rotated twice.
 template <typename T, int D, int SPIN>
 __global__ void __launch_bounds__(kThreads, 2) append_blocks_kernel(const AppendJob p, int units, int groups, int heads_cta, int tokens_cta, int per_token) {
   constexpr int LPR = D / 16, SLOTS = kThreads / LPR;

@@ -4,7 +4,7 @@
 //
 // Reads K and V once (64 sequences of up to 8192 keys, 8 heads x 128: 703 MB, 109 us at the measured copy rate, 118 to 133 here): bound by HBM.  One
 // sequence of 131 072 keys 41.6 and 57: ten microseconds are the start, the end and the combination.  Short calls are all that, 6.4 in clusters.
-// 16 rows a K/V head at 64 channels (91 MB) 14.1 and 33.6: the latency of two warps a scheduler, whose exp2 are per row and key.
+// 16 rows a K/V head at 64 channels (91 MB) 14.1 and 34.0: the latency of two warps a scheduler, whose exp2 are per row and key.
 //
 // Work.  A unit is (sequence, K/V head, tile of RT = 8 NT rows); the rows of all query heads that share the K/V head are packed into it, so
 // that K and V are read once for all of them.  Its keys are cut into chunks of G = 32, 64 at head dim 64.  The chunks of all units in a row are
@@ -950,6 +950,9 @@ struct Plan {
 // channels 32 rows 39.1 / 36.4 and 96.9 / 71.3.  Few rows in all do not fill the GPU with tiles: one sequence of 8 heads, at 64 channels 256 rows
 // 20.4 / 21.7 and 31.3 / 25.8, four of one head and 512 rows 16.0 / 23.1 and 24.9 / 32.0; at 128 channels 128 rows 16.5 / 18.0 and 25.4 / 29.6, 256
 // rows 21.9 / 28.8 and 42.8 / 29.0; at 256 channels 64 rows 17.5 / 18.5 and 31.5 / 31.3, 128 rows 25.8 / 21.7 and 52.7 / 37.3.
+// The rule goes by the rows of an average sequence alone.  So it is off where few sequences have many keys (256 rows at 64 channels above: packed) and where
+// a call mixes row counts, which all take one path (32 / 8 heads x 128: 63 single rows with up to 8192 keys and 512 rows with 4608 in one call 349 / 441,
+// as two calls 117 and 79).
 bool takes_tiles(const IntfaPagedParams* a) {
   if (a->debug_path) return a->debug_path == 2;
   const double rows = (double)a->tokens * (a->H / a->cache.H_kv) / a->cache.S;          // of an average sequence and K/V head
@@ -1151,7 +1154,8 @@ int paged_attention(const IntfaPagedParams* a, cudaStream_t stream) {
   // Warps and chunks a ring, as timed with 64 sequences of one row and up to 8192 keys (NT 1), 32 of 4 rows, 4 query heads a K/V head, and
   // up to 4097 (NT 2), in us.  64 channels: 71.3 (12 warps with 2 chunks 73.1; chunks of 32 keys, 8 with 5: 92.8), NT 2 33.5 (7 with 3 37.8, 6 with 3
   // 39.4, 9 with 2 42; chunks of 32 keys, 8 with 4: 38.6).  128 channels: 118 (chunks of 64 keys, 6 with 2: 124, 4 with 3: 125), NT 2 49.8 (6 with 3
-  // 57.8, 4 with 5 63.7).  256 channels: what fits registers and shared memory.
+  // 57.8, 4 with 5 63.7).  256 channels: what fits shared memory (32 of one row 75, 55 at the copy rate; 32 of 4 rows 79 and 27: 372 bytes of its
+  // accumulators spill, 78 in the cluster form).
   switch (c.D) {
     case 64: return pl.NT == 2 ? run<64, 2, 8, 2, 64>(a, pl, p, stream) : run<64, 1, 8, 3, 64>(a, pl, p, stream);
     case 128: return pl.NT == 2 ? run<128, 2, 8, 2>(a, pl, p, stream) : run<128, 1, 8, 3>(a, pl, p, stream);

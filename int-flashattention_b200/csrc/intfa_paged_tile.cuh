@@ -6,8 +6,10 @@
 // contiguous shares; parts of units that are cut go to scratch and combine_tiles_kernel adds them up, as in the kernel for few rows.
 //
 // Four sequences of up to 512 new rows, 32 / 8 heads x 128, and up to 8192 keys: 4 * rows * keys * D operations, 94 us at the fp16 rate of P V and S
-// (70 with S at the int8 rate, 67 for the exp2 alone), 217 here; six prompts of up to 4096 306 and 707.  Bound by the latency of the chain from
-// S to P (scores, exponents, exp2, sums, P) with two softmax warps a scheduler: issue slots 47 %, exp2 40 %, tensor pipe 31 %.
+// (70 with S at the int8 rate, 67 for the exp2 alone), 217 here; six prompts of up to 4096 306 and 695.  Bound by the latency of the chain from
+// S to P (scores, exponents, exp2, sums, P) with two softmax warps a scheduler: issue slots 47 %, exp2 40 %, tensor pipe 31 %.  Eight sequences of up to
+// 256 rows and 4096 keys: 64 channels, 32 / 8 heads 19 and 115, 256 channels, 16 / 4 heads 38 and 122 (one tile: four of the eight softmax warps have
+// no rows).  Spilled: 32 bytes at 128 channels, 40 at 256, 12 at 64.
 //
 // 512 threads:
 //   warp 0       TMA: Q once per unit (heads x tokens boxes), K and V pages of 8 rows and more each
@@ -19,9 +21,10 @@
 // TMEM: two S buffers of each tile, P (fp16) over the scores it was made of, two accumulators of D columns.  S is two chunks ahead of P V.
 //
 // The arithmetic is that of the kernel for few rows: w = p v_scale relative to a reference near its running maximum, P = fp16(w), l = sum p
-// relative to a reference of its own.  The references follow only where w gets 2^8 ahead: the accumulator is rescaled in a few chunks of
-// a unit, and w <= 2^8 loses no bits in fp16.  Where a chunk's V scales are within 2^60 of what the references differ by (nearly
-// always: the general way is for zeros and for scales of very different sizes) p = w / v_scale needs no exp2 of its own.
+// relative to a reference of its own.  The reference of w follows only where the sum of p times the largest V scale does not say that all w
+// are below 2^15: the accumulator is rescaled in a few chunks of a unit, and w below 2^15 (fp16 ends at 65504) loses no bits in fp16.  Where a chunk's V scales are within 2^60 of what the references differ by (nearly
+// always: the general way is for zeros and for scales of very different sizes; there p is summed up by itself and its reference follows where it
+// gets 2^8 ahead) p = w / v_scale needs no exp2 of its own.
 // S starts from the bit pattern of 1.5*2^23, written by a small fp16 MMA, and reads as fp32 1.5*2^23 + dot.
 #pragma once
 
@@ -69,7 +72,8 @@ __device__ __forceinline__ int tile_chunks(const PParams& p, const TileSeq& q, i
   if (!q.uniform) vis = min(vis, q.first + (long long)(tile + 1) * p.unit_tokens);
   return vis > G ? (int)((vis + G - 1) / G) : 1;
 }
-// sum of floor((a t + b) / m), t = 0 .. n-1 (a, b >= 0)
+// sum of floor((a t + b) / m), t = 0 .. n-1 (a, b >= 0): whole parts out, then the points below the line counted along the other axis, which
+// swaps a and m as Euclid's algorithm does
 __device__ __noinline__ long long floor_sum(long long n, long long m, long long a, long long b) {
   long long sum = 0;
   while (n > 0) {

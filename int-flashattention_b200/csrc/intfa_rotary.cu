@@ -1,6 +1,6 @@
 // Rotary positions of one or two tensors (q, and k with it) in one launch; the gradient of a rotation is the rotation back.
 //
-// Moves each value once in and once out (2 * 84 million bf16 values: 340 MB, 52.6 us at the measured copy rate, 62.7 here; 24 MB of fp32, half of
+// Moves each value once in and once out (2 * 84 million bf16 values: 340 MB, 52.6 us at the measured copy rate, 62.7 here; 148 MB of fp32, half of
 // the channels rotated, 22.9 and 32.2): bound by HBM, and for a few tokens by the launch (2.4 us in a graph).  All heads of
 // a token share the (cos, sin) of its position: a slot (the lanes that hold a row) reads what it needs of the table once, keeps it in
 // registers and goes through several heads of one token, a few rows in flight.  The first rows are asked for ahead of the table, so

@@ -239,7 +239,8 @@ def attention_int8_paged(q, k_cache, v_cache, q_scale, k_scale, v_scale, block_t
     cu_seqlens[s] .. cu_seqlens[s+1]-1 (None: one row each, decode); causal: they are its last tokens, row i of n sees keys up to
     seq_lens[s] - n + i, else all keys.  Sequences may share pages; keys whose page lies outside the cache do not count
     (check_status() tells).  Query heads share K/V heads in order, as in attention_int8.  A row that sees no key is
-    zero.  Returns o [tokens, query heads, D] in out_dtype (torch.float16 unless given, or torch.bfloat16); with `out` it is written there,
+    zero.  Scores, softmax and sums are float32; p times the key's V scale is rounded to float16 (2^-11 of each, 2^-25 of the row's largest) for the
+    product with the codes of v.  Returns o [tokens, query heads, D] in out_dtype (torch.float16 unless given, or torch.bfloat16); with `out` it is written there,
     and rows behind the last sequence stay as they were (without it they are not set).  return_lse: and the log2-domain LSE
     [tokens, query heads].  (debug_path: test hook, 1 or 2 for one of the two kernels whatever the sizes.)"""
     return (_native_mod or _native()).paged(q, k_cache, v_cache, q_scale, k_scale, v_scale, block_table, seq_lens, cu_seqlens, causal, sm_scale,
