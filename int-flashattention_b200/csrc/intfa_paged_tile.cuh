@@ -23,8 +23,8 @@
 // The arithmetic is that of the kernel for few rows: w = p v_scale relative to a reference near its running maximum, P = fp16(w), l = sum p
 // relative to a reference of its own.  The reference of w follows only where the sum of p times the largest V scale does not say that all w
 // are below 2^15: the accumulator is rescaled in a few chunks of a unit, and w below 2^15 (fp16 ends at 65504) loses no bits in fp16.
-// Where a chunk's V scales are within 2^60 of what the references differ by (nearly always: the general way is for zeros and for scales of very different sizes; there p is summed up by itself and its reference follows where it
-// gets 2^8 ahead) p = w / v_scale needs no exp2 of its own.
+// Where a chunk's V scales are within 2^60 of what the references differ by (nearly always: the general way is for zeros and for scales of very
+// different sizes; there p is summed up by itself and its reference follows where it gets 2^8 ahead) p = w / v_scale needs no exp2 of its own.
 // S starts from the bit pattern of 1.5*2^23, written by a small fp16 MMA, and reads as fp32 1.5*2^23 + dot.
 #pragma once
 
