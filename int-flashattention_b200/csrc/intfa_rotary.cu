@@ -25,7 +25,8 @@ struct RotaryJob {
   int* status;
 };
 
-template <typename T, int SPIN>
+// PART: rot is no multiple of 8, so that a piece is rotated in part (2 % of the time of large calls, so not for the others)
+template <typename T, int SPIN, bool PART>
 __global__ void __launch_bounds__(kThreads, SPIN == kAny ? 2 : 3) rotary_kernel(const RotaryJob p) {
   constexpr int U = sizeof(T) == 4 ? 1 : 2;                  // rows in flight
   const int slot = threadIdx.x >> p.lpr_log, slots = kThreads >> p.lpr_log;
@@ -85,6 +86,14 @@ __global__ void __launch_bounds__(kThreads, SPIN == kAny ? 2 : 3) rotary_kernel(
         // (what is not rotated as it is, a NaN's bits too)
         if (at.a >= p.rot) a = in[u].a;
         if (at.b >= p.rot) c = in[u].b;
+        if constexpr (PART) {
+          constexpr int W = Raw<T>::W;
+#pragma unroll
+          for (int i = 0; i < W; ++i) {
+            if (at.a + i * (8 / W) >= p.rot) a.w[i] = in[u].a.w[i];
+            if (at.b + i * (8 / W) >= p.rot) c.w[i] = in[u].b.w[i];
+          }
+        }
         if (!ok) {
           a.zero();
           c.zero();
@@ -115,7 +124,8 @@ int run(const RotaryJob& job, int D, bool interleaved, cudaStream_t stream) {
   const long long grid = (p.tokens + tokens_cta - 1) / tokens_cta;
   if (grid > 0x7fffffffLL) return set_error(INTFA_ERR_TOO_LARGE, "too many tokens");
   auto go = [&](auto kernel) { return launch_kernel("rotary", kernel, (unsigned)grid, kThreads, 0, stream, p); };
-  return interleaved ? go(rotary_kernel<T, kPairs>) : p.rot % 16 == 0 ? go(rotary_kernel<T, kHalf>) : go(rotary_kernel<T, kAny>);
+  if (interleaved) return p.rot % 8 ? go(rotary_kernel<T, kPairs, true>) : go(rotary_kernel<T, kPairs, false>);
+  return p.rot % 16 == 0 ? go(rotary_kernel<T, kHalf, false>) : go(rotary_kernel<T, kAny, true>);
 }
 
 }  // namespace

@@ -276,3 +276,20 @@ def test_single_tokens_and_chunks_in_one_call(news, lens, D, pkg):
             both.append(s.check(pkg, causal))
         s.path = 0
         assert any(torch.equal(o, x) for x in both)
+
+
+@pytest.mark.parametrize("D,rot", [(64, 20), (64, 2), (128, 100), (256, 66), (64, 32), (16, 6)])
+@pytest.mark.parametrize("dtype,words", [(torch.float16, torch.int16), (torch.bfloat16, torch.int16), (torch.float32, torch.int32)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_channels_that_are_not_rotated_keep_their_bits(D, rot, dtype, words, interleaved, pkg):
+    """Whatever they hold, and wherever the rotated part ends."""
+    g = torch.Generator(device="cuda").manual_seed(rot)
+    top = torch.iinfo(words)
+    x = torch.randint(top.min, top.max, (5, 3, D), device="cuda", generator=g, dtype=words)          # NaN of all kinds among them
+    x[..., rot::3] = top.max - x[..., rot::3].abs() % 100                                              # (these are)
+    x = x.view(dtype)
+    x[..., :rot] = torch.randn(5, 3, rot, device="cuda", generator=g).to(dtype)
+    cs, pos = pkg.rotary_table(50, rot, device="cuda"), torch.arange(45, 50, device="cuda")
+    y = pkg.rotary(x, None, cs, pos, interleaved=interleaved)
+    assert torch.equal(y[..., rot:].view(words), x[..., rot:].view(words))
+    assert torch.equal(y[..., :rot], O.turn(x[..., :rot].float(), cs[pos][:, None], interleaved).to(dtype))
