@@ -312,8 +312,8 @@ int intfa_paged_append(const IntfaAppendParams* p, void* stream);
  * cu_seqlens[s] .. cu_seqlens[s+1]-1 (NULL: one row a sequence); causal: row i of n sees the keys up to seq_lens[s] - n + i, else all.
  * Softmax, sums and the running output in fp32, p * v_scale rounded to fp16 for the product with v.  A row that sees nothing is zero
  * (lse -inf); rows behind the last sequence are not written.  o [tokens, H, D]: strides for (token, head), multiples of 8.
- * Sequences may share pages.  Keys of a page outside the cache do not count.  cu_seqlens must not fall; where it does, or a length does not fit its table row, nothing is read or written
- * outside and `status` tells.  lse_out (or NULL): [tokens, H] fp32 contiguous, log2 domain, as intfa_fwd's.
+ * Sequences may share pages.  Keys of a page outside the cache do not count.  cu_seqlens must not fall; where it does, or a length does not
+ * fit its table row, nothing is read or written outside and `status` tells.  lse_out (or NULL): [tokens, H] fp32 contiguous, log2 domain, as intfa_fwd's.
  * workspace: device scratch of intfa_paged_workspace_bytes() bytes, 256-byte aligned, contents irrelevant.
  */
 typedef struct IntfaPagedParams {

@@ -317,10 +317,11 @@ __device__ __forceinline__ void write_part(float* part, float* ml, int stride, c
   }
 }
 
-// One chunk.  sK, sV: its rows in shared memory; sS: its K scales, then the logarithms of its V scales; last[n]: the last key of the chunk that row n*8 + g sees.
-// MASKED: not all rows see all keys, or the K scales say kNoKey.
 constexpr float kNoKey = -INFINITY;               // in place of the K scale: no key, its page lies outside the cache (the V scale is 0)
 __device__ const float no_key = kNoKey;
+
+// One chunk.  sK, sV: its rows in shared memory; sS: its K scales, then the logarithms of its V scales; last[n]: the last key of the chunk that row n*8 + g sees.
+// MASKED: not all rows see all keys, or the K scales say kNoKey.
 template <int D, int NT, int G, bool MASKED>
 __device__ __forceinline__ void chunk_step(RowState<D, NT>& st, const uint32_t (&q)[D / 64][NT][4], const float (&qs)[NT], const int (&last)[NT],
                                            uint32_t sK, uint32_t sV, uint32_t sS) {
